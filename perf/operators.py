@@ -1,0 +1,391 @@
+"""Measured cases of the operators that stand beside the FP8 linears in a training step: layer normalisation, the
+vocabulary projection with its softmax cross entropy, and the AdamW update of many tensors.
+
+Every case is a dict of plain values.  `kind` says which operator it calls:
+
+  norm   layer_norm over the last dimension: forward, or forward and backward with the gradients of weight and bias
+  head   linear_cross_entropy, the loss of hidden states x [tokens, hidden] against labels under a projection
+         weight [vocab, hidden]: the loss with both gradients, or the losses of the single tokens without any
+  adamw  one AdamW step over a list of tensors, moments held in 32 bits, or in 8 (E4M3 codes of the first moment and of
+         the root of the second, each block of 256 elements with a power-of-two scale, stochastically rounded)
+
+With `own` false, `run` computes them in 32 bits from elementary torch operations.  Sizes: the decoder layer and token
+counts of this repository's benchmark, the layer sizes of its tests, and generic ones (vocabularies of 6 to 128
+thousand).  Activations are ~N(0, 1), projection weights give logits of standard deviation 1.3, hidden states lean
+towards their label's row by anything between nothing and ten, as those of a model in training do.
+"""
+import math
+
+import torch
+
+own = False
+
+DEVICE = torch.device("cuda", 0)
+TORCH = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+BYTES = {"fp32": 4, "fp16": 2, "bf16": 2}
+EPS = 1e-5
+IGNORE = -100
+BLOCK = 256          # elements of an 8-bit moment that share a scale
+LR, BETAS, ADAM_EPS, DECAY = 1e-4, (0.9, 0.95), 1e-8, 0.1
+
+
+def listed():
+    return [
+        # one token through a norm of a full-size model, as in token-by-token evaluation: launch and host time
+        dict(name="norm eval 1 token", kind="norm", rows=1, cols=4096, dtype="bf16", wdtype="fp32", train=False),
+        # a size that is a multiple of nothing, everything in 32 bits
+        dict(name="norm step 1021x1037 fp32", kind="norm", rows=1021, cols=1037, dtype="fp32", wdtype="fp32", train=True),
+        # the norm before a linear of the benchmark layer
+        dict(name="norm step 4096x4096", kind="norm", rows=4096, cols=4096, dtype="bf16", wdtype="fp32", train=True),
+        # a long batch through a wide model
+        dict(name="norm step 16384x8192", kind="norm", rows=16384, cols=8192, dtype="bf16", wdtype="bf16", train=True),
+        # the losses of a few tokens under a full vocabulary: scoring answers
+        dict(name="head losses of 16 tokens", kind="head", tokens=16, hidden=4096, vocab=128000, dtype="bf16", train=False, ignored=0.0),
+        # sizes that are multiples of nothing, fp16
+        dict(name="head step 333x515x6001", kind="head", tokens=333, hidden=515, vocab=6001, dtype="fp16", train=True, ignored=0.1),
+        # a small model's head on an unpadded batch, part of it prompt
+        dict(name="head step 1021x1024x50001", kind="head", tokens=1021, hidden=1024, vocab=50001, dtype="bf16", train=True, ignored=0.25),
+        # the head beside the benchmark layer
+        dict(name="head step 4096x4096x128000", kind="head", tokens=4096, hidden=4096, vocab=128000, dtype="bf16", train=True, ignored=0.0),
+        # the small tensors of a model, norms and biases, odd sizes: one launch for all of them
+        dict(name="adamw 200 small tensors", kind="adamw", sizes="small", tensors=200, most=20000, dtype="fp32", gdtype="fp32", copies="none", bits=32),
+        # a low-precision model without master weights
+        dict(name="adamw 8-bit 33 tensors bf16", kind="adamw", sizes="small", tensors=33, most=300000, dtype="bf16", gdtype="bf16", copies="none", bits=8),
+        # the benchmark's decoder layer: fp32 masters with 16-bit model weights and gradients
+        dict(name="adamw layer", kind="adamw", sizes="layer", hidden=4096, qkv=6144, inter=14336, dtype="fp32", gdtype="bf16", copies="bf16", bits=32),
+        # the same with moments in 8 bits and the fp32 gradients of FP8 linears
+        dict(name="adamw 8-bit layer", kind="adamw", sizes="layer", hidden=4096, qkv=6144, inter=14336, dtype="fp32", gdtype="fp32", copies="none", bits=8),
+    ]
+
+
+def _log(rng, lo, hi):
+    return math.exp(rng.uniform(math.log(lo), math.log(hi)))
+
+
+def _size(rng, lo, hi, grid):
+    """A size between lo and hi, spread over its logarithm, on a grid (clipped to the range)."""
+    v = int(_log(rng, lo, hi))
+    v = max(lo, min(hi, (v + grid // 2) // grid * grid)) if v >= grid else max(lo, v)
+    return v + grid if v == 3072 else v
+
+
+def draw(rng):
+    kind = rng.choice(["norm", "head", "adamw"])
+    grid = rng.choice([128, 16, 1])
+    if kind == "norm":
+        dtype = rng.choice(["bf16", "bf16", "fp16", "fp32"])
+        return dict(kind=kind, rows=_size(rng, 1, 16384, rng.choice([128, 1])), cols=_size(rng, 64, 4096 if dtype == "fp32" else 8192, grid),
+                    dtype=dtype, wdtype=rng.choice(["fp32", dtype]), train=rng.random() < 0.7)
+    if kind == "head":
+        train = rng.random() < 0.7
+        c = dict(kind=kind, tokens=_size(rng, 16, 4096, rng.choice([128, 1])) if train else _size(rng, 1, 512, 1),
+                 hidden=_size(rng, 128, 4096, grid), vocab=_size(rng, 1000, 128000, rng.choice([128, 1])),
+                 dtype=rng.choice(["bf16", "bf16", "fp16"]), train=train, ignored=rng.choice([0.0, 0.1, 0.5]))
+        return c
+    dtype = rng.choice(["fp32", "fp32", "bf16", "fp16"])
+    c = dict(kind=kind, dtype=dtype, gdtype=rng.choice(["fp32", "bf16"]) if dtype == "fp32" else dtype,
+             copies=rng.choice(["none", "bf16"]) if dtype == "fp32" else "none", bits=rng.choice([32, 8]))
+    if rng.random() < 0.6:
+        return dict(c, sizes="small", tensors=_size(rng, 1, 300, 1), most=_size(rng, 100, 400000, 1))
+    hidden = _size(rng, 512, 4096, rng.choice([256, 16]))
+    return dict(c, sizes="layer", hidden=hidden, qkv=hidden + hidden // 4, inter=_size(rng, int(2.5 * hidden), int(3.5 * hidden), 16))
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _lengths(case):
+    """Elements of each tensor of an adamw case."""
+    if case["sizes"] == "layer":
+        h, q, i = case["hidden"], case["qkv"], case["inter"]
+        return [h, h * q, h * h, h, h * i, h * i, i * h]
+    n, most = case["tensors"], case["most"]
+    return [1 + (k * 7919 + 13) * 104729 % most for k in range(n)]
+
+
+def _normal(g, shape, std, dtype):
+    return (torch.randn(shape, generator=g, device=DEVICE) * std).to(dtype)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device=DEVICE).manual_seed(seed)
+    s = dict(case)
+    dt = TORCH[case["dtype"]]
+    if case["kind"] == "norm":
+        rows, cols, wd = case["rows"], case["cols"], TORCH[case["wdtype"]]
+        x = torch.randn((rows, cols), generator=g, device=DEVICE)
+        # a residual stream: a mean of its own for every token, a few large channels
+        x = x * (1 + 8 * (torch.rand(cols, generator=g, device=DEVICE) < 0.01)) + _normal(g, (rows, 1), 0.3, torch.float32)
+        s.update(x=x.to(dt), w=(1 + _normal(g, (cols,), 0.1, torch.float32)).to(wd), b=_normal(g, (cols,), 0.1, wd))
+        if case["train"]:
+            s["dy"] = _normal(g, (rows, cols), 1e-3 if case["dtype"] != "fp16" else 1e-1, dt)
+            for k in ("x", "w", "b"):
+                s[k].requires_grad_(True)
+    elif case["kind"] == "head":
+        n, h, v = case["tokens"], case["hidden"], case["vocab"]
+        w = _normal(g, (v, h), 1.28 / math.sqrt(h), dt)
+        labels = torch.randint(0, v, (n,), generator=g, device=DEVICE)
+        lean = 6 * torch.rand((n, 1), generator=g, device=DEVICE)
+        x = (torch.randn((n, h), generator=g, device=DEVICE) + lean * w[labels].float()).to(dt)
+        if case["ignored"]:
+            labels = torch.where(torch.rand(n, generator=g, device=DEVICE) < case["ignored"], IGNORE, labels)
+        s.update(x=x, w=w, labels=labels)
+        if case["train"]:
+            x.requires_grad_(True)
+            w.requires_grad_(True)
+    else:
+        lens = _lengths(case)
+        room = [-(-n // BLOCK) for n in lens]   # blocks
+        first, at = [], 0
+        for r in room:
+            first.append(at)
+            at += r
+        total = at * BLOCK
+        # every tensor is a view of one buffer and begins on a block; what is behind it in its last block stays zero
+        where = torch.tensor(first, device=DEVICE).repeat_interleave(torch.tensor(room, device=DEVICE))
+        inside = ((torch.arange(at, device=DEVICE) - where)[:, None] * BLOCK + torch.arange(BLOCK, device=DEVICE)).to(torch.int32)
+        ends = torch.tensor(lens, device=DEVICE).repeat_interleave(torch.tensor(room, device=DEVICE))
+        live = inside < ends[:, None]
+
+        def flat(std, dtype):
+            # every block with a level of its own
+            level = torch.exp(torch.randn((at, 1), generator=g, device=DEVICE))
+            return (torch.randn((at, BLOCK), generator=g, device=DEVICE) * level * std * live).to(dtype).reshape(total)
+
+        def views(t):
+            return [t[f * BLOCK:f * BLOCK + n] for f, n in zip(first, lens)]
+
+        p = (torch.randn((at, BLOCK), generator=g, device=DEVICE) * 0.02 * live).to(dt).reshape(total)
+        grad = flat(1e-3, TORCH[case["gdtype"]])
+        m = flat(3e-4, torch.float32)
+        r = flat(1e-3, torch.float32).abs_().add_(m.abs())   # a root of the second moment, nowhere below the first
+        s.update(p=p, grad=grad, blocks=at, index=inside, step=1000, clip=torch.full((1,), 0.75, device=DEVICE),
+                 ps=views(p), grads=views(grad), copy=None, copies_=None)
+        if case["copies"] != "none":
+            s["copy"] = p.to(TORCH[case["copies"]])
+            s["copies_"] = views(s["copy"])
+        if case["bits"] == 32:
+            v = r.square_()
+            s.update(m=m, v=v, ms=views(m), vs=views(v))
+        else:
+            half = torch.full((at, BLOCK), 32768, dtype=torch.int32, device=DEVICE)
+            mc, msc = _encode(m.view(at, BLOCK), half, False)
+            rc, rsc = _encode(r.view(at, BLOCK), half, True)
+
+            def scales(t):
+                return [t[f:f + k] for f, k in zip(first, room)]
+
+            s.update(m=mc.reshape(total), r=rc.reshape(total), msc=msc, rsc=rsc)
+            s.update(ms=views(s["m"]), rs=views(s["r"]), mscs=scales(msc), rscs=scales(rsc))
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ the operators
+def run(s):
+    if s["kind"] == "norm":
+        return _norm(s)
+    if s["kind"] == "head":
+        return _head(s)
+    return _adamw8(s) if s["bits"] == 8 else _adamw(s)
+
+
+def _norm(s):
+    if own:
+        from nanotron_amd.nn import layer_norm
+
+        if not s["train"]:
+            with torch.no_grad():
+                return layer_norm(s["x"], s["w"], s["b"], eps=EPS)
+        y = layer_norm(s["x"], s["w"], s["b"], eps=EPS)
+        return (y.detach(), *torch.autograd.grad(y, (s["x"], s["w"], s["b"]), s["dy"]))
+    with torch.no_grad():
+        x, w, b = s["x"].float(), s["w"].float(), s["b"].float()
+        mean = x.mean(-1, keepdim=True)
+        c = x - mean
+        rstd = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + EPS)
+        xhat = c * rstd
+        y = (xhat * w + b).to(s["x"].dtype)
+        if not s["train"]:
+            return y
+        dy = s["dy"].float()
+        gw = dy * w
+        dx = rstd * (gw - gw.mean(-1, keepdim=True) - xhat * (gw * xhat).mean(-1, keepdim=True))
+        return y, dx.to(s["x"].dtype), (dy * xhat).sum(0).to(s["w"].dtype), dy.sum(0).to(s["b"].dtype)
+
+
+def _head(s):
+    if own:
+        from nanotron_amd.nn import linear_cross_entropy
+
+        if not s["train"]:
+            with torch.no_grad():
+                return linear_cross_entropy(s["x"], s["w"], s["labels"], ignore_index=IGNORE, reduction="none")
+        loss = linear_cross_entropy(s["x"], s["w"], s["labels"], ignore_index=IGNORE)
+        return (loss.detach(), *torch.autograd.grad(loss, (s["x"], s["w"])))
+    with torch.no_grad():
+        x, w = s["x"].float(), s["w"].float()
+        logits = x @ w.t()
+        valid = s["labels"] != IGNORE
+        label = torch.where(valid, s["labels"], 0)[:, None]
+        top = logits.amax(-1, keepdim=True)
+        at_label = logits.gather(1, label)
+        e = torch.exp(logits - top)
+        total = e.sum(-1, keepdim=True)
+        losses = torch.where(valid, (torch.log(total) + top - at_label)[:, 0], 0.0)
+        if not s["train"]:
+            return losses
+        count = valid.sum()
+        p = e * (valid[:, None] / (total * count))
+        p.scatter_add_(1, label, -(valid / count)[:, None])
+        return losses.sum() / count, (p @ w).to(s["x"].dtype), (p.t() @ x).to(s["w"].dtype)
+
+
+def _adamw(s):
+    if own:
+        from nanotron_amd.optim import adamw_step
+
+        adamw_step(s["ps"], s["grads"], s["ms"], s["vs"], lr=LR, betas=BETAS, eps=ADAM_EPS, weight_decay=DECAY, step=s["step"],
+                   grad_scale=s["clip"], copies=s["copies_"])
+    else:
+        g = s["grad"].float() * s["clip"]
+        s["m"].copy_(BETAS[0] * s["m"] + (1 - BETAS[0]) * g)
+        s["v"].copy_(BETAS[1] * s["v"] + (1 - BETAS[1]) * (g * g))
+        _update(s, s["m"], torch.sqrt(s["v"]))
+    return [t for t in (s["p"], s["m"], s["v"], s["copy"]) if t is not None]
+
+
+def _update(s, m, r):
+    """The step of the parameters from the first moment and the root of the second."""
+    to = LR / (1 - BETAS[0] ** s["step"])
+    root = 1 / math.sqrt(1 - BETAS[1] ** s["step"])
+    p = s["p"].float() * (1 - LR * DECAY) - to * (m / (r * root + ADAM_EPS))
+    s["p"].copy_(p)
+    if s["copy"] is not None:
+        s["copy"].copy_(p)
+
+
+def _i32(v):
+    return v - (1 << 32) if v >= 1 << 31 else v
+
+
+def _dither(index, seed):
+    """16 pseudo-random bits for each element, from its place in its tensor and the seed: an integer hash of the pair of
+    elements it belongs to, of which the even one takes the low half."""
+    def down(x, k):   # unsigned shift
+        return (x >> k) & ((1 << (32 - k)) - 1)
+
+    x = (index >> 1) * _i32(0x9E3779B1) + _i32(seed * 0xBB67AE85 & 0xFFFFFFFF)
+    x = (x ^ down(x, 15)) * _i32(0x6A09E667)
+    x = (x ^ down(x, 13)) * _i32(0x3C6EF373)
+    x = x ^ down(x, 16)
+    return torch.where(index & 1 == 1, down(x, 16), x & 0xFFFF)
+
+
+def _encode(x, dither, keep):
+    """fp32 [blocks, BLOCK] -> E4M3 codes and the scale of each block, the power of two that brings its largest magnitude
+    into (224, 448]; code = x scale, rounded up where the dither exceeds what is missing.  `keep`: no value above zero
+    becomes zero."""
+    a = x.abs()
+    top = a.amax(-1, keepdim=True).view(torch.int32)
+    k = 8 - ((top >> 23) - 127) - ((top & 0x7FFFFF) > 0x600000).int()
+    k = torch.where(top == 0, 0, k.clamp(-126, 126))
+    scale = ((k + 127) << 23).view(torch.float32)
+    y = a * scale
+    normal = ((y.view(torch.int32) + (dither << 4)) >> 20) - 960
+    small = torch.floor(y * 512 + dither.float() * 2.0 ** -16).int()
+    code = torch.where(y >= 2.0 ** -6, normal, small)
+    if keep:
+        code = torch.where((code == 0) & (a > 0), 1, code)
+    code = torch.where(torch.isfinite(a), code, 0x7F)
+    code = code | ((x.view(torch.int32) >> 24) & 0x80)
+    return code.to(torch.uint8), scale[:, 0].contiguous()
+
+
+def _decode(codes, scale):
+    return codes.view(torch.float8_e4m3fn).float().view(-1, BLOCK) / scale[:, None]
+
+
+def _adamw8(s):
+    if own:
+        from nanotron_amd.optim import adamw_8bit_step
+
+        adamw_8bit_step(s["ps"], s["grads"], s["ms"], s["mscs"], s["rs"], s["rscs"], lr=LR, betas=BETAS, eps=ADAM_EPS, weight_decay=DECAY,
+                        step=s["step"], seed=s["step"], grad_scale=s["clip"], copies=s["copies_"])
+    else:
+        g = (s["grad"].float() * s["clip"]).view(-1, BLOCK)
+        m = BETAS[0] * _decode(s["m"], s["msc"]) + (1 - BETAS[0]) * g
+        r = _decode(s["r"], s["rsc"])
+        r = torch.sqrt(BETAS[1] * (r * r) + (1 - BETAS[1]) * (g * g))
+        _update(s, m.reshape(-1), r.reshape(-1))
+        d = _dither(s["index"], s["step"])
+        for x, keep, codes, scales in ((m, False, "m", "msc"), (r, True, "r", "rsc")):
+            c, k = _encode(x, d, keep)
+            s[codes].copy_(c.reshape(-1))
+            s[scales].copy_(k)
+    # the codes as the numbers that they are, beside their scales
+    f8 = torch.float8_e4m3fn
+    return [t for t in (s["p"], s["m"].view(f8), s["msc"], s["r"].view(f8), s["rsc"], s["copy"]) if t is not None]
+
+
+# ------------------------------------------------------------------------------------------------ 64 bits
+def exact(case, seed):
+    s = prepare(case, seed)
+    with torch.no_grad():
+        if case["kind"] == "norm":
+            x, w, b = (s[k].detach().double() for k in ("x", "w", "b"))
+            var, mean = torch.var_mean(x, -1, unbiased=False, keepdim=True)
+            rstd = torch.rsqrt(var + EPS)
+            xhat = (x - mean) * rstd
+            y = xhat * w + b
+            if not case["train"]:
+                return y
+            dy = s["dy"].double()
+            u = dy * w
+            dx = (u - u.mean(-1, keepdim=True) - xhat * (u * xhat).mean(-1, keepdim=True)) * rstd
+            return y, dx, (dy * xhat).sum(0), dy.sum(0)
+        if case["kind"] == "head":
+            x, w, labels = s["x"].detach().double(), s["w"].detach().double(), s["labels"]
+            logp = torch.log_softmax(x @ w.t(), -1)
+            keep = labels != IGNORE
+            rows = torch.nonzero(keep)[:, 0]
+            losses = torch.zeros_like(labels, dtype=torch.float64)
+            losses[rows] = -logp[rows, labels[rows]]
+            if not case["train"]:
+                return losses
+            count = rows.numel()
+            d = logp.exp_()
+            d[rows, labels[rows]] -= 1
+            d[~keep] = 0
+            d /= count
+            return losses.sum() / count, d @ w, d.t() @ x
+        g = s["grad"].double() * 0.75
+        if case["bits"] == 8:
+            spread = torch.ones(BLOCK, dtype=torch.float64, device=DEVICE)
+            m = s["m"].view(torch.float8_e4m3fn).double() / torch.outer(s["msc"].double(), spread).reshape(-1)
+            r = s["r"].view(torch.float8_e4m3fn).double() / torch.outer(s["rsc"].double(), spread).reshape(-1)
+            v = r * r
+        else:
+            m, v = s["m"].double(), s["v"].double()
+        m = m + (1 - BETAS[0]) * (g - m)
+        v = v + (1 - BETAS[1]) * (g * g - v)
+        mh, vh = m / (1 - BETAS[0] ** s["step"]), v / (1 - BETAS[1] ** s["step"])
+        p = s["p"].double() * (1 - LR * DECAY) - LR * mh / (vh.sqrt() + ADAM_EPS)
+        out = [p, m, v] if case["bits"] == 32 else [p, None, None, None, None]
+        return out if s["copy"] is None else out + [p]
+
+
+# ------------------------------------------------------------------------------------------------ work
+def work(case):
+    b = BYTES[case["dtype"]]
+    if case["kind"] == "norm":
+        n, c, wb = case["rows"] * case["cols"], case["cols"], BYTES[case["wdtype"]]
+        if not case["train"]:
+            return {"bytes": 2 * n * b + 2 * c * wb, "flops": 8 * n}
+        return {"bytes": 4 * n * b + 4 * c * wb, "flops": 24 * n}
+    if case["kind"] == "head":
+        n, h, v = case["tokens"], case["hidden"], case["vocab"]
+        if not case["train"]:
+            return {"bytes": (n * h + v * h) * b + 12 * n, "flops": 2 * n * h * v}
+        return {"bytes": 2 * (n * h + v * h) * b + 8 * n + 4, "flops": 6 * n * h * v}
+    n = sum(_lengths(case))
+    per = 2 * b + BYTES[case["gdtype"]] + (0 if case["copies"] == "none" else BYTES[case["copies"]])
+    per += 16 if case["bits"] == 32 else 4 + 16 / BLOCK
+    return {"bytes": n * per, "flops": (15 if case["bits"] == 32 else 50) * n}
