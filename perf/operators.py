@@ -83,8 +83,9 @@ def draw(rng):
                  dtype=rng.choice(["bf16", "bf16", "fp16"]), train=train, ignored=rng.choice([0.0, 0.1, 0.5]))
         return c
     dtype = rng.choice(["fp32", "fp32", "bf16", "fp16"])
-    c = dict(kind=kind, dtype=dtype, gdtype=rng.choice(["fp32", "bf16"]) if dtype == "fp32" else dtype,
-             copies=rng.choice(["none", "bf16"]) if dtype == "fp32" else "none", bits=rng.choice([32, 8]))
+    # a master in 32 bits has gradients in 32, or the 16 of the model weights that are written beside it
+    grads, copies = rng.choice([("fp32", "none"), ("bf16", "none"), ("bf16", "bf16")]) if dtype == "fp32" else (dtype, "none")
+    c = dict(kind=kind, dtype=dtype, gdtype=grads, copies=copies, bits=rng.choice([32, 8]))
     if rng.random() < 0.6:
         return dict(c, sizes="small", tensors=_size(rng, 1, 300, 1), most=_size(rng, 100, 400000, 1))
     hidden = _size(rng, 512, 4096, rng.choice([256, 16]))
@@ -98,7 +99,7 @@ def _lengths(case):
         h, q, i = case["hidden"], case["qkv"], case["inter"]
         return [h, h * q, h * h, h, h * i, h * i, i * h]
     n, most = case["tensors"], case["most"]
-    return [1 + (k * 7919 + 13) * 104729 % most for k in range(n)]
+    return [n + (n == 3072) for n in (1 + (k * 7919 + 13) * 104729 % most for k in range(n))]
 
 
 def _normal(g, shape, std, dtype):
