@@ -6,7 +6,8 @@
 The libraries are built in-tree so that they travel with the source tree to the GPU box; nothing is
 JIT-compiled at import time.
 
-nanotron_amd/_hostcall.so is a CPython extension on top of libntfp8.so: the host side of the hot calls.
+nanotron_amd/_hostcall.so and _opscall.so are CPython extensions on top of libntfp8.so: the host side of the fp8 calls and of
+the operators of include/ntops.h.
 
 Profiling libraries (nanotron_amd/profiling/, loaded by nothing but the benchmark's wg-timeline workload):
 libntfp8_stamps.so is the product library with per-workgroup time stamps compiled into the GEMM kernel
@@ -24,9 +25,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libntfp8.so")
 HOSTCALL = os.path.join(HERE, "_hostcall.so")
+OPSCALL = os.path.join(HERE, "_opscall.so")
 PROFILING_DIR = os.path.join(HERE, "profiling")
 LIB_STAMPS = os.path.join(PROFILING_DIR, "libntfp8_stamps.so")
-SOURCES = ["quant.hip", "gemm.hip", "gemm_mid.hip", "gemm_few.hip", "gemm_any.hip", "capi.hip"]
+SOURCES = ["quant.hip", "gemm.hip", "gemm_mid.hip", "gemm_few.hip", "gemm_any.hip", "capi.hip",
+           "layer_norm.hip", "adamw.hip", "head.hip", "ops_capi.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
@@ -59,8 +62,8 @@ def _link(out: str, objs) -> None:
     subprocess.check_call([HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out, *objs])
 
 
-def _build_hostcall() -> str:
-    """The host extension: plain C++ against torch's headers, linked to the libntfp8.so beside it."""
+def _build_extension(source: str, out: str) -> str:
+    """A host extension: plain C++ against torch's headers, linked to the libntfp8.so beside it."""
     import sysconfig
 
     import torch
@@ -68,14 +71,15 @@ def _build_hostcall() -> str:
 
     inc = [f"-I{p}" for p in [*include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]]]
     libs = [f"-L{p}" for p in library_paths()]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, os.path.join(CSRC, "hostcall.cpp"),
-           "-o", HOSTCALL, *libs, "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python", f"-L{HERE}", "-l:libntfp8.so",
+    name = os.path.basename(out)[:-len(".so")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-DTORCH_EXTENSION_NAME={name}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, os.path.join(CSRC, source),
+           "-o", out, *libs, "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python", f"-L{HERE}", "-l:libntfp8.so",
            "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"g++ failed for hostcall.cpp:\n{r.stderr}")
-    return HOSTCALL
+        raise RuntimeError(f"g++ failed for {source}:\n{r.stderr}")
+    return out
 
 
 def build(verbose: bool = True, profiling: bool = False) -> str:
@@ -88,7 +92,8 @@ def build(verbose: bool = True, profiling: bool = False) -> str:
         objs = list(ex.map(_compile, jobs))
     plain = objs[:len(SOURCES)]
     _link(LIB, plain)
-    built = [LIB, _build_hostcall()]
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        built = [LIB, *ex.map(_build_extension, ["hostcall.cpp", "opscall.cpp"], [HOSTCALL, OPSCALL])]
     if profiling:
         os.makedirs(PROFILING_DIR, exist_ok=True)
         for obj, out in zip(objs[len(SOURCES):], [LIB_STAMPS] + [experiment_lib(n) for n in EXPERIMENTS]):

@@ -1,0 +1,248 @@
+// AdamW over many tensors, moments in fp32 or in 8 bits.
+//
+// Bound by memory: an fp32 parameter with a 16-bit gradient moves 26 bytes with fp32 moments, 14 with 8-bit ones.  One launch
+// takes up to kMostTensors tensors, their pointers and sizes with the launch's arguments, so that nothing has to be copied to
+// the device first; a block takes kChunk elements of one tensor.
+//
+// 8-bit moments.  The first moment m and the root r of the second are kept as E4M3 codes, blocks of 256 elements with a
+// power-of-two scale each, found from the new values: a wave holds a block, four elements a lane, so that the block's
+// largest magnitude is a fold over the lanes and the codes never exist anywhere but in registers and the state.
+//   * r and not r^2: the format's 17 binades then span 34 of the second moment.
+//   * Stochastic rounding: beta2 = 0.95 moves r by at most 2.5 % a step downwards, less than half a step of the format (3 to
+//     6 %); rounded to nearest it would never fall.  The 16 bits are hashed from the element's place and the caller's seed,
+//     and both moments of an element use the same ones, so that their errors partly cancel in m / r.
+//   * r above zero keeps the smallest code: a root of zero under a first moment that is not would divide by eps.
+#include "ops_common.h"
+
+namespace ntfp8 {
+namespace {
+
+constexpr int kMostTensors = 40;
+constexpr int kThreads = 256, kEach = 4;
+constexpr int kTurns = 4;                              // pieces of kEach elements a thread, all requested before the first is used
+constexpr int kChunk = kThreads * kEach * kTurns;
+constexpr int kBlock = NTOPS_ADAMW_BLOCK;
+static_assert(kBlock == 64 * kEach, "a wave holds a block of 8-bit moments");
+
+struct Tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    void* copy;
+    float* ms;
+    float* vs;
+    int64_t n;
+};
+struct Step {
+    Tensor t[kMostTensors];
+    int first[kMostTensors + 1];   // first block of the launch for each tensor
+    int count;
+    int copy_dtype;                // -1: none
+    const float* grad_scale;
+    float beta1, rest1, beta2, rest2, keep, to, root, eps;
+    uint32_t seed;
+};
+
+// 16 bits for each of the two elements of a pair, the even one's in the low half
+__device__ __forceinline__ uint32_t dither_of(uint32_t pair, uint32_t seed) {
+    uint32_t x = pair * 0x9E3779B1u + seed;   // (seed times an odd constant, from the host)
+    x = (x ^ (x >> 15)) * 0x6A09E667u;
+    x = (x ^ (x >> 13)) * 0x3C6EF373u;
+    return x ^ (x >> 16);
+}
+
+// exponent k of the block scale 2^k from the bits of its largest magnitude: 2^k times it lies in (224, 448]
+__device__ __forceinline__ int scale_exponent(uint32_t top) {
+    const int k = 135 - (int)(top >> 23) - ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return top == 0u ? 0 : min(max(k, -126), 126);
+}
+
+// |value| times the scale, at most 448, plus its dither -> code without sign
+__device__ __forceinline__ uint32_t encode(float a, float scale, uint32_t dither) {
+    const float y = a * scale;
+    const uint32_t normal = ((__float_as_uint(y) + (dither << 4)) >> 20) - 960u;
+    const uint32_t small = (uint32_t)(y * 512.0f + (float)dither * 0x1p-16f);   // below 2^-6 codes are 2^-9 apart
+    uint32_t c = y >= 0x1p-6f ? normal : small;
+    return (__float_as_uint(a) & 0x7fffffffu) >= kInfBits ? 0x7fu : c;
+}
+
+template <int N>
+__device__ __forceinline__ void decode(uint32_t w, float inverse, float (&v)[N]) {
+    static_assert(N == 4, "");
+    typedef float v2 __attribute__((ext_vector_type(2)));
+    const v2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    v[0] = lo.x * inverse, v[1] = lo.y * inverse, v[2] = hi.x * inverse, v[3] = hi.y * inverse;
+}
+
+template <int P, int G, bool k8>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Step s) {
+    int which = 0;
+    for (int half = 32; half >= 1; half /= 2)   // the last tensor whose first block is not behind this one
+        if (which + half < s.count && s.first[which + half] <= (int)blockIdx.x) which += half;
+    const Tensor& T = s.t[which];
+    const int64_t n = T.n, at = (int64_t)((int)blockIdx.x - s.first[which]) * kChunk + threadIdx.x * kEach;
+    Piece<P, kEach> pr[kTurns];
+    Piece<G, kEach> gr[kTurns];
+    Piece<NTFP8_F32, kEach> mr[kTurns], vr[kTurns];
+    uint32_t mc[kTurns], vc[kTurns];
+    float ms[kTurns], vs[kTurns];
+    int left[kTurns];
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+        const int64_t i = at + u * (kThreads * kEach);
+        left[u] = i < n ? (int)min((int64_t)kEach, n - i) : 0;
+        pr[u] = load_piece<P, kEach>(T.p, i, left[u]);
+        gr[u] = load_piece<G, kEach>(T.g, i, left[u]);
+        if constexpr (k8) {
+            mc[u] = vc[u] = 0;
+            ms[u] = vs[u] = 1.0f;
+            if (left[u] == kEach) {
+                mc[u] = reinterpret_cast<const Word*>(static_cast<const uint8_t*>(T.m) + i)->w;
+                vc[u] = reinterpret_cast<const Word*>(static_cast<const uint8_t*>(T.v) + i)->w;
+            } else {
+                for (int e = 0; e < left[u]; ++e) {
+                    mc[u] |= (uint32_t)static_cast<const uint8_t*>(T.m)[i + e] << (8 * e);
+                    vc[u] |= (uint32_t)static_cast<const uint8_t*>(T.v)[i + e] << (8 * e);
+                }
+            }
+            if (left[u]) {
+                ms[u] = T.ms[i / kBlock];
+                vs[u] = T.vs[i / kBlock];
+            }
+        } else {
+            mr[u] = load_piece<NTFP8_F32, kEach>(T.m, i, left[u]);
+            vr[u] = load_piece<NTFP8_F32, kEach>(T.v, i, left[u]);
+        }
+    }
+    const float factor = s.grad_scale ? *s.grad_scale : 1.0f;
+#pragma unroll
+    for (int u = 0; u < kTurns; ++u) {
+        const int64_t i = at + u * (kThreads * kEach);
+        float p[kEach], g[kEach], m[kEach], v[kEach], r[kEach];
+        unpack<P, kEach>(pr[u], p);
+        unpack<G, kEach>(gr[u], g);
+        if constexpr (k8) {
+            decode(mc[u], 1.0f / ms[u], m);
+            decode(vc[u], 1.0f / vs[u], v);
+        } else {
+            unpack<NTFP8_F32, kEach>(mr[u], m);
+            unpack<NTFP8_F32, kEach>(vr[u], v);
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            g[e] *= factor;
+            m[e] = s.beta1 * m[e] + s.rest1 * g[e];
+            if constexpr (k8) v[e] *= v[e];
+            v[e] = s.beta2 * v[e] + s.rest2 * (g[e] * g[e]);
+            r[e] = sqrtf(v[e]);
+            p[e] = p[e] * s.keep - s.to * (m[e] / (r[e] * s.root + s.eps));
+        }
+        store_piece<P, kEach>(T.p, i, p, left[u]);
+        if (T.copy) {
+            if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach>(T.copy, i, p, left[u]);
+            else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach>(T.copy, i, p, left[u]);
+            else store_piece<NTFP8_F32, kEach>(T.copy, i, p, left[u]);
+        }
+        if constexpr (k8) {
+            uint32_t mt = 0, rt = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                mt = max(mt, __float_as_uint(m[e]) & 0x7fffffffu);   // (NaN lies above all others)
+                rt = max(rt, __float_as_uint(r[e]) & 0x7fffffffu);
+            }
+            const int mk = scale_exponent(wave_most(mt)), rk = scale_exponent(wave_most(rt));
+            const float mf = __uint_as_float((uint32_t)(mk + 127) << 23), rf = __uint_as_float((uint32_t)(rk + 127) << 23);
+            uint32_t mw = 0, rw = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; e += 2) {
+                const uint32_t d = dither_of((uint32_t)(i >> 1) + e / 2, s.seed);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t d16 = h ? d >> 16 : d & 0xffffu;
+                    const float a = __uint_as_float(__float_as_uint(m[e + h]) & 0x7fffffffu);
+                    mw |= (encode(a, mf, d16) | ((__float_as_uint(m[e + h]) >> 24) & 0x80u)) << (8 * (e + h));
+                    const uint32_t c = encode(r[e + h], rf, d16);
+                    rw |= ((c == 0u && r[e + h] > 0.0f ? 1u : c) | ((__float_as_uint(r[e + h]) >> 24) & 0x80u)) << (8 * (e + h));
+                }
+            }
+            if (left[u] == kEach) {
+                reinterpret_cast<Word*>(static_cast<uint8_t*>(T.m) + i)->w = mw;
+                reinterpret_cast<Word*>(static_cast<uint8_t*>(T.v) + i)->w = rw;
+            } else {
+                for (int e = 0; e < left[u]; ++e) {
+                    static_cast<uint8_t*>(T.m)[i + e] = (uint8_t)(mw >> (8 * e));
+                    static_cast<uint8_t*>(T.v)[i + e] = (uint8_t)(rw >> (8 * e));
+                }
+            }
+            if ((threadIdx.x & 63) == 0 && left[u]) {
+                T.ms[i / kBlock] = mf;
+                T.vs[i / kBlock] = rf;
+            }
+        } else {
+            store_piece<NTFP8_F32, kEach>(T.m, i, m, left[u]);
+            store_piece<NTFP8_F32, kEach>(T.v, i, v, left[u]);
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void adamw_unpack_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scale, int64_t n,
+                                                           float* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        out[i] = __builtin_amdgcn_cvt_f32_fp8((int)codes[i], 0) / scale[i / kBlock];
+}
+
+}  // namespace
+
+int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st) {
+    Step s = {};
+    s.copy_dtype = o.copy_dtype;
+    s.grad_scale = o.grad_scale;
+    s.beta1 = (float)o.beta1, s.rest1 = (float)(1.0 - o.beta1);
+    s.beta2 = (float)o.beta2, s.rest2 = (float)(1.0 - o.beta2);
+    s.keep = (float)(1.0 - o.lr * o.weight_decay);
+    s.to = (float)(o.lr / (1.0 - pow(o.beta1, (double)o.step)));
+    s.root = (float)(1.0 / sqrt(1.0 - pow(o.beta2, (double)o.step)));
+    s.eps = (float)o.eps;
+    s.seed = o.seed * 0xBB67AE85u;
+    auto launch = [&]() {
+        if (s.count == 0) return (int)NTFP8_OK;
+        const unsigned blocks = (unsigned)s.first[s.count];
+        return with_dtype(o.param_dtype, [&](auto p) {
+            constexpr int P = decltype(p)::value;
+            return with_dtype(o.grad_dtype, [&](auto g) {
+                constexpr int G = decltype(g)::value;
+                if (o.bits == 8) adamw_kernel<P, G, true><<<blocks, kThreads, 0, st>>>(s);
+                else adamw_kernel<P, G, false><<<blocks, kThreads, 0, st>>>(s);
+                return launch_status();
+            });
+        });
+    };
+    for (int i = 0; i < count; ++i) {
+        const ntops_adamw_tensor& t = tensors[i];
+        // a tensor of more blocks than a launch should have is split where a block of 8-bit moments ends
+        constexpr int64_t kPart = (int64_t)kChunk << 20;
+        const int ps = size_of(o.param_dtype), gs = size_of(o.grad_dtype), ss = o.bits == 8 ? 1 : 4;
+        for (int64_t at = 0; at < t.n; at += kPart) {
+            const int64_t n = std::min(kPart, t.n - at);
+            const int blocks = (int)((n + kChunk - 1) / kChunk);
+            if (s.count == kMostTensors || (int64_t)s.first[s.count] + blocks > (1 << 30)) {
+                if (const int rc = launch(); rc != NTFP8_OK) return rc;
+                s.count = 0;
+            }
+            s.t[s.count] = Tensor{static_cast<char*>(t.param) + at * ps, static_cast<const char*>(t.grad) + at * gs, static_cast<char*>(t.exp_avg) + at * ss,
+                                  static_cast<char*>(t.exp_avg_sq) + at * ss, t.copy ? static_cast<char*>(t.copy) + at * size_of(o.copy_dtype) : nullptr,
+                                  t.exp_avg_scale ? t.exp_avg_scale + at / kBlock : nullptr, t.exp_avg_sq_scale ? t.exp_avg_sq_scale + at / kBlock : nullptr, n};
+            s.first[s.count + 1] = s.first[s.count] + blocks;
+            ++s.count;
+        }
+    }
+    return launch();
+}
+
+int run_adamw_unpack(const void* codes, const float* scale, int64_t n, float* out, hipStream_t st) {
+    adamw_unpack_kernel<<<(unsigned)std::min<int64_t>((n + 255) / 256, 1 << 16), 256, 0, st>>>(static_cast<const uint8_t*>(codes), scale, n, out);
+    return launch_status();
+}
+
+}  // namespace ntfp8

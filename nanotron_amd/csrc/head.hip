@@ -1,0 +1,368 @@
+// Softmax cross entropy of a projection, without the logits: launches and the small kernels around the matrix products of
+// head_gemm.h.
+//
+// With P = softmax(x W^T) and dl = P - onehot(labels): loss = mean or sum of logsumexp - logit of the label, dx = dl W,
+// dW = dl^T x, three products of 2 tokens hidden vocab operations each.  The first one's epilogue turns a piece of 128 logits into
+// its maximum, its sum and (where gradients are wanted) its exponentials below that maximum, rounded once to fp16, 2 bytes
+// a logit that hold the softmax up to one factor a row and piece.  softmax_rows_kernel knows the whole row and makes dl of
+// them in place, 16 bits again, as the matrix cores take it.  Nothing is computed twice and nothing of 4 bytes a logit exists; what
+// there is of 2 bytes a logit is bounded by taking the tokens in pieces (head_piece).
+#include "head_gemm.h"
+
+namespace ntfp8 {
+namespace {
+
+constexpr int64_t kMostHeld = (int64_t)1 << 31;   // bytes of exponentials at a time
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t held_cols(int64_t vocab) { return up(vocab, kHeadK); }
+
+// One block: how many labels count, 1 / that (or 1) as the factor of loss and gradients.  With `place`, the tokens that count
+// are numbered in their order: place[token] = number or -1, kept[number] = its label, losses of the others 0.
+// No label has been found yet: label_logit = NaN.
+__global__ __launch_bounds__(1024) void head_begin_kernel(const int64_t* __restrict__ labels, int64_t tokens, int64_t ignore, int mean, float lift,
+                                                          float* __restrict__ label_logit, float* __restrict__ factors, int* __restrict__ rows,
+                                                          int* __restrict__ place, int* __restrict__ token_of, int64_t* __restrict__ kept,
+                                                          float* __restrict__ losses) {
+    __shared__ uint32_t part[17];
+    const int64_t each = (tokens + 1023) / 1024, first = threadIdx.x * each, last = std::min(first + each, tokens);
+    uint32_t count = 0;
+    for (int64_t i = first; i < last; ++i) {
+        count += labels[i] != ignore;
+        label_logit[i] = __uint_as_float(kNanBits);
+    }
+    // numbers before this thread's: inside the wave, then over the waves
+    uint32_t before = count;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = (uint32_t)__shfl_up((int)before, d, 64);
+        if ((threadIdx.x & 63) >= d) before += o;
+    }
+    if ((threadIdx.x & 63) == 63) part[1 + (threadIdx.x >> 6)] = before;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        part[0] = 0;
+        for (int w = 1; w <= 16; ++w) part[w] += part[w - 1];
+        const uint32_t n = part[16];
+        const float f = !mean ? 1.0f : n ? 1.0f / (float)n : 0.0f;
+        factors[0] = f;
+        factors[1] = f * lift;   // of the gradients: dl is kept times 1 / lift
+        *rows = (int)n;
+    }
+    __syncthreads();
+    if (!place) return;
+    int at = (int)(part[threadIdx.x >> 6] + before - count);
+    for (int64_t i = first; i < last; ++i) {
+        const int64_t label = labels[i];
+        if (label == ignore) {
+            place[i] = -1;
+            losses[i] = 0.0f;
+        } else {
+            place[i] = at;
+            token_of[at] = (int)i;
+            kept[at] = label;
+            ++at;
+        }
+    }
+}
+
+// A row to a block: its maximum and sum from its pieces, its loss, and dl in the place of its exponentials (rows beyond those
+// that count have neither).
+// dl = e 2^(piece's maximum - logsumexp) and, at the label, softmax - 1 from the fp32 logit.  T = bf16: the one rounding that
+// counts is that of dl to 8 bits of significand, e has 11.  T = fp16: dl is kept times 2^15, as its smallest values
+// would fall below fp16's normal numbers.
+template <int T, bool kGradient>
+__global__ __launch_bounds__(256) void softmax_rows_kernel(const float2* __restrict__ stats, int pieces, const int64_t* __restrict__ labels, int64_t ignore,
+                                                           const float* __restrict__ label_logit, float* __restrict__ losses, const int* __restrict__ rows, int row0,
+                                                           const int* __restrict__ token_of, uint16_t* held, int64_t ldd) {
+    const int64_t row = blockIdx.x;
+    if (kGradient && row0 + row >= *rows) return;   // uniform
+    const int64_t label = labels[row];
+    uint16_t* const d = held + row * ldd;
+    float* const own = losses + (kGradient ? token_of[row] : row);
+    if (!kGradient && label == ignore) {   // uniform
+        if (threadIdx.x == 0) *own = 0.0f;
+        return;
+    }
+    __shared__ float part[4];
+    const float2* const p = stats + row * pieces;
+    float top = -__builtin_inff();
+    for (int i = threadIdx.x; i < pieces; i += 256) top = __builtin_elementwise_maximum(top, p[i].x);
+    auto over_waves = [&](float v, auto f) {
+        v = __uint_as_float(wave_fold(__float_as_uint(v), [&](uint32_t a, uint32_t b) { return __float_as_uint(f(__uint_as_float(a), __uint_as_float(b))); }));
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        return f(f(part[0], part[1]), f(part[2], part[3]));
+    };
+    top = over_waves(top, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
+    float sum = 0.0f;
+    for (int i = threadIdx.x; i < pieces; i += 256) sum += p[i].y * __builtin_amdgcn_exp2f(p[i].x - top);   // (top -inf or inf: NaN, as the softmax is)
+    sum = over_waves(sum, [](float a, float b) { return a + b; });
+    const float log_sum = __builtin_amdgcn_logf(sum);   // (base 2; sum >= 1)
+    // in base 2, from the maximum down: the logit's product is exact inside the fma
+    const float loss = __builtin_fmaf(-label_logit[row], kLog2e, top) + log_sum;
+    if (threadIdx.x == 0) *own = loss * 0.693147180559945309417f;
+    if constexpr (kGradient) {
+        constexpr float kScale = T == NTFP8_BF16 ? 1.0f : 32768.0f;
+        const bool bad = loss != loss;   // no such label, or logits that are not numbers: the row says so
+        const float lse = bad ? loss : top + log_sum;
+        const float at_label = (__builtin_amdgcn_exp2f(-loss) - 1.0f) * kScale;
+        for (int64_t c = threadIdx.x * 8; c < ldd; c += 256 * 8) {
+            const v4i raw = *reinterpret_cast<const v4i*>(d + c);
+            const float f = __builtin_amdgcn_exp2f(p[c / kPieceCols].x - lse) * (kScale * 0x1p-15f);
+            v4i out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float a, b;
+                unpack_pair<NTFP8_F16>((uint32_t)raw[k], a, b);
+                a *= f;
+                b *= f;
+                if (c + 2 * k == label) a = at_label;
+                if (c + 2 * k + 1 == label) b = at_label;
+                out[k] = (int)pack_pair<T>(a, b);
+            }
+            *reinterpret_cast<v4i*>(d + c) = out;
+        }
+    }
+}
+
+// the losses' sum times the factor
+__global__ __launch_bounds__(1024) void head_end_kernel(const float* __restrict__ losses, int64_t tokens, const float* __restrict__ factors, float* __restrict__ loss) {
+    __shared__ float part[16];
+    float s = 0.0f;
+    for (int64_t i = threadIdx.x; i < tokens; i += 1024) s += losses[i];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = 0.0f;
+        for (int w = 0; w < 16; ++w) s += part[w];
+        *loss = factors[0] == 0.0f ? 0.0f : s * factors[0];
+    }
+}
+
+// rows padded with zeros to a multiple of 8 elements, for operands whose rows do not begin on 16-byte boundaries; with `from`
+// the first *rows of them, each from its place
+__global__ __launch_bounds__(256) void take_rows_kernel(const uint16_t* __restrict__ x, int64_t ld, int64_t count, int cols, int padded, const int* __restrict__ rows,
+                                                        const int* __restrict__ from, uint16_t* __restrict__ out) {
+    if (rows) count = *rows;
+    const int chunks = padded / 8;
+    for (int64_t r = blockIdx.x; r < count; r += gridDim.x) {
+        const int64_t src = (from ? from[r] : r) * ld;
+        for (int k = threadIdx.x; k < chunks; k += 256) {
+            const Piece<NTFP8_BF16, 8> v = load_piece<NTFP8_BF16, 8>(x, src + k * 8, cols - k * 8);
+            *reinterpret_cast<v4i*>(out + r * padded + k * 8) = (v4i){(int)v.w[0], (int)v.w[1], (int)v.w[2], (int)v.w[3]};
+        }
+    }
+}
+
+// dx: row place[token] - row0 of what was computed for the tokens that count, zeros for the others (if row0 is 0; the other
+// launches of a call leave rows that are not theirs alone).  Computed is alpha times the sum of `splits` runs of K in fp32, or,
+// splits 0, the row itself.
+template <int D>
+__global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ from, int splits, int64_t split_stride, const float* __restrict__ alpha,
+                                                       const int* __restrict__ place, int64_t tokens, int row0, int count, int cols, void* __restrict__ out) {
+    const float a = splits ? *alpha : 1.0f;
+    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
+        const int at = place[t];
+        const int64_t r = at - row0;
+        if (at < 0 ? row0 != 0 : r < 0 || r >= count) continue;
+        for (int c = threadIdx.x * 8; c < cols; c += 2048) {
+            const int left = cols - c;
+            float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (at >= 0) {
+                if (splits == 0) unpack<D, 8>(load_piece<D, 8>(from, r * cols + c, left), s);
+                for (int k = 0; k < splits; ++k) {
+                    float v[8];
+                    unpack<NTFP8_F32, 8>(load_piece<NTFP8_F32, 8>(from, k * split_stride + r * cols + c, left), v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[e] += v[e];
+                }
+                if (splits) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[e] *= a;
+                }
+            }
+            store_piece<D, 8>(out, t * cols + c, s, left);
+        }
+    }
+}
+
+template <int S, int D>
+__global__ __launch_bounds__(256) void scale_kernel(const void* x, const float* __restrict__ factor, int64_t n, void* out) {
+    const float f = *factor;
+    if (x == out && f == 1.0f) return;
+    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+        const int left = (int)std::min<int64_t>(8, n - i);
+        float v[8];
+        unpack<S, 8>(load_piece<S, 8>(x, i, left), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f;
+        store_piece<D, 8>(out, i, v, left);
+    }
+}
+
+template <int T, bool kAT, bool kBT, int EPI>
+int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
+    g.tiles_m = (int)((g.M + 32 * (int64_t)mi - 1) / (32 * mi));
+    g.tiles_n = (int)(((EPI == kLosses || EPI == kSoftmax ? g.ldd : g.N) + kBigN - 1) / kBigN);
+    g.magic = magic_of((uint32_t)(kGroupM * g.tiles_n));
+    const unsigned blocks = (unsigned)((int64_t)g.tiles_m * g.tiles_n * (EPI == kPartial ? g.splits : 1));
+    if constexpr (kAT) {
+        head_gemm_kernel<T, kAT, kBT, 8, EPI><<<blocks, kBigThreads, 0, st>>>(g);
+    } else {
+        if (mi == 8) head_gemm_kernel<T, kAT, kBT, 8, EPI><<<blocks, kBigThreads, 0, st>>>(g);
+        else if (mi == 4) head_gemm_kernel<T, kAT, kBT, 4, EPI><<<blocks, kBigThreads, 0, st>>>(g);
+        else if (mi == 2) head_gemm_kernel<T, kAT, kBT, 2, EPI><<<blocks, kBigThreads, 0, st>>>(g);
+        else head_gemm_kernel<T, kAT, kBT, 1, EPI><<<blocks, kBigThreads, 0, st>>>(g);
+    }
+    return launch_status();
+}
+
+// rows of a tile / 32: the smallest tile that holds all rows, the largest beyond
+int tile_rows(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
+
+struct Plan {
+    int64_t piece;            // tokens at a time
+    int64_t ldd, pieces;
+    bool pad_x, pad_w;
+    int64_t padded;           // hidden, up to a multiple of 8
+    int splits, kt_split;     // of dx
+    int64_t at_factors, at_label, at_place, at_token, at_kept, at_stats, at_held, at_x, at_w, at_dx, bytes;
+};
+int64_t piece_of(int64_t vocab) { return std::max<int64_t>(256, kMostHeld / (2 * held_cols(vocab)) / 256 * 256); }
+
+Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
+    Plan p = {};
+    const bool gradient = d.dx || d.dweight;
+    p.piece = gradient ? std::min(d.tokens, piece_of(d.vocab)) : d.tokens;
+    p.ldd = held_cols(d.vocab);
+    p.pieces = (p.ldd + kPieceCols - 1) / kPieceCols;
+    p.padded = up(d.hidden, 8);
+    // (with gradients the tokens that count are gathered: those that are ignored cost nothing, and what is in them, NaN say, is
+    // seen by nobody)
+    p.pad_x = gradient || d.hidden % 8 || d.x_stride % 8 || reinterpret_cast<uintptr_t>(d.x) % 16;
+    p.pad_w = d.hidden % 8 || d.weight_stride % 8 || reinterpret_cast<uintptr_t>(d.weight) % 16;
+    p.splits = 1;
+    p.kt_split = 0;
+    if (d.dx) {
+        // few tiles: K, the vocabulary, is cut into runs until there is one workgroup for each CU, of 8 K-tiles or more
+        const int64_t rows = p.piece, mi = tile_rows(rows), tiles = up(rows, 32 * mi) / (32 * mi) * (up(d.hidden, kBigN) / kBigN), kts = p.ldd / kHeadK;
+        const int64_t want = std::max<int64_t>(1, std::min(256 / tiles, kts / 8));
+        p.kt_split = (int)((kts + want - 1) / want);
+        p.splits = (int)((kts + p.kt_split - 1) / p.kt_split);
+    }
+    int64_t at = 0;
+    auto room = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += up(bytes, 256);
+        return here;
+    };
+    p.at_factors = room(256);
+    p.at_label = room(d.tokens * 4);
+    if (gradient) {
+        p.at_place = room(d.tokens * 4);
+        p.at_token = room(d.tokens * 4);
+        p.at_kept = room(d.tokens * 8);
+    }
+    p.at_stats = room(p.piece * p.pieces * 8);
+    p.at_held = gradient ? room(p.piece * p.ldd * 2) : 0;
+    p.at_x = p.pad_x ? room(d.tokens * p.padded * 2) : 0;
+    p.at_w = p.pad_w ? room(d.vocab * p.padded * 2) : 0;
+    p.at_dx = d.dx ? room(p.piece * d.hidden * (p.splits > 1 ? 4 * p.splits : size_of(d.grad_dtype))) : 0;
+    p.bytes = at;
+    return p;
+}
+
+template <int T>
+int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
+    const Plan p = plan_of(d);
+    char* const ws = static_cast<char*>(d.workspace);
+    float* const factors = reinterpret_cast<float*>(ws + p.at_factors);
+    float* const label_logit = reinterpret_cast<float*>(ws + p.at_label);
+    float2* const stats = reinterpret_cast<float2*>(ws + p.at_stats);
+    uint16_t* const held = reinterpret_cast<uint16_t*>(ws + p.at_held);
+    const bool gradient = d.dx || d.dweight;
+    const char* x = static_cast<const char*>(d.x);
+    const char* w = static_cast<const char*>(d.weight);
+    int64_t ldx = d.x_stride, ldw = d.weight_stride;
+    auto status = [](int rc) { return rc != NTFP8_OK; };
+    int* const count = reinterpret_cast<int*>(factors + 2);
+    int* const place = gradient ? reinterpret_cast<int*>(ws + p.at_place) : nullptr;
+    int* const token_of = gradient ? reinterpret_cast<int*>(ws + p.at_token) : nullptr;
+    int64_t* const kept = gradient ? reinterpret_cast<int64_t*>(ws + p.at_kept) : nullptr;
+    const int64_t* const labels = gradient ? kept : d.labels;
+    head_begin_kernel<<<1, 1024, 0, st>>>(d.labels, d.tokens, d.ignore_index, d.mean, T == NTFP8_F16 ? 0x1p-15f : 1.0f, label_logit, factors, count, place, token_of, kept, d.losses);
+    auto take = [&](const char*& from, int64_t& ld, int64_t rows, int64_t at, const int* live, const int* which) {
+        uint16_t* const to = reinterpret_cast<uint16_t*>(ws + at);
+        take_rows_kernel<<<(unsigned)std::min<int64_t>(rows, 8192), 256, 0, st>>>(reinterpret_cast<const uint16_t*>(from), ld, rows, (int)d.hidden, (int)p.padded, live, which, to);
+        from = reinterpret_cast<const char*>(to);
+        ld = p.padded;
+    };
+    if (p.pad_x) take(x, ldx, d.tokens, p.at_x, gradient ? count : nullptr, token_of);
+    if (p.pad_w) take(w, ldw, d.vocab, p.at_w, nullptr, nullptr);
+    if (status(launch_status())) return NTFP8_ERR_LAUNCH;
+    for (int64_t row = 0; row < d.tokens; row += p.piece) {
+        const int64_t rows = std::min(p.piece, d.tokens - row);
+        const int mi = tile_rows(rows);
+        HeadGemm g = {};
+        g.A = x + row * ldx * 2, g.lda = ldx, g.a_cols = (int)p.padded;
+        g.B = w, g.ldb = ldw, g.b_cols = (int)p.padded, g.b_rows = 0;
+        g.M = (int)rows, g.N = (int)d.vocab, g.K = (int)p.padded;
+        g.rows = gradient ? count : nullptr, g.row0 = (int)row;
+        g.D = held, g.ldd = p.ldd, g.stats = stats, g.pieces = (int)p.pieces;
+        g.labels = labels + row, g.label_logit = label_logit + row;
+        if (status(gradient ? launch_gemm<T, false, false, kSoftmax>(g, mi, st) : launch_gemm<T, false, false, kLosses>(g, mi, st))) return NTFP8_ERR_LAUNCH;
+        auto rows_kernel = gradient ? softmax_rows_kernel<T, true> : softmax_rows_kernel<T, false>;
+        rows_kernel<<<(unsigned)rows, 256, 0, st>>>(stats, (int)p.pieces, labels + row, d.ignore_index, label_logit + row, gradient ? d.losses : d.losses + row, count, (int)row,
+                                                    gradient ? token_of + row : nullptr, held, p.ldd);
+        if (status(launch_status())) return NTFP8_ERR_LAUNCH;
+        if (d.dx) {
+            HeadGemm h = {};
+            h.A = held, h.lda = p.ldd, h.a_cols = (int)p.ldd;
+            h.B = w, h.ldb = ldw, h.b_cols = (int)p.padded, h.b_rows = (int)d.vocab;
+            h.M = (int)rows, h.N = (int)d.hidden, h.K = (int)p.ldd;
+            h.rows = count, h.row0 = (int)row;
+            h.D = ws + p.at_dx, h.d_dtype = d.grad_dtype, h.alpha = factors + 1;
+            h.splits = p.splits, h.kt_split = p.kt_split, h.partial = reinterpret_cast<float*>(ws + p.at_dx);
+            if (status(p.splits == 1 ? launch_gemm<T, false, true, kStore>(h, mi, st) : launch_gemm<T, false, true, kPartial>(h, mi, st))) return NTFP8_ERR_LAUNCH;
+            auto put = d.grad_dtype == T ? put_rows_kernel<T> : put_rows_kernel<NTFP8_F32>;
+            put<<<(unsigned)std::min<int64_t>(d.tokens, 8192), 256, 0, st>>>(ws + p.at_dx, p.splits == 1 ? 0 : p.splits, rows * d.hidden, h.alpha, place, d.tokens, (int)row, (int)rows,
+                                                                            (int)d.hidden, d.dx);
+            if (status(launch_status())) return NTFP8_ERR_LAUNCH;
+        }
+        if (d.dweight) {
+            HeadGemm h = {};
+            h.A = held, h.lda = p.ldd, h.a_cols = (int)p.ldd;
+            h.B = x + row * ldx * 2, h.ldb = ldx, h.b_cols = (int)p.padded, h.b_rows = (int)rows;
+            h.M = (int)d.vocab, h.N = (int)d.hidden, h.K = (int)rows;
+            h.rows = count, h.row0 = (int)row;
+            h.D = d.dweight, h.d_dtype = d.grad_dtype, h.accumulate = row > 0, h.alpha = factors + 1;
+            if (status(launch_gemm<T, true, true, kStore>(h, 8, st))) return NTFP8_ERR_LAUNCH;
+        }
+    }
+    if (d.loss) {
+        head_end_kernel<<<1, 1024, 0, st>>>(d.losses, d.tokens, factors, d.loss);
+        return launch_status();
+    }
+    return NTFP8_OK;
+}
+
+}  // namespace
+
+int64_t head_piece(int64_t vocab) { return piece_of(vocab); }
+int64_t head_workspace(const ntops_linear_cross_entropy_desc& d) { return plan_of(d).bytes; }
+int run_head(const ntops_linear_cross_entropy_desc& d, hipStream_t st) { return d.x_dtype == NTFP8_BF16 ? run<NTFP8_BF16>(d, st) : run<NTFP8_F16>(d, st); }
+
+int run_scale(const void* x, int x_dtype, const float* factor, int64_t n, void* out, int out_dtype, hipStream_t st) {
+    const unsigned blocks = (unsigned)std::min<int64_t>((n + 2047) / 2048, 8192);
+    return with_dtype(x_dtype, [&](auto s) {
+        return with_dtype(out_dtype, [&](auto d) {
+            scale_kernel<decltype(s)::value, decltype(d)::value><<<blocks, 256, 0, st>>>(x, factor, n, out);
+            return launch_status();
+        });
+    });
+}
+
+}  // namespace ntfp8

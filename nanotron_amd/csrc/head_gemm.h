@@ -1,0 +1,351 @@
+// Matrix products of 16-bit operands for gfx950, in the forms that a projection with a softmax cross entropy needs:
+//   logits   A [M, K] rows, B [N, K] rows            x . weight^T, with the softmax's maxima and sums in the epilogue
+//   dx       A [M, K] rows, B [K, N] (transposed)    dl . weight
+//   dweight  A [K, M] and B [K, N] (transposed)      dl^T . x
+//
+// Block tile (32 MI) x 256 x 64 (128 bytes of K), four waves in a 2 x 2 arrangement, a wave owning (16 MI) x 128 outputs as MI x 8
+// accumulator blocks of V_MFMA_F32_16X16X32.  Tiles travel from memory straight into LDS, 16 bytes a lane, and lie there as
+// those of the fp8 GEMM do: rows of 128 bytes with their 16-byte chunks swizzled; a transposed operand as 64 rows of k with 512
+// bytes of n (or m) each, its 32-byte pieces swizzled, gathered with the transposing 64-bit LDS read.
+#pragma once
+#include "gemm_common.h"
+#include "gemm_big.h"
+#include "ops_common.h"
+
+namespace ntfp8 {
+
+constexpr int kHeadK = kBK / 2;   // elements of K per LDS stage
+constexpr int kPieceCols = 128;   // columns of logits that share a maximum: those of a wave
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+template <int T>
+__device__ __forceinline__ v4f mfma_16x16x32(v4i b_frag, v4i a_frag, v4f c) {
+    // B first: a lane owns 4 consecutive n (n = 4 (lane / 16) + r) of one output row m = lane % 16
+    if constexpr (T == NTFP8_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, b_frag), __builtin_bit_cast(v8bf, a_frag), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, b_frag), __builtin_bit_cast(v8h, a_frag), c, 0, 0, 0);
+}
+
+enum HeadEpilogue {
+    kStore,     // D = alpha * sums, rounded to d_dtype (fp32: optionally added to D)
+    kPartial,   // the sums of a run of K, fp32, to partial[split][M][N]
+    kLosses,    // per row and 128 columns: the largest logit and the sum of exponentials below it; the labels' logits
+    kSoftmax,   // the same, and the exponentials themselves in fp16
+};
+
+struct HeadGemm {
+    const void* A;
+    const void* B;
+    int64_t lda, ldb;            // elements between rows, a multiple of 8; both operands on 16-byte boundaries
+    int M, N, K;                 // K: a multiple of 8 unless both operands are transposed
+    const int* rows;             // NULL, or how many of the tokens count, known to the device alone, ...
+    int row0;                    // ... of which this launch has those from row0 on: M is at most that many, K where A is transposed
+    int a_cols, b_cols;          // columns of a row that may be read, a multiple of 8
+    int b_rows;                  // rows of a transposed B (K or fewer; those behind count as zeros)
+    int tiles_m, tiles_n;
+    uint32_t magic;              // magic_of(kGroupM tiles_n)
+    int splits, kt_split;        // runs of K, and K-tiles of each
+    void* D;
+    int d_dtype, accumulate;
+    const float* alpha;
+    float* partial;
+    // logits
+    int64_t ldd;                 // elements between rows of the exponentials, N of them or more (a multiple of 8)
+    float2* stats;               // [M][pieces]: base-2 maximum, sum
+    int pieces;
+    const int64_t* labels;
+    float* label_logit;
+};
+
+// LDS stages: what fits beside each other in 160 KB
+template <int MI>
+constexpr int head_stages() { return MI == 8 ? 2 : MI == 1 ? 4 : 3; }
+
+// One operand's loads: `kRows` rows of 128 bytes (or 64 rows of 2 kRows bytes of a transposed one) a K-tile
+template <bool kT, int kRows>
+struct HeadOperand {
+    static constexpr int kLoads = kRows * kBK / 1024 / kBigWaves;   // 1 KB wave-level loads per wave
+    static_assert(!kT || kRows == 256, "a transposed operand is 256 columns wide");
+    const char* base;
+    int64_t step;        // bytes from K-tile to K-tile
+    int64_t row_bytes;
+    int rows, cols;      // that may be read from base on (transposed: of all of K, from the first column of the matrix on)
+    uint32_t off[kLoads];
+
+    __device__ __forceinline__ void init(const void* p, int64_t ld, int first, int count, int readable, int k_rows, int wave, int lane) {
+        row_bytes = ld * 2;
+        cols = readable;
+        if constexpr (kT) {
+            base = static_cast<const char*>(p);
+            step = kHeadK * row_bytes;
+            rows = k_rows;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                // 2 rows of k a wave-level load, 32 chunks of 16 bytes each; 32-byte piece c of row k is stored at piece
+                // c ^ ((k mod 4) | 4 (k / 16 mod 2)): the 4 rows that one transposing read of 16 lanes touches, and the two
+                // groups of 16 lanes that go through LDS together, then use different banks
+                const int k = (wave + kBigWaves * i) * 2 + (lane >> 5);
+                const int piece = ((lane & 31) >> 1) ^ ((k & 3) | (((k >> 4) & 1) << 2));
+                off[i] = (uint32_t)k * (uint32_t)row_bytes + (uint32_t)first * 2u + (uint32_t)(piece * 32 + (lane & 1) * 16);
+            }
+        } else {
+            base = static_cast<const char*>(p) + (int64_t)first * row_bytes;
+            step = kBK;
+            rows = min(count, kRows);
+            const int chunk = ((lane & 7) ^ (lane >> 3) ^ (wave & 1)) << 4;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) off[i] = (uint32_t)((wave + kBigWaves * i) * 8 + (lane >> 3)) * (uint32_t)row_bytes + chunk;
+        }
+    }
+    // the descriptor of a K-tile; one past the last has no bytes
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t at(int ktile, bool live) const {
+        int r = rows;
+        if constexpr (kT) r = max(0, min(rows - ktile * kHeadK, kHeadK));
+        const uint32_t bytes = live && r > 0 ? (uint32_t)(r - 1) * (uint32_t)row_bytes + (uint32_t)cols * 2u : 0u;
+        const char* p = base;
+        if constexpr (kT) p += (int64_t)ktile * step;
+        return make_rsrc(p, (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
+    }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, uint8_t* stage, int l, int ktile, int wave) const {
+        lds_load16(r, (lds_ptr)(uintptr_t)(stage + (wave + kBigWaves * l) * 1024), off[l], kT ? 0 : ktile * kBK);
+    }
+    // lanes whose chunk of the last K-tile lies behind K: nothing is read there, zeros instead
+    __device__ __forceinline__ void poison() {
+        if constexpr (!kT) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) off[i] = kDropped;
+        }
+    }
+};
+
+// Fragment reads.  Plain: block i is 16 rows, 2048 bytes, further on.  Transposed: lane u of a group of 16 (k 16 g .. + 15) addresses
+// row k0 + u / 4, columns 4 (u mod 4) .. + 3 of the block's 32-byte piece, and receives rows k0 .. k0 + 3 of column u.
+template <bool kT>
+struct HeadFragment {
+    int at[2];
+    int turn;
+    __device__ __forceinline__ void init(int first, int lane) {   // first: row (column) of the wave's block 0 within the tile
+        const int g = lane >> 4, u = lane & 15;
+        if constexpr (kT) {
+            at[0] = (16 * g + (u >> 2)) * 512 + (first >> 7) * 256 + (u & 3) * 8;
+            at[1] = at[0];
+            turn = ((u >> 2) | ((g & 1) << 2)) << 5;
+        } else {
+            at[0] = lds_off16(first + u, 2 * g);
+            at[1] = lds_off16(first + u, 2 * g + 1);
+            turn = 0;
+        }
+    }
+    // half h of block i: k 8 h .. + 7 of the lane group's 16
+    __device__ __forceinline__ v4i read(uint8_t* stage, int i, int h) const {
+        if constexpr (kT) {
+            typedef short v4s __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) v4s* tr_ptr;
+            typedef int v2i __attribute__((ext_vector_type(2)));
+            uint8_t* p = stage + at[0] + ((i << 5) ^ turn) + h * (8 * 512);
+            const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)p));
+            const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(p + 4 * 512)));
+            return (v4i){lo.x, lo.y, hi.x, hi.y};
+        } else {
+            return *reinterpret_cast<const v4i*>(stage + at[h] + i * 2048);
+        }
+    }
+};
+
+__device__ __forceinline__ float lanes_over_rows_max(float v) {   // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __builtin_elementwise_maximum(__uint_as_float(r.x), __uint_as_float(r.y));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __builtin_elementwise_maximum(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ __forceinline__ float lanes_over_rows_sum(float v) {
+    typedef unsigned v2u __attribute__((ext_vector_type(2)));
+    v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r.x) + __uint_as_float(r.y);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLift = 15.0f;   // exponentials are kept in fp16 as 2^15 e, 1 at the maximum: 29 binades below it are normal numbers
+
+// Logits of a wave, MI x 8 blocks at rows m_base, columns n_base (a piece of kPieceCols columns).  For each row the largest
+// logit (NaN if one is) and the sum of exponentials below it, both in base 2 and fp32; with kKeep the exponentials as well,
+// once rounded, which the gradient is later made of by one multiplication a row and piece.
+template <int MI, bool kKeep>
+__device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const HeadGemm& G, int M, int m_base, int n_base, int lane) {
+    if (n_base >= (int)G.ldd) return;   // uniform
+    const int mrow = lane & 15, q = lane >> 4;
+    const float none = -__builtin_inff();
+    if (n_base + kPieceCols > G.N) {   // uniform: columns behind the vocabulary count for nothing
+#pragma unroll
+        for (int j = 0; j < kBigNJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool out = n_base + 16 * j + 4 * q + e >= G.N;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) acc[i][j][e] = out ? none : acc[i][j][e];
+            }
+    }
+    uint16_t* const D = static_cast<uint16_t*>(G.D);
+    const int piece = n_base / kPieceCols;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int m = m_base + 16 * i + mrow;
+        float top = acc[i][0][0];
+#pragma unroll
+        for (int j = 0; j < kBigNJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, acc[i][j][e]);
+        top = lanes_over_rows_max(top);
+        // the label's logit, where it is one of these columns
+        int rel = -1;
+        if (m < M) {
+            const int64_t label = G.labels[m];
+            if (label >= 0 && label < G.N) rel = (int)(label - n_base);
+        }
+        if (__any(rel >= 0 && rel < kPieceCols)) {
+#pragma unroll
+            for (int j = 0; j < kBigNJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (rel == 16 * j + 4 * q + e) G.label_logit[m] = acc[i][j][e];
+        }
+        const float base = top == none ? 0.0f : top * kLog2e;
+        const float lift = (kKeep ? kLift : 0.0f) - base;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kBigNJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, lift));
+                acc[i][j][e] = p;
+                sum += p;
+            }
+        sum = lanes_over_rows_sum(sum);
+        if (q == 0 && m < M) G.stats[(int64_t)m * G.pieces + piece] = make_float2(top == none ? none : base, kKeep ? sum * 0x1p-15f : sum);
+        if constexpr (kKeep) {
+#pragma unroll
+            for (int j = 0; j < kBigNJ; j += 2) {
+                // (as 16-bit outputs of the fp8 GEMM: 16 bytes a lane, a full 32-byte sector per row)
+                uint32_t x0 = OutT<NTFP8_F16>::pack2(acc[i][j][0], acc[i][j][1]);
+                uint32_t x1 = OutT<NTFP8_F16>::pack2(acc[i][j][2], acc[i][j][3]);
+                uint32_t y0 = OutT<NTFP8_F16>::pack2(acc[i][j + 1][0], acc[i][j + 1][1]);
+                uint32_t y1 = OutT<NTFP8_F16>::pack2(acc[i][j + 1][2], acc[i][j + 1][3]);
+                swap_rows16(x0, y0);
+                swap_rows16(x1, y1);
+                const int n = n_base + (j + (q & 1)) * 16 + (q >> 1) * 8;
+                if (m < M && n < (int)G.ldd) store16_through(D + (int64_t)m * G.ldd + n, (v4i){(int)x0, (int)x1, (int)y0, (int)y1});
+            }
+        }
+    }
+}
+
+template <int T, bool kAT, bool kBT, int MI, int EPI>
+__global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G) {
+    constexpr int NS = head_stages<MI>();
+    __shared__ __attribute__((aligned(1024))) uint8_t sA[NS][32 * MI * kBK];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB[NS][kBigN * kBK];
+    int M = G.M, K = G.K, b_rows = G.b_rows, tiles_m = G.tiles_m;
+    if (G.rows) {   // uniform
+        const int live = max(0, *G.rows - G.row0);
+        if constexpr (kAT) {
+            K = min(K, live);
+            b_rows = min(b_rows, live);
+            if (G.accumulate && live == 0) return;
+        } else {
+            M = min(M, live);
+            tiles_m = (M + 32 * MI - 1) / (32 * MI);
+        }
+    }
+    // Within each round of 256 workgroups an XCD takes a contiguous run of the tiles
+    int pid = blockIdx.x;
+    const int tiles = tiles_m * G.tiles_n, total = tiles * (EPI == kPartial ? G.splits : 1), round0 = pid & ~255;
+    if (pid >= total) return;
+    pid = round0 + run_of_xcd(pid - round0, min(256, total - round0));
+    const int split = EPI == kPartial ? pid / tiles : 0;
+    int pid_m, pid_n;
+    tile_in_group(EPI == kPartial ? pid - split * tiles : pid, tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
+    const int m0 = pid_m * 32 * MI, n0 = pid_n * kBigN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = (wave >> 1) * (MI * 16), wn = (wave & 1) * 128;
+    const int kt_all = (K + kHeadK - 1) / kHeadK;
+    const int kt0 = EPI == kPartial ? split * G.kt_split : 0;
+    const int kt1 = EPI == kPartial ? min(kt_all, kt0 + G.kt_split) : kt_all;
+
+    HeadOperand<kAT, 32 * MI> a;
+    HeadOperand<kBT, kBigN> b;
+    a.init(G.A, G.lda, m0, M - m0, G.a_cols, K, wave, lane);
+    b.init(G.B, G.ldb, n0, G.N - n0, G.b_cols, b_rows, wave, lane);
+    constexpr int NL = HeadOperand<kAT, 32 * MI>::kLoads + HeadOperand<kBT, kBigN>::kLoads;
+    HeadFragment<kAT> ra;
+    HeadFragment<kBT> rb;
+    ra.init(wm, lane);
+    rb.init(wn, lane);
+    // chunks of the last K-tile behind K read as zeros, not as the start of the next row
+    const bool dead = (kt_all - 1) * kHeadK + (((lane & 7) ^ (lane >> 3) ^ (wave & 1)) << 3) >= K;
+    auto poison = [&]() {
+        if (dead) {
+            a.poison();
+            b.poison();
+        }
+    };
+    auto issue = [&](int kt) {   // one K-tile into its stage; tiles behind the last are empty, so that every tile is NL loads
+        const bool live = kt < kt1;
+        const int s = kt % NS;
+        const __amdgpu_buffer_rsrc_t r0 = a.at(kt, live), r1 = b.at(kt, live);
+#pragma unroll
+        for (int l = 0; l < a.kLoads; ++l) a.load(r0, sA[s], l, kt, wave);
+#pragma unroll
+        for (int l = 0; l < b.kLoads; ++l) b.load(r1, sB[s], l, kt, wave);
+    };
+
+    v4f acc[MI][kBigNJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < kBigNJ; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int l = 0; l < NS - 1; ++l) {
+        if (kt0 + l == kt_all - 1) poison();
+        issue(kt0 + l);
+    }
+    for (int kt = kt0; kt < kt1; ++kt) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * NL) : "memory");   // this tile has landed ...
+        wg_barrier();                                                          // ... for every wave, and all are done with the one before
+        if (kt + NS - 1 == kt_all - 1) poison();
+        issue(kt + NS - 1);
+        const int s = kt % NS;
+        v4i fa[MI][2], fb[2];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            fa[i][0] = ra.read(sA[s], i, 0);
+            fa[i][1] = ra.read(sA[s], i, 1);
+        }
+#pragma unroll
+        for (int j = 0; j < kBigNJ; ++j) {
+            fb[0] = rb.read(sB[s], j, 0);
+            fb[1] = rb.read(sB[s], j, 1);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MI; ++i) acc[i][j] = mfma_16x16x32<T>(fb[h], fa[i][h], acc[i][j]);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the empty tiles too: nothing may land in LDS behind the workgroup)
+
+    if constexpr (EPI == kLosses || EPI == kSoftmax) {
+        softmax_epilogue<MI, EPI == kSoftmax>(acc, G, M, m0 + wm, n0 + wn, lane);
+    } else if constexpr (EPI == kPartial) {
+        store_wave_tile16<NTFP8_F32, false, MI, kBigNJ>(acc, G.partial + (int64_t)split * G.M * G.N, 1.0f, M, G.N, m0 + wm, n0 + wn, lane);
+    } else {
+        const float alpha = *G.alpha;
+        if (G.d_dtype == T) store_wave_tile16<T, false, MI, kBigNJ>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+        else if (G.accumulate) store_wave_tile16<NTFP8_F32, true, MI, kBigNJ>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+        else store_wave_tile16<NTFP8_F32, false, MI, kBigNJ>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+    }
+}
+
+}  // namespace ntfp8

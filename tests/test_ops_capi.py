@@ -1,0 +1,156 @@
+"""CPU-side checks of the operators' C ABI: every declared symbol is exported and bound, struct layouts agree, argument
+errors come back as codes before any launch, and the public functions refuse what they cannot serve."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+from nanotron_amd import _native as nt
+from nanotron_amd import _ops
+from nanotron_amd.nn import LayerNorm, layer_norm, linear_cross_entropy
+from nanotron_amd.optim import AdamW, adamw_step
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "ntops.h")
+P, Q, R = 0x10000, 0x20000000, 0x40000000   # never dereferenced: validation fails first
+NULL, ENUM, SIZE, ALIGN, UNSUPPORTED, ALIAS = -1, -2, -3, -4, -5, -7
+
+
+def source():
+    return re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+
+
+def test_library_exports_every_declared_symbol():
+    names = sorted(set(re.findall(r"\b(ntops_[a-z0-9_]+)\s*\(", source())))
+    assert sorted(_ops.SIGNATURES) == names
+    for n in names:
+        assert hasattr(_ops.lib, n)
+    assert int(re.search(r"#define NTOPS_ADAMW_BLOCK (\d+)", open(HEADER).read()).group(1)) == _ops.ADAMW_BLOCK
+
+
+@pytest.mark.parametrize("name,struct", [("ntops_adamw_tensor", _ops.AdamWTensor), ("ntops_adamw_options", _ops.AdamWOptions),
+                                         ("ntops_linear_cross_entropy_desc", _ops.LinearCrossEntropyDesc)])
+def test_struct_fields_match_header(name, struct):
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), source(), flags=re.S).group(1)
+    fields = []
+    for line in body.split(";"):
+        if line.strip():
+            fields += [re.split(r"[\s*]+", part.strip())[-1] for part in line.split(",")]
+    assert fields == [f[0] for f in struct._fields_]
+
+
+def test_layer_norm_argument_errors():
+    f, b = _ops.lib.ntops_layer_norm_forward, _ops.lib.ntops_layer_norm_backward
+    assert f(None, 2, 4, 8, 8, P, P, 0, 1e-5, Q, None, None, None) == NULL
+    assert f(P, 2, 4, 8, 8, P, P, 0, 1e-5, None, None, None, None) == NULL
+    assert f(P, 2, 4, 8, 8, P, P, 0, 1e-5, Q, R, None, None) == NULL
+    assert f(P, 7, 4, 8, 8, P, P, 0, 1e-5, Q, None, None, None) == ENUM
+    assert f(P, 2, 4, 8, 8, P, P, 1, 1e-5, Q, None, None, None) == ENUM      # fp16 weights beside bf16 rows
+    assert f(P, 2, 0, 8, 8, P, P, 0, 1e-5, Q, None, None, None) == SIZE
+    assert f(P, 2, 4, 8, 7, P, P, 0, 1e-5, Q, None, None, None) == SIZE
+    assert f(P, 2, 4, 32769, 32769, P, P, 0, 1e-5, Q, None, None, None) == UNSUPPORTED
+    assert f(P, 0, 4, 16385, 16385, P, P, 0, 1e-5, Q, None, None, None) == UNSUPPORTED
+    assert f(P + 1, 2, 4, 8, 8, P, P, 0, 1e-5, Q, None, None, None) == ALIGN
+    assert f(P, 2, 4, 8, 8, P + 2, P, 0, 1e-5, Q, None, None, None) == ALIGN
+    assert f(P, 2, 4, 8, 8, Q, Q, 0, 1e-5, P + 16, None, None, None) == ALIAS
+    assert b(None, 8, P, 2, 4, 8, 8, P, 0, P, P, Q, Q, Q, R, None) == NULL
+    assert b(P, 8, P, 2, 4, 8, 8, P, 0, P, P, None, None, None, R, None) == NULL
+    assert b(P, 8, P, 2, 4, 8, 8, P, 0, P, P, Q, Q, Q, None, None) == NULL
+    assert b(P, 4, P, 2, 4, 8, 8, P, 0, P, P, Q, Q, Q, R, None) == SIZE
+    assert b(P, 8, P, 2, 4, 8, 8, P, 0, P, P, Q, Q, Q, R + 4, None) == ALIGN
+    assert b(P, 8, Q, 2, 4, 8, 8, Q, 0, Q, Q, P, None, None, None, None) == ALIAS
+    assert _ops.lib.ntops_layer_norm_scratch(2, 0, 8) == 0
+    assert _ops.lib.ntops_layer_norm_scratch(2, 1, 8) == 64
+
+
+def options(**kw):
+    o = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, weight_decay=0.1, step=1, param_dtype=0, grad_dtype=0, copy_dtype=0, bits=32, seed=0, grad_scale=None)
+    return _ops.AdamWOptions(**{**o, **kw})
+
+
+def tensors(**kw):
+    t = dict(param=P, grad=Q, exp_avg=R, exp_avg_sq=R + 4096, copy=None, exp_avg_scale=None, exp_avg_sq_scale=None, n=16)
+    return (_ops.AdamWTensor * 1)(_ops.AdamWTensor(**{**t, **kw}))
+
+
+def test_adamw_argument_errors():
+    f = _ops.lib.ntops_adamw
+    assert f(tensors(), 1, None, None) == NULL
+    assert f(None, 1, options(), None) == NULL
+    for k in ("param", "grad", "exp_avg", "exp_avg_sq"):
+        assert f(tensors(**{k: None}), 1, options(), None) == NULL
+        assert f(tensors(**{k: P + 0x800001}), 1, options(), None) == ALIGN
+    assert f(tensors(), 1, options(bits=8), None) == NULL          # no scales
+    assert f(tensors(), 1, options(bits=16), None) == ENUM
+    assert f(tensors(), 1, options(grad_dtype=5), None) == ENUM
+    assert f(tensors(copy=P + 0x100000), 1, options(copy_dtype=-1), None) == ENUM
+    assert f(tensors(), 1, options(step=0), None) == SIZE
+    assert f(tensors(n=-1), 1, options(), None) == SIZE
+    assert f(tensors(), 1, options(beta2=1.0), None) == UNSUPPORTED
+    assert f(tensors(), 1, options(eps=float("nan")), None) == UNSUPPORTED
+    assert f(tensors(grad=P), 1, options(), None) == ALIAS
+    assert f(tensors(copy=R), 1, options(), None) == ALIAS
+    assert f(tensors(n=0, param=None), 1, options(), None) == 0    # nothing to do, nothing launched
+    assert f(None, 0, options(), None) == 0
+    g = _ops.lib.ntops_adamw_unpack
+    assert g(None, P, 4, Q, None) == NULL and g(P, P, 0, Q, None) == SIZE and g(P, R, 64, P + 16, None) == ALIAS
+
+
+def desc(**kw):
+    d = dict(x=P, weight=0x1000000, labels=0x2000000, tokens=16, hidden=64, vocab=1000, x_stride=64, weight_stride=64, ignore_index=-100,
+             x_dtype=nt.BF16, mean=1, grad_dtype=nt.BF16, losses=0x3000000, loss=0x3100000, dx=0x4000000, dweight=0x5000000, workspace=0x10000000)
+    return _ops.LinearCrossEntropyDesc(**{**d, **kw})
+
+
+def test_linear_cross_entropy_argument_errors():
+    f = _ops.lib.ntops_linear_cross_entropy
+    assert f(None, None) == NULL
+    for k in ("x", "weight", "labels", "losses", "workspace"):
+        assert f(desc(**{k: None}), None) == NULL
+    assert f(desc(x_dtype=nt.F32), None) == ENUM
+    assert f(desc(grad_dtype=nt.F16), None) == ENUM
+    for k in ("tokens", "hidden", "vocab"):
+        assert f(desc(**{k: 0}), None) == SIZE
+    assert f(desc(x_stride=63), None) == SIZE and f(desc(vocab=1 << 23), None) == SIZE
+    piece = _ops.lib.ntops_linear_cross_entropy_piece(128000)
+    assert piece == 8192
+    assert f(desc(vocab=128000, tokens=piece + 1), None) == UNSUPPORTED
+    assert f(desc(x=P + 1), None) == ALIGN and f(desc(workspace=0x10000010), None) == ALIGN and f(desc(dx=0x4000004), None) == ALIGN
+    assert f(desc(dx=P), None) == ALIAS and f(desc(loss=0x3000000), None) == ALIAS and f(desc(workspace=0x5000000), None) == ALIAS
+    size = _ops.lib.ntops_linear_cross_entropy_workspace
+    assert size(desc(tokens=0)) == 0
+    # two bytes a logit, bounded
+    assert size(desc(tokens=64, vocab=128000)) < 2 * 64 * 128000 * 1.3
+    assert size(desc(tokens=1 << 16, vocab=128000, grad_dtype=nt.F32)) < (1 << 31) * 1.2
+
+
+def test_scale_argument_errors():
+    f = _ops.lib.ntops_scale
+    assert f(None, 0, P, 4, Q, 0, None) == NULL and f(P, 3, P, 4, Q, 0, None) == ENUM and f(P, 0, P, 0, Q, 0, None) == SIZE
+    assert f(P, 0, R, 4, P, 2, None) == ALIAS and f(P + 2, 0, R, 4, Q, 0, None) == ALIGN
+
+
+def test_public_functions_refuse_host_tensors():
+    x = torch.ones(3, 8)
+    with pytest.raises(ValueError, match="CUDA"):
+        layer_norm(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        linear_cross_entropy(x, x, torch.zeros(3, dtype=torch.int64))
+    with pytest.raises(ValueError, match="CUDA"):
+        adamw_step([x], [x], [x], [x], lr=1e-3, step=1)
+    adamw_step([], [], [], [], lr=1e-3, step=1)
+
+
+def test_constructors_refuse():
+    with pytest.raises(ValueError, match="last dimension"):
+        LayerNorm((4, 8))
+    with pytest.raises(ValueError, match="last dimension"):
+        LayerNorm(8)(torch.ones(3, 7))
+    p = torch.nn.Parameter(torch.ones(4))
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8)):
+        with pytest.raises(ValueError):
+            AdamW([p], **kw)
+    with pytest.raises(ValueError, match="copies"):
+        AdamW([dict(params=[p], copies=[None, None])])
+    assert ctypes.sizeof(_ops.AdamWTensor) == 64
