@@ -143,9 +143,12 @@ struct HeadFragment {
             typedef short v4s __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) v4s* tr_ptr;
             typedef int v2i __attribute__((ext_vector_type(2)));
-            uint8_t* p = stage + at[0] + ((i << 5) ^ turn) + h * (8 * 512);
-            const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)p));
-            const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(p + 4 * 512)));
+            // (one index each: the compiler follows a pointer back to its array over few steps only, and where it does not, it
+            // waits for every direct-to-LDS load in flight before the read)
+            int off = at[0] + ((i << 5) ^ turn);
+            asm("" : "+v"(off));
+            const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[off + h * (8 * 512)]));
+            const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[off + h * (8 * 512) + 4 * 512]));
             return (v4i){lo.x, lo.y, hi.x, hi.y};
         } else {
             return *reinterpret_cast<const v4i*>(stage + at[h] + i * 2048);
@@ -307,31 +310,106 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < kBigNJ; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    if constexpr (MI == 8) {
+        // Whole tiles: the schedule of the fp8 GEMM's (gemm_big.h), a slot being two MFMAs of 16 cycles where it has one of
+        // 32, ordered so that no MFMA waits for the accumulator of the one before it.  front(f), groups 0-5 of K-tile f: the B
+        // fragments 2-7 are read behind every other one of the first 24 slots, a barrier releases the stage, and the loads of tile
+        // f + 2 go into it, behind every third slot up to the end of back(f); a second barrier publishes tile f + 1.  back(f): groups 6
+        // and 7, interleaved per A fragment, which is dead after them and refilled from tile f + 1.
+        constexpr int kRelease = 25, kEvery = 3, kFront = (MI * 6 - 1 - kRelease) / kEvery;
+        const int n = kt1 - kt0;
+        v4i fa[MI][2], fw[kBigNJ][2];
+        __amdgpu_buffer_rsrc_t r0, r1;
+        auto load = [&](int f, int l) {
+            if (l < a.kLoads) a.load(r0, sA[f & 1], l, kt0 + f, wave);
+            else b.load(r1, sB[f & 1], l - a.kLoads, kt0 + f, wave);
+        };
+        auto ready = [&](int f) {   // for the loads of tile f
+            if (kt0 + f == kt_all - 1) poison();
+            r0 = a.at(kt0 + f, f < n);
+            r1 = b.at(kt0 + f, f < n);
+        };
 #pragma unroll
-    for (int l = 0; l < NS - 1; ++l) {
-        if (kt0 + l == kt_all - 1) poison();
-        issue(kt0 + l);
-    }
-    for (int kt = kt0; kt < kt1; ++kt) {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * NL) : "memory");   // this tile has landed ...
-        wg_barrier();                                                          // ... for every wave, and all are done with the one before
-        if (kt + NS - 1 == kt_all - 1) poison();
-        issue(kt + NS - 1);
-        const int s = kt % NS;
-        v4i fa[MI][2], fb[2];
+        for (int f = 0; f < 2; ++f) {
+            ready(f);
+#pragma unroll
+            for (int l = 0; l < NL; ++l) load(f, l);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+        wg_barrier();
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            fa[i][0] = ra.read(sA[s], i, 0);
-            fa[i][1] = ra.read(sA[s], i, 1);
+            fa[i][0] = ra.read(sA[0], i, 0);
+            fa[i][1] = ra.read(sA[0], i, 1);
         }
 #pragma unroll
-        for (int j = 0; j < kBigNJ; ++j) {
-            fb[0] = rb.read(sB[s], j, 0);
-            fb[1] = rb.read(sB[s], j, 1);
+        for (int h = 0; h < 4; ++h) fw[h >> 1][h & 1] = rb.read(sB[0], h >> 1, h & 1);
+        for (int f = 0; f < n; ++f) {
+            const int s = f & 1;
+            ready(f + 2);
+            sched_fence();
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int x = 0; x < MI * 6; ++x) {
+                const int j = x / MI, h = x % MI / (MI / 2), i = x % (MI / 2) * 2;
+                acc[i][j] = mfma_16x16x32<T>(fw[j][h], fa[i][h], acc[i][j]);
+                acc[i + 1][j] = mfma_16x16x32<T>(fw[j][h], fa[i + 1][h], acc[i + 1][j]);
+                if (x < 24 && x % 2 == 0) fw[2 + x / 4][x / 2 % 2] = rb.read(sB[s], 2 + x / 4, x / 2 % 2);
+                if (x == kRelease) {
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // every fragment of tile f is in registers
+                    wg_barrier();
+                }
+                if (x > kRelease && (x - kRelease) % kEvery == 0) load(f + 2, (x - kRelease) / kEvery - 1);
+                sched_fence();
+            }
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kFront) : "memory");   // all but tile f + 2's
+            wg_barrier();
 #pragma unroll
-                for (int i = 0; i < MI; ++i) acc[i][j] = mfma_16x16x32<T>(fb[h], fa[i][h], acc[i][j]);
+            for (int i = 0; i < MI; ++i) {
+                acc[i][6] = mfma_16x16x32<T>(fw[6][0], fa[i][0], acc[i][6]);
+                acc[i][7] = mfma_16x16x32<T>(fw[7][0], fa[i][0], acc[i][7]);
+                if (i > 0) {
+                    fa[i - 1][0] = ra.read(sA[s ^ 1], i - 1, 0);
+                    fa[i - 1][1] = ra.read(sA[s ^ 1], i - 1, 1);
+                }
+                sched_fence();
+                acc[i][6] = mfma_16x16x32<T>(fw[6][1], fa[i][1], acc[i][6]);
+                acc[i][7] = mfma_16x16x32<T>(fw[7][1], fa[i][1], acc[i][7]);
+                if (i < 4) fw[i >> 1][i & 1] = rb.read(sB[s ^ 1], i >> 1, i & 1);
+#pragma unroll
+                for (int l = kFront + i * (NL - kFront) / MI; l < kFront + (i + 1) * (NL - kFront) / MI; ++l) load(f + 2, l);
+                sched_fence();
+            }
+            fa[MI - 1][0] = ra.read(sA[s ^ 1], MI - 1, 0);
+            fa[MI - 1][1] = ra.read(sA[s ^ 1], MI - 1, 1);
+            sched_fence();
+        }
+    } else {
+#pragma unroll
+        for (int l = 0; l < NS - 1; ++l) {
+            if (kt0 + l == kt_all - 1) poison();
+            issue(kt0 + l);
+        }
+        for (int kt = kt0; kt < kt1; ++kt) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 2) * NL) : "memory");   // this tile has landed ...
+            wg_barrier();                                                          // ... for every wave, and all are done with the one before
+            if (kt + NS - 1 == kt_all - 1) poison();
+            issue(kt + NS - 1);
+            const int s = kt % NS;
+            v4i fa[MI][2], fb[2];
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                fa[i][0] = ra.read(sA[s], i, 0);
+                fa[i][1] = ra.read(sA[s], i, 1);
+            }
+#pragma unroll
+            for (int j = 0; j < kBigNJ; ++j) {
+                fb[0] = rb.read(sB[s], j, 0);
+                fb[1] = rb.read(sB[s], j, 1);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) acc[i][j] = mfma_16x16x32<T>(fb[h], fa[i][h], acc[i][j]);
+            }
         }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the empty tiles too: nothing may land in LDS behind the workgroup)
