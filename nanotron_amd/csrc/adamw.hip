@@ -1,8 +1,8 @@
 // AdamW over many tensors, moments in fp32 or in 8 bits.
 //
 // Bound by memory: an fp32 parameter with a 16-bit gradient moves 26 bytes with fp32 moments, 14 with 8-bit ones.  One launch
-// takes up to kMostTensors tensors, their pointers and sizes with the launch's arguments, so that nothing has to be copied to
-// the device first; a block takes kChunk elements of one tensor.
+// takes as many tensors as its arguments hold (84 with fp32 moments), their pointers and sizes among them, so that nothing has
+// to be copied to the device first; a workgroup takes a run of elements of one tensor.
 //
 // 8-bit moments.  The first moment m and the root r of the second are kept as E4M3 codes, blocks of 256 elements with a
 // power-of-two scale each, found from the new values: a wave holds a block, four elements a lane, so that the block's
@@ -17,32 +17,36 @@
 namespace ntfp8 {
 namespace {
 
-constexpr int kMostTensors = 40;
 constexpr int kThreads = 256, kEach = 4;
-constexpr int kTurns = 4;                              // pieces of kEach elements a thread, all requested before the first is used
-constexpr int kChunk = kThreads * kEach * kTurns;
 constexpr int kBlock = NTOPS_ADAMW_BLOCK;
 static_assert(kBlock == 64 * kEach, "a wave holds a block of 8-bit moments");
+constexpr int chunk_of(int turns) { return kThreads * kEach * turns; }   // elements a workgroup takes
 
-struct Tensor {
+// what a launch knows of a tensor: as little as its kind needs, the arguments of a launch being 4 KB
+struct Moments {
     void* p;
     const void* g;
     void* m;
     void* v;
-    void* copy;
-    float* ms;
-    float* vs;
     int64_t n;
 };
+struct Scales {
+    float* m;
+    float* v;
+};
+template <bool k8, bool kCopy>
 struct Step {
-    Tensor t[kMostTensors];
-    int first[kMostTensors + 1];   // first block of the launch for each tensor
-    int count;
-    int copy_dtype;                // -1: none
+    static constexpr int kMost = (3968 - 64) / (int)(sizeof(Moments) + 4 + (k8 ? sizeof(Scales) : 0) + (kCopy ? sizeof(void*) : 0));
+    Moments t[kMost];
+    int first[kMost];              // first workgroup of the launch for each tensor; 2^31 - 1 behind the last
+    Scales scales[k8 ? kMost : 1];
+    void* copy[kCopy ? kMost : 1];
     const float* grad_scale;
     float beta1, rest1, beta2, rest2, keep, to, root, eps;
     uint32_t seed;
+    int copy_dtype;
 };
+static_assert(sizeof(Step<false, false>) <= 4096 && sizeof(Step<true, true>) <= 4096 && Step<false, false>::kMost <= 128, "");
 
 // 16 bits for each of the two elements of a pair, the even one's in the low half
 __device__ __forceinline__ uint32_t dither_of(uint32_t pair, uint32_t seed) {
@@ -75,13 +79,20 @@ __device__ __forceinline__ void decode(uint32_t w, float inverse, float (&v)[N])
     v[0] = lo.x * inverse, v[1] = lo.y * inverse, v[2] = hi.x * inverse, v[3] = hi.y * inverse;
 }
 
-template <int P, int G, bool k8>
-__global__ __launch_bounds__(kThreads) void adamw_kernel(const Step s) {
-    int which = 0;
-    for (int half = 32; half >= 1; half /= 2)   // the last tensor whose first block is not behind this one
-        if (which + half < s.count && s.first[which + half] <= (int)blockIdx.x) which += half;
-    const Tensor& T = s.t[which];
-    const int64_t n = T.n, at = (int64_t)((int)blockIdx.x - s.first[which]) * kChunk + threadIdx.x * kEach;
+// kTurns pieces of 4 elements a thread, all requested before the first is used
+template <int P, int G, bool k8, bool kCopy, int kTurns>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s) {
+    // The last tensor whose first workgroup is not behind this one: every lane compares one, so that the arguments are read
+    // in one trip (looked up by halves they are seven dependent ones, 3 us in front of a workgroup's first load)
+    const int lane = threadIdx.x & 63;
+    int which = __popcll(__ballot(lane < s.kMost && s.first[lane] <= (int)blockIdx.x));
+    if constexpr (s.kMost > 64) which += __popcll(__ballot(lane + 64 < s.kMost && s.first[min(lane + 64, s.kMost - 1)] <= (int)blockIdx.x));
+    which = __builtin_amdgcn_readfirstlane(which - 1);
+    const Moments T = s.t[which];
+    const int64_t n = T.n, at = (int64_t)((int)blockIdx.x - s.first[which]) * chunk_of(kTurns) + threadIdx.x * kEach;
+    float* const scale_m = k8 ? s.scales[k8 ? which : 0].m : nullptr;
+    float* const scale_v = k8 ? s.scales[k8 ? which : 0].v : nullptr;
+    void* const copy = kCopy ? s.copy[kCopy ? which : 0] : nullptr;
     Piece<P, kEach> pr[kTurns];
     Piece<G, kEach> gr[kTurns];
     Piece<NTFP8_F32, kEach> mr[kTurns], vr[kTurns];
@@ -107,8 +118,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step s) {
                 }
             }
             if (left[u]) {
-                ms[u] = T.ms[i / kBlock];
-                vs[u] = T.vs[i / kBlock];
+                ms[u] = scale_m[i / kBlock];
+                vs[u] = scale_v[i / kBlock];
             }
         } else {
             mr[u] = load_piece<NTFP8_F32, kEach>(T.m, i, left[u]);
@@ -139,10 +150,10 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step s) {
             p[e] = p[e] * s.keep - s.to * (m[e] / (r[e] * s.root + s.eps));
         }
         store_piece<P, kEach>(T.p, i, p, left[u]);
-        if (T.copy) {
-            if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach>(T.copy, i, p, left[u]);
-            else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach>(T.copy, i, p, left[u]);
-            else store_piece<NTFP8_F32, kEach>(T.copy, i, p, left[u]);
+        if (kCopy && copy) {
+            if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach>(copy, i, p, left[u]);
+            else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach>(copy, i, p, left[u]);
+            else store_piece<NTFP8_F32, kEach>(copy, i, p, left[u]);
         }
         if constexpr (k8) {
             uint32_t mt = 0, rt = 0;
@@ -176,8 +187,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step s) {
                 }
             }
             if ((threadIdx.x & 63) == 0 && left[u]) {
-                T.ms[i / kBlock] = mf;
-                T.vs[i / kBlock] = rf;
+                scale_m[i / kBlock] = mf;
+                scale_v[i / kBlock] = rf;
             }
         } else {
             store_piece<NTFP8_F32, kEach>(T.m, i, m, left[u]);
@@ -194,8 +205,12 @@ __global__ __launch_bounds__(256) void adamw_unpack_kernel(const uint8_t* __rest
 
 }  // namespace
 
-int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st) {
-    Step s = {};
+namespace {
+
+template <int P, int G, bool k8, bool kCopy>
+int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st) {
+    using S = Step<k8, kCopy>;
+    S s = {};
     s.copy_dtype = o.copy_dtype;
     s.grad_scale = o.grad_scale;
     s.beta1 = (float)o.beta1, s.rest1 = (float)(1.0 - o.beta1);
@@ -205,39 +220,54 @@ int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_op
     s.root = (float)(1.0 / sqrt(1.0 - pow(o.beta2, (double)o.step)));
     s.eps = (float)o.eps;
     s.seed = o.seed * 0xBB67AE85u;
+    // Few elements in all: a piece a thread, for as many workgroups as there can be; else four, for loads enough in flight.
+    int64_t all = 0;
+    for (int i = 0; i < count; ++i) all += tensors[i].n;
+    const bool few = all < (int64_t)cu_count() * chunk_of(4) * 4;
+    const int chunk = chunk_of(few ? 1 : 4);
+    const int64_t part = (int64_t)chunk << 20;   // a tensor of more workgroups than a launch should have is split
+    int used = 0, blocks = 0;
     auto launch = [&]() {
-        if (s.count == 0) return (int)NTFP8_OK;
-        const unsigned blocks = (unsigned)s.first[s.count];
-        return with_dtype(o.param_dtype, [&](auto p) {
-            constexpr int P = decltype(p)::value;
-            return with_dtype(o.grad_dtype, [&](auto g) {
-                constexpr int G = decltype(g)::value;
-                if (o.bits == 8) adamw_kernel<P, G, true><<<blocks, kThreads, 0, st>>>(s);
-                else adamw_kernel<P, G, false><<<blocks, kThreads, 0, st>>>(s);
-                return launch_status();
-            });
-        });
+        if (used == 0) return (int)NTFP8_OK;
+        for (int i = used; i < S::kMost; ++i) s.first[i] = 0x7fffffff;
+        if (few) adamw_kernel<P, G, k8, kCopy, 1><<<(unsigned)blocks, kThreads, 0, st>>>(s);
+        else adamw_kernel<P, G, k8, kCopy, 4><<<(unsigned)blocks, kThreads, 0, st>>>(s);
+        used = blocks = 0;
+        return launch_status();
     };
+    constexpr int kState = k8 ? 1 : 4;
     for (int i = 0; i < count; ++i) {
         const ntops_adamw_tensor& t = tensors[i];
-        // a tensor of more blocks than a launch should have is split where a block of 8-bit moments ends
-        constexpr int64_t kPart = (int64_t)kChunk << 20;
-        const int ps = size_of(o.param_dtype), gs = size_of(o.grad_dtype), ss = o.bits == 8 ? 1 : 4;
-        for (int64_t at = 0; at < t.n; at += kPart) {
-            const int64_t n = std::min(kPart, t.n - at);
-            const int blocks = (int)((n + kChunk - 1) / kChunk);
-            if (s.count == kMostTensors || (int64_t)s.first[s.count] + blocks > (1 << 30)) {
+        for (int64_t at = 0; at < t.n; at += part) {
+            const int64_t n = std::min(part, t.n - at);
+            const int more = (int)((n + chunk - 1) / chunk);
+            if (used == S::kMost || blocks + more > (1 << 30))
                 if (const int rc = launch(); rc != NTFP8_OK) return rc;
-                s.count = 0;
-            }
-            s.t[s.count] = Tensor{static_cast<char*>(t.param) + at * ps, static_cast<const char*>(t.grad) + at * gs, static_cast<char*>(t.exp_avg) + at * ss,
-                                  static_cast<char*>(t.exp_avg_sq) + at * ss, t.copy ? static_cast<char*>(t.copy) + at * size_of(o.copy_dtype) : nullptr,
-                                  t.exp_avg_scale ? t.exp_avg_scale + at / kBlock : nullptr, t.exp_avg_sq_scale ? t.exp_avg_sq_scale + at / kBlock : nullptr, n};
-            s.first[s.count + 1] = s.first[s.count] + blocks;
-            ++s.count;
+            s.t[used] = Moments{static_cast<char*>(t.param) + at * size_of(P), static_cast<const char*>(t.grad) + at * size_of(G),
+                                static_cast<char*>(t.exp_avg) + at * kState, static_cast<char*>(t.exp_avg_sq) + at * kState, n};
+            s.first[used] = blocks;
+            if constexpr (k8) s.scales[used] = Scales{t.exp_avg_scale + at / kBlock, t.exp_avg_sq_scale + at / kBlock};
+            if constexpr (kCopy) s.copy[used] = t.copy ? static_cast<char*>(t.copy) + at * size_of(o.copy_dtype) : nullptr;
+            blocks += more;
+            ++used;
         }
     }
     return launch();
+}
+
+}  // namespace
+
+int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st) {
+    bool copies = false;
+    for (int i = 0; i < count; ++i) copies = copies || tensors[i].copy;
+    return with_dtype(o.param_dtype, [&](auto p) {
+        constexpr int P = decltype(p)::value;
+        return with_dtype(o.grad_dtype, [&](auto g) {
+            constexpr int G = decltype(g)::value;
+            if (o.bits == 8) return copies ? run<P, G, true, true>(tensors, count, o, st) : run<P, G, true, false>(tensors, count, o, st);
+            return copies ? run<P, G, false, true>(tensors, count, o, st) : run<P, G, false, false>(tensors, count, o, st);
+        });
+    });
 }
 
 int run_adamw_unpack(const void* codes, const float* scale, int64_t n, float* out, hipStream_t st) {

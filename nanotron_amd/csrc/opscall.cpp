@@ -6,8 +6,11 @@
 
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/ntops.h"
+
+namespace py = pybind11;
 
 namespace {
 
@@ -234,14 +237,34 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& labe
 }
 
 // ---------------------------------------------------------------------------------------------- AdamW
-using List = std::vector<Tensor>;
-using MaybeList = std::optional<std::vector<Tensor>>;
+// A list or tuple of tensors as the objects that it holds: hundreds of them come in every step, and as a vector of tensors each
+// would cost a reference more
+struct List {
+    py::object own;
+    PyObject** items = nullptr;
+    size_t n = 0;
+    explicit List(const py::object& o, const char* name) {
+        if (o.is_none()) return;
+        own = py::reinterpret_steal<py::object>(PySequence_Fast(o.ptr(), "a list of tensors is expected"));
+        if (!own) throw py::error_already_set();
+        items = PySequence_Fast_ITEMS(own.ptr());
+        n = (size_t)PySequence_Fast_GET_SIZE(own.ptr());
+        for (size_t i = 0; i < n; ++i) TORCH_CHECK_TYPE(items[i] == Py_None || THPVariable_Check(items[i]), name, " must be a list of tensors");
+    }
+    bool given() const { return items != nullptr || own; }
+    bool none(size_t i) const { return items[i] == Py_None; }
+    const Tensor& operator[](size_t i) const {
+        TORCH_CHECK_TYPE(items[i] != Py_None, "a tensor is expected, got None");
+        return THPVariable_Unpack(items[i]);
+    }
+};
 
-void adamw(const List& params, const List& grads, const List& m, const List& v, const MaybeList& ms, const MaybeList& vs, const MaybeList& copies, double lr, double beta1,
-           double beta2, double eps, double weight_decay, int64_t step, int64_t seed, const std::optional<Tensor>& grad_scale) {
-    const size_t n = params.size();
-    const bool small = ms.has_value();
-    TORCH_CHECK_VALUE(grads.size() == n && m.size() == n && v.size() == n && (!small || (ms->size() == n && vs->size() == n)) && (!copies || copies->size() == n),
+void adamw(const py::object& params_, const py::object& grads_, const py::object& m_, const py::object& v_, const py::object& ms_, const py::object& vs_,
+           const py::object& copies_, double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step, int64_t seed, const std::optional<Tensor>& grad_scale) {
+    const List params(params_, "params"), grads(grads_, "grads"), m(m_, "first moments"), v(v_, "second moments"), ms(ms_, "scales"), vs(vs_, "scales"), copies(copies_, "copies");
+    const size_t n = params.n;
+    const bool small = ms.given();
+    TORCH_CHECK_VALUE(grads.n == n && m.n == n && v.n == n && (!small || (ms.n == n && vs.n == n)) && (!copies.given() || copies.n == n),
                       "the lists of an AdamW step must have one length (", n, " parameters)");
     TORCH_CHECK_VALUE(step >= 1, "step counts from 1, got ", step);
     TORCH_CHECK_VALUE(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "betas must lie in [0, 1), got ", beta1, " and ", beta2);
@@ -249,7 +272,8 @@ void adamw(const List& params, const List& grads, const List& m, const List& v, 
     if (n == 0) return;
     const Tensor& p0 = params[0];
     on_gpu(p0, "a parameter");
-    Guard guard(p0.device());
+    const c10::Device device = p0.device();
+    Guard guard(device);
     ntops_adamw_options o = {};
     o.lr = lr, o.beta1 = beta1, o.beta2 = beta2, o.eps = eps, o.weight_decay = weight_decay, o.step = step, o.seed = (uint32_t)seed, o.bits = small ? 8 : 32;
     if (grad_scale) {
@@ -263,36 +287,38 @@ void adamw(const List& params, const List& grads, const List& m, const List& v, 
         std::vector<ntops_adamw_tensor> t;
     };
     std::vector<Kind> kinds;
+    const auto state = small ? at::kByte : at::kFloat;
     for (size_t i = 0; i < n; ++i) {
         const Tensor& p = params[i];
-        auto fits = [&](const Tensor& t, const char* name, int64_t count) {
-            same_device(t, p0, name);
-            TORCH_CHECK_VALUE(t.numel() == count && t.is_contiguous(), name, " ", i, " must be contiguous with ", count, " elements, got shape ", t.sizes(), " and strides ", t.strides());
-        };
-        fits(p, "parameter", p.numel());
-        fits(grads[i], "gradient", p.numel());
-        fits(m[i], "first moment", p.numel());
-        fits(v[i], "second moment", p.numel());
-        const auto state = small ? at::kByte : at::kFloat;
-        TORCH_CHECK_TYPE(m[i].scalar_type() == state && v[i].scalar_type() == state, "moments must be ", state, ", got ", m[i].scalar_type(), " and ", v[i].scalar_type());
-        ntops_adamw_tensor t = {};
-        t.param = p.data_ptr(), t.grad = grads[i].data_ptr(), t.exp_avg = m[i].data_ptr(), t.exp_avg_sq = v[i].data_ptr(), t.n = p.numel();
-        if (small) {
-            const int64_t blocks = (p.numel() + NTOPS_ADAMW_BLOCK - 1) / NTOPS_ADAMW_BLOCK;
-            for (const auto& [list, name] : {std::pair<const List&, const char*>(*ms, "scales of the first moment"), std::pair<const List&, const char*>(*vs, "scales of the second moment")}) {
-                fits(list[i], name, blocks);
-                TORCH_CHECK_TYPE(list[i].scalar_type() == at::kFloat, name, " must be float32");
+        const int64_t count = p.numel();
+        auto fits = [&](const Tensor& t, const char* name, int64_t want) -> void* {
+            if (C10_UNLIKELY(t.device() != device || t.numel() != want || !t.is_contiguous())) {
+                same_device(t, p0, name);
+                TORCH_CHECK_VALUE(false, name, " ", i, " must be contiguous with ", want, " elements, got shape ", t.sizes(), " and strides ", t.strides());
             }
-            t.exp_avg_scale = (*ms)[i].data_ptr<float>(), t.exp_avg_sq_scale = (*vs)[i].data_ptr<float>();
+            return t.data_ptr();
+        };
+        ntops_adamw_tensor t = {};
+        t.param = fits(p, "parameter", count), t.grad = fits(grads[i], "gradient", count), t.exp_avg = fits(m[i], "first moment", count);
+        t.exp_avg_sq = fits(v[i], "second moment", count), t.n = count;
+        TORCH_CHECK_TYPE(m[i].scalar_type() == state && v[i].scalar_type() == state, "moments must be ", state, ", got ", m[i].scalar_type(), " and ", v[i].scalar_type());
+        if (small) {
+            const int64_t blocks = (count + NTOPS_ADAMW_BLOCK - 1) / NTOPS_ADAMW_BLOCK;
+            TORCH_CHECK_TYPE(ms[i].scalar_type() == at::kFloat && vs[i].scalar_type() == at::kFloat, "scales of moments must be float32");
+            t.exp_avg_scale = static_cast<float*>(fits(ms[i], "scales of the first moment", blocks));
+            t.exp_avg_sq_scale = static_cast<float*>(fits(vs[i], "scales of the second moment", blocks));
         }
-        Kind k = {code_of(p, "a parameter"), code_of(grads[i], "a gradient"), -1, {}};
-        if (copies && (*copies)[i].defined()) {
-            fits((*copies)[i], "copy", p.numel());
-            k.c = code_of((*copies)[i], "a copy");
-            t.copy = (*copies)[i].data_ptr();
+        const int pc = code_of(p, "a parameter"), gc = code_of(grads[i], "a gradient");
+        int cc = -1;
+        if (copies.given() && !copies.none(i)) {
+            t.copy = fits(copies[i], "copy", count);
+            cc = code_of(copies[i], "a copy");
         }
-        auto at = std::find_if(kinds.begin(), kinds.end(), [&](const Kind& q) { return q.p == k.p && q.g == k.g && q.c == k.c; });
-        if (at == kinds.end()) at = kinds.insert(kinds.end(), std::move(k));
+        auto at = std::find_if(kinds.begin(), kinds.end(), [&](const Kind& q) { return q.p == pc && q.g == gc && q.c == cc; });
+        if (at == kinds.end()) {
+            at = kinds.insert(kinds.end(), Kind{pc, gc, cc, {}});
+            at->t.reserve(n - i);
+        }
         at->t.push_back(t);
     }
     for (const Kind& k : kinds) {
@@ -300,8 +326,8 @@ void adamw(const List& params, const List& grads, const List& m, const List& v, 
         call(ntops_adamw(k.t.data(), (int)k.t.size(), &o, stream_of(p0)), "ntops_adamw");
     }
     // (autograd's record of in-place changes: a graph that saved a parameter finds out)
-    for (const Tensor& p : params)
-        if (!p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+    for (size_t i = 0; i < n; ++i)
+        if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
 }
 
 Tensor adamw_unpack(const Tensor& codes, const Tensor& scale) {
