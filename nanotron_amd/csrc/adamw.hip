@@ -20,7 +20,7 @@ namespace {
 constexpr int kThreads = 256, kEach = 4;
 constexpr int kBlock = NTOPS_ADAMW_BLOCK;
 static_assert(kBlock == 64 * kEach, "a wave holds a block of 8-bit moments");
-constexpr int chunk_of(int turns) { return kThreads * kEach * turns; }   // elements a workgroup takes
+constexpr int kChunk = kThreads * kEach;   // elements of a workgroup
 
 // what a launch knows of a tensor: as little as its kind needs, the arguments of a launch being 4 KB
 struct Moments {
@@ -62,13 +62,12 @@ __device__ __forceinline__ int scale_exponent(uint32_t top) {
     return top == 0u ? 0 : min(max(k, -126), 126);
 }
 
-// |value| times the scale, at most 448, plus its dither -> code without sign
+// |value| times the scale (at most 448) plus its dither -> code without sign.  Below 2^-6 codes are 2^-9 apart, as they are
+// from 2^-6 to 2^-5: moved up by 2^-6 a value is rounded like one of those, 8 codes further on.
 __device__ __forceinline__ uint32_t encode(float a, float scale, uint32_t dither) {
     const float y = a * scale;
-    const uint32_t normal = ((__float_as_uint(y) + (dither << 4)) >> 20) - 960u;
-    const uint32_t small = (uint32_t)(y * 512.0f + (float)dither * 0x1p-16f);   // below 2^-6 codes are 2^-9 apart
-    uint32_t c = y >= 0x1p-6f ? normal : small;
-    return (__float_as_uint(a) & 0x7fffffffu) >= kInfBits ? 0x7fu : c;
+    const bool small = y < 0x1p-6f;
+    return ((__float_as_uint(y + (small ? 0x1p-6f : 0.0f)) + (dither << 4)) >> 20) - (small ? 968u : 960u);
 }
 
 template <int N>
@@ -79,8 +78,10 @@ __device__ __forceinline__ void decode(uint32_t w, float inverse, float (&v)[N])
     v[0] = lo.x * inverse, v[1] = lo.y * inverse, v[2] = hi.x * inverse, v[3] = hi.y * inverse;
 }
 
-// kTurns pieces of 4 elements a thread, all requested before the first is used
-template <int P, int G, bool k8, bool kCopy, int kTurns>
+// Four elements a thread and no loop: with four such pieces a thread, all requested before the first was used, steps were
+// as fast from 4 million elements on with fp32 moments, slower with 8-bit ones (12.7 million bf16 parameters 35.5 / 40.2 us) and
+// below (0.9 million fp32 ones 6.0 / 8.0).
+template <int P, int G, bool k8, bool kCopy>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s) {
     // The last tensor whose first workgroup is not behind this one: every lane compares one, so that the arguments are read
     // in one trip (looked up by halves they are seven dependent ones, 3 us in front of a workgroup's first load)
@@ -89,111 +90,105 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
     if constexpr (s.kMost > 64) which += __popcll(__ballot(lane + 64 < s.kMost && s.first[min(lane + 64, s.kMost - 1)] <= (int)blockIdx.x));
     which = __builtin_amdgcn_readfirstlane(which - 1);
     const Moments T = s.t[which];
-    const int64_t n = T.n, at = (int64_t)((int)blockIdx.x - s.first[which]) * chunk_of(kTurns) + threadIdx.x * kEach;
+    const int64_t n = T.n, i = (int64_t)((int)blockIdx.x - s.first[which]) * kChunk + threadIdx.x * kEach;
+    const int left = i < n ? (int)min((int64_t)kEach, n - i) : 0;
     float* const scale_m = k8 ? s.scales[k8 ? which : 0].m : nullptr;
     float* const scale_v = k8 ? s.scales[k8 ? which : 0].v : nullptr;
     void* const copy = kCopy ? s.copy[kCopy ? which : 0] : nullptr;
-    Piece<P, kEach> pr[kTurns];
-    Piece<G, kEach> gr[kTurns];
-    Piece<NTFP8_F32, kEach> mr[kTurns], vr[kTurns];
-    uint32_t mc[kTurns], vc[kTurns];
-    float ms[kTurns], vs[kTurns];
-    int left[kTurns];
-#pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-        const int64_t i = at + u * (kThreads * kEach);
-        left[u] = i < n ? (int)min((int64_t)kEach, n - i) : 0;
-        pr[u] = load_piece<P, kEach>(T.p, i, left[u]);
-        gr[u] = load_piece<G, kEach>(T.g, i, left[u]);
-        if constexpr (k8) {
-            mc[u] = vc[u] = 0;
-            ms[u] = vs[u] = 1.0f;
-            if (left[u] == kEach) {
-                mc[u] = reinterpret_cast<const Word*>(static_cast<const uint8_t*>(T.m) + i)->w;
-                vc[u] = reinterpret_cast<const Word*>(static_cast<const uint8_t*>(T.v) + i)->w;
-            } else {
-                for (int e = 0; e < left[u]; ++e) {
-                    mc[u] |= (uint32_t)static_cast<const uint8_t*>(T.m)[i + e] << (8 * e);
-                    vc[u] |= (uint32_t)static_cast<const uint8_t*>(T.v)[i + e] << (8 * e);
-                }
-            }
-            if (left[u]) {
-                ms[u] = scale_m[i / kBlock];
-                vs[u] = scale_v[i / kBlock];
-            }
+    float p[kEach], g[kEach], m[kEach], v[kEach], r[kEach];
+    const Piece<P, kEach> pr = load_piece<P, kEach>(T.p, i, left);
+    const Piece<G, kEach> gr = load_piece<G, kEach>(T.g, i, left);
+    if constexpr (k8) {
+        uint32_t mc = 0, vc = 0;
+        float ms = 1.0f, vs = 1.0f;
+        if (left == kEach) {
+            mc = reinterpret_cast<const Word*>(static_cast<const uint8_t*>(T.m) + i)->w;
+            vc = reinterpret_cast<const Word*>(static_cast<const uint8_t*>(T.v) + i)->w;
         } else {
-            mr[u] = load_piece<NTFP8_F32, kEach>(T.m, i, left[u]);
-            vr[u] = load_piece<NTFP8_F32, kEach>(T.v, i, left[u]);
+            for (int e = 0; e < left; ++e) {
+                mc |= (uint32_t)static_cast<const uint8_t*>(T.m)[i + e] << (8 * e);
+                vc |= (uint32_t)static_cast<const uint8_t*>(T.v)[i + e] << (8 * e);
+            }
         }
+        if (left) {
+            ms = scale_m[i / kBlock];
+            vs = scale_v[i / kBlock];
+        }
+        decode(mc, __builtin_amdgcn_rcpf(ms), m);   // (exact: powers of two)
+        decode(vc, __builtin_amdgcn_rcpf(vs), v);
+    } else {
+        unpack<NTFP8_F32, kEach>(load_piece<NTFP8_F32, kEach>(T.m, i, left), m);
+        unpack<NTFP8_F32, kEach>(load_piece<NTFP8_F32, kEach>(T.v, i, left), v);
     }
     const float factor = s.grad_scale ? *s.grad_scale : 1.0f;
+    unpack<P, kEach>(pr, p);
+    unpack<G, kEach>(gr, g);
 #pragma unroll
-    for (int u = 0; u < kTurns; ++u) {
-        const int64_t i = at + u * (kThreads * kEach);
-        float p[kEach], g[kEach], m[kEach], v[kEach], r[kEach];
-        unpack<P, kEach>(pr[u], p);
-        unpack<G, kEach>(gr[u], g);
+    for (int e = 0; e < kEach; ++e) {
+        g[e] *= factor;
+        m[e] = s.beta1 * m[e] + s.rest1 * g[e];
+        if constexpr (k8) v[e] *= v[e];
+        v[e] = s.beta2 * v[e] + s.rest2 * (g[e] * g[e]);
         if constexpr (k8) {
-            decode(mc[u], 1.0f / ms[u], m);
-            decode(vc[u], 1.0f / vs[u], v);
+            // (to the last bit but one: with 8-bit moments the arithmetic bounds the step, and correctly rounded roots and
+            // quotients are a fifth of it)
+            r[e] = __builtin_amdgcn_sqrtf(v[e]);
+            p[e] = p[e] * s.keep - s.to * (m[e] * __builtin_amdgcn_rcpf(r[e] * s.root + s.eps));
         } else {
-            unpack<NTFP8_F32, kEach>(mr[u], m);
-            unpack<NTFP8_F32, kEach>(vr[u], v);
+            p[e] = p[e] * s.keep - s.to * (m[e] / (sqrtf(v[e]) * s.root + s.eps));
         }
+    }
+    store_piece<P, kEach>(T.p, i, p, left);
+    if (kCopy && copy) {
+        if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach>(copy, i, p, left);
+        else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach>(copy, i, p, left);
+        else store_piece<NTFP8_F32, kEach>(copy, i, p, left);
+    }
+    if constexpr (k8) {
+        uint32_t mt = 0, rt = 0;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
-            g[e] *= factor;
-            m[e] = s.beta1 * m[e] + s.rest1 * g[e];
-            if constexpr (k8) v[e] *= v[e];
-            v[e] = s.beta2 * v[e] + s.rest2 * (g[e] * g[e]);
-            r[e] = sqrtf(v[e]);
-            p[e] = p[e] * s.keep - s.to * (m[e] / (r[e] * s.root + s.eps));
+            mt = max(mt, __float_as_uint(m[e]) & 0x7fffffffu);   // (NaN lies above all others)
+            rt = max(rt, __float_as_uint(r[e]) & 0x7fffffffu);
         }
-        store_piece<P, kEach>(T.p, i, p, left[u]);
-        if (kCopy && copy) {
-            if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach>(copy, i, p, left[u]);
-            else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach>(copy, i, p, left[u]);
-            else store_piece<NTFP8_F32, kEach>(copy, i, p, left[u]);
+        mt = wave_most(mt);
+        rt = wave_most(rt);
+        const int mk = scale_exponent(mt), rk = scale_exponent(rt);
+        const float mf = __uint_as_float((uint32_t)(mk + 127) << 23), rf = __uint_as_float((uint32_t)(rk + 127) << 23);
+        uint32_t mw = 0, rw = 0;
+#pragma unroll
+        for (int e = 0; e < kEach; e += 2) {
+            const uint32_t d = dither_of((uint32_t)(i >> 1) + e / 2, s.seed);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t d16 = h ? d >> 16 : d & 0xffffu, bits = __float_as_uint(m[e + h]);
+                mw |= (encode(__builtin_fabsf(m[e + h]), mf, d16) | ((bits >> 24) & 0x80u)) << (8 * (e + h));
+                rw |= max(encode(r[e + h], rf, d16), min(__float_as_uint(r[e + h]), 1u)) << (8 * (e + h));
+            }
         }
-        if constexpr (k8) {
-            uint32_t mt = 0, rt = 0;
+        if (max(mt, rt) >= kInfBits) {   // uniform: a block with something that is not finite in it
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
-                mt = max(mt, __float_as_uint(m[e]) & 0x7fffffffu);   // (NaN lies above all others)
-                rt = max(rt, __float_as_uint(r[e]) & 0x7fffffffu);
+                if ((__float_as_uint(m[e]) & 0x7fffffffu) >= kInfBits) mw |= 0x7fu << (8 * e);
+                if ((__float_as_uint(r[e]) & 0x7fffffffu) >= kInfBits) rw |= 0x7fu << (8 * e);
             }
-            const int mk = scale_exponent(wave_most(mt)), rk = scale_exponent(wave_most(rt));
-            const float mf = __uint_as_float((uint32_t)(mk + 127) << 23), rf = __uint_as_float((uint32_t)(rk + 127) << 23);
-            uint32_t mw = 0, rw = 0;
-#pragma unroll
-            for (int e = 0; e < kEach; e += 2) {
-                const uint32_t d = dither_of((uint32_t)(i >> 1) + e / 2, s.seed);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t d16 = h ? d >> 16 : d & 0xffffu;
-                    const float a = __uint_as_float(__float_as_uint(m[e + h]) & 0x7fffffffu);
-                    mw |= (encode(a, mf, d16) | ((__float_as_uint(m[e + h]) >> 24) & 0x80u)) << (8 * (e + h));
-                    const uint32_t c = encode(r[e + h], rf, d16);
-                    rw |= ((c == 0u && r[e + h] > 0.0f ? 1u : c) | ((__float_as_uint(r[e + h]) >> 24) & 0x80u)) << (8 * (e + h));
-                }
-            }
-            if (left[u] == kEach) {
-                reinterpret_cast<Word*>(static_cast<uint8_t*>(T.m) + i)->w = mw;
-                reinterpret_cast<Word*>(static_cast<uint8_t*>(T.v) + i)->w = rw;
-            } else {
-                for (int e = 0; e < left[u]; ++e) {
-                    static_cast<uint8_t*>(T.m)[i + e] = (uint8_t)(mw >> (8 * e));
-                    static_cast<uint8_t*>(T.v)[i + e] = (uint8_t)(rw >> (8 * e));
-                }
-            }
-            if ((threadIdx.x & 63) == 0 && left[u]) {
-                scale_m[i / kBlock] = mf;
-                scale_v[i / kBlock] = rf;
-            }
-        } else {
-            store_piece<NTFP8_F32, kEach>(T.m, i, m, left[u]);
-            store_piece<NTFP8_F32, kEach>(T.v, i, v, left[u]);
         }
+        if (left == kEach) {
+            reinterpret_cast<Word*>(static_cast<uint8_t*>(T.m) + i)->w = mw;
+            reinterpret_cast<Word*>(static_cast<uint8_t*>(T.v) + i)->w = rw;
+        } else {
+            for (int e = 0; e < left; ++e) {
+                static_cast<uint8_t*>(T.m)[i + e] = (uint8_t)(mw >> (8 * e));
+                static_cast<uint8_t*>(T.v)[i + e] = (uint8_t)(rw >> (8 * e));
+            }
+        }
+        if ((threadIdx.x & 63) == 0 && left) {
+            scale_m[i / kBlock] = mf;
+            scale_v[i / kBlock] = rf;
+        }
+    } else {
+        store_piece<NTFP8_F32, kEach>(T.m, i, m, left);
+        store_piece<NTFP8_F32, kEach>(T.v, i, v, left);
     }
 }
 
@@ -220,18 +215,12 @@ int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options&
     s.root = (float)(1.0 / sqrt(1.0 - pow(o.beta2, (double)o.step)));
     s.eps = (float)o.eps;
     s.seed = o.seed * 0xBB67AE85u;
-    // Few elements in all: a piece a thread, for as many workgroups as there can be; else four, for loads enough in flight.
-    int64_t all = 0;
-    for (int i = 0; i < count; ++i) all += tensors[i].n;
-    const bool few = all < (int64_t)cu_count() * chunk_of(4) * 4;
-    const int chunk = chunk_of(few ? 1 : 4);
-    const int64_t part = (int64_t)chunk << 20;   // a tensor of more workgroups than a launch should have is split
+    constexpr int64_t part = (int64_t)kChunk << 20;   // a tensor of more workgroups than a launch should have is split
     int used = 0, blocks = 0;
     auto launch = [&]() {
         if (used == 0) return (int)NTFP8_OK;
         for (int i = used; i < S::kMost; ++i) s.first[i] = 0x7fffffff;
-        if (few) adamw_kernel<P, G, k8, kCopy, 1><<<(unsigned)blocks, kThreads, 0, st>>>(s);
-        else adamw_kernel<P, G, k8, kCopy, 4><<<(unsigned)blocks, kThreads, 0, st>>>(s);
+        adamw_kernel<P, G, k8, kCopy><<<(unsigned)blocks, kThreads, 0, st>>>(s);
         used = blocks = 0;
         return launch_status();
     };
@@ -240,7 +229,7 @@ int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options&
         const ntops_adamw_tensor& t = tensors[i];
         for (int64_t at = 0; at < t.n; at += part) {
             const int64_t n = std::min(part, t.n - at);
-            const int more = (int)((n + chunk - 1) / chunk);
+            const int more = (int)((n + kChunk - 1) / kChunk);
             if (used == S::kMost || blocks + more > (1 << 30))
                 if (const int rc = launch(); rc != NTFP8_OK) return rc;
             s.t[used] = Moments{static_cast<char*>(t.param) + at * size_of(P), static_cast<const char*>(t.grad) + at * size_of(G),
