@@ -81,7 +81,10 @@ __device__ __forceinline__ void decode(uint32_t w, float inverse, float (&v)[N])
 // Four elements a thread and no loop: with four such pieces a thread, all requested before the first was used, steps were
 // as fast from 4 million elements on with fp32 moments, slower with 8-bit ones (12.7 million bf16 parameters 35.5 / 40.2 us) and
 // below (0.9 million fp32 ones 6.0 / 8.0).
-template <int P, int G, bool k8, bool kCopy>
+// kStream: what a step moves does not fit the memory-side cache (256 MB) and is read and written past the caches.  us, with /
+// without: a decoder layer of 218 million fp32 parameters with fp32 moments 1016 / 1130, with 8-bit ones 554 / 596; 12.7 million,
+// which fit, 54 / 49 where the same ones were stepped just before.
+template <int P, int G, bool k8, bool kCopy, bool kStream>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s) {
     // The last tensor whose first workgroup is not behind this one: every lane compares one, so that the arguments are read
     // in one trip (looked up by halves they are seven dependent ones, 3 us in front of a workgroup's first load)
@@ -96,8 +99,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
     float* const scale_v = k8 ? s.scales[k8 ? which : 0].v : nullptr;
     void* const copy = kCopy ? s.copy[kCopy ? which : 0] : nullptr;
     float p[kEach], g[kEach], m[kEach], v[kEach], r[kEach];
-    const Piece<P, kEach> pr = load_piece<P, kEach>(T.p, i, left);
-    const Piece<G, kEach> gr = load_piece<G, kEach>(T.g, i, left);
+    const Piece<P, kEach> pr = load_piece<P, kEach, kStream>(T.p, i, left);
+    const Piece<G, kEach> gr = load_piece<G, kEach, kStream>(T.g, i, left);
     if constexpr (k8) {
         uint32_t mc = 0, vc = 0;
         float ms = 1.0f, vs = 1.0f;
@@ -117,8 +120,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
         decode(mc, __builtin_amdgcn_rcpf(ms), m);   // (exact: powers of two)
         decode(vc, __builtin_amdgcn_rcpf(vs), v);
     } else {
-        unpack<NTFP8_F32, kEach>(load_piece<NTFP8_F32, kEach>(T.m, i, left), m);
-        unpack<NTFP8_F32, kEach>(load_piece<NTFP8_F32, kEach>(T.v, i, left), v);
+        unpack<NTFP8_F32, kEach>(load_piece<NTFP8_F32, kEach, kStream>(T.m, i, left), m);
+        unpack<NTFP8_F32, kEach>(load_piece<NTFP8_F32, kEach, kStream>(T.v, i, left), v);
     }
     const float factor = s.grad_scale ? *s.grad_scale : 1.0f;
     unpack<P, kEach>(pr, p);
@@ -138,11 +141,11 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
             p[e] = p[e] * s.keep - s.to * (m[e] / (sqrtf(v[e]) * s.root + s.eps));
         }
     }
-    store_piece<P, kEach>(T.p, i, p, left);
+    store_piece<P, kEach, kStream>(T.p, i, p, left);
     if (kCopy && copy) {
-        if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach>(copy, i, p, left);
-        else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach>(copy, i, p, left);
-        else store_piece<NTFP8_F32, kEach>(copy, i, p, left);
+        if (s.copy_dtype == NTFP8_BF16) store_piece<NTFP8_BF16, kEach, kStream>(copy, i, p, left);
+        else if (s.copy_dtype == NTFP8_F16) store_piece<NTFP8_F16, kEach, kStream>(copy, i, p, left);
+        else store_piece<NTFP8_F32, kEach, kStream>(copy, i, p, left);
     }
     if constexpr (k8) {
         uint32_t mt = 0, rt = 0;
@@ -187,8 +190,8 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
             scale_v[i / kBlock] = rf;
         }
     } else {
-        store_piece<NTFP8_F32, kEach>(T.m, i, m, left);
-        store_piece<NTFP8_F32, kEach>(T.v, i, v, left);
+        store_piece<NTFP8_F32, kEach, kStream>(T.m, i, m, left);
+        store_piece<NTFP8_F32, kEach, kStream>(T.v, i, v, left);
     }
 }
 
@@ -215,12 +218,16 @@ int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options&
     s.root = (float)(1.0 / sqrt(1.0 - pow(o.beta2, (double)o.step)));
     s.eps = (float)o.eps;
     s.seed = o.seed * 0xBB67AE85u;
+    int64_t all = 0;
+    for (int i = 0; i < count; ++i) all += tensors[i].n;
+    const bool stream = all * (2 * size_of(P) + size_of(G) + (k8 ? 4 : 16) + (kCopy ? 2 : 0)) > ((int64_t)256 << 20);
     constexpr int64_t part = (int64_t)kChunk << 20;   // a tensor of more workgroups than a launch should have is split
     int used = 0, blocks = 0;
     auto launch = [&]() {
         if (used == 0) return (int)NTFP8_OK;
         for (int i = used; i < S::kMost; ++i) s.first[i] = 0x7fffffff;
-        adamw_kernel<P, G, k8, kCopy><<<(unsigned)blocks, kThreads, 0, st>>>(s);
+        if (stream) adamw_kernel<P, G, k8, kCopy, true><<<(unsigned)blocks, kThreads, 0, st>>>(s);
+        else adamw_kernel<P, G, k8, kCopy, false><<<(unsigned)blocks, kThreads, 0, st>>>(s);
         used = blocks = 0;
         return launch_status();
     };

@@ -50,14 +50,22 @@ struct __attribute__((packed, aligned(D == NTFP8_F32 ? 4 : 2))) Piece {
     static constexpr int kWords = N * size_of(D) / 4;
     uint32_t w[kWords];
 };
+// the same words as the vector that a non-temporal access takes
 template <int D, int N>
+struct PieceVector {
+    typedef uint32_t type __attribute__((ext_vector_type(Piece<D, N>::kWords), aligned(D == NTFP8_F32 ? 4 : 2)));
+};
+// kStream: read or written once, not kept in the caches
+template <int D, int N, bool kStream = false>
 __device__ __forceinline__ Piece<D, N> load_piece(const void* p, int64_t i) {
-    return *reinterpret_cast<const Piece<D, N>*>(static_cast<const char*>(p) + i * size_of(D));
+    const char* const at = static_cast<const char*>(p) + i * size_of(D);
+    if constexpr (kStream) return __builtin_bit_cast(Piece<D, N>, __builtin_nontemporal_load(reinterpret_cast<const typename PieceVector<D, N>::type*>(at)));
+    else return *reinterpret_cast<const Piece<D, N>*>(at);
 }
 // the first `count` elements, zeros behind them
-template <int D, int N>
+template <int D, int N, bool kStream = false>
 __device__ __forceinline__ Piece<D, N> load_piece(const void* p, int64_t i, int count) {
-    if (count >= N) return load_piece<D, N>(p, i);
+    if (count >= N) return load_piece<D, N, kStream>(p, i);
     Piece<D, N> r;
 #pragma unroll
     for (int k = 0; k < Piece<D, N>::kWords; ++k) {
@@ -81,7 +89,7 @@ __device__ __forceinline__ void unpack(const Piece<D, N>& r, float (&v)[N]) {
         for (int k = 0; k < N / 2; ++k) unpack_pair<D>(r.w[k], v[2 * k], v[2 * k + 1]);
     }
 }
-template <int D, int N>
+template <int D, int N, bool kStream = false>
 __device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&v)[N], int count = N) {
     if (count >= N) {
         Piece<D, N> r;
@@ -92,7 +100,9 @@ __device__ __forceinline__ void store_piece(void* p, int64_t i, const float (&v)
 #pragma unroll
             for (int k = 0; k < N / 2; ++k) r.w[k] = pack_pair<D>(v[2 * k], v[2 * k + 1]);
         }
-        *reinterpret_cast<Piece<D, N>*>(static_cast<char*>(p) + i * size_of(D)) = r;
+        char* const at = static_cast<char*>(p) + i * size_of(D);
+        if constexpr (kStream) __builtin_nontemporal_store(__builtin_bit_cast(typename PieceVector<D, N>::type, r), reinterpret_cast<typename PieceVector<D, N>::type*>(at));
+        else *reinterpret_cast<Piece<D, N>*>(at) = r;
     } else {
 #pragma unroll
         for (int k = 0; k < N; ++k)
