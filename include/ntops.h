@@ -86,9 +86,14 @@ int64_t ntops_linear_cross_entropy_piece(int64_t vocab);
 int64_t ntops_linear_cross_entropy_workspace(const ntops_linear_cross_entropy_desc* d);
 int ntops_linear_cross_entropy(const ntops_linear_cross_entropy_desc* d, void* stream);
 
-/* out = out_dtype(x * *factor), n elements of x_dtype; out may be x (same type): then nothing is read or written where
- * *factor is 1.  What a backward pass does with the gradient that reaches a loss. */
-int ntops_scale(const void* x, int x_dtype, const float* factor, int64_t n, void* out, int out_dtype, void* stream);
+/* out = out_dtype(x * *factor) for `count` tensors of n elements of x_dtype; out may be x (same type): then nothing is read or
+ * written where *factor is 1.  What a backward pass does with the gradient that reaches a loss. */
+typedef struct ntops_scale_tensor {
+    const void* x;
+    void* out;
+    int64_t n;
+} ntops_scale_tensor;
+int ntops_scale(const ntops_scale_tensor* tensors, int count, int x_dtype, const float* factor, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -36,6 +36,11 @@ class LinearCrossEntropyDesc(ctypes.Structure):
                 ("loss", _vp), ("dx", _vp), ("dweight", _vp), ("workspace", _vp)]
 
 
+class ScaleTensor(ctypes.Structure):
+    """`ntops_scale_tensor` of include/ntops.h."""
+    _fields_ = [("x", _vp), ("out", _vp), ("n", _i64)]
+
+
 SIGNATURES = {
     "ntops_layer_norm_forward": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp]),
     "ntops_layer_norm_scratch": (_i64, [_i, _i64, _i64]),
@@ -45,7 +50,7 @@ SIGNATURES = {
     "ntops_linear_cross_entropy_piece": (_i64, [_i64]),
     "ntops_linear_cross_entropy_workspace": (_i64, [_c.POINTER(LinearCrossEntropyDesc)]),
     "ntops_linear_cross_entropy": (_i, [_c.POINTER(LinearCrossEntropyDesc), _vp]),
-    "ntops_scale": (_i, [_vp, _i, _vp, _i64, _vp, _i, _vp]),
+    "ntops_scale": (_i, [_c.POINTER(ScaleTensor), _i, _i, _vp, _i, _vp]),
 }
 for _name, (_res, _args) in SIGNATURES.items():
     _fn = getattr(nt.lib, _name)  # AttributeError here = library / header mismatch

@@ -127,19 +127,24 @@ __global__ __launch_bounds__(256) void softmax_rows_kernel(const float2* __restr
     }
 }
 
-// the losses' sum times the factor
-__global__ __launch_bounds__(1024) void head_end_kernel(const float* __restrict__ losses, int64_t tokens, const float* __restrict__ factors, float* __restrict__ loss) {
-    __shared__ float part[16];
+// one workgroup: the losses' sum times the factor
+template <int kThreads>
+__device__ __forceinline__ void sum_losses(const float* __restrict__ losses, int64_t tokens, const float* __restrict__ factors, float* __restrict__ loss) {
+    __shared__ float part[kThreads / 64];
     float s = 0.0f;
-    for (int64_t i = threadIdx.x; i < tokens; i += 1024) s += losses[i];
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < tokens; i += kThreads) s += losses[i];
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         s = 0.0f;
-        for (int w = 0; w < 16; ++w) s += part[w];
+        for (int w = 0; w < kThreads / 64; ++w) s += part[w];
         *loss = factors[0] == 0.0f ? 0.0f : s * factors[0];
     }
+}
+__global__ __launch_bounds__(1024) void head_end_kernel(const float* __restrict__ losses, int64_t tokens, const float* __restrict__ factors, float* __restrict__ loss) {
+    sum_losses<1024>(losses, tokens, factors, loss);
 }
 
 // rows padded with zeros to a multiple of 8 elements, for operands whose rows do not begin on 16-byte boundaries; with `from`
@@ -159,47 +164,62 @@ __global__ __launch_bounds__(256) void take_rows_kernel(const uint16_t* __restri
 
 // dx: row place[token] - row0 of what was computed for the tokens that count, zeros for the others (if row0 is 0; the other
 // launches of a call leave rows that are not theirs alone).  Computed is alpha times the sum of `splits` runs of K in fp32, or,
-// splits 0, the row itself.
+// splits 0, the row itself.  With `loss`, one more workgroup sums the losses.
 template <int D>
-__global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ from, int splits, int64_t split_stride, const float* __restrict__ alpha,
-                                                       const int* __restrict__ place, int64_t tokens, int row0, int count, int cols, void* __restrict__ out) {
-    const float a = splits ? *alpha : 1.0f;
-    for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
-        const int at = place[t];
+__global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ from, int splits, int64_t split_stride, const float* __restrict__ factors,
+                                                       const int* __restrict__ place, int64_t tokens, int row0, int count, int cols, void* __restrict__ out,
+                                                       const float* __restrict__ losses, float* __restrict__ loss) {
+    if (loss && blockIdx.x == gridDim.x - 1) {   // uniform
+        sum_losses<256>(losses, tokens, factors, loss);
+        return;
+    }
+    const float a = factors[1];
+    const int chunks = (cols + 7) / 8;
+    const int64_t all = tokens * chunks, step = (int64_t)(gridDim.x - (loss ? 1 : 0)) * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
+        const int64_t t = i / chunks;
+        const int c = (int)(i - t * chunks) * 8, left = cols - c, at = place[t];
         const int64_t r = at - row0;
         if (at < 0 ? row0 != 0 : r < 0 || r >= count) continue;
-        for (int c = threadIdx.x * 8; c < cols; c += 2048) {
-            const int left = cols - c;
-            float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (at >= 0) {
-                if (splits == 0) unpack<D, 8>(load_piece<D, 8>(from, r * cols + c, left), s);
-                for (int k = 0; k < splits; ++k) {
-                    float v[8];
-                    unpack<NTFP8_F32, 8>(load_piece<NTFP8_F32, 8>(from, k * split_stride + r * cols + c, left), v);
+        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (at >= 0) {
+            if (splits == 0) unpack<D, 8>(load_piece<D, 8>(from, r * cols + c, left), s);
+#pragma unroll 8
+            for (int k = 0; k < splits; ++k) {
+                float v[8];
+                unpack<NTFP8_F32, 8>(load_piece<NTFP8_F32, 8>(from, k * split_stride + r * cols + c, left), v);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) s[e] += v[e];
-                }
-                if (splits) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s[e] *= a;
-                }
+                for (int e = 0; e < 8; ++e) s[e] += v[e];
             }
-            store_piece<D, 8>(out, t * cols + c, s, left);
+            if (splits) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[e] *= a;
+            }
         }
+        store_piece<D, 8>(out, t * cols + c, s, left);
     }
 }
 
+struct Scaled {
+    const void* x[2];
+    void* out[2];
+    int64_t n[2];
+};
 template <int S, int D>
-__global__ __launch_bounds__(256) void scale_kernel(const void* x, const float* __restrict__ factor, int64_t n, void* out) {
+__global__ __launch_bounds__(256) void scale_kernel(const Scaled t, const float* __restrict__ factor) {
     const float f = *factor;
-    if (x == out && f == 1.0f) return;
-    for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
-        const int left = (int)std::min<int64_t>(8, n - i);
-        float v[8];
-        unpack<S, 8>(load_piece<S, 8>(x, i, left), v);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= f;
-        store_piece<D, 8>(out, i, v, left);
+    for (int k = 0; k < 2; ++k) {
+        const int64_t n = t.n[k];
+        if (t.x[k] == t.out[k] && f == 1.0f) continue;
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+            const int left = (int)std::min<int64_t>(8, n - i);
+            float v[8];
+            unpack<S, 8>(load_piece<S, 8>(t.x[k], i, left), v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] *= f;
+            store_piece<D, 8>(t.out[k], i, v, left);
+        }
     }
 }
 
@@ -220,15 +240,55 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
     return launch_status();
 }
 
-// rows of a tile / 32: the smallest tile that holds all rows, the largest beyond
-int tile_rows(int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
+// What a launch of `tiles` workgroups takes, us, each of `kts` K-tiles of (32 mi) x 256 outputs: rounds of one workgroup a CU, a
+// K-tile's time and what a workgroup takes besides.  A K-tile of fewer rows takes more of their share, since the 256 columns
+// are the larger part of what it loads.  (Measured at 64 to 2048 tokens, 512 to 4096 hidden, vocabularies of 6 to 50 thousand; with a
+// transposed operand a K-tile takes a tenth more.)
+float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed) {
+    const int at = mi == 1 ? 0 : mi == 2 ? 1 : mi == 4 ? 2 : 3;
+    constexpr float kTile[4] = {0.55f, 0.72f, 1.0f, 1.4f}, kRest[4] = {4.0f, 5.0f, 8.0f, 12.0f};
+    return (float)((tiles + 255) / 256) * ((float)kts * kTile[at] * (transposed ? 1.1f : 1.0f) + kRest[at]);
+}
+int64_t tiles_of(int64_t rows, int64_t cols, int mi) { return (rows + 32 * mi - 1) / (32 * mi) * ((cols + kBigN - 1) / kBigN); }
+
+// Rows of a tile / 32, and runs that K is cut into, for the products with an untransposed A
+struct Tiling {
+    int mi, splits, kt_split;
+};
+// logits: 333 tokens against 6001 rows of 512, us with 256 / 128 / 64 / 32 rows a tile: 25.4, 18.0, 12.5, 16.3; 512 tokens, 32000 rows of 2048: 57.6,
+// 81.6, 107.7, 167.9
+Tiling tiling_of_logits(int64_t rows, int64_t cols, int64_t kts) {
+    Tiling best = {8, 1, 0};
+    float least = 1e30f;
+    for (int mi = 8; mi >= 1; mi /= 2) {
+        const float us = launch_us(mi, tiles_of(rows, cols, mi), kts, false);
+        if (us < least) least = us, best.mi = mi;
+    }
+    return best;
+}
+// dx: K is the vocabulary, and there are few tiles; runs of K fill the chip, for their fp32 sums' way to memory and back
+Tiling tiling_of_dx(int64_t rows, int64_t cols, int64_t kts) {
+    Tiling best = {8, 1, (int)kts};
+    float least = 1e30f;
+    for (int mi = 8; mi >= 1; mi /= 2) {
+        const int64_t tiles = tiles_of(rows, cols, mi);
+        for (int64_t want = 1; want <= 64 && want <= std::max<int64_t>(1, kts / 4); ++want) {
+            const int64_t each = (kts + want - 1) / want, splits = (kts + each - 1) / each;
+            if (splits > 1 && tiles * splits > 1024) break;
+            float us = launch_us(mi, tiles * splits, each, true);
+            if (splits > 1) us += (float)(rows * cols) * (float)splits * 8.0f / 4.5e6f;
+            if (us < least) least = us, best = {mi, (int)splits, (int)each};
+        }
+    }
+    return best;
+}
 
 struct Plan {
     int64_t piece;            // tokens at a time
     int64_t ldd, pieces;
     bool pad_x, pad_w;
     int64_t padded;           // hidden, up to a multiple of 8
-    int splits, kt_split;     // of dx
+    Tiling logits, dx;
     int64_t at_factors, at_label, at_place, at_token, at_kept, at_stats, at_held, at_x, at_w, at_dx, bytes;
 };
 int64_t piece_of(int64_t vocab) { return std::max<int64_t>(256, kMostHeld / (2 * held_cols(vocab)) / 256 * 256); }
@@ -244,15 +304,8 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     // seen by nobody)
     p.pad_x = gradient || d.hidden % 8 || d.x_stride % 8 || reinterpret_cast<uintptr_t>(d.x) % 16;
     p.pad_w = d.hidden % 8 || d.weight_stride % 8 || reinterpret_cast<uintptr_t>(d.weight) % 16;
-    p.splits = 1;
-    p.kt_split = 0;
-    if (d.dx) {
-        // few tiles: K, the vocabulary, is cut into runs until there is one workgroup for each CU, of 8 K-tiles or more
-        const int64_t rows = p.piece, mi = tile_rows(rows), tiles = up(rows, 32 * mi) / (32 * mi) * (up(d.hidden, kBigN) / kBigN), kts = p.ldd / kHeadK;
-        const int64_t want = std::max<int64_t>(1, std::min(256 / tiles, kts / 8));
-        p.kt_split = (int)((kts + want - 1) / want);
-        p.splits = (int)((kts + p.kt_split - 1) / p.kt_split);
-    }
+    p.logits = tiling_of_logits(p.piece, p.ldd, (p.padded + kHeadK - 1) / kHeadK);
+    if (d.dx) p.dx = tiling_of_dx(p.piece, d.hidden, p.ldd / kHeadK);
     int64_t at = 0;
     auto room = [&](int64_t bytes) {
         const int64_t here = at;
@@ -270,7 +323,7 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     p.at_held = gradient ? room(p.piece * p.ldd * 2) : 0;
     p.at_x = p.pad_x ? room(d.tokens * p.padded * 2) : 0;
     p.at_w = p.pad_w ? room(d.vocab * p.padded * 2) : 0;
-    p.at_dx = d.dx ? room(p.piece * d.hidden * (p.splits > 1 ? 4 * p.splits : size_of(d.grad_dtype))) : 0;
+    p.at_dx = d.dx ? room(p.piece * d.hidden * (p.dx.splits > 1 ? 4 * p.dx.splits : size_of(d.grad_dtype))) : 0;
     p.bytes = at;
     return p;
 }
@@ -305,7 +358,7 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
     if (status(launch_status())) return NTFP8_ERR_LAUNCH;
     for (int64_t row = 0; row < d.tokens; row += p.piece) {
         const int64_t rows = std::min(p.piece, d.tokens - row);
-        const int mi = tile_rows(rows);
+        const bool last = row + rows == d.tokens;
         HeadGemm g = {};
         g.A = x + row * ldx * 2, g.lda = ldx, g.a_cols = (int)p.padded;
         g.B = w, g.ldb = ldw, g.b_cols = (int)p.padded, g.b_rows = 0;
@@ -313,7 +366,7 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
         g.rows = gradient ? count : nullptr, g.row0 = (int)row;
         g.D = held, g.ldd = p.ldd, g.stats = stats, g.pieces = (int)p.pieces;
         g.labels = labels + row, g.label_logit = label_logit + row;
-        if (status(gradient ? launch_gemm<T, false, false, kSoftmax>(g, mi, st) : launch_gemm<T, false, false, kLosses>(g, mi, st))) return NTFP8_ERR_LAUNCH;
+        if (status(gradient ? launch_gemm<T, false, false, kSoftmax>(g, p.logits.mi, st) : launch_gemm<T, false, false, kLosses>(g, p.logits.mi, st))) return NTFP8_ERR_LAUNCH;
         auto rows_kernel = gradient ? softmax_rows_kernel<T, true> : softmax_rows_kernel<T, false>;
         rows_kernel<<<(unsigned)rows, 256, 0, st>>>(stats, (int)p.pieces, labels + row, d.ignore_index, label_logit + row, gradient ? d.losses : d.losses + row, count, (int)row,
                                                     gradient ? token_of + row : nullptr, held, p.ldd);
@@ -325,11 +378,13 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
             h.M = (int)rows, h.N = (int)d.hidden, h.K = (int)p.ldd;
             h.rows = count, h.row0 = (int)row;
             h.D = ws + p.at_dx, h.d_dtype = d.grad_dtype, h.alpha = factors + 1;
-            h.splits = p.splits, h.kt_split = p.kt_split, h.partial = reinterpret_cast<float*>(ws + p.at_dx);
-            if (status(p.splits == 1 ? launch_gemm<T, false, true, kStore>(h, mi, st) : launch_gemm<T, false, true, kPartial>(h, mi, st))) return NTFP8_ERR_LAUNCH;
+            h.splits = p.dx.splits, h.kt_split = p.dx.kt_split, h.partial = reinterpret_cast<float*>(ws + p.at_dx);
+            const bool whole = p.dx.splits == 1;
+            if (status(whole ? launch_gemm<T, false, true, kStore>(h, p.dx.mi, st) : launch_gemm<T, false, true, kPartial>(h, p.dx.mi, st))) return NTFP8_ERR_LAUNCH;
             auto put = d.grad_dtype == T ? put_rows_kernel<T> : put_rows_kernel<NTFP8_F32>;
-            put<<<(unsigned)std::min<int64_t>(d.tokens, 8192), 256, 0, st>>>(ws + p.at_dx, p.splits == 1 ? 0 : p.splits, rows * d.hidden, h.alpha, place, d.tokens, (int)row, (int)rows,
-                                                                            (int)d.hidden, d.dx);
+            const int64_t n = d.tokens * ((d.hidden + 7) / 8);
+            put<<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192) + (last && d.loss ? 1 : 0), 256, 0, st>>>(
+                ws + p.at_dx, whole ? 0 : p.dx.splits, rows * d.hidden, factors, place, d.tokens, (int)row, (int)rows, (int)d.hidden, d.dx, d.losses, last ? d.loss : nullptr);
             if (status(launch_status())) return NTFP8_ERR_LAUNCH;
         }
         if (d.dweight) {
@@ -342,7 +397,7 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
             if (status(launch_gemm<T, true, true, kStore>(h, 8, st))) return NTFP8_ERR_LAUNCH;
         }
     }
-    if (d.loss) {
+    if (d.loss && !d.dx) {
         head_end_kernel<<<1, 1024, 0, st>>>(d.losses, d.tokens, factors, d.loss);
         return launch_status();
     }
@@ -355,14 +410,24 @@ int64_t head_piece(int64_t vocab) { return piece_of(vocab); }
 int64_t head_workspace(const ntops_linear_cross_entropy_desc& d) { return plan_of(d).bytes; }
 int run_head(const ntops_linear_cross_entropy_desc& d, hipStream_t st) { return d.x_dtype == NTFP8_BF16 ? run<NTFP8_BF16>(d, st) : run<NTFP8_F16>(d, st); }
 
-int run_scale(const void* x, int x_dtype, const float* factor, int64_t n, void* out, int out_dtype, hipStream_t st) {
-    const unsigned blocks = (unsigned)std::min<int64_t>((n + 2047) / 2048, 8192);
-    return with_dtype(x_dtype, [&](auto s) {
-        return with_dtype(out_dtype, [&](auto d) {
-            scale_kernel<decltype(s)::value, decltype(d)::value><<<blocks, 256, 0, st>>>(x, factor, n, out);
-            return launch_status();
+int run_scale(const ntops_scale_tensor* t, int count, int x_dtype, const float* factor, int out_dtype, hipStream_t st) {
+    for (int i = 0; i < count; i += 2) {
+        Scaled g = {};
+        int64_t most = 0;
+        for (int k = 0; k < 2 && i + k < count; ++k) {
+            g.x[k] = t[i + k].x, g.out[k] = t[i + k].out, g.n[k] = t[i + k].n;
+            most = std::max(most, t[i + k].n);
+        }
+        const unsigned blocks = (unsigned)std::min<int64_t>((most + 2047) / 2048, 2048);
+        const int rc = with_dtype(x_dtype, [&](auto s) {
+            return with_dtype(out_dtype, [&](auto d) {
+                scale_kernel<decltype(s)::value, decltype(d)::value><<<blocks, 256, 0, st>>>(g, factor);
+                return launch_status();
+            });
         });
-    });
+        if (rc != NTFP8_OK) return rc;
+    }
+    return NTFP8_OK;
 }
 
 }  // namespace ntfp8

@@ -16,7 +16,7 @@ int run_adamw_unpack(const void* codes, const float* scale, int64_t n, float* ou
 int64_t head_piece(int64_t vocab);
 int64_t head_workspace(const ntops_linear_cross_entropy_desc& d);
 int run_head(const ntops_linear_cross_entropy_desc& d, hipStream_t st);
-int run_scale(const void* x, int x_dtype, const float* factor, int64_t n, void* out, int out_dtype, hipStream_t st);
+int run_scale(const ntops_scale_tensor* t, int count, int x_dtype, const float* factor, int out_dtype, hipStream_t st);
 
 namespace {
 
@@ -156,13 +156,19 @@ int ntops_linear_cross_entropy(const ntops_linear_cross_entropy_desc* d, void* s
     return run_head(*d, static_cast<hipStream_t>(stream));
 }
 
-int ntops_scale(const void* x, int x_dtype, const float* factor, int64_t n, void* out, int out_dtype, void* stream) {
-    if (!x || !factor || !out) return NTFP8_ERR_NULL;
+int ntops_scale(const ntops_scale_tensor* tensors, int count, int x_dtype, const float* factor, int out_dtype, void* stream) {
+    if (!factor || (count > 0 && !tensors)) return NTFP8_ERR_NULL;
     if (!dtype_ok(x_dtype) || !dtype_ok(out_dtype)) return NTFP8_ERR_ENUM;
-    if (n <= 0 || n > kMostElements) return NTFP8_ERR_SIZE;
-    if (!aligned(x, size_of(x_dtype)) || !aligned(factor, 4) || !aligned(out, size_of(out_dtype))) return NTFP8_ERR_ALIGN;
-    if ((x != out || x_dtype != out_dtype) && overlap(x, n * size_of(x_dtype), out, n * size_of(out_dtype))) return NTFP8_ERR_ALIAS;
-    return run_scale(x, x_dtype, factor, n, out, out_dtype, static_cast<hipStream_t>(stream));
+    if (count < 0) return NTFP8_ERR_SIZE;
+    if (!aligned(factor, 4)) return NTFP8_ERR_ALIGN;
+    for (int i = 0; i < count; ++i) {
+        const ntops_scale_tensor& t = tensors[i];
+        if (!t.x || !t.out) return NTFP8_ERR_NULL;
+        if (t.n <= 0 || t.n > kMostElements) return NTFP8_ERR_SIZE;
+        if (!aligned(t.x, size_of(x_dtype)) || !aligned(t.out, size_of(out_dtype))) return NTFP8_ERR_ALIGN;
+        if ((t.x != t.out || x_dtype != out_dtype) && overlap(t.x, t.n * size_of(x_dtype), t.out, t.n * size_of(out_dtype))) return NTFP8_ERR_ALIAS;
+    }
+    return run_scale(tensors, count, x_dtype, factor, out_dtype, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -174,11 +174,18 @@ Head head(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore
     return h;
 }
 
-Tensor scaled(const Tensor& t, const Tensor& factor, at::ScalarType to) {
-    const Tensor out = t.scalar_type() == to ? t : at::empty(t.sizes(), t.options().dtype(to));
-    if (t.numel())
-        call(ntops_scale(t.data_ptr(), code_of(t, "gradient"), factor.const_data_ptr<float>(), t.numel(), out.data_ptr(), code_of(out, "gradient"), stream_of(t)), "ntops_scale");
-    return out;
+// the gradients times what arrives from above, of type `to`
+void scale(Tensor* const (&t)[2], const Tensor& factor, at::ScalarType to) {
+    ntops_scale_tensor d[2];
+    int n = 0, from = -1;
+    for (Tensor* g : t) {
+        if (!g->defined()) continue;
+        from = code_of(*g, "a gradient");
+        const Tensor out = g->scalar_type() == to ? *g : at::empty(g->sizes(), g->options().dtype(to));
+        d[n++] = {g->data_ptr(), out.data_ptr(), g->numel()};
+        *g = out;
+    }
+    if (n) call(ntops_scale(d, n, from, factor.const_data_ptr<float>(), to == at::kHalf ? NTFP8_F16 : NTFP8_BF16, stream_of(factor)), "ntops_scale");
 }
 
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
@@ -205,8 +212,8 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         Guard guard(grads[0].device());
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = grads[0].to(at::kFloat);
-        if (dx.defined()) dx = scaled(dx, g, type);
-        if (dw.defined()) dw = scaled(dw, g, type);
+        const Tensor held_dx = dx, held_dw = dw;   // (until the launch that reads them is queued)
+        scale({&dx, &dw}, g, type);
         return {dx, dw, Variable(), Variable(), Variable(), Variable(), Variable()};
     }
 };

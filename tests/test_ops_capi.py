@@ -30,7 +30,7 @@ def test_library_exports_every_declared_symbol():
 
 
 @pytest.mark.parametrize("name,struct", [("ntops_adamw_tensor", _ops.AdamWTensor), ("ntops_adamw_options", _ops.AdamWOptions),
-                                         ("ntops_linear_cross_entropy_desc", _ops.LinearCrossEntropyDesc)])
+                                         ("ntops_linear_cross_entropy_desc", _ops.LinearCrossEntropyDesc), ("ntops_scale_tensor", _ops.ScaleTensor)])
 def test_struct_fields_match_header(name, struct):
     body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), source(), flags=re.S).group(1)
     fields = []
@@ -126,9 +126,12 @@ def test_linear_cross_entropy_argument_errors():
 
 
 def test_scale_argument_errors():
-    f = _ops.lib.ntops_scale
-    assert f(None, 0, P, 4, Q, 0, None) == NULL and f(P, 3, P, 4, Q, 0, None) == ENUM and f(P, 0, P, 0, Q, 0, None) == SIZE
-    assert f(P, 0, R, 4, P, 2, None) == ALIAS and f(P + 2, 0, R, 4, Q, 0, None) == ALIGN
+    def f(x=P, out=Q, n=4, x_dtype=0, factor=R, out_dtype=0, count=1):
+        return _ops.lib.ntops_scale((_ops.ScaleTensor * 1)(_ops.ScaleTensor(x, out, n)), count, x_dtype, factor, out_dtype, None)
+
+    assert f(x=None) == NULL and f(out=None) == NULL and f(factor=None) == NULL and _ops.lib.ntops_scale(None, 1, 0, R, 0, None) == NULL
+    assert f(x_dtype=3) == ENUM and f(out_dtype=-1) == ENUM and f(n=0) == SIZE and f(count=-1) == SIZE
+    assert f(out=P, out_dtype=2) == ALIAS and f(x=P + 2) == ALIGN and f(count=0) == 0
 
 
 def test_public_functions_refuse_host_tensors():
