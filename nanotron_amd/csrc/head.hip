@@ -205,14 +205,16 @@ struct Scaled {
     void* out[2];
     int64_t n[2];
 };
+// (as few workgroups as can keep the memory busy: where the factor is 1 the launch is nothing but their coming and going)
 template <int S, int D>
-__global__ __launch_bounds__(256) void scale_kernel(const Scaled t, const float* __restrict__ factor) {
+__global__ __launch_bounds__(1024) void scale_kernel(const Scaled t, const float* __restrict__ factor) {
     const float f = *factor;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int64_t n = t.n[k];
         if (t.x[k] == t.out[k] && f == 1.0f) continue;
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 2048) {
+#pragma unroll 4
+        for (int64_t i = ((int64_t)blockIdx.x * 1024 + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * 8192) {
             const int left = (int)std::min<int64_t>(8, n - i);
             float v[8];
             unpack<S, 8>(load_piece<S, 8>(t.x[k], i, left), v);
@@ -418,10 +420,10 @@ int run_scale(const ntops_scale_tensor* t, int count, int x_dtype, const float* 
             g.x[k] = t[i + k].x, g.out[k] = t[i + k].out, g.n[k] = t[i + k].n;
             most = std::max(most, t[i + k].n);
         }
-        const unsigned blocks = (unsigned)std::min<int64_t>((most + 2047) / 2048, 2048);
+        const unsigned blocks = (unsigned)std::min<int64_t>((most + 8191) / 8192, 2 * cu_count());
         const int rc = with_dtype(x_dtype, [&](auto s) {
             return with_dtype(out_dtype, [&](auto d) {
-                scale_kernel<decltype(s)::value, decltype(d)::value><<<blocks, 256, 0, st>>>(g, factor);
+                scale_kernel<decltype(s)::value, decltype(d)::value><<<blocks, 1024, 0, st>>>(g, factor);
                 return launch_status();
             });
         });

@@ -246,6 +246,38 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
     }
 }
 
+// Stores of a wave's tile.  Rows of whole pieces go as those of the fp8 GEMM do; others, whose rows begin anywhere, a lane's
+// 4 consecutive outputs at a time at whatever address they have (element by element, the weight's gradient of 6001 x 515 in fp32 took
+// twice as long).
+template <int DT, bool kAcc, int MI>
+__device__ __forceinline__ void store_tile(const v4f (&acc)[MI][kBigNJ], void* D, float alpha, int M, int N, int m_base, int n_base, int lane) {
+    if ((N & 7) == 0) {
+        store_wave_tile16<DT, kAcc, MI, kBigNJ>(acc, D, alpha, M, N, m_base, n_base, lane);
+        return;
+    }
+    const int mrow = lane & 15, q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int m = m_base + 16 * i + mrow;
+        if (m >= M) continue;
+#pragma unroll
+        for (int j = 0; j < kBigNJ; ++j) {
+            const int n = n_base + 16 * j + 4 * q, left = N - n;
+            if (left <= 0) continue;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * alpha;
+            if constexpr (kAcc) {
+                float old[4];
+                unpack<DT, 4>(load_piece<DT, 4>(D, (int64_t)m * N + n, left), old);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] += old[e];
+            }
+            store_piece<DT, 4>(D, (int64_t)m * N + n, v, left);
+        }
+    }
+}
+
 template <int T, bool kAT, bool kBT, int MI, int EPI>
 __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G) {
     constexpr int NS = head_stages<MI>();
@@ -417,12 +449,12 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
     if constexpr (EPI == kLosses || EPI == kSoftmax) {
         softmax_epilogue<MI, EPI == kSoftmax>(acc, G, M, m0 + wm, n0 + wn, lane);
     } else if constexpr (EPI == kPartial) {
-        store_wave_tile16<NTFP8_F32, false, MI, kBigNJ>(acc, G.partial + (int64_t)split * G.M * G.N, 1.0f, M, G.N, m0 + wm, n0 + wn, lane);
+        store_tile<NTFP8_F32, false, MI>(acc, G.partial + (int64_t)split * G.M * G.N, 1.0f, M, G.N, m0 + wm, n0 + wn, lane);
     } else {
         const float alpha = *G.alpha;
-        if (G.d_dtype == T) store_wave_tile16<T, false, MI, kBigNJ>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
-        else if (G.accumulate) store_wave_tile16<NTFP8_F32, true, MI, kBigNJ>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
-        else store_wave_tile16<NTFP8_F32, false, MI, kBigNJ>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+        if (G.d_dtype == T) store_tile<T, false, MI>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+        else if (G.accumulate) store_tile<NTFP8_F32, true, MI>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+        else store_tile<NTFP8_F32, false, MI>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
     }
 }
 
