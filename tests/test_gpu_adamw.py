@@ -198,6 +198,31 @@ def test_many_tensors_in_one_call():
         near(d[0], want[0], bound[0], "param")
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_than_the_memory_side_cache(bits):
+    """Steps that move over 256 MB take another path to memory: 24 million elements beside an odd few."""
+    hyper = dict(HYPER, step=4)
+    big = 24_000_003
+    for dtype, gdtype in ((torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16)):
+        data = [draw(n, dtype, gdtype, n) for n in (big, 77)]
+        if bits == 32:
+            old = [[t.clone() for t in d] for d in data]
+            adamw_step(*[list(c) for c in zip(*data)], **hyper)
+            for d, o in zip(data, old):
+                want, bound = exact(*o, **hyper)
+                for k, name in ((0, "param"), (2, "exp_avg"), (3, "exp_avg_sq")):
+                    near(d[k], want[(0, 0, 1, 2)[k]], bound[(0, 0, 1, 2)[k]], name)
+        else:
+            full = [(p, g, *packed(p.numel(), m, v.sqrt())) for p, g, m, v in data]
+            old = [(p.clone(), g, dequantize_moment(a, b), dequantize_moment(c, e)) for p, g, a, b, c, e in full]
+            adamw_8bit_step(*[list(c) for c in zip(*full)], seed=8, **hyper)
+            for d, o in zip(full, old):
+                want, bound = exact(o[0], o[1], o[2], o[3].double() ** 2, **hyper)
+                near(d[0], want[0], bound[0], "param")
+                check_codes(d[2], d[3], want[1], bound[1], False)
+                check_codes(d[4], d[5], want[2].sqrt(), 8 * U32 * want[2].sqrt(), True)
+
+
 def test_optimizer_follows_torch():
     """32-bit moments: the optimizer beside torch.optim.AdamW in 64 bits, over 20 steps; 8-bit moments stay near."""
     torch.manual_seed(0)
