@@ -64,14 +64,18 @@ __global__ __launch_bounds__(forward_block(TPR)) void layer_norm_forward_kernel(
         const int c = (t + k * TPR) * VE;
         raw[k] = load_piece<D, VE>(n.x, x0 + c, live && c < n.cols ? n.cols - c : 0);
     }
-    // (weight and bias are asked for before the row's sums are waited for)
+    // weight and bias are asked for before the row's sums are waited for, unless a row takes 1024 threads: held that long they
+    // leave registers for one block a CU only, 8192 rows of 16384 168 us instead of 117
+    constexpr bool kEarly = TPR < 1024;
     float w[VPT][VE], b[VPT][VE];
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {
+    auto affine = [&](int k) {
         const int c = (t + k * TPR) * VE, left = c < n.cols ? n.cols - c : 0;
         if (n.weight) unpack<W, VE>(load_piece<W, VE>(n.weight, c, left), w[k]);
         if (n.bias) unpack<W, VE>(load_piece<W, VE>(n.bias, c, left), b[k]);
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+        if constexpr (kEarly) affine(k);
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         unpack<D, VE>(raw[k], v[k]);
@@ -103,6 +107,7 @@ __global__ __launch_bounds__(forward_block(TPR)) void layer_norm_forward_kernel(
     for (int k = 0; k < VPT; ++k) {
         const int c = (t + k * TPR) * VE;
         if (c >= n.cols) continue;
+        if constexpr (!kEarly) affine(k);
         float y[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
@@ -272,7 +277,19 @@ __global__ __launch_bounds__(kSumColumns * kSumRuns) void column_sums_kernel(con
     }
 }
 
-// threads of a row and pieces a thread, by the row's length in 16-byte pieces
+// Threads of a row and pieces a thread, by the row's length in 16-byte pieces.  Forward: two pieces a thread, requested together
+template <typename F>
+int by_width_forward(int pieces, F&& f) {
+    using std::integral_constant;
+    if (pieces <= 64) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (pieces <= 128) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if (pieces <= 256) return f(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+    if (pieces <= 512) return f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    if (pieces <= 1024) return f(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+    if (pieces <= 2048) return f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+    return f(integral_constant<int, 1024>{}, integral_constant<int, kMostPieces>{});
+}
+// backward: one, whose sums for weight and bias take the registers
 template <typename F>
 int by_width(int pieces, F&& f) {
     using std::integral_constant;
@@ -309,7 +326,7 @@ int run_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t col
     Norm n = {x, nullptr, weight, bias, y, mean, rstd, nullptr, x_stride, 0, rows, (int)cols, eps};
     return with_dtype(x_dtype, [&](auto d) {
         return with_weight<decltype(d)::value>(w_dtype, [&](auto w) {
-            return by_width(pieces_of(x_dtype, cols), [&](auto tpr, auto vpt) {
+            return by_width_forward(pieces_of(x_dtype, cols), [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, kBlock = forward_block(TPR), kRows = kBlock / TPR;
                 layer_norm_forward_kernel<decltype(d)::value, decltype(w)::value, TPR, decltype(vpt)::value>
                     <<<(unsigned)((rows + kRows - 1) / kRows), kBlock, 0, st>>>(n);
