@@ -58,6 +58,32 @@ struct HeadGemm {
     float* label_logit;
 };
 
+// What a workgroup needs behind its K loop, read in front of it: a launch's arguments are in no cache, and one trip after
+// another to them and to what they point to, between the last product and the first store, was a quarter of a small product's time
+struct HeadOutput {
+    void* D;
+    int64_t ldd;
+    float2* stats;
+    const int64_t* labels;
+    float* label_logit;
+    float alpha;
+    int N, pieces, d_dtype, accumulate;
+};
+template <int EPI>
+__device__ __forceinline__ HeadOutput head_output(const HeadGemm& G) {
+    HeadOutput o = {G.D, G.ldd, G.stats, G.labels, G.label_logit, 1.0f, G.N, G.pieces, G.d_dtype, G.accumulate};
+    if constexpr (EPI == kLosses || EPI == kSoftmax) {
+        asm volatile("" ::"s"(o.D), "s"(o.ldd), "s"(o.stats), "s"(o.labels), "s"(o.label_logit), "s"(o.N), "s"(o.pieces));
+    } else if constexpr (EPI == kPartial) {
+        o.D = G.partial;
+        asm volatile("" ::"s"(o.D), "s"(o.N));
+    } else {
+        o.alpha = *G.alpha;
+        asm volatile("" ::"s"(o.D), "s"(o.N), "s"(o.d_dtype), "s"(o.accumulate) : "memory");
+    }
+    return o;
+}
+
 // LDS stages: what fits beside each other in 160 KB
 template <int MI>
 constexpr int head_stages() { return MI == 8 ? 2 : MI == 1 ? 4 : 3; }
@@ -178,7 +204,7 @@ constexpr float kLift = 15.0f;   // exponentials are kept in fp16 as 2^15 e, 1 a
 // logit (NaN if one is) and the sum of exponentials below it, both in base 2 and fp32; with kKeep the exponentials as well,
 // once rounded, which the gradient is later made of by one multiplication a row and piece.
 template <int MI, bool kKeep>
-__device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const HeadGemm& G, int M, int m_base, int n_base, int lane) {
+__device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const HeadOutput& G, int M, int m_base, int n_base, int lane) {
     if (n_base >= (int)G.ldd) return;   // uniform
     const int mrow = lane & 15, q = lane >> 4;
     const float none = -__builtin_inff();
@@ -194,6 +220,13 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
     }
     uint16_t* const D = static_cast<uint16_t*>(G.D);
     const int piece = n_base / kPieceCols;
+    // the label's column within this piece, -1 for none; all rows' are asked for at once
+    int64_t label[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) label[i] = m_base + 16 * i + mrow < M ? G.labels[m_base + 16 * i + mrow] : -1;
+    int rel[MI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i) rel[i] = label[i] >= n_base && label[i] < min(n_base + kPieceCols, G.N) ? (int)(label[i] - n_base) : -1;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         const int m = m_base + 16 * i + mrow;
@@ -203,18 +236,12 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, acc[i][j][e]);
         top = lanes_over_rows_max(top);
-        // the label's logit, where it is one of these columns
-        int rel = -1;
-        if (m < M) {
-            const int64_t label = G.labels[m];
-            if (label >= 0 && label < G.N) rel = (int)(label - n_base);
-        }
-        if (__any(rel >= 0 && rel < kPieceCols)) {
+        if (__any(rel[i] >= 0)) {   // the label's logit
 #pragma unroll
             for (int j = 0; j < kBigNJ; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (rel == 16 * j + 4 * q + e) G.label_logit[m] = acc[i][j][e];
+                    if (rel[i] == 16 * j + 4 * q + e) G.label_logit[m] = acc[i][j][e];
         }
         const float base = top == none ? 0.0f : top * kLog2e;
         const float lift = (kKeep ? kLift : 0.0f) - base;
@@ -243,6 +270,7 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
                 if (m < M && n < (int)G.ldd) store16_through(D + (int64_t)m * G.ldd + n, (v4i){(int)x0, (int)x1, (int)y0, (int)y1});
             }
         }
+        sched_fence();
     }
 }
 
@@ -252,7 +280,13 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
 template <int DT, bool kAcc, int MI>
 __device__ __forceinline__ void store_tile(const v4f (&acc)[MI][kBigNJ], void* D, float alpha, int M, int N, int m_base, int n_base, int lane) {
     if ((N & 7) == 0) {
-        store_wave_tile16<DT, kAcc, MI, kBigNJ>(acc, D, alpha, M, N, m_base, n_base, lane);
+        // (16 rows at a time: the compiler would have the values of all of them at once, and no registers for them)
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const v4f (&part)[1][kBigNJ] = reinterpret_cast<const v4f (&)[1][kBigNJ]>(acc[i]);
+            store_wave_tile16<DT, kAcc, 1, kBigNJ>(part, D, alpha, M, N, m_base + 16 * i, n_base, lane);
+            sched_fence();
+        }
         return;
     }
     const int mrow = lane & 15, q = lane >> 4;
@@ -275,6 +309,7 @@ __device__ __forceinline__ void store_tile(const v4f (&acc)[MI][kBigNJ], void* D
             }
             store_piece<DT, 4>(D, (int64_t)m * N + n, v, left);
         }
+        sched_fence();
     }
 }
 
@@ -285,7 +320,7 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
     __shared__ __attribute__((aligned(1024))) uint8_t sB[NS][kBigN * kBK];
     int M = G.M, K = G.K, b_rows = G.b_rows, tiles_m = G.tiles_m;
     if (G.rows) {   // uniform
-        const int live = max(0, *G.rows - G.row0);
+        const int live = __builtin_amdgcn_readfirstlane(max(0, *G.rows - G.row0));   // (loaded by vector: sizes, tiles and descriptors are scalars)
         if constexpr (kAT) {
             K = min(K, live);
             b_rows = min(b_rows, live);
@@ -337,6 +372,7 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
         for (int l = 0; l < b.kLoads; ++l) b.load(r1, sB[s], l, kt, wave);
     };
 
+    const HeadOutput out = head_output<EPI>(G);
     v4f acc[MI][kBigNJ];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
@@ -447,14 +483,13 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the empty tiles too: nothing may land in LDS behind the workgroup)
 
     if constexpr (EPI == kLosses || EPI == kSoftmax) {
-        softmax_epilogue<MI, EPI == kSoftmax>(acc, G, M, m0 + wm, n0 + wn, lane);
+        softmax_epilogue<MI, EPI == kSoftmax>(acc, out, M, m0 + wm, n0 + wn, lane);
     } else if constexpr (EPI == kPartial) {
-        store_tile<NTFP8_F32, false, MI>(acc, G.partial + (int64_t)split * G.M * G.N, 1.0f, M, G.N, m0 + wm, n0 + wn, lane);
+        store_tile<NTFP8_F32, false, MI>(acc, static_cast<float*>(out.D) + (int64_t)split * G.M * out.N, 1.0f, M, out.N, m0 + wm, n0 + wn, lane);
     } else {
-        const float alpha = *G.alpha;
-        if (G.d_dtype == T) store_tile<T, false, MI>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
-        else if (G.accumulate) store_tile<NTFP8_F32, true, MI>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
-        else store_tile<NTFP8_F32, false, MI>(acc, G.D, alpha, M, G.N, m0 + wm, n0 + wn, lane);
+        if (out.d_dtype == T) store_tile<T, false, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
+        else if (out.accumulate) store_tile<NTFP8_F32, true, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
+        else store_tile<NTFP8_F32, false, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
     }
 }
 

@@ -94,6 +94,13 @@ def test_sum_and_large_vocabulary(dtype):
     check(*draw(70, 128, 50001, dtype, 0.3, 5), reduction="sum")
 
 
+@pytest.mark.parametrize("tokens,hidden,vocab", [(700, 136, 40000), (520, 512, 30001), (1100, 64, 25000), (300, 1000, 52001)])
+def test_large_tiles(tokens, hidden, vocab):
+    """Sizes whose products are made of 256-row tiles, several to a workgroup: one K-tile and many, and K-tiles that end inside."""
+    check(*draw(tokens, hidden, vocab, torch.bfloat16, 0.2, 8))
+    check(*draw(tokens, hidden, vocab, torch.float16, 0.0, 9))
+
+
 def test_long_batch():
     check(*draw(2500, 256, 1501, torch.bfloat16, 0.1, 6))
 
