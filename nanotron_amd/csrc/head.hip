@@ -298,9 +298,10 @@ int64_t piece_of(int64_t vocab) { return std::max<int64_t>(256, kMostHeld / (2 *
 Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     Plan p = {};
     const bool gradient = d.dx || d.dweight;
-    p.piece = gradient ? std::min(d.tokens, piece_of(d.vocab)) : d.tokens;
     p.ldd = held_cols(d.vocab);
     p.pieces = (p.ldd + kPieceCols - 1) / kPieceCols;
+    // (without gradients nothing is held but 8 bytes for 128 logits)
+    p.piece = std::min(d.tokens, gradient ? piece_of(d.vocab) : std::max<int64_t>(256, kMostHeld / (8 * p.pieces) / 256 * 256));
     p.padded = up(d.hidden, 8);
     // (with gradients the tokens that count are gathered: those that are ignored cost nothing, and what is in them, NaN say, is
     // seen by nobody)

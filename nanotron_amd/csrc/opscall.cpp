@@ -40,6 +40,10 @@ void same_device(const Tensor& t, const Tensor& x, const char* name) {
     TORCH_CHECK_VALUE(t.device() == x.device(), name, " must be on ", x.device(), ", got ", t.device());
 }
 
+// The operators here are differentiable once, and in reverse: what asks for more is told so instead of given zeros
+void once(const char* name) { TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its backward pass cannot be recorded (create_graph)"); }
+void no_tangent(const Tensor& t, const char* name) { TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), name, " has no forward-mode derivative"); }
+
 // x as rows of its last dimension that a kernel can walk with one stride
 struct Rows {
     Tensor t;
@@ -92,6 +96,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return n.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("layer_norm");
         const variable_list s = ctx->get_saved_variables();
         const Variable &x = s[0], &w = s[1], &b = s[2];
         Guard guard(x.device());
@@ -136,6 +141,7 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     }
     TORCH_CHECK_TYPE(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias must have one type");
     TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
+    for (const Tensor* t : {&x, &w, &b}) no_tangent(*t, "layer_norm");
     const bool gx = x.requires_grad(), gw = w.defined() && w.requires_grad(), gb = b.defined() && b.requires_grad();
     if (at::GradMode::is_enabled() && (gx || gw || gb)) return LayerNorm::apply(x, weight, bias, eps, gx, gw, gb);
     Guard guard(x.device());
@@ -201,6 +207,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         return h.loss;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("linear_cross_entropy");
         TORCH_CHECK(ctx->saved_data.count("type"),
                     "linear_cross_entropy: its gradients are handed over once and not kept; compute the loss again for another backward pass");
         Tensor dx, dw;
@@ -232,6 +239,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& labe
     TORCH_CHECK_VALUE(mean || none || reduction == "sum", "reduction must be 'mean', 'sum' or 'none', got '", reduction, "'");
     const bool gx = x.requires_grad(), gw = w.requires_grad(), wants = at::GradMode::is_enabled() && (gx || gw);
     TORCH_CHECK_VALUE(!(none && wants), "reduction='none' gives the losses of single tokens without gradients: call it under torch.no_grad()");
+    for (const Tensor* t : {&x, &w}) no_tangent(*t, "linear_cross_entropy");
     if (x.numel() == 0) {   // no tokens: a loss of 0 without gradient
         const auto f32 = x.options().dtype(at::kFloat);
         return none ? at::zeros(labels.sizes(), f32) : (x.sum() + w.sum()).to(at::kFloat).mul(0);

@@ -53,11 +53,12 @@ class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update in few launches; `state_bits` 32 or 8 chooses the moments (`adamw_step`,
     `adamw_8bit_step`).
 
-    A parameter without `.grad` but with a `main_grad` (what an FP8Linear with a 16-bit master accumulates in fp32) is
-    stepped by that.  `grad_scale` of step() multiplies all gradients (a clipping factor left on the device).  Where a
-    parameter is an fp32 master, `copies` of add_param_group / the constructor's group dicts (a list beside `params`) names the
-    16-bit tensors that take its new values.  Every parameter counts its own steps.  `seed` shifts the stochastic
-    rounding of 8-bit moments.  State dicts hold the moments as they are."""
+    Where a parameter is an fp32 master, `copies` in its group (a list beside `params`, None for a parameter without) names
+    the 16-bit tensors of the model that take its new values.  A parameter is stepped by its `.grad`, or else its `main_grad`
+    (what an FP8Linear with a 16-bit master leaves in fp32), or else the `.grad` of its copy (`grad_of`); zero_grad() clears
+    all three.  `grad_scale` of step() multiplies all gradients (a clipping factor left on the device).  Every parameter
+    counts its own steps.  `seed` shifts the stochastic rounding of 8-bit moments.  State dicts hold the moments as they are,
+    and no copies."""
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0):
@@ -72,6 +73,33 @@ class AdamW(torch.optim.Optimizer):
         group = self.param_groups[-1]
         if group.get("copies") is not None and len(group["copies"]) != len(group["params"]):
             raise ValueError(f"copies must name one tensor (or None) for each of {len(group['params'])} parameters, got {len(group['copies'])}")
+
+    @staticmethod
+    def grad_of(param: torch.Tensor, copy: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+        """The gradient that a parameter is stepped by, None if it has none."""
+        for grad in (param.grad, getattr(param, "main_grad", None), None if copy is None else copy.grad):
+            if grad is not None:
+                return grad
+        return None
+
+    def params_and_copies(self):
+        """(parameter, copy or None) of all groups."""
+        for group in self.param_groups:
+            yield from zip(group["params"], group["copies"] or [None] * len(group["params"]))
+
+    def zero_grad(self, set_to_none: bool = True) -> None:
+        super().zero_grad(set_to_none)
+        for p, copy in self.params_and_copies():
+            if getattr(p, "main_grad", None) is not None:
+                if set_to_none:
+                    p.main_grad = None
+                else:
+                    p.main_grad.zero_()
+            if copy is not None and copy.grad is not None:
+                if set_to_none:
+                    copy.grad = None
+                else:
+                    copy.grad.zero_()
 
     def state_dict(self) -> dict:
         # (the copies are other people's tensors)
@@ -100,8 +128,8 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             # parameters that have taken the same number of steps share launches; so do those of one device
             runs: dict = {}
-            for i, p in enumerate(group["params"]):
-                grad = p.grad if p.grad is not None else getattr(p, "main_grad", None)
+            for p, copy in zip(group["params"], group["copies"] or [None] * len(group["params"])):
+                grad = self.grad_of(p, copy)
                 if grad is None:
                     continue
                 if grad.is_sparse:
@@ -115,7 +143,6 @@ class AdamW(torch.optim.Optimizer):
                         state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                         state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 state["step"] += 1
-                copy = group["copies"][i] if group["copies"] is not None else None
                 runs.setdefault((state["step"], p.device), []).append((_plain(p), _plain(grad).contiguous(), state, copy))
             for (step, _), run in runs.items():
                 params, grads, states, copies = zip(*run)

@@ -232,3 +232,12 @@ def test_refusals():
             layer_norm(*bad)
     with pytest.raises(RuntimeError, match="not supported"):
         layer_norm(torch.zeros(1, 40000, device=DEV, dtype=torch.bfloat16))
+
+
+def test_differentiable_once():
+    x = torch.randn(4, 64, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(layer_norm(x).sum(), x, create_graph=True)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            layer_norm(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)))

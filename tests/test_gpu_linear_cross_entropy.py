@@ -317,3 +317,25 @@ def test_refusals():
                             ((x, w, labels), dict(reduction="max"), ValueError), ((x.requires_grad_(True), w, labels), dict(reduction="none"), ValueError)):
         with pytest.raises(error):
             linear_cross_entropy(*args, **kw)
+
+
+def test_differentiable_once():
+    x, w, labels = draw(10, 64, 100, torch.bfloat16)
+    x.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(linear_cross_entropy(x, w, labels), x, create_graph=True)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            linear_cross_entropy(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)), w, labels)
+
+
+def test_losses_in_pieces():
+    """Losses alone, of more tokens than are taken at a time."""
+    vocab = 1 << 21
+    tokens = (1 << 31) // (8 * (vocab // 128)) + 300
+    x, w, labels = draw(tokens, 8, vocab, torch.bfloat16, 0.1, 19)
+    got = linear_cross_entropy(x, w, labels, reduction="none")
+    for r in (0, 5000, tokens - 301, tokens - 40):
+        part = slice(r, r + 40)
+        want, bound = exact(x[part], w, labels[part])
+        near(got[part], want[0], bound[0], "losses")
