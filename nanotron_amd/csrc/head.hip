@@ -248,7 +248,7 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
 // transposed operand a K-tile takes a tenth more.)
 float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed) {
     const int at = mi == 1 ? 0 : mi == 2 ? 1 : mi == 4 ? 2 : 3;
-    constexpr float kTile[4] = {0.55f, 0.72f, 1.0f, 1.4f}, kRest[4] = {4.0f, 5.0f, 8.0f, 12.0f};
+    constexpr float kTile[4] = {0.48f, 0.62f, 0.72f, 1.37f}, kRest[4] = {4.0f, 5.0f, 6.0f, 9.0f};
     return (float)((tiles + 255) / 256) * ((float)kts * kTile[at] * (transposed ? 1.1f : 1.0f) + kRest[at]);
 }
 int64_t tiles_of(int64_t rows, int64_t cols, int mi) { return (rows + 32 * mi - 1) / (32 * mi) * ((cols + kBigN - 1) / kBigN); }
@@ -257,8 +257,8 @@ int64_t tiles_of(int64_t rows, int64_t cols, int mi) { return (rows + 32 * mi - 
 struct Tiling {
     int mi, splits, kt_split;
 };
-// logits: 333 tokens against 6001 rows of 512, us with 256 / 128 / 64 / 32 rows a tile: 25.4, 18.0, 12.5, 16.3; 512 tokens, 32000 rows of 2048: 57.6,
-// 81.6, 107.7, 167.9
+// logits: 333 tokens against 6001 rows of 512, us with 256 / 128 / 64 / 32 rows a tile: 21.4, 13.6, 11.6, 16.2; 512 tokens, 32000 rows of 2048: 53.3,
+// 58.8, 99.6, 156.9
 Tiling tiling_of_logits(int64_t rows, int64_t cols, int64_t kts) {
     Tiling best = {8, 1, 0};
     float least = 1e30f;

@@ -451,6 +451,99 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
             fa[MI - 1][1] = ra.read(sA[s ^ 1], MI - 1, 1);
             sched_fence();
         }
+    } else if constexpr (MI == 4) {
+        // Half tiles: the schedule of the fp8 GEMM's, three stages and one barrier a K-tile.  front: groups 0-5, the B fragments
+        // read three groups ahead; the barrier behind it releases this K-tile's stage and publishes the next one.  back: groups
+        // 6 and 7, whose A fragments are refilled from the next K-tile.  The loads of the K-tile after next but one go into the
+        // released stage, a third during back, the others during the next front.
+        constexpr int kBackLoads = NL / 3, kFrontLoads = NL - kBackLoads, kSlots = 5 * (MI / 2);
+        const int n = kt1 - kt0;
+        v4i fa[MI][2], fb[4][2];
+        __amdgpu_buffer_rsrc_t r0, r1;
+        int coming = 0, to = 0;   // the K-tile being loaded, and its stage
+        auto ready = [&](int f) {
+            if (kt0 + f == kt_all - 1) poison();
+            coming = kt0 + f;
+            to = f % NS;
+            r0 = a.at(kt0 + f, f < n);
+            r1 = b.at(kt0 + f, f < n);
+        };
+        auto load = [&](int l) {
+            if (l < a.kLoads) a.load(r0, sA[to], l, coming, wave);
+            else b.load(r1, sB[to], l - a.kLoads, coming, wave);
+        };
+#pragma unroll
+        for (int f = 0; f < NS; ++f) {
+            ready(f);
+#pragma unroll
+            for (int l = 0; l < NL; ++l) load(l);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+        wg_barrier();
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            fa[i][0] = ra.read(sA[0], i, 0);
+            fa[i][1] = ra.read(sA[0], i, 1);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) fb[h >> 1][h & 1] = rb.read(sB[0], h >> 1, h & 1);
+        auto front = [&](auto loads_tag, int s) __attribute__((always_inline)) {
+            constexpr bool loads = decltype(loads_tag)::value;
+            sched_fence();
+#pragma unroll
+            for (int j = 0; j < 6; ++j) {
+#pragma unroll
+                for (int x = 0; x < MI; ++x) {   // two MFMAs each, neither on the accumulator of the one before
+                    const int h = x / (MI / 2), i = x % (MI / 2) * 2;
+                    acc[i][j] = mfma_16x16x32<T>(fb[j & 3][h], fa[i][h], acc[i][j]);
+                    acc[i + 1][j] = mfma_16x16x32<T>(fb[j & 3][h], fa[i + 1][h], acc[i + 1][j]);
+                    // B fragment j + 3 (behind group 0 fragments 2 and 3), so that none is on its way at the barrier
+                    if (x < 2 && j < 5) fb[(j + (j ? 3 : 2)) & 3][x] = rb.read(sB[s], j + (j ? 3 : 2), x);
+                    else if (j == 0) fb[3][x - 2] = rb.read(sB[s], 3, x - 2);
+                    if (loads && j > 0 && x >= 2) {
+                        const int y = (j - 1) * (MI - 2) + x - 2;
+#pragma unroll
+                        for (int l = kBackLoads + y * kFrontLoads / kSlots; l < kBackLoads + (y + 1) * kFrontLoads / kSlots; ++l) load(l);
+                    }
+                    sched_fence();
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");   // all but the newest K-tile
+            wg_barrier();
+        };
+        auto back = [&](int next) __attribute__((always_inline)) {   // next: stage of the K-tile behind this one
+            sched_fence();
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                acc[i][6] = mfma_16x16x32<T>(fb[2][0], fa[i][0], acc[i][6]);
+                acc[i][7] = mfma_16x16x32<T>(fb[3][0], fa[i][0], acc[i][7]);
+                if (i > 0) {
+                    fa[i - 1][0] = ra.read(sA[next], i - 1, 0);
+                    fa[i - 1][1] = ra.read(sA[next], i - 1, 1);
+                }
+                sched_fence();
+                acc[i][6] = mfma_16x16x32<T>(fb[2][1], fa[i][1], acc[i][6]);
+                acc[i][7] = mfma_16x16x32<T>(fb[3][1], fa[i][1], acc[i][7]);
+#pragma unroll
+                for (int l = i * kBackLoads / MI; l < (i + 1) * kBackLoads / MI; ++l) load(l);
+                fb[i >> 1][i & 1] = rb.read(sB[next], i >> 1, i & 1);
+                sched_fence();
+            }
+            fa[MI - 1][0] = ra.read(sA[next], MI - 1, 0);
+            fa[MI - 1][1] = ra.read(sA[next], MI - 1, 1);
+            sched_fence();
+        };
+        front(std::false_type{}, 0);   // (K-tile 3 goes into the stage that it still reads)
+        int s = 0;
+        for (int f = 1; f < n; ++f) {
+            const int next = s == NS - 1 ? 0 : s + 1;
+            ready(f + 2);
+            back(next);
+            front(std::true_type{}, next);
+            s = next;
+        }
+        back(s == NS - 1 ? 0 : s + 1);   // (loads nothing more: the last of them are those of an empty K-tile again)
     } else {
 #pragma unroll
         for (int l = 0; l < NS - 1; ++l) {
