@@ -61,24 +61,29 @@ Rows rows_of(const Tensor& x) {
     return r;
 }
 
+// row `i` of a dense 2-D tensor
+Tensor row_of(const Tensor& t, int64_t i) {
+    Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(t.storage()), t.key_set(), t.dtype());
+    const int64_t size = t.size(1), stride = 1;
+    v.unsafeGetTensorImpl()->set_sizes_and_strides(size, stride, t.storage_offset() + i * size);
+    return v;
+}
+
 // ---------------------------------------------------------------------------------------------- layer norm
 struct Norm {
-    Tensor y, mean, rstd;
+    Tensor y, stats;   // stats: the rows' means and, behind them, their 1 / root of the variance
     Rows x;
 };
 Norm norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool keep) {
-    Norm n{Tensor(), Tensor(), Tensor(), rows_of(x)};
+    Norm n{Tensor(), Tensor(), rows_of(x)};
     n.y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
-    if (keep) {
-        const Tensor both = at::empty({2, n.x.rows}, x.options().dtype(at::kFloat));
-        n.mean = both.select(0, 0);
-        n.rstd = both.select(0, 1);
-    }
+    if (keep) n.stats = at::empty({2, n.x.rows}, x.options().dtype(at::kFloat));
     if (x.numel() == 0) return n;
     const Tensor wd = w.defined() ? w.contiguous() : w, bd = b.defined() ? b.contiguous() : b;
     const int xd = code_of(x, "x"), wc = w.defined() ? code_of(w, "weight") : b.defined() ? code_of(b, "bias") : xd;
+    float* const mean = static_cast<float*>(at_or_null(n.stats));
     call(ntops_layer_norm_forward(n.x.t.data_ptr(), xd, n.x.rows, n.x.cols, n.x.stride, at_or_null(wd), at_or_null(bd), wc, (float)eps, n.y.data_ptr(),
-                                  static_cast<float*>(at_or_null(n.mean)), static_cast<float*>(at_or_null(n.rstd)), stream_of(x)),
+                                  mean, mean ? mean + n.x.rows : nullptr, stream_of(x)),
          "ntops_layer_norm_forward");
     return n;
 }
@@ -92,7 +97,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         ctx->saved_data["want"] = (int64_t)(gx | gw << 1 | gb << 2);
         Norm n = norm_forward(x, w, b, eps, true);
         // (a non-dense x is saved as the dense rows that were made of it: one copy serves both passes)
-        ctx->save_for_backward({n.x.t.is_same(x) ? x : n.x.t, w, b, n.mean, n.rstd});
+        ctx->save_for_backward({n.x.t.is_same(x) ? x : n.x.t, w, b, n.stats});
         return n.y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -114,13 +119,20 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         }
         const Rows xr = rows_of(x), gr = rows_of(grads[0].scalar_type() == x.scalar_type() ? grads[0] : grads[0].to(x.scalar_type()));
         const int xd = code_of(x, "x"), wc = w.defined() ? code_of(w, "weight") : b.defined() ? code_of(b, "bias") : xd;
-        if (gw) dw = at::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
-        if (gb) db = at::empty(b.sizes(), b.options().memory_format(at::MemoryFormat::Contiguous));
+        if (gw && gb) {   // (one type: one allocation, and two views of it without a dispatch each)
+            const Tensor both = at::empty({2, xr.cols}, w.options().memory_format(at::MemoryFormat::Contiguous));
+            dw = row_of(both, 0);
+            db = row_of(both, 1);
+        } else if (gw) {
+            dw = at::empty(w.sizes(), w.options().memory_format(at::MemoryFormat::Contiguous));
+        } else if (gb) {
+            db = at::empty(b.sizes(), b.options().memory_format(at::MemoryFormat::Contiguous));
+        }
         Tensor scratch;
         if (gw || gb) scratch = at::empty({ntops_layer_norm_scratch(xd, xr.rows, xr.cols)}, x.options().dtype(at::kByte));
         const Tensor wd = w.defined() ? w.contiguous() : w;
         call(ntops_layer_norm_backward(gr.t.data_ptr(), gr.stride, xr.t.data_ptr(), xd, xr.rows, xr.cols, xr.stride, at_or_null(wd), wc, s[3].const_data_ptr<float>(),
-                                       s[4].const_data_ptr<float>(), at_or_null(dx), at_or_null(dw), at_or_null(db), at_or_null(scratch), stream_of(x)),
+                                       s[3].const_data_ptr<float>() + xr.rows, at_or_null(dx), at_or_null(dw), at_or_null(db), at_or_null(scratch), stream_of(x)),
              "ntops_layer_norm_backward");
         return given();
     }
@@ -167,15 +179,19 @@ Head head(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore
     const bool wide = xd == NTFP8_F16 || (gw && d.tokens > ntops_linear_cross_entropy_piece(d.vocab));
     d.grad_dtype = wide ? NTFP8_F32 : xd;
     Head h;
-    h.losses = at::empty({xr.rows}, f32);
+    const bool gradient = gx || gw;
+    if (!gradient) h.losses = at::empty({xr.rows}, f32);
     h.loss = at::empty({}, f32);
     const auto go = wide ? f32 : x.options().memory_format(at::MemoryFormat::Contiguous);
     if (gx) h.dx = at::empty(x.sizes(), go);
     if (gw) h.dw = at::empty(w.sizes(), go);
-    d.losses = h.losses.data_ptr<float>(), d.loss = h.loss.data_ptr<float>(), d.dx = at_or_null(h.dx), d.dweight = at_or_null(h.dw);
-    const int64_t bytes = ntops_linear_cross_entropy_workspace(&d);
-    const Tensor ws = at::empty({bytes + 256}, x.options().dtype(at::kByte));
-    d.workspace = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws.data_ptr()) + 255) / 256 * 256);
+    d.loss = h.loss.data_ptr<float>(), d.dx = at_or_null(h.dx), d.dweight = at_or_null(h.dw);
+    // (with gradients the tokens' losses are nobody's: they lie behind the workspace)
+    const int64_t bytes = (ntops_linear_cross_entropy_workspace(&d) + 255) / 256 * 256;
+    const Tensor ws = at::empty({256 + bytes + (gradient ? 4 * xr.rows : 0)}, x.options().dtype(at::kByte));
+    char* const at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws.data_ptr()) + 255) / 256 * 256);
+    d.workspace = at;
+    d.losses = gradient ? reinterpret_cast<float*>(at + bytes) : h.losses.data_ptr<float>();
     call(ntops_linear_cross_entropy(&d, stream_of(x)), "ntops_linear_cross_entropy");
     return h;
 }
