@@ -227,10 +227,11 @@ __global__ __launch_bounds__(1024) void scale_kernel(const Scaled t, const float
 
 template <int T, bool kAT, bool kBT, int EPI>
 int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
-    g.tiles_m = (int)((g.M + 32 * (int64_t)mi - 1) / (32 * mi));
     g.tiles_n = (int)(((EPI == kLosses || EPI == kSoftmax ? g.ldd : g.N) + kBigN - 1) / kBigN);
     g.magic = magic_of((uint32_t)(kGroupM * g.tiles_n));
-    const unsigned blocks = (unsigned)((int64_t)g.tiles_m * g.tiles_n * (EPI == kPartial ? g.splits : 1));
+    const int64_t tiles = (g.M + 32 * (int64_t)mi - 1) / (32 * mi) * g.tiles_n;
+    // (with 256-row tiles up to 128 more, for those of a last round that go in halves; how many is known to the device)
+    const unsigned blocks = (unsigned)(EPI == kPartial ? tiles * g.splits : mi == 8 ? tiles + 128 : tiles);
     if constexpr (kAT) {
         head_gemm_kernel<T, kAT, kBT, 8, EPI><<<blocks, kBigThreads, 0, st>>>(g);
     } else {
@@ -245,11 +246,13 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
 // What a launch of `tiles` workgroups takes, us, each of `kts` K-tiles of (32 mi) x 256 outputs: rounds of one workgroup a CU, a
 // K-tile's time and what a workgroup takes besides.  A K-tile of fewer rows takes more of their share, since the 256 columns
 // are the larger part of what it loads.  (Measured at 64 to 2048 tokens, 512 to 4096 hidden, vocabularies of 6 to 50 thousand; with a
-// transposed operand a K-tile takes a tenth more.)
-float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed) {
-    const int at = mi == 1 ? 0 : mi == 2 ? 1 : mi == 4 ? 2 : 3;
+// transposed operand a K-tile takes a tenth more.)  halves: a last round of up to 128 tiles of 256 rows goes in tiles of 128.
+float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed, bool halves) {
     constexpr float kTile[4] = {0.48f, 0.62f, 0.72f, 1.37f}, kRest[4] = {4.0f, 5.0f, 6.0f, 9.0f};
-    return (float)((tiles + 255) / 256) * ((float)kts * kTile[at] * (transposed ? 1.1f : 1.0f) + kRest[at]);
+    auto round = [&](int at) { return (float)kts * kTile[at] * (transposed ? 1.1f : 1.0f) + kRest[at]; };
+    const int at = mi == 1 ? 0 : mi == 2 ? 1 : mi == 4 ? 2 : 3;
+    const int64_t rest = tiles % 256;
+    return (float)(tiles / 256) * round(at) + (rest == 0 ? 0.0f : mi == 8 && halves && rest <= 128 ? round(2) : round(at));
 }
 int64_t tiles_of(int64_t rows, int64_t cols, int mi) { return (rows + 32 * mi - 1) / (32 * mi) * ((cols + kBigN - 1) / kBigN); }
 
@@ -263,7 +266,7 @@ Tiling tiling_of_logits(int64_t rows, int64_t cols, int64_t kts) {
     Tiling best = {8, 1, 0};
     float least = 1e30f;
     for (int mi = 8; mi >= 1; mi /= 2) {
-        const float us = launch_us(mi, tiles_of(rows, cols, mi), kts, false);
+        const float us = launch_us(mi, tiles_of(rows, cols, mi), kts, false, true);
         if (us < least) least = us, best.mi = mi;
     }
     return best;
@@ -277,7 +280,7 @@ Tiling tiling_of_dx(int64_t rows, int64_t cols, int64_t kts) {
         for (int64_t want = 1; want <= 64 && want <= std::max<int64_t>(1, kts / 4); ++want) {
             const int64_t each = (kts + want - 1) / want, splits = (kts + each - 1) / each;
             if (splits > 1 && tiles * splits > 1024) break;
-            float us = launch_us(mi, tiles * splits, each, true);
+            float us = launch_us(mi, tiles * splits, each, true, splits == 1);
             if (splits > 1) us += (float)(rows * cols) * (float)splits * 8.0f / 4.5e6f;
             if (us < least) least = us, best = {mi, (int)splits, (int)each};
         }

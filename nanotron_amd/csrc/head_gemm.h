@@ -43,7 +43,7 @@ struct HeadGemm {
     int row0;                    // ... of which this launch has those from row0 on: M is at most that many, K where A is transposed
     int a_cols, b_cols;          // columns of a row that may be read, a multiple of 8
     int b_rows;                  // rows of a transposed B (K or fewer; those behind count as zeros)
-    int tiles_m, tiles_n;
+    int tiles_n;
     uint32_t magic;              // magic_of(kGroupM tiles_n)
     int splits, kt_split;        // runs of K, and K-tiles of each
     void* D;
@@ -92,7 +92,7 @@ constexpr int head_stages() { return MI == 8 ? 2 : MI == 1 ? 4 : 3; }
 template <bool kT, int kRows>
 struct HeadOperand {
     static constexpr int kLoads = kRows * kBK / 1024 / kBigWaves;   // 1 KB wave-level loads per wave
-    static_assert(!kT || kRows == 256, "a transposed operand is 256 columns wide");
+    static_assert(!kT || kRows == 256 || kRows == 128, "");
     const char* base;
     int64_t step;        // bytes from K-tile to K-tile
     int64_t row_bytes;
@@ -108,11 +108,12 @@ struct HeadOperand {
             rows = k_rows;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                // 2 rows of k a wave-level load, 32 chunks of 16 bytes each; 32-byte piece c of row k is stored at piece
-                // c ^ ((k mod 4) | 4 (k / 16 mod 2)): the 4 rows that one transposing read of 16 lanes touches, and the two
-                // groups of 16 lanes that go through LDS together, then use different banks
-                const int k = (wave + kBigWaves * i) * 2 + (lane >> 5);
-                const int piece = ((lane & 31) >> 1) ^ ((k & 3) | (((k >> 4) & 1) << 2));
+                // 2 rows of k a wave-level load (4 of a 128-column operand), in chunks of 16 bytes; 32-byte piece c of row k is
+                // stored at piece c ^ ((k mod 4) | 4 (k / 16 mod 2)): the 4 rows that one transposing read of 16 lanes touches, and
+                // the two groups of 16 lanes that go through LDS together, then use different banks
+                constexpr int kChunks = kRows / 8;
+                const int k = (wave + kBigWaves * i) * (64 / kChunks) + lane / kChunks;
+                const int piece = (lane % kChunks >> 1) ^ ((k & 3) | (((k >> 4) & 1) << 2));
                 off[i] = (uint32_t)k * (uint32_t)row_bytes + (uint32_t)first * 2u + (uint32_t)(piece * 32 + (lane & 1) * 16);
             }
         } else {
@@ -147,16 +148,18 @@ struct HeadOperand {
 
 // Fragment reads.  Plain: block i is 16 rows, 2048 bytes, further on.  Transposed: lane u of a group of 16 (k 16 g .. + 15) addresses
 // row k0 + u / 4, columns 4 (u mod 4) .. + 3 of the block's 32-byte piece, and receives rows k0 .. k0 + 3 of column u.
-template <bool kT>
+template <bool kT, int kCols>
 struct HeadFragment {
+    static constexpr int kPitch = 2 * kCols;   // bytes of a row of k of a transposed operand
     int at[2];
     int turn;
     __device__ __forceinline__ void init(int first, int lane) {   // first: row (column) of the wave's block 0 within the tile
         const int g = lane >> 4, u = lane & 15;
         if constexpr (kT) {
-            at[0] = (16 * g + (u >> 2)) * 512 + (first >> 7) * 256 + (u & 3) * 8;
+            // (a wave's blocks are pieces 0 .. 7 or 8 .. 15 of 16, or 0 .. 3 or 4 .. 7 of 8: the swizzle reaches over 8)
+            at[0] = (16 * g + (u >> 2)) * kPitch + (first >> 7) * 256 + (u & 3) * 8;
             at[1] = at[0];
-            turn = ((u >> 2) | ((g & 1) << 2)) << 5;
+            turn = (((u >> 2) | ((g & 1) << 2)) << 5) ^ (first << 1 & 128);
         } else {
             at[0] = lds_off16(first + u, 2 * g);
             at[1] = lds_off16(first + u, 2 * g + 1);
@@ -173,8 +176,8 @@ struct HeadFragment {
             // waits for every direct-to-LDS load in flight before the read)
             int off = at[0] + ((i << 5) ^ turn);
             asm("" : "+v"(off));
-            const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[off + h * (8 * 512)]));
-            const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[off + h * (8 * 512) + 4 * 512]));
+            const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[off + h * (8 * kPitch)]));
+            const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[off + h * (8 * kPitch) + 4 * kPitch]));
             return (v4i){lo.x, lo.y, hi.x, hi.y};
         } else {
             return *reinterpret_cast<const v4i*>(stage + at[h] + i * 2048);
@@ -313,45 +316,40 @@ __device__ __forceinline__ void store_tile(const v4f (&acc)[MI][kBigNJ], void* D
     }
 }
 
-template <int T, bool kAT, bool kBT, int MI, int EPI>
-__global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G) {
-    constexpr int NS = head_stages<MI>();
-    __shared__ __attribute__((aligned(1024))) uint8_t sA[NS][32 * MI * kBK];
-    __shared__ __attribute__((aligned(1024))) uint8_t sB[NS][kBigN * kBK];
-    int M = G.M, K = G.K, b_rows = G.b_rows, tiles_m = G.tiles_m;
+// What the launch's arguments say of sizes, or less of them where the device knows better
+struct HeadSizes {
+    int M, K, b_rows;
+};
+template <bool kAT>
+__device__ __forceinline__ HeadSizes head_sizes(const HeadGemm& G) {
+    HeadSizes z = {G.M, G.K, G.b_rows};
     if (G.rows) {   // uniform
         const int live = __builtin_amdgcn_readfirstlane(max(0, *G.rows - G.row0));   // (loaded by vector: sizes, tiles and descriptors are scalars)
         if constexpr (kAT) {
-            K = min(K, live);
-            b_rows = min(b_rows, live);
-            if (G.accumulate && live == 0) return;
+            z.K = min(z.K, live);
+            z.b_rows = min(z.b_rows, live);
         } else {
-            M = min(M, live);
-            tiles_m = (M + 32 * MI - 1) / (32 * MI);
+            z.M = min(z.M, live);
         }
     }
-    // Within each round of 256 workgroups an XCD takes a contiguous run of the tiles
-    int pid = blockIdx.x;
-    const int tiles = tiles_m * G.tiles_n, total = tiles * (EPI == kPartial ? G.splits : 1), round0 = pid & ~255;
-    if (pid >= total) return;
-    pid = round0 + run_of_xcd(pid - round0, min(256, total - round0));
-    const int split = EPI == kPartial ? pid / tiles : 0;
-    int pid_m, pid_n;
-    tile_in_group(EPI == kPartial ? pid - split * tiles : pid, tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
-    const int m0 = pid_m * 32 * MI, n0 = pid_n * kBigN;
+    return z;
+}
+
+// The tile of 32 MI x 256 outputs at (m0, n0), K-tiles kt0 .. kt1 - 1 of kt_all.  sA, sB: the LDS stages.
+template <int T, bool kAT, bool kBT, int MI, int EPI>
+__device__ __forceinline__ void head_tile(const HeadGemm& G, const HeadSizes& z, int m0, int n0, int split, int kt0, int kt1, int kt_all, uint8_t* sA, uint8_t* sB) {
+    constexpr int NS = head_stages<MI>(), kStageA = 32 * MI * kBK, kStageB = kBigN * kBK;
+    const int M = z.M, K = z.K, b_rows = z.b_rows;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = (wave >> 1) * (MI * 16), wn = (wave & 1) * 128;
-    const int kt_all = (K + kHeadK - 1) / kHeadK;
-    const int kt0 = EPI == kPartial ? split * G.kt_split : 0;
-    const int kt1 = EPI == kPartial ? min(kt_all, kt0 + G.kt_split) : kt_all;
 
     HeadOperand<kAT, 32 * MI> a;
     HeadOperand<kBT, kBigN> b;
     a.init(G.A, G.lda, m0, M - m0, G.a_cols, K, wave, lane);
     b.init(G.B, G.ldb, n0, G.N - n0, G.b_cols, b_rows, wave, lane);
     constexpr int NL = HeadOperand<kAT, 32 * MI>::kLoads + HeadOperand<kBT, kBigN>::kLoads;
-    HeadFragment<kAT> ra;
-    HeadFragment<kBT> rb;
+    HeadFragment<kAT, 32 * MI> ra;
+    HeadFragment<kBT, kBigN> rb;
     ra.init(wm, lane);
     rb.init(wn, lane);
     // chunks of the last K-tile behind K read as zeros, not as the start of the next row
@@ -367,9 +365,9 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
         const int s = kt % NS;
         const __amdgpu_buffer_rsrc_t r0 = a.at(kt, live), r1 = b.at(kt, live);
 #pragma unroll
-        for (int l = 0; l < a.kLoads; ++l) a.load(r0, sA[s], l, kt, wave);
+        for (int l = 0; l < a.kLoads; ++l) a.load(r0, sA + (s) * kStageA, l, kt, wave);
 #pragma unroll
-        for (int l = 0; l < b.kLoads; ++l) b.load(r1, sB[s], l, kt, wave);
+        for (int l = 0; l < b.kLoads; ++l) b.load(r1, sB + (s) * kStageB, l, kt, wave);
     };
 
     const HeadOutput out = head_output<EPI>(G);
@@ -389,8 +387,8 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
         v4i fa[MI][2], fw[kBigNJ][2];
         __amdgpu_buffer_rsrc_t r0, r1;
         auto load = [&](int f, int l) {
-            if (l < a.kLoads) a.load(r0, sA[f & 1], l, kt0 + f, wave);
-            else b.load(r1, sB[f & 1], l - a.kLoads, kt0 + f, wave);
+            if (l < a.kLoads) a.load(r0, sA + (f & 1) * kStageA, l, kt0 + f, wave);
+            else b.load(r1, sB + (f & 1) * kStageB, l - a.kLoads, kt0 + f, wave);
         };
         auto ready = [&](int f) {   // for the loads of tile f
             if (kt0 + f == kt_all - 1) poison();
@@ -407,11 +405,11 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
         wg_barrier();
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            fa[i][0] = ra.read(sA[0], i, 0);
-            fa[i][1] = ra.read(sA[0], i, 1);
+            fa[i][0] = ra.read(sA + (0) * kStageA, i, 0);
+            fa[i][1] = ra.read(sA + (0) * kStageA, i, 1);
         }
 #pragma unroll
-        for (int h = 0; h < 4; ++h) fw[h >> 1][h & 1] = rb.read(sB[0], h >> 1, h & 1);
+        for (int h = 0; h < 4; ++h) fw[h >> 1][h & 1] = rb.read(sB + (0) * kStageB, h >> 1, h & 1);
         for (int f = 0; f < n; ++f) {
             const int s = f & 1;
             ready(f + 2);
@@ -421,7 +419,7 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
                 const int j = x / MI, h = x % MI / (MI / 2), i = x % (MI / 2) * 2;
                 acc[i][j] = mfma_16x16x32<T>(fw[j][h], fa[i][h], acc[i][j]);
                 acc[i + 1][j] = mfma_16x16x32<T>(fw[j][h], fa[i + 1][h], acc[i + 1][j]);
-                if (x < 24 && x % 2 == 0) fw[2 + x / 4][x / 2 % 2] = rb.read(sB[s], 2 + x / 4, x / 2 % 2);
+                if (x < 24 && x % 2 == 0) fw[2 + x / 4][x / 2 % 2] = rb.read(sB + (s) * kStageB, 2 + x / 4, x / 2 % 2);
                 if (x == kRelease) {
                     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // every fragment of tile f is in registers
                     wg_barrier();
@@ -436,19 +434,19 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
                 acc[i][6] = mfma_16x16x32<T>(fw[6][0], fa[i][0], acc[i][6]);
                 acc[i][7] = mfma_16x16x32<T>(fw[7][0], fa[i][0], acc[i][7]);
                 if (i > 0) {
-                    fa[i - 1][0] = ra.read(sA[s ^ 1], i - 1, 0);
-                    fa[i - 1][1] = ra.read(sA[s ^ 1], i - 1, 1);
+                    fa[i - 1][0] = ra.read(sA + (s ^ 1) * kStageA, i - 1, 0);
+                    fa[i - 1][1] = ra.read(sA + (s ^ 1) * kStageA, i - 1, 1);
                 }
                 sched_fence();
                 acc[i][6] = mfma_16x16x32<T>(fw[6][1], fa[i][1], acc[i][6]);
                 acc[i][7] = mfma_16x16x32<T>(fw[7][1], fa[i][1], acc[i][7]);
-                if (i < 4) fw[i >> 1][i & 1] = rb.read(sB[s ^ 1], i >> 1, i & 1);
+                if (i < 4) fw[i >> 1][i & 1] = rb.read(sB + (s ^ 1) * kStageB, i >> 1, i & 1);
 #pragma unroll
                 for (int l = kFront + i * (NL - kFront) / MI; l < kFront + (i + 1) * (NL - kFront) / MI; ++l) load(f + 2, l);
                 sched_fence();
             }
-            fa[MI - 1][0] = ra.read(sA[s ^ 1], MI - 1, 0);
-            fa[MI - 1][1] = ra.read(sA[s ^ 1], MI - 1, 1);
+            fa[MI - 1][0] = ra.read(sA + (s ^ 1) * kStageA, MI - 1, 0);
+            fa[MI - 1][1] = ra.read(sA + (s ^ 1) * kStageA, MI - 1, 1);
             sched_fence();
         }
     } else if constexpr (MI == 4) {
@@ -469,8 +467,8 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
             r1 = b.at(kt0 + f, f < n);
         };
         auto load = [&](int l) {
-            if (l < a.kLoads) a.load(r0, sA[to], l, coming, wave);
-            else b.load(r1, sB[to], l - a.kLoads, coming, wave);
+            if (l < a.kLoads) a.load(r0, sA + (to) * kStageA, l, coming, wave);
+            else b.load(r1, sB + (to) * kStageB, l - a.kLoads, coming, wave);
         };
 #pragma unroll
         for (int f = 0; f < NS; ++f) {
@@ -482,11 +480,11 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
         wg_barrier();
 #pragma unroll
         for (int i = 0; i < MI; ++i) {
-            fa[i][0] = ra.read(sA[0], i, 0);
-            fa[i][1] = ra.read(sA[0], i, 1);
+            fa[i][0] = ra.read(sA + (0) * kStageA, i, 0);
+            fa[i][1] = ra.read(sA + (0) * kStageA, i, 1);
         }
 #pragma unroll
-        for (int h = 0; h < 4; ++h) fb[h >> 1][h & 1] = rb.read(sB[0], h >> 1, h & 1);
+        for (int h = 0; h < 4; ++h) fb[h >> 1][h & 1] = rb.read(sB + (0) * kStageB, h >> 1, h & 1);
         auto front = [&](auto loads_tag, int s) __attribute__((always_inline)) {
             constexpr bool loads = decltype(loads_tag)::value;
             sched_fence();
@@ -498,8 +496,8 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
                     acc[i][j] = mfma_16x16x32<T>(fb[j & 3][h], fa[i][h], acc[i][j]);
                     acc[i + 1][j] = mfma_16x16x32<T>(fb[j & 3][h], fa[i + 1][h], acc[i + 1][j]);
                     // B fragment j + 3 (behind group 0 fragments 2 and 3), so that none is on its way at the barrier
-                    if (x < 2 && j < 5) fb[(j + (j ? 3 : 2)) & 3][x] = rb.read(sB[s], j + (j ? 3 : 2), x);
-                    else if (j == 0) fb[3][x - 2] = rb.read(sB[s], 3, x - 2);
+                    if (x < 2 && j < 5) fb[(j + (j ? 3 : 2)) & 3][x] = rb.read(sB + (s) * kStageB, j + (j ? 3 : 2), x);
+                    else if (j == 0) fb[3][x - 2] = rb.read(sB + (s) * kStageB, 3, x - 2);
                     if (loads && j > 0 && x >= 2) {
                         const int y = (j - 1) * (MI - 2) + x - 2;
 #pragma unroll
@@ -519,19 +517,19 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
                 acc[i][6] = mfma_16x16x32<T>(fb[2][0], fa[i][0], acc[i][6]);
                 acc[i][7] = mfma_16x16x32<T>(fb[3][0], fa[i][0], acc[i][7]);
                 if (i > 0) {
-                    fa[i - 1][0] = ra.read(sA[next], i - 1, 0);
-                    fa[i - 1][1] = ra.read(sA[next], i - 1, 1);
+                    fa[i - 1][0] = ra.read(sA + (next) * kStageA, i - 1, 0);
+                    fa[i - 1][1] = ra.read(sA + (next) * kStageA, i - 1, 1);
                 }
                 sched_fence();
                 acc[i][6] = mfma_16x16x32<T>(fb[2][1], fa[i][1], acc[i][6]);
                 acc[i][7] = mfma_16x16x32<T>(fb[3][1], fa[i][1], acc[i][7]);
 #pragma unroll
                 for (int l = i * kBackLoads / MI; l < (i + 1) * kBackLoads / MI; ++l) load(l);
-                fb[i >> 1][i & 1] = rb.read(sB[next], i >> 1, i & 1);
+                fb[i >> 1][i & 1] = rb.read(sB + (next) * kStageB, i >> 1, i & 1);
                 sched_fence();
             }
-            fa[MI - 1][0] = ra.read(sA[next], MI - 1, 0);
-            fa[MI - 1][1] = ra.read(sA[next], MI - 1, 1);
+            fa[MI - 1][0] = ra.read(sA + (next) * kStageA, MI - 1, 0);
+            fa[MI - 1][1] = ra.read(sA + (next) * kStageA, MI - 1, 1);
             sched_fence();
         };
         front(std::false_type{}, 0);   // (K-tile 3 goes into the stage that it still reads)
@@ -559,13 +557,13 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
             v4i fa[MI][2], fb[2];
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
-                fa[i][0] = ra.read(sA[s], i, 0);
-                fa[i][1] = ra.read(sA[s], i, 1);
+                fa[i][0] = ra.read(sA + (s) * kStageA, i, 0);
+                fa[i][1] = ra.read(sA + (s) * kStageA, i, 1);
             }
 #pragma unroll
             for (int j = 0; j < kBigNJ; ++j) {
-                fb[0] = rb.read(sB[s], j, 0);
-                fb[1] = rb.read(sB[s], j, 1);
+                fb[0] = rb.read(sB + (s) * kStageB, j, 0);
+                fb[1] = rb.read(sB + (s) * kStageB, j, 1);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -584,6 +582,42 @@ __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G
         else if (out.accumulate) store_tile<NTFP8_F32, true, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
         else store_tile<NTFP8_F32, false, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
     }
+}
+
+template <int T, bool kAT, bool kBT, int MI, int EPI>
+__global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G) {
+    // 256-row tiles that do not fill a last round (kTail): its tiles in halves of 128 rows, twice the workgroups for half as long.
+    // us, whole / so: weight gradients of 6001 x 515 from 333 tokens 18.3 / 13.1, of 50001 x 1024 from 766 101 / 95, of 128000 x 4096 from 4096 3404 / 3300
+    constexpr bool kTail = MI == 8 && EPI != kPartial;
+    constexpr int kBytesA = head_stages<MI>() * 32 * MI * kBK, kBytesB = head_stages<kTail ? 4 : MI>() * kBigN * kBK;
+    __shared__ __attribute__((aligned(1024))) uint8_t sA[kBytesA];
+    __shared__ __attribute__((aligned(1024))) uint8_t sB[kBytesB];
+    static_assert(!kTail || kBytesA >= head_stages<4>() * 128 * kBK, "half tiles use the same arrays");
+    const HeadSizes z = head_sizes<kAT>(G);
+    if (kAT && G.accumulate && z.K == 0) return;
+    const int tiles_m = (z.M + 32 * MI - 1) / (32 * MI), tiles = tiles_m * G.tiles_n, total = tiles * (EPI == kPartial ? G.splits : 1);
+    const int kt_all = (z.K + kHeadK - 1) / kHeadK;
+    int pid = blockIdx.x, pid_m, pid_n;
+    if constexpr (kTail) {
+        const int rest = total & 255, whole = rest > 128 ? total : total - rest;
+        if (pid >= whole) {
+            const int half = pid - whole;
+            if (rest > 128 || half >= 2 * rest) return;
+            const int at = run_of_xcd(half, 2 * rest);
+            tile_in_group(whole + (at >> 1), tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
+            const int m0 = pid_m * 256 + (at & 1) * 128;
+            if (m0 < z.M) head_tile<T, kAT, kBT, 4, EPI>(G, z, m0, pid_n * kBigN, 0, 0, kt_all, kt_all, sA, sB);
+            return;
+        }
+    }
+    // Within each round of 256 workgroups an XCD takes a contiguous run of the tiles
+    if (pid >= total) return;
+    const int round0 = pid & ~255;
+    pid = round0 + run_of_xcd(pid - round0, min(256, total - round0));
+    const int split = EPI == kPartial ? pid / tiles : 0;
+    tile_in_group(EPI == kPartial ? pid - split * tiles : pid, tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
+    const int kt0 = EPI == kPartial ? split * G.kt_split : 0;
+    head_tile<T, kAT, kBT, MI, EPI>(G, z, pid_m * 32 * MI, pid_n * kBigN, split, kt0, EPI == kPartial ? min(kt_all, kt0 + G.kt_split) : kt_all, kt_all, sA, sB);
 }
 
 }  // namespace ntfp8
