@@ -356,9 +356,14 @@ void adamw(const py::object& params_, const py::object& grads_, const py::object
         o.param_dtype = k.p, o.grad_dtype = k.g, o.copy_dtype = k.c;
         call(ntops_adamw(k.t.data(), (int)k.t.size(), &o, stream_of(p0)), "ntops_adamw");
     }
-    // (autograd's record of in-place changes: a graph that saved a parameter finds out)
-    for (size_t i = 0; i < n; ++i)
-        if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
+    // (autograd's record of in-place changes: a graph that saved a parameter or its copy finds out)
+    const auto changed = [](const Tensor& t) {
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    };
+    for (size_t i = 0; i < n; ++i) {
+        changed(params[i]);
+        if (copies.given() && !copies.none(i)) changed(copies[i]);
+    }
 }
 
 Tensor adamw_unpack(const Tensor& codes, const Tensor& scale) {

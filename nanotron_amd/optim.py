@@ -16,7 +16,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
     params and grads: float32, float16 or bfloat16, in any mixture; exp_avgs and exp_avg_sqs: float32.  All contiguous and
     on one device.  Arithmetic is fp32; a 16-bit parameter is rounded to nearest once a step.  grad_scale (one float32 on the
-    device: a clipping factor, the inverse of a loss scale) multiplies every gradient.  copies: for each parameter a tensor
+    device: a clipping factor, the inverse of a loss scale) multiplies every gradient.  lr and step are part of the launch: a
+    captured graph repeats them.  copies: for each parameter a tensor
     (or None) that receives its new value in that tensor's type, as the 16-bit weights beside fp32 masters."""
     _ops.host.adamw(params, grads, exp_avgs, exp_avg_sqs, None, None, copies, lr, betas[0], betas[1], eps, weight_decay, step, 0, grad_scale)
 
@@ -142,8 +143,7 @@ class AdamW(torch.optim.Optimizer):
                     else:
                         state["exp_avg"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                         state["exp_avg_sq"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-                state["step"] += 1
-                runs.setdefault((state["step"], p.device), []).append((_plain(p), _plain(grad).contiguous(), state, copy))
+                runs.setdefault((state["step"] + 1, p.device), []).append((_plain(p), _plain(grad).contiguous(), state, copy))
             for (step, _), run in runs.items():
                 params, grads, states, copies = zip(*run)
                 common = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], step=step,
@@ -156,6 +156,8 @@ class AdamW(torch.optim.Optimizer):
                     adamw_8bit_step(params, grads, of("exp_avg"), of("exp_avg_scale"), of("exp_rms"), of("exp_rms_scale"), seed=group["seed"] + step, **common)
                 else:
                     adamw_step(params, grads, of("exp_avg"), of("exp_avg_sq"), **common)
+                for state in states:   # (a call that refused its arguments has stepped nothing)
+                    state["step"] = step
         return loss
 
 

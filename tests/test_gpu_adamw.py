@@ -307,3 +307,25 @@ def test_refusals():
         adamw_step([p], [p], [m], [v], **good)
     with pytest.raises(ValueError, match="scales"):
         adamw_8bit_step([p], [g], [m.byte()], [torch.ones(2, device=DEV)], [v.byte()], [torch.ones(1, device=DEV)], seed=0, **good)
+
+
+def test_autograd_sees_new_copies():
+    """A product that saved a 16-bit copy cannot be differentiated through once a step has changed it."""
+    master = torch.nn.Parameter(torch.randn(8, 8, device=DEV))
+    model = master.detach().bfloat16().requires_grad_(True)
+    out = (torch.ones(2, 8, device=DEV, dtype=torch.bfloat16, requires_grad=True) * model[:2]).sum()
+    master.grad = torch.ones_like(master)
+    AdamW([dict(params=[master], copies=[model])], **HYPER).step()
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.backward()
+
+
+def test_a_refused_step_is_not_counted():
+    p = torch.nn.Parameter(torch.randn(8, 8, device=DEV))
+    o = AdamW([p], **HYPER)
+    p.grad = torch.ones_like(p)
+    with pytest.raises(TypeError, match="grad_scale"):
+        o.step(grad_scale=torch.ones(2, device=DEV))
+    assert o.state[p]["step"] == 0
+    o.step()
+    assert o.state[p]["step"] == 1
