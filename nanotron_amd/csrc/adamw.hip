@@ -1,7 +1,7 @@
 // AdamW over many tensors, moments in fp32 or in 8 bits.
 //
 // Bound by memory: an fp32 parameter with a 16-bit gradient moves 26 bytes with fp32 moments, 14 with 8-bit ones.  One launch
-// takes as many tensors as its arguments hold (84 with fp32 moments), their pointers and sizes among them, so that nothing has
+// takes as many tensors as its arguments hold (57 to 88), their pointers and sizes among them, so that nothing has
 // to be copied to the device first; a workgroup takes a run of elements of one tensor.
 //
 // 8-bit moments.  The first moment m and the root r of the second are kept as E4M3 codes, blocks of 256 elements with a
@@ -237,7 +237,7 @@ int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options&
         for (int64_t at = 0; at < t.n; at += part) {
             const int64_t n = std::min(part, t.n - at);
             const int more = (int)((n + kChunk - 1) / kChunk);
-            if (used == S::kMost || blocks + more > (1 << 30))
+            if (used == S::kMost || blocks + more > (1 << 23))   // (a launch takes fewer than 2^32 threads)
                 if (const int rc = launch(); rc != NTFP8_OK) return rc;
             s.t[used] = Moments{static_cast<char*>(t.param) + at * size_of(P), static_cast<const char*>(t.grad) + at * size_of(G),
                                 static_cast<char*>(t.exp_avg) + at * kState, static_cast<char*>(t.exp_avg_sq) + at * kState, n};

@@ -296,7 +296,9 @@ struct Plan {
     Tiling logits, dx;
     int64_t at_factors, at_label, at_place, at_token, at_kept, at_stats, at_held, at_x, at_w, at_dx, bytes;
 };
-int64_t piece_of(int64_t vocab) { return std::max<int64_t>(256, kMostHeld / (2 * held_cols(vocab)) / 256 * 256); }
+// tokens at a time that `each` bytes of a token allow (and a launch with a row to a block, of fewer than 2^32 threads)
+int64_t piece_with(int64_t each) { return std::min<int64_t>(1 << 23, std::max<int64_t>(256, kMostHeld / each / 256 * 256)); }
+int64_t piece_of(int64_t vocab) { return piece_with(2 * held_cols(vocab)); }
 
 Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     Plan p = {};
@@ -304,7 +306,7 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     p.ldd = held_cols(d.vocab);
     p.pieces = (p.ldd + kPieceCols - 1) / kPieceCols;
     // (without gradients nothing is held but 8 bytes for 128 logits)
-    p.piece = std::min(d.tokens, gradient ? piece_of(d.vocab) : std::max<int64_t>(256, kMostHeld / (8 * p.pieces) / 256 * 256));
+    p.piece = std::min(d.tokens, gradient ? piece_of(d.vocab) : piece_with(8 * p.pieces));
     p.padded = up(d.hidden, 8);
     // (with gradients the tokens that count are gathered: those that are ignored cost nothing, and what is in them, NaN say, is
     // seen by nobody)

@@ -323,14 +323,20 @@ int layer_norm_blocks(int dtype, int64_t rows, int64_t cols) {
 
 int run_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride, const void* weight, const void* bias,
                            int w_dtype, float eps, void* y, float* mean, float* rstd, hipStream_t st) {
-    Norm n = {x, nullptr, weight, bias, y, mean, rstd, nullptr, x_stride, 0, rows, (int)cols, eps};
     return with_dtype(x_dtype, [&](auto d) {
         return with_weight<decltype(d)::value>(w_dtype, [&](auto w) {
             return by_width_forward(pieces_of(x_dtype, cols), [&](auto tpr, auto vpt) {
                 constexpr int TPR = decltype(tpr)::value, kBlock = forward_block(TPR), kRows = kBlock / TPR;
-                layer_norm_forward_kernel<decltype(d)::value, decltype(w)::value, TPR, decltype(vpt)::value>
-                    <<<(unsigned)((rows + kRows - 1) / kRows), kBlock, 0, st>>>(n);
-                return launch_status();
+                // (a launch takes fewer than 2^32 threads)
+                constexpr int64_t kMost = (int64_t)kRows << 21;
+                for (int64_t row = 0; row < rows; row += kMost) {
+                    const int64_t some = std::min(kMost, rows - row);
+                    const Norm n = {static_cast<const char*>(x) + row * x_stride * size_of(x_dtype), nullptr, weight, bias, static_cast<char*>(y) + row * cols * size_of(x_dtype),
+                                    mean ? mean + row : nullptr, mean ? rstd + row : nullptr, nullptr, x_stride, 0, some, (int)cols, eps};
+                    layer_norm_forward_kernel<decltype(d)::value, decltype(w)::value, TPR, decltype(vpt)::value><<<(unsigned)((some + kRows - 1) / kRows), kBlock, 0, st>>>(n);
+                    if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+                }
+                return (int)NTFP8_OK;
             });
         });
     });

@@ -241,3 +241,20 @@ def test_differentiable_once():
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(NotImplementedError):
             layer_norm(torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x)))
+
+
+def test_more_rows_than_a_launch_takes():
+    """Rows of a few elements, more of them than threads of one launch can take (2^32, 64 a row)."""
+    rows, cols = (1 << 26) + 1003, 3
+    g = torch.Generator(device=DEV).manual_seed(2)
+    x, dy = (torch.randn(rows, cols, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    w, b = (torch.randn(cols, generator=g, device=DEV) for _ in range(2))
+    x.requires_grad_(True)
+    y = layer_norm(x, w, b)
+    y.backward(dy)
+    # a launch ends at 2^21 workgroups of four rows each
+    for first in (0, (1 << 23) - 500, (1 << 25) - 500, rows - 1000):
+        part = slice(first, first + 1000)
+        want, bound = exact(x.detach()[part], w, b, dy[part], 1e-5)
+        near(y.detach()[part], want[0], bound[0], y.dtype, "y")
+        near(x.grad[part], want[1], bound[1], x.dtype, "dx")

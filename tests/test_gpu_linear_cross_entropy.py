@@ -339,3 +339,18 @@ def test_losses_in_pieces():
         part = slice(r, r + 40)
         want, bound = exact(x[part], w, labels[part])
         near(got[part], want[0], bound[0], "losses")
+
+
+def test_many_tokens_of_few_labels():
+    """More tokens than a launch with a token to a workgroup takes."""
+    tokens = (1 << 24) + 300
+    x, w, labels = draw(tokens, 8, 5, torch.bfloat16, 0.1, 20)
+    x.requires_grad_(True)
+    linear_cross_entropy(x, w, labels, reduction="sum").backward()
+    with torch.no_grad():
+        losses = linear_cross_entropy(x, w, labels, reduction="none")
+    for first in (0, (1 << 23) - 500, (1 << 24) - 500, tokens - 1000):
+        part = slice(first, first + 1000)
+        want, bound = exact(x.detach()[part], w, labels[part], mean=False)
+        near(losses[part], want[0], bound[0], "losses")
+        near(x.grad[part], want[2], bound[2], "dx")
