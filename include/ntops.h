@@ -36,7 +36,7 @@ int ntops_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, 
  * scale (value = code / scale), the power of two that brings the block's largest magnitude into (224, 448]; codes are rounded
  * stochastically with 16 bits hashed from the element's index and `seed`, a root above zero never to zero, and a value that is
  * not finite becomes NaN.  The parameters move by the moments before they are rounded.
- * Tensors must not overlap.  An empty tensor (n = 0) is passed over. */
+ * Tensors must not overlap, and lie below 2^48 (NTFP8_ERR_UNSUPPORTED).  An empty tensor (n = 0) is passed over. */
 #define NTOPS_ADAMW_BLOCK 256
 typedef struct ntops_adamw_tensor {
     void* param;

@@ -157,3 +157,8 @@ def test_constructors_refuse():
     with pytest.raises(ValueError, match="copies"):
         AdamW([dict(params=[p], copies=[None, None])])
     assert ctypes.sizeof(_ops.AdamWTensor) == 64
+
+
+def test_adamw_addresses():
+    for k in ("param", "grad", "exp_avg", "exp_avg_sq", "copy"):
+        assert _ops.lib.ntops_adamw(tensors(**{k: 1 << 48}), 1, options(copy_dtype=nt.BF16), None) == UNSUPPORTED
