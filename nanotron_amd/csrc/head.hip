@@ -195,10 +195,11 @@ __global__ __launch_bounds__(1024) void head_end_kernel(const float* __restrict_
 }
 
 // dx: row place[token] - row0 of what was computed for the tokens that count, zeros for the others (if row0 is 0; the other
-// launches of a call leave rows that are not theirs alone).  Computed is alpha times the sum of `splits` runs of K in fp32, or,
-// splits 0, the row itself.  With `loss`, one more workgroup sums the losses.
+// launches of a call leave rows that are not theirs alone).  Computed is the row itself or, with K cut into runs
+// (`groups` workgroups, tiles of tile_rows, tiles_n of them across, kt_all K-tiles), the sum of the runs in fp32 times alpha.  With `loss`, one more workgroup sums the losses.
 template <int D>
-__global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ from, int splits, int64_t split_stride, const float* __restrict__ factors,
+__global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ from, int groups, int tile_rows, int tiles_n, int kt_all, const int* __restrict__ rows,
+                                                       const float* __restrict__ factors,
                                                        const int* __restrict__ place, int64_t tokens, int row0, int count, int cols, void* __restrict__ out,
                                                        const float* __restrict__ losses, float* __restrict__ loss) {
     if (loss && blockIdx.x == gridDim.x - 1) {   // uniform
@@ -206,6 +207,8 @@ __global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ 
         return;
     }
     const float a = factors[1];
+    const int live = max(0, min(*rows - row0, count)), splits = runs_of(groups, (live + tile_rows - 1) / tile_rows * tiles_n, kt_all).splits;
+    const int64_t split_stride = (int64_t)live * cols;
     const int chunks = (cols + 7) / 8;
     const int64_t all = tokens * chunks, step = (int64_t)(gridDim.x - (loss ? 1 : 0)) * 256;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += step) {
@@ -215,15 +218,16 @@ __global__ __launch_bounds__(256) void put_rows_kernel(const void* __restrict__ 
         if (at < 0 ? row0 != 0 : r < 0 || r >= count) continue;
         float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (at >= 0) {
-            if (splits == 0) unpack<D, 8>(load_piece<D, 8>(from, r * cols + c, left), s);
+            if (splits == 1) {
+                unpack<D, 8>(load_piece<D, 8>(from, r * cols + c, left), s);
+            } else {
 #pragma unroll 8
-            for (int k = 0; k < splits; ++k) {
-                float v[8];
-                unpack<NTFP8_F32, 8>(load_piece<NTFP8_F32, 8>(from, k * split_stride + r * cols + c, left), v);
+                for (int k = 0; k < splits; ++k) {
+                    float v[8];
+                    unpack<NTFP8_F32, 8>(load_piece<NTFP8_F32, 8>(from, k * split_stride + r * cols + c, left), v);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] += v[e];
-            }
-            if (splits) {
+                    for (int e = 0; e < 8; ++e) s[e] += v[e];
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) s[e] *= a;
             }
@@ -263,7 +267,7 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
     g.magic = magic_of((uint32_t)(kGroupM * g.tiles_n));
     const int64_t tiles = (g.M + 32 * (int64_t)mi - 1) / (32 * mi) * g.tiles_n;
     // (with 256-row tiles up to 128 more, for those of a last round that go in halves; how many is known to the device)
-    const unsigned blocks = (unsigned)(EPI == kPartial ? tiles * g.splits : mi == 8 ? tiles + 128 : tiles);
+    const unsigned blocks = (unsigned)((EPI == kPartial ? g.groups : tiles) + (mi == 8 ? 128 : 0));
     if constexpr (kAT) {
         head_gemm_kernel<T, kAT, kBT, 8, EPI><<<blocks, kBigThreads, 0, st>>>(g);
     } else {
@@ -278,43 +282,43 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
 // What a launch of `tiles` workgroups takes, us, each of `kts` K-tiles of (32 mi) x 256 outputs: rounds of one workgroup a CU, a
 // K-tile's time and what a workgroup takes besides.  A K-tile of fewer rows takes more of their share, since the 256 columns
 // are the larger part of what it loads.  (Measured at 64 to 2048 tokens, 512 to 4096 hidden, vocabularies of 6 to 50 thousand; with a
-// transposed operand a K-tile takes a tenth more.)  halves: a last round of up to 128 tiles of 256 rows goes in tiles of 128.
-float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed, bool halves) {
+// transposed operand a K-tile takes a tenth more.)  A last round of up to 128 tiles of 256 rows goes in tiles of 128.
+float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed) {
     constexpr float kTile[4] = {0.48f, 0.62f, 0.72f, 1.37f}, kRest[4] = {4.0f, 5.0f, 6.0f, 9.0f};
     auto round = [&](int at) { return (float)kts * kTile[at] * (transposed ? 1.1f : 1.0f) + kRest[at]; };
     const int at = mi == 1 ? 0 : mi == 2 ? 1 : mi == 4 ? 2 : 3;
     const int64_t rest = tiles % 256;
-    return (float)(tiles / 256) * round(at) + (rest == 0 ? 0.0f : mi == 8 && halves && rest <= 128 ? round(2) : round(at));
+    return (float)(tiles / 256) * round(at) + (rest == 0 ? 0.0f : mi == 8 && rest <= 128 ? round(2) : round(at));
 }
 int64_t tiles_of(int64_t rows, int64_t cols, int mi) { return (rows + 32 * mi - 1) / (32 * mi) * ((cols + kBigN - 1) / kBigN); }
 
-// Rows of a tile / 32, and runs that K is cut into, for the products with an untransposed A
+// Rows of a tile / 32, and runs that K is cut into if all tokens count, for the products with an untransposed A
 struct Tiling {
-    int mi, splits, kt_split;
+    int mi, splits;
 };
 // logits: 333 tokens against 6001 rows of 512, us with 256 / 128 / 64 / 32 rows a tile: 21.4, 13.6, 11.6, 16.2; 512 tokens, 32000 rows of 2048: 53.3,
 // 58.8, 99.6, 156.9
 Tiling tiling_of_logits(int64_t rows, int64_t cols, int64_t kts) {
-    Tiling best = {8, 1, 0};
+    Tiling best = {8, 1};
     float least = 1e30f;
     for (int mi = 8; mi >= 1; mi /= 2) {
-        const float us = launch_us(mi, tiles_of(rows, cols, mi), kts, false, true);
+        const float us = launch_us(mi, tiles_of(rows, cols, mi), kts, false);
         if (us < least) least = us, best.mi = mi;
     }
     return best;
 }
 // dx: K is the vocabulary, and there are few tiles; runs of K fill the chip, for their fp32 sums' way to memory and back
 Tiling tiling_of_dx(int64_t rows, int64_t cols, int64_t kts) {
-    Tiling best = {8, 1, (int)kts};
+    Tiling best = {8, 1};
     float least = 1e30f;
     for (int mi = 8; mi >= 1; mi /= 2) {
         const int64_t tiles = tiles_of(rows, cols, mi);
         for (int64_t want = 1; want <= 64 && want <= std::max<int64_t>(1, kts / 4); ++want) {
             const int64_t each = (kts + want - 1) / want, splits = (kts + each - 1) / each;
             if (splits > 1 && tiles * splits > 1024) break;
-            float us = launch_us(mi, tiles * splits, each, true, splits == 1);
+            float us = launch_us(mi, tiles * splits, each, true);
             if (splits > 1) us += (float)(rows * cols) * (float)splits * 8.0f / 4.5e6f;
-            if (us < least) least = us, best = {mi, (int)splits, (int)each};
+            if (us < least) least = us, best = {mi, (int)splits};
         }
     }
     return best;
@@ -363,7 +367,7 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     p.at_held = gradient ? room(p.piece * p.ldd * 2) : 0;
     p.at_x = p.pad_x ? room(d.tokens * p.padded * 2) : 0;
     p.at_w = p.pad_w ? room(d.vocab * p.padded * 2) : 0;
-    p.at_dx = d.dx ? room(p.piece * d.hidden * (p.dx.splits > 1 ? 4 * p.dx.splits : size_of(d.grad_dtype))) : 0;
+    p.at_dx = d.dx ? room(up(p.piece, 32 * p.dx.mi) * d.hidden * 4 * p.dx.splits) : 0;
     p.bytes = at;
     return p;
 }
@@ -423,13 +427,12 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
             h.M = (int)rows, h.N = (int)d.hidden, h.K = (int)p.ldd;
             h.rows = count, h.row0 = (int)row;
             h.D = ws + p.at_dx, h.d_dtype = d.grad_dtype, h.alpha = factors + 1;
-            h.splits = p.dx.splits, h.kt_split = p.dx.kt_split, h.partial = reinterpret_cast<float*>(ws + p.at_dx);
-            const bool whole = p.dx.splits == 1;
-            if (status(whole ? launch_gemm<T, false, true, kStore>(h, p.dx.mi, st) : launch_gemm<T, false, true, kPartial>(h, p.dx.mi, st))) return NTFP8_ERR_LAUNCH;
+            h.groups = (int)tiles_of(rows, d.hidden, p.dx.mi) * p.dx.splits;
+            if (status(launch_gemm<T, false, true, kPartial>(h, p.dx.mi, st))) return NTFP8_ERR_LAUNCH;
             auto put = d.grad_dtype == T ? put_rows_kernel<T> : put_rows_kernel<NTFP8_F32>;
             const int64_t n = d.tokens * ((d.hidden + 7) / 8);
             put<<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192) + (last && d.loss ? 1 : 0), 256, 0, st>>>(
-                ws + p.at_dx, whole ? 0 : p.dx.splits, rows * d.hidden, factors, place, d.tokens, (int)row, (int)rows, (int)d.hidden, d.dx, d.losses, last ? d.loss : nullptr);
+                ws + p.at_dx, h.groups, 32 * p.dx.mi, (int)((d.hidden + kBigN - 1) / kBigN), (int)(p.ldd / kHeadK), count, factors, place, d.tokens, (int)row, (int)rows, (int)d.hidden, d.dx, d.losses, last ? d.loss : nullptr);
             if (status(launch_status())) return NTFP8_ERR_LAUNCH;
         }
         if (d.dweight) {

@@ -29,7 +29,7 @@ __device__ __forceinline__ v4f mfma_16x16x32(v4i b_frag, v4i a_frag, v4f c) {
 
 enum HeadEpilogue {
     kStore,     // D = alpha * sums, rounded to d_dtype (fp32: optionally added to D)
-    kPartial,   // the sums of a run of K, fp32, to partial[split][M][N]
+    kPartial,   // with K cut into runs, the sums of a run in fp32, D[run][M][N]; of all of K as kStore
     kLosses,    // per row and 128 columns: the largest logit and the sum of exponentials below it; the labels' logits
     kSoftmax,   // the same, and the exponentials themselves in fp16
 };
@@ -45,11 +45,10 @@ struct HeadGemm {
     int b_rows;                  // rows of a transposed B (K or fewer; those behind count as zeros)
     int tiles_n;
     uint32_t magic;              // magic_of(kGroupM tiles_n)
-    int splits, kt_split;        // runs of K, and K-tiles of each
+    int groups;                  // kPartial: workgroups (tiles times runs of K)
     void* D;
     int d_dtype, accumulate;
     const float* alpha;
-    float* partial;
     // logits
     int64_t ldd;                 // elements between rows of the exponentials, N of them or more (a multiple of 8)
     float2* stats;               // [M][pieces]: base-2 maximum, sum
@@ -74,14 +73,23 @@ __device__ __forceinline__ HeadOutput head_output(const HeadGemm& G) {
     HeadOutput o = {G.D, G.ldd, G.stats, G.labels, G.label_logit, 1.0f, G.N, G.pieces, G.d_dtype, G.accumulate};
     if constexpr (EPI == kLosses || EPI == kSoftmax) {
         asm volatile("" ::"s"(o.D), "s"(o.ldd), "s"(o.stats), "s"(o.labels), "s"(o.label_logit), "s"(o.N), "s"(o.pieces));
-    } else if constexpr (EPI == kPartial) {
-        o.D = G.partial;
-        asm volatile("" ::"s"(o.D), "s"(o.N));
     } else {
         o.alpha = *G.alpha;
         asm volatile("" ::"s"(o.D), "s"(o.N), "s"(o.d_dtype), "s"(o.accumulate) : "memory");
     }
     return o;
+}
+
+// Runs that K is cut into where there are fewer tiles than workgroups, and K-tiles of each.  The device does it, who knows how many
+// tokens count.  us of a step, three of four tokens ignored, with the runs that all tokens would have / so: 2048 tokens, 2048 hidden,
+// 32000 labels 357 / 274; 4096, 2048, 50000 1036 / 650; where all count, 4096, 4096, 128000 9935 / 9950 (dx's kernel takes either).
+struct HeadRuns {
+    int splits, kts;
+};
+__host__ __device__ __forceinline__ HeadRuns runs_of(int groups, int tiles, int kt_all) {
+    if (tiles <= 0 || kt_all <= 0) return {1, kt_all};
+    const int most = groups / tiles, want = kt_all / 4 < most ? kt_all / 4 : most, kts = (kt_all + (want > 1 ? want : 1) - 1) / (want > 1 ? want : 1);
+    return {(kt_all + kts - 1) / kts, kts};
 }
 
 // LDS stages: what fits beside each other in 160 KB
@@ -575,12 +583,13 @@ __device__ __forceinline__ void head_tile(const HeadGemm& G, const HeadSizes& z,
 
     if constexpr (EPI == kLosses || EPI == kSoftmax) {
         softmax_epilogue<MI, EPI == kSoftmax>(acc, out, M, m0 + wm, n0 + wn, lane);
-    } else if constexpr (EPI == kPartial) {
-        store_tile<NTFP8_F32, false, MI>(acc, static_cast<float*>(out.D) + (int64_t)split * G.M * out.N, 1.0f, M, out.N, m0 + wm, n0 + wn, lane);
     } else {
-        if (out.d_dtype == T) store_tile<T, false, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
-        else if (out.accumulate) store_tile<NTFP8_F32, true, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
-        else store_tile<NTFP8_F32, false, MI>(acc, out.D, out.alpha, M, out.N, m0 + wm, n0 + wn, lane);
+        const bool part = EPI == kPartial && kt1 - kt0 < kt_all;
+        void* const D = part ? static_cast<float*>(out.D) + (int64_t)split * M * out.N : out.D;
+        const float alpha = part ? 1.0f : out.alpha;
+        if (!part && out.d_dtype == T) store_tile<T, false, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane);
+        else if (EPI == kStore && out.accumulate) store_tile<NTFP8_F32, true, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane);
+        else store_tile<NTFP8_F32, false, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane);
     }
 }
 
@@ -588,36 +597,43 @@ template <int T, bool kAT, bool kBT, int MI, int EPI>
 __global__ __launch_bounds__(kBigThreads) void head_gemm_kernel(const HeadGemm G) {
     // 256-row tiles that do not fill a last round (kTail): its tiles in halves of 128 rows, twice the workgroups for half as long.
     // us, whole / so: weight gradients of 6001 x 515 from 333 tokens 18.3 / 13.1, of 50001 x 1024 from 766 101 / 95, of 128000 x 4096 from 4096 3404 / 3300
-    constexpr bool kTail = MI == 8 && EPI != kPartial;
+    constexpr bool kTail = MI == 8;
     constexpr int kBytesA = head_stages<MI>() * 32 * MI * kBK, kBytesB = head_stages<kTail ? 4 : MI>() * kBigN * kBK;
     __shared__ __attribute__((aligned(1024))) uint8_t sA[kBytesA];
     __shared__ __attribute__((aligned(1024))) uint8_t sB[kBytesB];
     static_assert(!kTail || kBytesA >= head_stages<4>() * 128 * kBK, "half tiles use the same arrays");
     const HeadSizes z = head_sizes<kAT>(G);
     if (kAT && G.accumulate && z.K == 0) return;
-    const int tiles_m = (z.M + 32 * MI - 1) / (32 * MI), tiles = tiles_m * G.tiles_n, total = tiles * (EPI == kPartial ? G.splits : 1);
+    const int tiles_m = (z.M + 32 * MI - 1) / (32 * MI), tiles = tiles_m * G.tiles_n;
     const int kt_all = (z.K + kHeadK - 1) / kHeadK;
+    HeadRuns runs = {1, kt_all};
+    if constexpr (EPI == kPartial) {   // (quotients are vector arithmetic: what descriptors are made of is scalar)
+        runs = runs_of(G.groups, tiles, kt_all);
+        runs.splits = __builtin_amdgcn_readfirstlane(runs.splits);
+        runs.kts = __builtin_amdgcn_readfirstlane(runs.kts);
+    }
+    const int total = tiles * runs.splits;
     int pid = blockIdx.x, pid_m, pid_n;
+    auto place = [&](int tile) {   // -> its run of K
+        const int split = EPI == kPartial ? __builtin_amdgcn_readfirstlane(tile / tiles) : 0;
+        tile_in_group(EPI == kPartial ? tile - split * tiles : tile, tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
+        return split;
+    };
     if constexpr (kTail) {
         const int rest = total & 255, whole = rest > 128 ? total : total - rest;
         if (pid >= whole) {
             const int half = pid - whole;
             if (rest > 128 || half >= 2 * rest) return;
-            const int at = run_of_xcd(half, 2 * rest);
-            tile_in_group(whole + (at >> 1), tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
+            const int at = run_of_xcd(half, 2 * rest), split = place(whole + (at >> 1)), kt0 = split * runs.kts;
             const int m0 = pid_m * 256 + (at & 1) * 128;
-            if (m0 < z.M) head_tile<T, kAT, kBT, 4, EPI>(G, z, m0, pid_n * kBigN, 0, 0, kt_all, kt_all, sA, sB);
+            if (m0 < z.M) head_tile<T, kAT, kBT, 4, EPI>(G, z, m0, pid_n * kBigN, split, kt0, min(kt_all, kt0 + runs.kts), kt_all, sA, sB);
             return;
         }
     }
     // Within each round of 256 workgroups an XCD takes a contiguous run of the tiles
     if (pid >= total) return;
-    const int round0 = pid & ~255;
-    pid = round0 + run_of_xcd(pid - round0, min(256, total - round0));
-    const int split = EPI == kPartial ? pid / tiles : 0;
-    tile_in_group(EPI == kPartial ? pid - split * tiles : pid, tiles_m, G.tiles_n, G.magic, pid_m, pid_n);
-    const int kt0 = EPI == kPartial ? split * G.kt_split : 0;
-    head_tile<T, kAT, kBT, MI, EPI>(G, z, pid_m * 32 * MI, pid_n * kBigN, split, kt0, EPI == kPartial ? min(kt_all, kt0 + G.kt_split) : kt_all, kt_all, sA, sB);
+    const int round0 = pid & ~255, split = place(round0 + run_of_xcd(pid - round0, min(256, total - round0))), kt0 = split * runs.kts;
+    head_tile<T, kAT, kBT, MI, EPI>(G, z, pid_m * 32 * MI, pid_n * kBigN, split, kt0, min(kt_all, kt0 + runs.kts), kt_all, sA, sB);
 }
 
 }  // namespace ntfp8
