@@ -282,13 +282,14 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
 // What a launch of `tiles` workgroups takes, us, each of `kts` K-tiles of (32 mi) x 256 outputs: rounds of one workgroup a CU, a
 // K-tile's time and what a workgroup takes besides.  A K-tile of fewer rows takes more of their share, since the 256 columns
 // are the larger part of what it loads.  (Measured at 64 to 2048 tokens, 512 to 4096 hidden, vocabularies of 6 to 50 thousand; with a
-// transposed operand a K-tile takes a tenth more.)  A last round of up to 128 tiles of 256 rows goes in tiles of 128.
+// transposed operand a K-tile takes a tenth more.)  A last round of up to 128 tiles of 256 rows goes in halves, a little slower
+// than a launch of such tiles (dx of 766 x 1024 from 50001 labels, all of it in halves 80, in tiles of 128 rows 73).
 float launch_us(int mi, int64_t tiles, int64_t kts, bool transposed) {
     constexpr float kTile[4] = {0.48f, 0.62f, 0.72f, 1.37f}, kRest[4] = {4.0f, 5.0f, 6.0f, 9.0f};
     auto round = [&](int at) { return (float)kts * kTile[at] * (transposed ? 1.1f : 1.0f) + kRest[at]; };
     const int at = mi == 1 ? 0 : mi == 2 ? 1 : mi == 4 ? 2 : 3;
     const int64_t rest = tiles % 256;
-    return (float)(tiles / 256) * round(at) + (rest == 0 ? 0.0f : mi == 8 && rest <= 128 ? round(2) : round(at));
+    return (float)(tiles / 256) * round(at) + (rest == 0 ? 0.0f : mi == 8 && rest <= 128 ? 1.08f * round(2) : round(at));
 }
 int64_t tiles_of(int64_t rows, int64_t cols, int mi) { return (rows + 32 * mi - 1) / (32 * mi) * ((cols + kBigN - 1) / kBigN); }
 
