@@ -329,3 +329,40 @@ def test_a_refused_step_is_not_counted():
     assert o.state[p]["step"] == 0
     o.step()
     assert o.state[p]["step"] == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph_replays(bits):
+    """A captured step, replayed with new gradients and other work in between, is the step launched from Python."""
+    tensors = [draw(n, torch.float32, torch.bfloat16, seed=n) for n in (70001, 256, 5)]
+    params, grads, ms, vs = ([t[i].clone() for t in tensors] for i in range(4))
+    factor = torch.full((1,), 0.5, device=DEV)
+    state = [moments_8bit(p) for p in params]
+
+    def step(params, ms, vs, state):
+        if bits == 32:
+            adamw_step(params, grads, ms, vs, step=3, grad_scale=factor, **HYPER)
+        else:
+            m, s, r, t = zip(*state)
+            adamw_8bit_step(params, grads, m, s, r, t, step=3, seed=11, grad_scale=factor, **HYPER)
+
+    def clones():
+        return [p.clone() for p in params], [m.clone() for m in ms], [v.clone() for v in vs], [tuple(t.clone() for t in s) for s in state]
+
+    mine = clones()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step(*clones())
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(params, ms, vs, state)
+    for k in range(4):
+        for g in grads:
+            g.copy_(torch.randn(g.shape, device=DEV) * 10.0 ** -k)
+        step(*mine)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(mine[0], params)), k
+        assert all(torch.equal(a, b) for s, t in zip(mine[3], state) for a, b in zip(s, t)), k
