@@ -32,12 +32,6 @@ __device__ __forceinline__ void unpack_pair(uint32_t w, float& a, float& b) {
 }
 
 template <int D>
-__device__ __forceinline__ float load_one(const void* p, int64_t i) {
-    if constexpr (D == NTFP8_F32) return static_cast<const float*>(p)[i];
-    else if constexpr (D == NTFP8_BF16) return bf16_bits_to_float(static_cast<const uint16_t*>(p)[i]);
-    else return half_bits_to_float(static_cast<const uint16_t*>(p)[i]);
-}
-template <int D>
 __device__ __forceinline__ void store_one(void* p, int64_t i, float v) {
     if constexpr (D == NTFP8_F32) static_cast<float*>(p)[i] = v;
     else static_cast<uint16_t*>(p)[i] = (uint16_t)pack_pair<D>(v, v);
