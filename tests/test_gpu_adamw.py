@@ -366,3 +366,34 @@ def test_graph_replays(bits):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(mine[0], params)), k
         assert all(torch.equal(a, b) for s, t in zip(mine[3], state) for a, b in zip(s, t)), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_beyond_32_bits(bits):
+    """A tensor of more than 2^32 bytes, which a launch takes as several: the elements where one ends and the last ones."""
+    n = (1 << 31) + 1027
+    p, g = (torch.randn(n, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    parts = [slice(0, 5000), slice((1 << 30) - 2560, (1 << 30) + 2560), slice((1 << 31) - 2560, n)]
+    before = [p[s].clone() for s in parts]
+    if bits == 32:
+        m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+        adamw_step([p], [g], [m], [v], step=1, **HYPER)
+    else:
+        state = moments_8bit(p)
+        adamw_8bit_step([p], [g], *([t] for t in state), step=1, seed=5, **HYPER)
+    for s, old in zip(parts, before):
+        zero = torch.zeros(old.shape, device=DEV)
+        want, bound = exact(old, g[s], zero, zero, step=1, **HYPER)
+        near(p[s], want[0], bound[0], "parameter")
+        if bits == 32:
+            near(m[s], want[1], bound[1], "first moment")
+            near(v[s], want[2], bound[2], "second moment")
+        else:
+            # a code is a neighbour of its value: an eighth of it off at most, or the distance of the smallest codes
+            blocks = slice(s.start // 256, -(-s.stop // 256))
+            for code, scale, value in ((state[0], state[1], want[1]), (state[2], state[3], want[2].sqrt())):
+                got = dequantize_moment(code[blocks.start * 256:s.stop], scale[blocks])[s.start - blocks.start * 256:]
+                each = scale[blocks].repeat_interleave(256)[s.start - blocks.start * 256:][:got.numel()].double()
+                assert ((got.double() - value).abs() <= value.abs() / 8 + 2.0 ** -9 / each).all()
+    del p, g
+    torch.cuda.empty_cache()

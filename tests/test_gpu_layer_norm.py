@@ -258,3 +258,21 @@ def test_more_rows_than_a_launch_takes():
         want, bound = exact(x.detach()[part], w, b, dy[part], 1e-5)
         near(y.detach()[part], want[0], bound[0], y.dtype, "y")
         near(x.grad[part], want[1], bound[1], x.dtype, "dx")
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes of x: the last rows are those of the formulas."""
+    rows, cols = 270001, 8192
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x, dy = (torch.randn(rows, cols, generator=g, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    w, b = (torch.randn(cols, generator=g, device=DEV) for _ in range(2))
+    x.requires_grad_(True)
+    y = layer_norm(x, w, b)
+    y.backward(dy)
+    assert x.numel() * 2 > 1 << 32
+    for part in (slice(0, 100), slice(rows // 2 - 50, rows // 2 + 50), slice(rows - 100, rows)):
+        want, bound = exact(x.detach()[part], w, b, dy[part], 1e-5)
+        near(y.detach()[part], want[0], bound[0], y.dtype, "y")
+        near(x.grad[part], want[1], bound[1], x.dtype, "dx")
+    del x, y, dy
+    torch.cuda.empty_cache()

@@ -354,3 +354,39 @@ def test_many_tokens_of_few_labels():
         want, bound = exact(x.detach()[part], w, labels[part], mean=False)
         near(losses[part], want[0], bound[0], "losses")
         near(x.grad[part], want[2], bound[2], "dx")
+
+
+def test_offsets_beyond_32_bits():
+    """A weight of more than 2^32 bytes, in 64 bits by runs of its rows."""
+    tokens, hidden, vocab, run = 40, 4096, (1 << 19) + 4099, 1 << 15
+    x, w, labels = draw(tokens, hidden, vocab, torch.bfloat16, 0.1, 21)
+    labels[:4] = torch.tensor([0, vocab - 1, vocab - 2, 1 << 19], device=DEV)
+    assert w.numel() * 2 > 1 << 32
+    a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(a, b, labels, reduction="sum")
+    loss.backward()
+    xd, ut = x.double(), UT[x.dtype]
+    runs = [slice(r, min(vocab, r + run)) for r in range(0, vocab, run)]
+    logits = torch.cat([xd @ w[r].double().t() for r in runs], 1)
+    e = (hidden / 32 + 40) * U32 * torch.stack([(xd.abs() @ w[r].double().abs().t()).amax(-1) for r in runs]).amax(0)
+    keep = labels != -100
+    at = torch.where(keep, labels, 0)
+    lse = torch.logsumexp(logits, -1)
+    losses = torch.where(keep, lse - logits.gather(1, at[:, None])[:, 0], 0.0)
+    near(loss.detach(), losses.sum(), (2 * e + 8 * U32 * (lse.abs() + losses.abs() + 20)).sum(), "loss")
+    p = torch.softmax(logits, -1)
+    dl = p.clone()
+    dl[torch.arange(tokens), at] -= 1
+    dl, p = dl * keep[:, None], p * keep[:, None]
+    edl = (2 * e + 40 * U32)[:, None] * p + (2.0 ** -11 + ut) * dl.abs() + 2.0 ** -40
+    dx, edx = torch.zeros_like(xd), torch.zeros_like(xd)
+    for r in runs:
+        wr = w[r].double()
+        dx += dl[:, r] @ wr
+        edx += edl[:, r] @ wr.abs() + (vocab / 32 + 300) * U32 * ((dl[:, r].abs() + edl[:, r]) @ wr.abs())
+    near(a.grad, dx, edx + 2 * U32 * dx.abs(), "dx")
+    for r in (slice(0, 1000), slice((1 << 19) - 500, (1 << 19) + 500), slice(vocab - 1000, vocab)):
+        dw = dl[:, r].t() @ xd
+        near(b.grad[r], dw, edl[:, r].t() @ xd.abs() + (tokens / 32 + 300) * U32 * ((dl[:, r].abs() + edl[:, r]).t() @ xd.abs()) + 2 * U32 * dw.abs(), "dweight")
+    del a, b, x, w
+    torch.cuda.empty_cache()
