@@ -258,7 +258,7 @@ Tensor linear_cross_entropy(const Tensor& x, const Tensor& w, const Tensor& labe
     for (const Tensor* t : {&x, &w}) no_tangent(*t, "linear_cross_entropy");
     if (x.numel() == 0) {   // no tokens: a loss of 0 without gradient
         const auto f32 = x.options().dtype(at::kFloat);
-        return none ? at::zeros(labels.sizes(), f32) : (x.sum() + w.sum()).to(at::kFloat).mul(0);
+        return none ? at::zeros(labels.sizes(), f32) : (x.sum() + w.narrow(0, 0, 0).sum()).to(at::kFloat);
     }
     if (wants) return LinearCrossEntropy::apply(x, w, labels, ignore, mean, gx, gw);
     Guard guard(x.device());

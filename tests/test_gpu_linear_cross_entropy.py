@@ -390,3 +390,12 @@ def test_offsets_beyond_32_bits():
         near(b.grad[r], dw, edl[:, r].t() @ xd.abs() + (tokens / 32 + 300) * U32 * ((dl[:, r].abs() + edl[:, r]).t() @ xd.abs()) + 2 * U32 * dw.abs(), "dweight")
     del a, b, x, w
     torch.cuda.empty_cache()
+
+
+def test_no_tokens_beside_a_weight_that_is_not_finite():
+    x = torch.empty(0, 64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    w = torch.full((500, 64), float("inf"), device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    loss = linear_cross_entropy(x, w, torch.empty(0, device=DEV, dtype=torch.int64))
+    loss.backward()
+    assert loss.dtype == torch.float32 and loss.item() == 0.0
+    assert x.grad.shape == x.shape and not w.grad.any()
