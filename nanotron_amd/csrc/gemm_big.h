@@ -119,7 +119,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(O* D, int M, int N, 
 // Epilogue of one wave: MI x NJ accumulator blocks of 16 x 16, block (i, j) at rows m_base + 16 i,
 // columns n_base + 16 j.  Descale, optional fp32 accumulate, one rounding, store.
 // kBias: bv[j][e] = bias of column n_base + 16 j + 4 (lane / 16) + e, added to the descaled value before the rounding.
-template <int DT, bool kAcc, int MI, int NJ, bool kBias = false>
+template <int DT, bool kAcc, int MI, int NJ, bool kBias = false, bool kThrough = true>
 __device__ __forceinline__ void store_wave_tile16(const v4f (&acc)[MI][NJ], void* __restrict__ Dv, float alpha, int M,
                                                   int N, int m_base, int n_base, int lane, const float (*bv)[4] = nullptr) {
     typedef typename OutT<DT>::type O;
@@ -149,8 +149,11 @@ __device__ __forceinline__ void store_wave_tile16(const v4f (&acc)[MI][NJ], void
                     swap_rows16(x1, y1);
                     // lane row q now holds n 8 (q / 2) .. + 7 of block j + (q & 1): x = first four, y = last four
                     const int n = n_base + (j + (q & 1)) * 16 + (q >> 1) * 8;
-                    if (m < M && n < N)
-                        store16_through(D + (int64_t)m * N + n, (v4i){(int)x0, (int)x1, (int)y0, (int)y1});
+                    const v4i out = {(int)x0, (int)x1, (int)y0, (int)y1};
+                    if (m < M && n < N) {
+                        if constexpr (kThrough) store16_through(D + (int64_t)m * N + n, out);
+                        else *reinterpret_cast<v4i*>(D + (int64_t)m * N + n) = out;
+                    }
                 }
             }
             return;

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(1024) void scale_kernel(const Scaled t, const float
 
 template <int T, bool kAT, bool kBT, int EPI>
 int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
-    g.tiles_n = (int)(((EPI == kLosses || EPI == kSoftmax ? g.ldd : g.N) + kBigN - 1) / kBigN);
+    g.tiles_n = (int)(((softmax_of(EPI) ? g.ldd : g.N) + kBigN - 1) / kBigN);
     g.magic = magic_of((uint32_t)(kGroupM * g.tiles_n));
     const int64_t tiles = (g.M + 32 * (int64_t)mi - 1) / (32 * mi) * g.tiles_n;
     // (with 256-row tiles up to 128 more, for those of a last round that go in halves; how many is known to the device)
@@ -271,6 +271,12 @@ int launch_gemm(HeadGemm g, int mi, hipStream_t st) {
     if constexpr (kAT) {
         head_gemm_kernel<T, kAT, kBT, 8, EPI><<<blocks, kBigThreads, 0, st>>>(g);
     } else {
+        if constexpr (EPI == kSoftmax) {
+            if (mi == 8 && g.K <= (kLongK - 1) * kHeadK && g.M * g.ldd * 2 > kFoundBytes) {
+                head_gemm_kernel<T, kAT, kBT, 8, kSoftmaxThrough><<<blocks, kBigThreads, 0, st>>>(g);
+                return launch_status();
+            }
+        }
         if (mi == 8) head_gemm_kernel<T, kAT, kBT, 8, EPI><<<blocks, kBigThreads, 0, st>>>(g);
         else if (mi == 4) head_gemm_kernel<T, kAT, kBT, 4, EPI><<<blocks, kBigThreads, 0, st>>>(g);
         else if (mi == 2) head_gemm_kernel<T, kAT, kBT, 2, EPI><<<blocks, kBigThreads, 0, st>>>(g);

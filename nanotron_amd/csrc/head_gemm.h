@@ -36,7 +36,19 @@ enum HeadEpilogue {
     kPartial,   // with K cut into runs, the sums of a run in fp32, D[run][M][N]; of all of K as kStore
     kLosses,    // per row and 128 columns: the largest logit and the sum of exponentials below it; the labels' logits
     kSoftmax,   // the same, and the exponentials themselves in fp16
+    kSoftmaxThrough,   // the same, written through to memory
 };
+constexpr bool softmax_of(int epilogue) { return epilogue >= kLosses; }
+constexpr bool keeps(int epilogue) { return epilogue >= kSoftmax; }
+
+// Written through, or left in the L2.  A tile's 128 KB of 16-bit outputs a CU, left in the L2s, are written back while the next round
+// of tiles computes; if that takes less time than the memory needs, they are in the way of its loads, and those of the last round
+// are at the cost of the kernels behind.  So they are left there where K is long, or where the kernel behind finds them there.  us, through / left:
+//   logits, with the pass over their rows: 4096 tokens, 4096 hidden, 128000 labels 3535 / 3475; 2048, 4096, 32000 452 / 440; 4096, 2048,
+//   50000 810 / 832; 766, 1024, 50001 133 / 130 and 4 more in the product behind; a step of 256, 2048, 50000 294 / 285
+//   weight gradients: 128000 x 4096 of 4096 tokens 3294 / 3212; 50001 x 1024 of 766 93 / 93 and 10 more in the kernels behind
+constexpr int kLongK = 64;                                // K-tiles
+constexpr int64_t kFoundBytes = (int64_t)64 << 20;        // exponentials
 
 struct HeadGemm {
     const void* A;
@@ -75,7 +87,7 @@ struct HeadOutput {
 template <int EPI>
 __device__ __forceinline__ HeadOutput head_output(const HeadGemm& G) {
     HeadOutput o = {G.D, G.ldd, G.stats, G.labels, G.label_logit, 1.0f, G.N, G.pieces, G.d_dtype, G.accumulate};
-    if constexpr (EPI == kLosses || EPI == kSoftmax) {
+    if constexpr (softmax_of(EPI)) {
         asm volatile("" ::"s"(o.D), "s"(o.ldd), "s"(o.stats), "s"(o.labels), "s"(o.label_logit), "s"(o.N), "s"(o.pieces));
     } else {
         o.alpha = *G.alpha;
@@ -218,7 +230,7 @@ constexpr float kLift = 15.0f;   // exponentials are kept in fp16 as 2^15 e, 1 a
 // Logits of a wave, MI x 8 blocks at rows m_base, columns n_base (a piece of kPieceCols columns).  For each row the largest
 // logit (NaN if one is) and the sum of exponentials below it, both in base 2 and fp32; with kKeep the exponentials as well,
 // once rounded, which the gradient is later made of by one multiplication a row and piece.
-template <int MI, bool kKeep>
+template <int MI, bool kKeep, bool kThrough>
 __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const HeadOutput& G, int M, int m_base, int n_base, int lane) {
     if (n_base >= (int)G.ldd) return;   // uniform
     const int mrow = lane & 15, q = lane >> 4;
@@ -282,7 +294,11 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
                 swap_rows16(x0, y0);
                 swap_rows16(x1, y1);
                 const int n = n_base + (j + (q & 1)) * 16 + (q >> 1) * 8;
-                if (m < M && n < (int)G.ldd) store16_through(D + (int64_t)m * G.ldd + n, (v4i){(int)x0, (int)x1, (int)y0, (int)y1});
+                const v4i out = {(int)x0, (int)x1, (int)y0, (int)y1};
+                if (m < M && n < (int)G.ldd) {
+                    if constexpr (kThrough) store16_through(D + (int64_t)m * G.ldd + n, out);
+                    else *reinterpret_cast<v4i*>(D + (int64_t)m * G.ldd + n) = out;
+                }
             }
         }
         sched_fence();
@@ -291,16 +307,22 @@ __device__ __forceinline__ void softmax_epilogue(v4f (&acc)[MI][kBigNJ], const H
 
 // Stores of a wave's tile.  Rows of whole pieces go as those of the fp8 GEMM do; others, whose rows begin anywhere, a lane's
 // 4 consecutive outputs at a time at whatever address they have (element by element, the weight's gradient of 6001 x 515 in fp32 took
-// twice as long).
+// twice as long).  `stay`: 16-bit outputs are left in the L2.
 template <int DT, bool kAcc, int MI>
-__device__ __forceinline__ void store_tile(const v4f (&acc)[MI][kBigNJ], void* D, float alpha, int M, int N, int m_base, int n_base, int lane) {
+__device__ __forceinline__ void store_tile(const v4f (&acc)[MI][kBigNJ], void* D, float alpha, int M, int N, int m_base, int n_base, int lane, bool stay = false) {
     if ((N & 7) == 0) {
         // (16 rows at a time: the compiler would have the values of all of them at once, and no registers for them)
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
+        auto rows = [&](auto through, int i) __attribute__((always_inline)) {
             const v4f (&part)[1][kBigNJ] = reinterpret_cast<const v4f (&)[1][kBigNJ]>(acc[i]);
-            store_wave_tile16<DT, kAcc, 1, kBigNJ>(part, D, alpha, M, N, m_base + 16 * i, n_base, lane);
+            store_wave_tile16<DT, kAcc, 1, kBigNJ, false, decltype(through)::value>(part, D, alpha, M, N, m_base + 16 * i, n_base, lane);
             sched_fence();
+        };
+        if (stay) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) rows(std::false_type{}, i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < MI; ++i) rows(std::true_type{}, i);
         }
         return;
     }
@@ -585,13 +607,13 @@ __device__ __forceinline__ void head_tile(const HeadGemm& G, const HeadSizes& z,
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the empty tiles too: nothing may land in LDS behind the workgroup)
 
-    if constexpr (EPI == kLosses || EPI == kSoftmax) {
-        softmax_epilogue<MI, EPI == kSoftmax>(acc, out, M, m0 + wm, n0 + wn, lane);
+    if constexpr (softmax_of(EPI)) {
+        softmax_epilogue<MI, keeps(EPI), EPI == kSoftmaxThrough>(acc, out, M, m0 + wm, n0 + wn, lane);
     } else {
         const bool part = EPI == kPartial && kt1 - kt0 < kt_all;
         void* const D = part ? static_cast<float*>(out.D) + (int64_t)split * M * out.N : out.D;
         const float alpha = part ? 1.0f : out.alpha;
-        if (!part && out.d_dtype == T) store_tile<T, false, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane);
+        if (!part && out.d_dtype == T) store_tile<T, false, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane, EPI == kPartial || kt_all >= kLongK);   // (dx: put_rows_kernel reads it next)
         else if (EPI == kStore && out.accumulate) store_tile<NTFP8_F32, true, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane);
         else store_tile<NTFP8_F32, false, MI>(acc, D, alpha, M, out.N, m0 + wm, n0 + wn, lane);
     }
