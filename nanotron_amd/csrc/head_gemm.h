@@ -8,9 +8,9 @@
 // those of the fp8 GEMM do: rows of 128 bytes with their 16-byte chunks swizzled; a transposed operand as 64 rows of k with 512
 // bytes of n (or m) each, its 32-byte pieces swizzled, gathered with the transposing 64-bit LDS read.
 //
-// bf16, 4096 tokens, 4096 hidden, 128000 labels: logits with their exponentials 3130 us (1.37 PFLOP/s), dx 2950 (1.46), dweight 3330 (1.29).
-// Bound by energy: the clock falls to 1.77 GHz while 70, 76 and 66 % of the MFMA slots are used, with 8 to 11 % of the waves' time spent
-// waiting.  Of 766 tokens, 1024 hidden, 50001 labels 101, 73 and 91 us: 12 to 16 K-tiles a tile, whose first loads and stores nothing hides.
+// bf16, 4096 tokens, 4096 hidden, 128000 labels: logits with their exponentials 3030 us (1.42 PFLOP/s), dx 2920 (1.47), dweight 3220 (1.33);
+// by card up to 3 % more.  Bound by energy: the clock falls to 1.77 GHz while 72, 77 and 67 % of the MFMA slots are used, with 8 to 11 % of the
+// waves' time spent waiting.  Of 766 tokens, 1024 hidden, 50001 labels 100, 73 and 90 us: 12 to 16 K-tiles a tile, whose first loads and stores nothing hides.
 #pragma once
 #include "gemm_common.h"
 #include "gemm_big.h"
