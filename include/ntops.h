@@ -33,9 +33,9 @@ int ntops_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, 
  * in fp32, every operation rounded by itself; param is rounded once to its type, and once more to copy_dtype into `copy`
  * where one is given.  bits 32: exp_avg and exp_avg_sq are fp32 m and v.  bits 8: exp_avg holds E4M3 codes of m and exp_avg_sq
  * those of sqrt(v); every NTOPS_ADAMW_BLOCK elements (counted from the tensor's start, the last block may be short) share a
- * scale (value = code / scale), the power of two that brings the block's largest magnitude into (224, 448]; codes are rounded
- * stochastically with 16 bits hashed from the element's index and `seed`, a root above zero never to zero, and a value that is
- * not finite becomes NaN.  The parameters move by the moments before they are rounded.
+ * scale (value = code / scale), the power of two that brings the largest finite magnitude of the block into (224, 448]; codes are
+ * rounded stochastically with 16 bits hashed from the element's index and `seed`, a root above zero never to zero, and a value
+ * that is not finite becomes NaN, at no cost to its neighbours.  The parameters move by the moments before they are rounded.
  * Tensors must not overlap, and lie below 2^48 (NTFP8_ERR_UNSUPPORTED).  An empty tensor (n = 0) is passed over. */
 #define NTOPS_ADAMW_BLOCK 256
 typedef struct ntops_adamw_tensor {

@@ -14,6 +14,8 @@
 //     6 %); rounded to nearest it would never fall.  The 16 bits are hashed from the element's place and the caller's seed,
 //     and both moments of an element use the same ones, so that their errors partly cancel in m / r.
 //   * r above zero keeps the smallest code: a root of zero under a first moment that is not would divide by eps.
+//   * What is not finite becomes NaN by itself: the scale is found from the block's finite values.  (A scale that made room for an
+//     infinity would leave its neighbours the smallest code alone, 2^111, whose square is infinite in the next step.)
 #include "ops_common.h"
 
 namespace ntfp8 {
@@ -175,9 +177,23 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
         }
         mt = wave_most(mt);
         rt = wave_most(rt);
+        uint32_t mbad = 0, rbad = 0;   // 0x7f in the byte of an element that is not finite, NaN whatever its sign
+        if (max(mt, rt) >= kInfBits) {   // uniform: a block with such an element in it, of which only the others count
+            mt = rt = 0;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                const uint32_t mb = __float_as_uint(m[e]) & 0x7fffffffu, rb = __float_as_uint(r[e]) & 0x7fffffffu;
+                if (mb >= kInfBits) mbad |= 0x7fu << (8 * e), m[e] = 0.0f;   // (whose code keeps to its byte)
+                else mt = max(mt, mb);
+                if (rb >= kInfBits) rbad |= 0x7fu << (8 * e), r[e] = 0.0f;
+                else rt = max(rt, rb);
+            }
+            mt = wave_most(mt);
+            rt = wave_most(rt);
+        }
         const int mk = scale_exponent(mt), rk = scale_exponent(rt);
         const float mf = __uint_as_float((uint32_t)(mk + 127) << 23), rf = __uint_as_float((uint32_t)(rk + 127) << 23);
-        uint32_t mw = 0, rw = 0;
+        uint32_t mw = mbad, rw = rbad;
 #pragma unroll
         for (int e = 0; e < kEach; e += 2) {
             const uint32_t d = dither_of((uint32_t)(i >> 1) + e / 2, s.seed);
@@ -186,13 +202,6 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
                 const uint32_t d16 = h ? d >> 16 : d & 0xffffu, bits = __float_as_uint(m[e + h]);
                 mw |= (encode(__builtin_fabsf(m[e + h]), mf, d16) | ((bits >> 24) & 0x80u)) << (8 * (e + h));
                 rw |= max(encode(r[e + h], rf, d16), min(__float_as_uint(r[e + h]), 1u)) << (8 * (e + h));
-            }
-        }
-        if (max(mt, rt) >= kInfBits) {   // uniform: a block with something that is not finite in it
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-                if ((__float_as_uint(m[e]) & 0x7fffffffu) >= kInfBits) mw |= 0x7fu << (8 * e);
-                if ((__float_as_uint(r[e]) & 0x7fffffffu) >= kInfBits) rw |= 0x7fu << (8 * e);
             }
         }
         if (left == kEach) {

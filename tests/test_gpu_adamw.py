@@ -397,3 +397,27 @@ def test_offsets_beyond_32_bits(bits):
                 assert ((got.double() - value).abs() <= value.abs() / 8 + 2.0 ** -9 / each).all()
     del p, g
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bad_gradient_costs_its_own_elements(dtype, value):
+    """8-bit moments: one step with gradients that are not finite, three with finite ones.  Only those elements are lost: their
+    neighbours' codes and scales, and the parameters that the next steps make of them, are as if the block held nothing else."""
+    n, where = 1500, [0, 5, 255, 700, 702, 1499]
+    p, g, m, v = draw(n, dtype, torch.float32, 3)
+    st = packed(n, m, v.sqrt())
+    bad = torch.zeros(n, dtype=torch.bool, device=DEV)
+    bad[where] = True
+    bad[256:512] = True      # a block with nothing else in it
+    for step in range(2, 6):
+        grad = torch.where(bad, value, g) if step == 2 else g * (step - 3.5)
+        old = (p.clone(), dequantize_moment(st[0], st[1]), dequantize_moment(st[2], st[3]))
+        adamw_8bit_step([p], [grad], *([t] for t in st), step=step, seed=step, **HYPER)
+        assert torch.equal(p.isnan(), bad), step
+        want, bound = exact(old[0], grad, old[1], old[2].double() ** 2, step=step, **HYPER)
+        near(p[~bad], want[0][~bad], bound[0][~bad], f"param in step {step}")
+        for codes, scales, value_of, off, root in ((st[0], st[1], want[1], bound[1], False), (st[2], st[3], want[2].sqrt(), 8 * U32 * want[2].sqrt(), True)):
+            assert torch.equal(dequantize_moment(codes, scales).isnan(), bad), step
+            clean = [torch.where(bad, torch.zeros_like(t), t) for t in (codes, value_of, off)]
+            check_codes(clean[0], scales, clean[1], clean[2], root)
