@@ -62,7 +62,8 @@ int ntops_adamw_unpack(const void* codes, const float* scale, int64_t n, float* 
 
 /* Softmax cross entropy of the logits x weight^T under int64 labels, the logits never in memory as such.
  *   x [tokens, hidden], weight [vocab, hidden], both of x_dtype (NTFP8_BF16 or NTFP8_F16), rows x_stride / weight_stride
- *   elements apart; labels [tokens].  Products on the matrix cores with fp32 sums, the softmax's maxima and sums in fp32.
+ *   elements apart (any number; more than 2^22, or no multiple of 8: a copy in the workspace); labels [tokens].  hidden and vocab
+ *   at most 2^22.  Products on the matrix cores with fp32 sums, the softmax's maxima and sums in fp32.
  * Outputs: losses [tokens] fp32 = logsumexp - logit of the label, 0 where the label is ignore_index, NaN where it is outside
  * [0, vocab).  loss (may be NULL): their sum, divided by the number of labels that are not ignored if `mean` (0 if all
  * are).  Gradients of `loss` (dx and dweight both NULL: none are made; each may be NULL by itself): dx [tokens, hidden]

@@ -13,6 +13,9 @@ namespace ntfp8 {
 namespace {
 
 constexpr int64_t kMostHeld = (int64_t)1 << 31;   // bytes of exponentials at a time
+// elements between rows of the products' operands: 256 of them are within reach of 32-bit offsets.  Rows further apart are copied, as
+// unaligned ones are
+constexpr int64_t kMostStride = (int64_t)1 << 22;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 int64_t held_cols(int64_t vocab) { return up(vocab, kHeadK); }
@@ -353,8 +356,8 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     p.padded = up(d.hidden, 8);
     // (with gradients the tokens that count are gathered: those that are ignored cost nothing, and what is in them, NaN say, is
     // seen by nobody)
-    p.pad_x = gradient || d.hidden % 8 || d.x_stride % 8 || reinterpret_cast<uintptr_t>(d.x) % 16;
-    p.pad_w = d.hidden % 8 || d.weight_stride % 8 || reinterpret_cast<uintptr_t>(d.weight) % 16;
+    p.pad_x = gradient || d.hidden % 8 || d.x_stride % 8 || d.x_stride > kMostStride || reinterpret_cast<uintptr_t>(d.x) % 16;
+    p.pad_w = d.hidden % 8 || d.weight_stride % 8 || d.weight_stride > kMostStride || reinterpret_cast<uintptr_t>(d.weight) % 16;
     p.logits = tiling_of_logits(p.piece, p.ldd, (p.padded + kHeadK - 1) / kHeadK);
     if (d.dx) p.dx = tiling_of_dx(p.piece, d.hidden, p.ldd / kHeadK);
     int64_t at = 0;

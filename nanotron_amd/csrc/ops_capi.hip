@@ -45,10 +45,9 @@ int check_norm(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x
 int check_head(const ntops_linear_cross_entropy_desc& d) {
     // sizes first: the workspace depends on them alone
     if (d.x_dtype != NTFP8_BF16 && d.x_dtype != NTFP8_F16) return NTFP8_ERR_ENUM;
-    // (rows of 2^22 elements keep 256 of them within reach of 32-bit offsets)
-    constexpr int64_t kMost = (int64_t)1 << 22;
+    constexpr int64_t kMost = (int64_t)1 << 22;   // (and so in head.hip)
     if (d.tokens <= 0 || d.hidden <= 0 || d.vocab <= 0 || d.tokens > ((int64_t)1 << 30) || d.hidden > kMost || d.vocab > kMost) return NTFP8_ERR_SIZE;
-    if (d.x_stride < d.hidden || d.weight_stride < d.hidden || d.x_stride > kMost || d.weight_stride > kMost) return NTFP8_ERR_SIZE;
+    if (!rows_ok(d.tokens, d.hidden, d.x_stride) || !rows_ok(d.vocab, d.hidden, d.weight_stride)) return NTFP8_ERR_SIZE;
     if ((d.dx || d.dweight) && d.grad_dtype != d.x_dtype && d.grad_dtype != NTFP8_F32) return NTFP8_ERR_ENUM;
     return NTFP8_OK;
 }

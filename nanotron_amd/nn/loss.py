@@ -20,7 +20,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     raises RuntimeError.  "none": the float32 losses of the tokens, without gradients (ValueError if any are wanted).
 
     Memory beside the gradients, freed when the call returns: 2 bytes a logit for at most 2 GiB worth of tokens at a time, a
-    copy of x, and one of weight if its rows do not begin on 16-byte boundaries.
+    copy of x, and one of weight if its rows do not begin on 16-byte boundaries or lie more than 2^22 elements apart.
     Tokens beyond that go in pieces, with the gradient of the weight summed in fp32 (4 bytes an element, freed likewise),
     which float16 inputs always use, so that a loss scale cannot overflow or underflow them."""
     return _ops.host.linear_cross_entropy(x, weight, labels, ignore_index, reduction)

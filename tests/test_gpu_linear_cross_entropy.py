@@ -399,3 +399,22 @@ def test_no_tokens_beside_a_weight_that_is_not_finite():
     loss.backward()
     assert loss.dtype == torch.float32 and loss.item() == 0.0
     assert x.grad.shape == x.shape and not w.grad.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_far_apart(dtype):
+    """The last token of every sequence of a long batch, and a weight whose rows lie as far apart: more than 2^22 elements."""
+    hidden, length, vocab = 4096, 1031, 33
+    h = torch.zeros(5, length, hidden, device=DEV, dtype=dtype)
+    x, w, labels = draw(5, hidden, vocab, dtype, 0.0, 24)
+    labels[3] = -100
+    h[:, -1] = x
+    wide = torch.zeros(vocab, (1 << 22) + 8, device=DEV, dtype=dtype)
+    wide[:, 8:8 + hidden] = w
+    assert h[:, -1].stride(0) > 1 << 22 and wide.stride(0) > 1 << 22
+    for rows, weight in ((h[:, -1], w), (x, wide[:, 8:8 + hidden]), (h[:, -1], wide[:, 8:8 + hidden])):
+        check(rows, weight, labels)
+        with torch.no_grad():
+            assert torch.equal(linear_cross_entropy(rows, weight, labels, reduction="none"), linear_cross_entropy(x, w, labels, reduction="none"))
+    del h, wide
+    torch.cuda.empty_cache()

@@ -162,3 +162,16 @@ def test_constructors_refuse():
 def test_adamw_addresses():
     for k in ("param", "grad", "exp_avg", "exp_avg_sq", "copy"):
         assert _ops.lib.ntops_adamw(tensors(**{k: 1 << 48}), 1, options(copy_dtype=nt.BF16), None) == UNSUPPORTED
+
+
+def test_linear_cross_entropy_takes_rows_far_apart():
+    """Strides are bounded by what can be addressed alone; rows further apart than tiles reach are copied, which the workspace says."""
+    size = _ops.lib.ntops_linear_cross_entropy_workspace
+    near, far = 1 << 22, (1 << 22) + 8
+    for g in (dict(), dict(dx=None, dweight=None)):
+        base = size(desc(x_stride=near, weight_stride=near, **g))
+        assert base > 0
+        assert size(desc(x_stride=far, weight_stride=near, **g)) == base + (0 if not g else 16 * 64 * 2)      # (with gradients x is gathered anyway)
+        assert size(desc(x_stride=near, weight_stride=far, **g)) == base + 1000 * 64 * 2
+    assert _ops.lib.ntops_linear_cross_entropy(desc(x_stride=(1 << 46) // 16 + 8), None) == SIZE
+    assert _ops.lib.ntops_linear_cross_entropy(desc(weight_stride=(1 << 46) // 1000 + 8), None) == SIZE
