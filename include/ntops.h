@@ -56,6 +56,9 @@ typedef struct ntops_adamw_options {
     const float* grad_scale;   /* device scalar, NULL: 1 */
 } ntops_adamw_options;
 int ntops_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options* options, void* stream);
+/* What ntops_adamw would say of these arguments, without a launch: for a caller whose step is several calls (types differ), of
+ * which none should be made if one is refused. */
+int ntops_adamw_check(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options* options);
 
 /* out = fp32 of what E4M3 codes and block scales as above stand for */
 int ntops_adamw_unpack(const void* codes, const float* scale, int64_t n, float* out, void* stream);

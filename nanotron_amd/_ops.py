@@ -46,6 +46,7 @@ SIGNATURES = {
     "ntops_layer_norm_scratch": (_i64, [_i, _i64, _i64]),
     "ntops_layer_norm_backward": (_i, [_vp, _i64, _vp, _i, _i64, _i64, _i64, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "ntops_adamw": (_i, [_c.POINTER(AdamWTensor), _i, _c.POINTER(AdamWOptions), _vp]),
+    "ntops_adamw_check": (_i, [_c.POINTER(AdamWTensor), _i, _c.POINTER(AdamWOptions)]),
     "ntops_adamw_unpack": (_i, [_vp, _vp, _i64, _vp, _vp]),
     "ntops_linear_cross_entropy_piece": (_i64, [_i64]),
     "ntops_linear_cross_entropy_workspace": (_i64, [_c.POINTER(LinearCrossEntropyDesc)]),

@@ -289,14 +289,18 @@ int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options&
 
 }  // namespace
 
-int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st) {
-    bool copies = false;
+bool adamw_within_reach(const ntops_adamw_tensor* tensors, int count) {
     for (int i = 0; i < count; ++i) {
         const ntops_adamw_tensor& t = tensors[i];
         for (const void* p : {(const void*)t.param, t.grad, (const void*)t.exp_avg, (const void*)t.exp_avg_sq, (const void*)t.exp_avg_scale, (const void*)t.exp_avg_sq_scale, (const void*)t.copy})
-            if (!within_reach(p)) return NTFP8_ERR_UNSUPPORTED;
-        copies = copies || t.copy;
+            if (!within_reach(p)) return false;
     }
+    return true;
+}
+
+int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st) {
+    bool copies = false;
+    for (int i = 0; i < count; ++i) copies = copies || tensors[i].copy;
     return with_dtype(o.param_dtype, [&](auto p) {
         constexpr int P = decltype(p)::value;
         return with_dtype(o.grad_dtype, [&](auto g) {

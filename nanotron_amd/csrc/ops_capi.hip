@@ -11,6 +11,7 @@ int run_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t col
 int run_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride,
                             const void* weight, int w_dtype, const float* mean, const float* rstd, void* dx, void* dweight, void* dbias,
                             float* scratch, hipStream_t st);
+bool adamw_within_reach(const ntops_adamw_tensor* tensors, int count);
 int run_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options& o, hipStream_t st);
 int run_adamw_unpack(const void* codes, const float* scale, int64_t n, float* out, hipStream_t st);
 int64_t head_piece(int64_t vocab);
@@ -91,7 +92,7 @@ int ntops_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, 
                                    static_cast<float*>(scratch), static_cast<hipStream_t>(stream));
 }
 
-int ntops_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options* options, void* stream) {
+int ntops_adamw_check(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options* options) {
     if (!options || (count > 0 && !tensors)) return NTFP8_ERR_NULL;
     const ntops_adamw_options& o = *options;
     if (count < 0 || o.step < 1) return NTFP8_ERR_SIZE;
@@ -115,7 +116,12 @@ int ntops_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_
             overlap(t.copy, cb, t.param, pb) || overlap(t.copy, cb, t.grad, gb) || overlap(t.copy, cb, t.exp_avg, sb) || overlap(t.copy, cb, t.exp_avg_sq, sb))
             return NTFP8_ERR_ALIAS;
     }
-    return run_adamw(tensors, count, o, static_cast<hipStream_t>(stream));
+    return adamw_within_reach(tensors, count) ? NTFP8_OK : NTFP8_ERR_UNSUPPORTED;
+}
+
+int ntops_adamw(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options* options, void* stream) {
+    if (const int rc = ntops_adamw_check(tensors, count, options)) return rc;
+    return run_adamw(tensors, count, *options, static_cast<hipStream_t>(stream));
 }
 
 int ntops_adamw_unpack(const void* codes, const float* scale, int64_t n, float* out, void* stream) {

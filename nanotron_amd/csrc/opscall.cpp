@@ -352,10 +352,15 @@ void adamw(const py::object& params_, const py::object& grads_, const py::object
         }
         at->t.push_back(t);
     }
-    for (const Kind& k : kinds) {
-        o.param_dtype = k.p, o.grad_dtype = k.g, o.copy_dtype = k.c;
-        call(ntops_adamw(k.t.data(), (int)k.t.size(), &o, stream_of(p0)), "ntops_adamw");
-    }
+    // all sets are looked over before the first is launched: a step that is refused has changed nothing
+    const auto each = [&](auto&& f) {
+        for (const Kind& k : kinds) {
+            o.param_dtype = k.p, o.grad_dtype = k.g, o.copy_dtype = k.c;
+            call(f(k.t.data(), (int)k.t.size()), "ntops_adamw");
+        }
+    };
+    if (kinds.size() > 1) each([&](const ntops_adamw_tensor* t, int count) { return ntops_adamw_check(t, count, &o); });
+    each([&](const ntops_adamw_tensor* t, int count) { return ntops_adamw(t, count, &o, stream_of(p0)); });
     // (autograd's record of in-place changes: a graph that saved a parameter or its copy finds out)
     const auto changed = [](const Tensor& t) {
         if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();

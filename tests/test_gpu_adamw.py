@@ -421,3 +421,23 @@ def test_a_bad_gradient_costs_its_own_elements(dtype, value):
             assert torch.equal(dequantize_moment(codes, scales).isnan(), bad), step
             clean = [torch.where(bad, torch.zeros_like(t), t) for t in (codes, value_of, off)]
             check_codes(clean[0], scales, clean[1], clean[2], root)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_call_has_stepped_nothing(bits):
+    """Of tensors of two sets of types the second set is refused: the first one stays as it was, too."""
+    data = [draw(1000, dtype, dtype, i) for i, dtype in enumerate((torch.bfloat16, torch.float32))]
+    params, grads = [d[0] for d in data], [data[0][1], data[1][0]]      # (the second gradient is the parameter itself)
+    state = [moments_8bit(p) for p in params] if bits == 8 else [(d[2], d[3]) for d in data]
+    held = [*params, *state[0], *state[1]]
+    before, versions = [t.clone() for t in held], [t._version for t in held]
+    with pytest.raises(RuntimeError, match="overlap"):
+        (adamw_step if bits == 32 else adamw_8bit_step)(params, grads, *map(list, zip(*state)), step=1, **HYPER, **({} if bits == 32 else dict(seed=2)))
+    assert all(torch.equal(a, b) for a, b in zip(held, before)) and versions == [t._version for t in held]
+    p = [torch.nn.Parameter(d[0].clone()) for d in data]
+    o = AdamW(p, state_bits=bits, **HYPER)
+    p[0].grad, p[1].grad = data[0][1], p[1].data
+    before = [q.detach().clone() for q in p]
+    with pytest.raises(RuntimeError, match="overlap"):
+        o.step()
+    assert all(torch.equal(q.detach(), b) for q, b in zip(p, before)) and o.state[p[0]]["step"] == 0

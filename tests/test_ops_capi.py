@@ -175,3 +175,11 @@ def test_linear_cross_entropy_takes_rows_far_apart():
         assert size(desc(x_stride=near, weight_stride=far, **g)) == base + 1000 * 64 * 2
     assert _ops.lib.ntops_linear_cross_entropy(desc(x_stride=(1 << 46) // 16 + 8), None) == SIZE
     assert _ops.lib.ntops_linear_cross_entropy(desc(weight_stride=(1 << 46) // 1000 + 8), None) == SIZE
+
+
+def test_adamw_check_says_what_a_step_would():
+    f, g = _ops.lib.ntops_adamw_check, _ops.lib.ntops_adamw
+    for t, o in ((tensors(), options(bits=8)), (tensors(), options(step=0)), (tensors(grad=P), options()), (tensors(param=P + 0x800001), options()),
+                 (tensors(exp_avg=1 << 48), options()), (tensors(n=0, param=None), options())):
+        assert f(t, 1, o) == g(t, 1, o, None)
+    assert f(tensors(), 1, options()) == 0 and f(None, 1, options()) == NULL and f(tensors(), 1, None) == NULL
