@@ -50,8 +50,14 @@ struct WholeAddresses {
 };
 template <bool k8>
 struct Entry {
-    std::conditional_t<k8, WholeAddresses<6>, Addresses<4>> at;   // parameter, gradient, moments, scales of 8-bit ones
+    Addresses<4> at;   // parameter, gradient, moments
     int n;
+};
+template <>
+struct Entry<true> {
+    WholeAddresses<6> at;   // and the scales of both moments
+    int n;
+    uint32_t pair;          // number of the first pair of elements in its tensor, which may have several entries
 };
 template <bool k8, bool kCopy>
 struct Step {
@@ -196,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(const Step<k8, kCopy> s
         uint32_t mw = mbad, rw = rbad;
 #pragma unroll
         for (int e = 0; e < kEach; e += 2) {
-            const uint32_t d = dither_of((uint32_t)(i >> 1) + e / 2, s.seed);
+            const uint32_t d = dither_of(entry.pair + (uint32_t)(i >> 1) + e / 2, s.seed);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const uint32_t d16 = h ? d >> 16 : d & 0xffffu, bits = __float_as_uint(m[e + h]);
@@ -276,6 +282,7 @@ int run(const ntops_adamw_tensor* tensors, int count, const ntops_adamw_options&
             s.t[used].n = (int)n;
             s.first[used] = blocks;
             if constexpr (k8) {
+                s.t[used].pair = (uint32_t)(at >> 1);
                 s.t[used].at.set(4, t.exp_avg_scale + at / kBlock);
                 s.t[used].at.set(5, t.exp_avg_sq_scale + at / kBlock);
             }

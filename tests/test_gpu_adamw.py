@@ -441,3 +441,30 @@ def test_a_refused_call_has_stepped_nothing(bits):
     with pytest.raises(RuntimeError, match="overlap"):
         o.step()
     assert all(torch.equal(q.detach(), b) for q, b in zip(p, before)) and o.state[p[0]]["step"] == 0
+
+
+def test_dither_of_a_tensor_beyond_a_launch():
+    """Codes are rounded by the hash of the element's index in its tensor, also where a launch takes the tensor in parts (of
+    2^30 elements): the hash in Python's integers says which of the two neighbours of 0.7371 every element gets."""
+    n, seed = (1 << 30) + 5003, 77
+    p, g = torch.zeros(n, device=DEV, dtype=torch.bfloat16), torch.full((n,), 0.7371, device=DEV, dtype=torch.bfloat16)
+    g[::256] = 1.0      # the blocks' largest: a scale of 256
+    state = moments_8bit(p)
+    adamw_8bit_step([p], [g], *([t] for t in state), lr=0.0, betas=(0.0, 0.0), step=1, seed=seed)
+    assert (state[1] == 256).all()
+
+    def code(i, value):
+        mask = 0xFFFFFFFF
+        x = ((i >> 1) * 0x9E3779B1 + seed * 0xBB67AE85) & mask
+        x = (x ^ x >> 15) * 0x6A09E667 & mask
+        x = (x ^ x >> 13) * 0x3C6EF373 & mask
+        x ^= x >> 16
+        bits = torch.tensor(value * 256).view(torch.int32).item()
+        return ((bits + ((x >> 16 if i & 1 else x & 0xFFFF) << 4)) >> 20) - 960
+
+    value = g[1].item()
+    for first in (0, (1 << 30) - 512, 1 << 30, n - 512):
+        want = [code(i, 1.0 if i % 256 == 0 else value) for i in range(first, first + 512)]
+        assert len(set(want)) == 3 and state[0][first:first + 512].tolist() == want, first
+    del p, g, state
+    torch.cuda.empty_cache()
