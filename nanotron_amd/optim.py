@@ -59,7 +59,7 @@ class AdamW(torch.optim.Optimizer):
     (what an FP8Linear with a 16-bit master leaves in fp32), or else the `.grad` of its copy (`grad_of`); zero_grad() clears
     all three.  `grad_scale` of step() multiplies all gradients (a clipping factor left on the device).  Every parameter
     counts its own steps.  `seed` shifts the stochastic rounding of 8-bit moments.  State dicts hold the moments as they are,
-    and no copies."""
+    and no copies; one of torch.optim.AdamW is taken over with its 32-bit moments (ValueError for amsgrad or maximize)."""
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0):
@@ -110,15 +110,28 @@ class AdamW(torch.optim.Optimizer):
         return d
 
     def load_state_dict(self, state_dict: dict) -> None:
-        copies = [g["copies"] for g in self.param_groups]
+        for g in state_dict["param_groups"]:   # (of torch.optim.AdamW or Adam)
+            for name in ("amsgrad", "maximize"):
+                if g.get(name):
+                    raise ValueError(f"AdamW has no {name}, with which this state was made")
+            if not g.get("decoupled_weight_decay", True) and g["weight_decay"]:
+                raise ValueError("AdamW decays weights decoupled from their gradients (decoupled_weight_decay), this state's optimizer did not")
+        own = [{k: g[k] for k in ("copies", "seed")} for g in self.param_groups]
         super().load_state_dict(state_dict)
-        for g, c in zip(self.param_groups, copies):
-            g["copies"] = c
-        # (the base class casts state to the parameter's type; moments keep theirs)
+        for g, kept in zip(self.param_groups, own):
+            g["copies"] = kept["copies"]
+            # what torch's groups do not say: moments that are not codes are 32-bit ones
+            g.setdefault("seed", kept["seed"])
+            g.setdefault("state_bits", 32)
+        # (the base class casts state to the parameter's type; moments keep theirs, or become the fp32 that a step takes)
         for g, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, key in zip(g["params"], saved["params"]):
                 if key in state_dict["state"]:
-                    self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v for k, v in state_dict["state"][key].items()}
+                    state = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v for k, v in state_dict["state"][key].items() if k != "step"}
+                    if g["state_bits"] == 32:
+                        state = {k: v.float() if isinstance(v, torch.Tensor) else v for k, v in state.items()}
+                    # (torch counts in a tensor; parameters share launches by their number of steps)
+                    self.state[p] = {"step": int(state_dict["state"][key]["step"]), **state}
 
     @torch.no_grad()
     def step(self, closure=None, *, grad_scale: Optional[torch.Tensor] = None):

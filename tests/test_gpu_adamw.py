@@ -468,3 +468,28 @@ def test_dither_of_a_tensor_beyond_a_launch():
         assert len(set(want)) == 3 and state[0][first:first + 512].tolist() == want, first
     del p, g, state
     torch.cuda.empty_cache()
+
+
+def test_goes_on_from_a_torch_optimizer():
+    """A state dict of torch.optim.AdamW: the moments (fp32, whatever the parameters' type) and counts of steps are taken over, and
+    the next step is that of the formula."""
+    start = [draw(n, dtype, dtype, n)[0] for n, dtype in ((300, torch.float32), (700, torch.bfloat16))]
+    ref = [torch.nn.Parameter(t.clone()) for t in start]
+    theirs = torch.optim.AdamW(ref, **HYPER)
+    for k in range(3):
+        for i, p in enumerate(ref):
+            p.grad = draw(p.numel(), p.dtype, p.dtype, 10 * k + i)[1]
+        theirs.step()
+    own = [torch.nn.Parameter(p.detach().clone()) for p in ref]
+    ours = AdamW(own, lr=1.0)
+    ours.load_state_dict(theirs.state_dict())
+    for p, q in zip(own, ref):
+        assert ours.state[p]["step"] == 3 and type(ours.state[p]["step"]) is int
+        m, v = (theirs.state[q][k] for k in ("exp_avg", "exp_avg_sq"))
+        p.grad = draw(p.numel(), p.dtype, p.dtype, 99)[1]
+        want, bound = exact(p.detach(), p.grad, m, v, step=4, **HYPER)
+        q.want = want[0], bound[0]
+    ours.step()
+    for p, q in zip(own, ref):
+        near(p.detach(), *q.want, "param")
+        assert ours.state[p]["step"] == 4

@@ -183,3 +183,27 @@ def test_adamw_check_says_what_a_step_would():
                  (tensors(exp_avg=1 << 48), options()), (tensors(n=0, param=None), options())):
         assert f(t, 1, o) == g(t, 1, o, None)
     assert f(tensors(), 1, options()) == 0 and f(None, 1, options()) == NULL and f(tensors(), 1, None) == NULL
+
+
+def test_adamw_takes_the_state_of_torch():
+    p = [torch.nn.Parameter(torch.ones(4)), torch.nn.Parameter(torch.ones(3, dtype=torch.bfloat16))]
+    theirs = torch.optim.AdamW(p, lr=0.25)
+    for q in p:
+        q.grad = torch.ones_like(q)
+    theirs.step()
+    ours = AdamW(p, state_bits=8, seed=5)
+    ours.load_state_dict(theirs.state_dict())
+    group = ours.param_groups[0]
+    # (its moments are 32-bit ones)
+    assert group["lr"] == 0.25 and group["state_bits"] == 32 and group["seed"] == 5 and group["copies"] is None
+    for q in p:
+        state = ours.state[q]
+        assert type(state["step"]) is int and state["step"] == 1
+        assert state["exp_avg"].dtype == state["exp_avg_sq"].dtype == torch.float32
+        assert torch.equal(state["exp_avg"], theirs.state[q]["exp_avg"].float())
+    for kw in (dict(amsgrad=True), dict(maximize=True)):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            AdamW(p).load_state_dict(torch.optim.AdamW(p, **kw).state_dict())
+    with pytest.raises(ValueError, match="decoupled"):
+        AdamW(p).load_state_dict(torch.optim.Adam(p, weight_decay=0.1).state_dict())
+    AdamW(p).load_state_dict(torch.optim.Adam(p).state_dict())
