@@ -63,17 +63,27 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params: Iterable, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, *, state_bits: int = 32, seed: int = 0):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
-        if lr < 0 or eps < 0 or weight_decay < 0 or not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"lr, eps and weight_decay must not be negative and betas lie in [0, 1), got {lr}, {eps}, {weight_decay}, {betas}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed, copies=None))
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, seed=seed, copies=None)
+        self._check(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check(group: dict) -> None:
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+        if group["lr"] < 0 or group["eps"] < 0 or group["weight_decay"] < 0 or not all(0 <= b < 1 for b in group["betas"]):
+            raise ValueError(f"lr, eps and weight_decay must not be negative and betas lie in [0, 1), got {group['lr']}, {group['eps']}, "
+                             f"{group['weight_decay']}, {group['betas']}")
+        if group.get("params") is not None and group["copies"] is not None and len(group["copies"]) != len(group["params"]):
+            raise ValueError(f"copies must name one tensor (or None) for each of {len(group['params'])} parameters, got {len(group['copies'])}")
 
     def add_param_group(self, param_group: dict) -> None:
         super().add_param_group(param_group)
-        group = self.param_groups[-1]
-        if group.get("copies") is not None and len(group["copies"]) != len(group["params"]):
-            raise ValueError(f"copies must name one tensor (or None) for each of {len(group['params'])} parameters, got {len(group['copies'])}")
+        try:
+            self._check(self.param_groups[-1])
+        except ValueError:
+            self.param_groups.pop()
+            raise
 
     @staticmethod
     def grad_of(param: torch.Tensor, copy: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:

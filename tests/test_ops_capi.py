@@ -207,3 +207,16 @@ def test_adamw_takes_the_state_of_torch():
     with pytest.raises(ValueError, match="decoupled"):
         AdamW(p).load_state_dict(torch.optim.Adam(p, weight_decay=0.1).state_dict())
     AdamW(p).load_state_dict(torch.optim.Adam(p).state_dict())
+
+
+def test_a_refused_group_is_not_added():
+    p, q = (torch.nn.Parameter(torch.ones(4)) for _ in range(2))
+    o = AdamW([p])
+    for kw in (dict(copies=[None, None]), dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1e-8), dict(weight_decay=-0.1)):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            o.add_param_group(dict(params=[q], **kw))
+        assert [g["params"] for g in o.param_groups] == [[p]]
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            AdamW([dict(params=[q], **kw)])
+    o.add_param_group(dict(params=[q], copies=[None], state_bits=8))
+    assert len(o.param_groups) == 2
