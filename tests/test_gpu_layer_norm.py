@@ -276,3 +276,26 @@ def test_offsets_beyond_32_bits():
         near(x.grad[part], want[1], bound[1], x.dtype, "dx")
     del x, y, dy
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("cols", [1000, 7168, 100, 33, 16384])
+def test_constant_rows(cols, dtype):
+    """Rows of one value have no deviation at all, whatever the value and their length: exactly the bias comes out.  (The sum may
+    round, and the mean with it, to a neighbour of the value at most; the sum of the differences from that is small whole
+    multiples of an ulp, exact, and so is its quotient.)"""
+    values = torch.tensor([1000.0, 100.0, 1000.1, 3.3, -17.77, 0.1, 1e-3, 60000.0, 1 / 3, 0.0], device=DEV).to(dtype)
+    x = values[:, None].expand(-1, cols).contiguous()
+    b = torch.randn(cols, device=DEV)
+    assert (layer_norm(x) == 0).all()
+    assert torch.equal(layer_norm(x, torch.full((cols,), 3.0, device=DEV), b), b.to(dtype).expand(len(values), -1))
+    # backward: xhat is 0, dx = rstd (g - mean g)
+    x.requires_grad_(True)
+    w = torch.ones(cols, device=DEV, requires_grad=True)
+    dy = torch.randn(len(values), cols, device=DEV).to(dtype)
+    dx, dw = torch.autograd.grad(layer_norm(x, w), (x, w), dy)
+    assert (dw == 0).all()
+    d = dy.double()
+    want = (d - d.mean(-1, keepdim=True)) / 1e-5 ** 0.5
+    # mean(g): a tree of sums, 34 u mean|g|; a difference, a product, rstd (4 u)
+    near(dx, want, U32 / 1e-5 ** 0.5 * (34 * d.abs().mean(-1, keepdim=True) + 6 * (d.abs() + d.abs().mean(-1, keepdim=True))), dtype, "dx")
