@@ -20,7 +20,8 @@ int ntops_layer_norm_forward(const void* x, int x_dtype, int64_t rows, int64_t c
                              const void* bias, int w_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
 
 /* Gradients of the above from dy [rows, cols] (rows dy_stride apart, type of x).  dx (dense, type of x), dweight and dbias
- * (type w_dtype) may each be NULL; the sums over rows are made in fp32, in an order that depends on the sizes alone.
+ * (type w_dtype) may each be NULL; the sums over rows are made in fp32 within a workgroup and in 64 bits over them,
+ * in an order that depends on the sizes alone.
  * `scratch`: ntops_layer_norm_scratch(...) bytes, 16-byte aligned; may be NULL where neither dweight nor dbias is asked for. */
 int64_t ntops_layer_norm_scratch(int x_dtype, int64_t rows, int64_t cols);
 int ntops_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t x_stride,

@@ -10,9 +10,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """Layer normalisation over the last dimension: `(x - mean) / sqrt(var + eps) * weight + bias`.
 
     x: float32, float16 or bfloat16, any number of dimensions; the result has its type.  weight and bias ([x.shape[-1]],
-    each optional) are float32 or of the type of x.  Mean, variance, the sums of the gradients of weight and bias and all
-    arithmetic are fp32; the last two are summed in an order that depends on the sizes alone, so gradients repeat bit for
-    bit.  Rows that are dense in themselves (a slice of a wider 2-D tensor) are read where they are.  Up to 32768 columns of
+    each optional) are float32 or of the type of x.  Arithmetic is fp32; the gradients of weight and bias are
+    summed in fp32 within a workgroup and in 64 bits over them, in an order that depends on the sizes alone, so gradients
+    repeat bit for bit.  Rows that are dense in themselves (a slice of a wider 2-D tensor) are read where they are.  Up to 32768 columns of
     a 16-bit x, 16384 of float32.  ValueError / TypeError for what does not fit; differentiable once."""
     return _ops.host.layer_norm(x, weight, bias, eps)
 

@@ -299,3 +299,25 @@ def test_constant_rows(cols, dtype):
     want = (d - d.mean(-1, keepdim=True)) / 1e-5 ** 0.5
     # mean(g): a tree of sums, 34 u mean|g|; a difference, a product, rstd (4 u)
     near(dx, want, U32 / 1e-5 ** 0.5 * (34 * d.abs().mean(-1, keepdim=True) + 6 * (d.abs() + d.abs().mean(-1, keepdim=True))), dtype, "dx")
+
+
+def test_weight_gradient_of_rows_that_cancel():
+    """Two rows of dy of 2^27 that cancel, among 1019 of ones.  In 32 bits a value passes the additions in its thread and its
+    workgroup only (two rows a thread and two threads of a column here, three additions with the one onto zero, which is exact);
+    everything behind them is summed in 64.  Of four additions at 2^27 each is off by half of 16 at most."""
+    rows, cols = 1021, 1037
+    x = torch.randn(rows, cols, device=DEV)
+    dy = torch.ones(rows, cols, device=DEV)
+    dy[0], dy[-1] = 2.0 ** 27, -2.0 ** 27
+    w, b = torch.ones(cols, device=DEV, requires_grad=True), torch.zeros(cols, device=DEV, requires_grad=True)
+    y = layer_norm(x, w, b)
+    db, = torch.autograd.grad(y, b, dy, retain_graph=True)
+    assert ((db - (rows - 2)).abs() <= 4 * 8).all()
+    # the same of xhat: rows 0 and last alike, and bounded entries (xhat of two values, +-1 but for eps)
+    x = torch.ones(rows, cols - 1, device=DEV)
+    x[:, ::2] = -1.0
+    y = layer_norm(x, w[:-1])
+    dw, = torch.autograd.grad(y, w, dy[:, :-1])
+    xh = torch.where(torch.arange(cols - 1, device=DEV) % 2 == 0, -1.0, 1.0).double() / (1 + 1e-5) ** 0.5
+    # (4 additions, and the product's own rounding of the two large ones, which are alike and cancel)
+    assert ((dw[:-1] - (rows - 2) * xh).abs() <= 4 * 8 + 1e-3).all()
