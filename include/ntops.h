@@ -72,7 +72,8 @@ int ntops_adamw_unpack(const void* codes, const float* scale, int64_t n, float* 
  * [0, vocab).  loss (may be NULL): their sum, divided by the number of labels that are not ignored if `mean` (0 if all
  * are).  Gradients of `loss` (dx and dweight both NULL: none are made; each may be NULL by itself): dx [tokens, hidden]
  * dense, dweight [vocab, hidden] dense, each of x_dtype, or fp32 (grad_dtype NTFP8_F32).
- * workspace: ntops_linear_cross_entropy_workspace(...) bytes, aligned to 256.  Tokens beyond ntops_linear_cross_entropy_piece(vocab) at a
+ * workspace: ntops_linear_cross_entropy_workspace(...) bytes, aligned to 256 (2 bytes a logit of a piece and 4 an element of dx,
+ * at most 2 GiB of each, and copies of x and, if need be, weight).  Tokens beyond ntops_linear_cross_entropy_piece(vocab) at a
  * time go through it in pieces; dweight of type fp32 then collects the pieces, and a 16-bit dweight needs all tokens in
  * one piece (NTFP8_ERR_UNSUPPORTED otherwise: take fp32). */
 typedef struct ntops_linear_cross_entropy_desc {

@@ -12,7 +12,7 @@
 namespace ntfp8 {
 namespace {
 
-constexpr int64_t kMostHeld = (int64_t)1 << 31;   // bytes of exponentials at a time
+constexpr int64_t kMostHeld = (int64_t)1 << 31;   // bytes of exponentials at a time, and of sums of dx
 // elements between rows of the products' operands: 256 of them are within reach of 32-bit offsets.  Rows further apart are copied, as
 // unaligned ones are
 constexpr int64_t kMostStride = (int64_t)1 << 22;
@@ -340,6 +340,7 @@ struct Plan {
     bool pad_x, pad_w;
     int64_t padded;           // hidden, up to a multiple of 8
     Tiling logits, dx;
+    int64_t dx_rows;          // tokens at a time of dx's product: with few labels a piece has so many that its sums are the larger part
     int64_t at_factors, at_label, at_place, at_token, at_kept, at_stats, at_held, at_x, at_w, at_dx, bytes;
 };
 // tokens at a time that `each` bytes of a token allow (and a launch with a row to a block, of fewer than 2^32 threads)
@@ -359,7 +360,8 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     p.pad_x = gradient || d.hidden % 8 || d.x_stride % 8 || d.x_stride > kMostStride || reinterpret_cast<uintptr_t>(d.x) % 16;
     p.pad_w = d.hidden % 8 || d.weight_stride % 8 || d.weight_stride > kMostStride || reinterpret_cast<uintptr_t>(d.weight) % 16;
     p.logits = tiling_of_logits(p.piece, p.ldd, (p.padded + kHeadK - 1) / kHeadK);
-    if (d.dx) p.dx = tiling_of_dx(p.piece, d.hidden, p.ldd / kHeadK);
+    p.dx_rows = std::min(p.piece, std::max<int64_t>(256, kMostHeld / (4 * d.hidden) / 256 * 256));
+    if (d.dx) p.dx = tiling_of_dx(p.dx_rows, d.hidden, p.ldd / kHeadK);
     int64_t at = 0;
     auto room = [&](int64_t bytes) {
         const int64_t here = at;
@@ -377,7 +379,7 @@ Plan plan_of(const ntops_linear_cross_entropy_desc& d) {
     p.at_held = gradient ? room(p.piece * p.ldd * 2) : 0;
     p.at_x = p.pad_x ? room(d.tokens * p.padded * 2) : 0;
     p.at_w = p.pad_w ? room(d.vocab * p.padded * 2) : 0;
-    p.at_dx = d.dx ? room(up(p.piece, 32 * p.dx.mi) * d.hidden * 4 * p.dx.splits) : 0;
+    p.at_dx = d.dx ? room(up(p.dx_rows, 32 * p.dx.mi) * d.hidden * 4 * p.dx.splits) : 0;
     p.bytes = at;
     return p;
 }
@@ -417,7 +419,6 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
     if (status(launch_status())) return NTFP8_ERR_LAUNCH;
     for (int64_t row = 0; row < d.tokens; row += p.piece) {
         const int64_t rows = std::min(p.piece, d.tokens - row);
-        const bool last = row + rows == d.tokens;
         HeadGemm g = {};
         g.A = x + row * ldx * 2, g.lda = ldx, g.a_cols = (int)p.padded;
         g.B = w, g.ldb = ldw, g.b_cols = (int)p.padded, g.b_rows = 0;
@@ -430,19 +431,21 @@ int run(const ntops_linear_cross_entropy_desc& d, hipStream_t st) {
         rows_kernel<<<(unsigned)rows, 256, 0, st>>>(stats, (int)p.pieces, labels + row, d.ignore_index, label_logit + row, gradient ? d.losses : d.losses + row, count, (int)row,
                                                     gradient ? token_of + row : nullptr, held, p.ldd);
         if (status(launch_status())) return NTFP8_ERR_LAUNCH;
-        if (d.dx) {
+        for (int64_t at = 0; d.dx && at < rows; at += p.dx_rows) {
+            const int64_t some = std::min(p.dx_rows, rows - at), row0 = row + at;
+            float* const loss = row0 + some == d.tokens ? d.loss : nullptr;
             HeadGemm h = {};
-            h.A = held, h.lda = p.ldd, h.a_cols = (int)p.ldd;
+            h.A = held + at * p.ldd, h.lda = p.ldd, h.a_cols = (int)p.ldd;
             h.B = w, h.ldb = ldw, h.b_cols = (int)p.padded, h.b_rows = (int)d.vocab;
-            h.M = (int)rows, h.N = (int)d.hidden, h.K = (int)p.ldd;
-            h.rows = count, h.row0 = (int)row;
+            h.M = (int)some, h.N = (int)d.hidden, h.K = (int)p.ldd;
+            h.rows = count, h.row0 = (int)row0;
             h.D = ws + p.at_dx, h.d_dtype = d.grad_dtype, h.alpha = factors + 1;
-            h.groups = (int)tiles_of(rows, d.hidden, p.dx.mi) * p.dx.splits;
+            h.groups = (int)tiles_of(some, d.hidden, p.dx.mi) * p.dx.splits;
             if (status(launch_gemm<T, false, true, kPartial>(h, p.dx.mi, st))) return NTFP8_ERR_LAUNCH;
             auto put = d.grad_dtype == T ? put_rows_kernel<T> : put_rows_kernel<NTFP8_F32>;
             const int64_t n = d.tokens * ((d.hidden + 7) / 8);
-            put<<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192) + (last && d.loss ? 1 : 0), 256, 0, st>>>(
-                ws + p.at_dx, h.groups, 32 * p.dx.mi, (int)((d.hidden + kBigN - 1) / kBigN), (int)(p.ldd / kHeadK), count, factors, place, d.tokens, (int)row, (int)rows, (int)d.hidden, d.dx, d.losses, last ? d.loss : nullptr);
+            put<<<(unsigned)std::min<int64_t>((n + 255) / 256, 8192) + (loss ? 1 : 0), 256, 0, st>>>(
+                ws + p.at_dx, h.groups, 32 * p.dx.mi, (int)((d.hidden + kBigN - 1) / kBigN), (int)(p.ldd / kHeadK), count, factors, place, d.tokens, (int)row0, (int)some, (int)d.hidden, d.dx, d.losses, loss);
             if (status(launch_status())) return NTFP8_ERR_LAUNCH;
         }
         if (d.dweight) {

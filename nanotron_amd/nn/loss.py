@@ -19,9 +19,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
     hand (three products in all, no recomputation), and handed to autograd once: a second backward through the same loss
     raises RuntimeError.  "none": the float32 losses of the tokens, without gradients (ValueError if any are wanted).
 
-    Memory beside the gradients, freed when the call returns: 2 bytes a logit for at most 2 GiB worth of tokens at a time, a
-    copy of x, and one of weight if its rows do not begin on 16-byte boundaries or lie more than 2^22 elements apart.
-    Tokens beyond that go in pieces, with the gradient of the weight summed in fp32 (4 bytes an element, freed likewise),
+    Memory beside the gradients, freed when the call returns: 2 bytes a logit for at most 2 GiB worth of tokens at a time, sums
+    of the gradient of x in fp32 (4 bytes an element, at most 2 GiB at a time, or 256 MiB where there are few tokens), a copy of
+    x, and one of weight if its rows do not begin on 16-byte boundaries or lie more than 2^22 elements apart.
+    Tokens beyond 2 GiB of logits go in pieces, with the gradient of the weight summed in fp32 (4 bytes an element, freed likewise),
     which float16 inputs always use, so that a loss scale cannot overflow or underflow them."""
     return _ops.host.linear_cross_entropy(x, weight, labels, ignore_index, reduction)
 

@@ -418,3 +418,27 @@ def test_rows_far_apart(dtype):
             assert torch.equal(linear_cross_entropy(rows, weight, labels, reduction="none"), linear_cross_entropy(x, w, labels, reduction="none"))
     del h, wide
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+def test_dx_in_pieces_of_its_own(reduction):
+    """So many tokens of so few labels that all logits are held at once and the sums of dx are not: its rows on both sides
+    of where a piece ends (2^31 bytes of sums, 65280 rows here), ignored ones among them, and the weight's whole gradient."""
+    tokens, hidden, vocab = 70001, 8200, 301
+    x, w, labels = draw(tokens, hidden, vocab, torch.bfloat16, 0.05, 23)
+    a, b = x.requires_grad_(True), w.requires_grad_(True)
+    linear_cross_entropy(a, b, labels, reduction=reduction).backward()
+    x, w = x.detach(), w.detach()
+    count = int((labels != -100).sum())
+    f = 1.0 / count if reduction == "mean" else 1.0
+    assert 65280 < count < 65280 + 2000
+    dw, bw = torch.zeros(vocab, hidden, device=DEV, dtype=torch.float64), torch.zeros(vocab, hidden, device=DEV, dtype=torch.float64)
+    for r in range(0, tokens, 10000):
+        part = slice(r, min(tokens, r + 10000))
+        want, bound = exact(x[part], w, labels[part], mean=False)
+        near(a.grad[part], want[2] * f, bound[2] * f, f"dx of {r}")
+        dw += want[3] * f
+        bw += bound[3] * f
+    near(b.grad, dw, bw, "dweight")
+    del a, b, x, w, dw, bw
+    torch.cuda.empty_cache()

@@ -220,3 +220,16 @@ def test_a_refused_group_is_not_added():
             AdamW([dict(params=[q], **kw)])
     o.add_param_group(dict(params=[q], copies=[None], state_bits=8))
     assert len(o.param_groups) == 2
+
+
+def test_workspace_of_many_tokens_of_few_labels():
+    """Beside the logits, the sums of dx in fp32, at most 2 GiB of each, with 8 bytes for 128 logits and 24 for a token on top."""
+    size = _ops.lib.ntops_linear_cross_entropy_workspace
+    for tokens, hidden, vocab in ((1 << 18, 8192, 1000), (1 << 16, 8192, 8000), (1 << 17, 16384, 500), (70000, 8200, 300), (4096, 4096, 128000), (3000, 65536, 1000)):
+        logits = min(1 << 31, 2 * tokens * (vocab + 63))
+        dx = min(1 << 31, 4 * (tokens + 255) * hidden)
+        # fewer rows than the chip has room for are cut into runs of the vocabulary: 1024 tiles of 256 x 256 at most
+        dx = max(dx, 1024 << 18)
+        d = desc(tokens=tokens, hidden=hidden, vocab=vocab, x_stride=hidden, weight_stride=hidden)
+        assert size(d) <= logits * 1.04 + dx + 2 * tokens * hidden + 24 * tokens + (1 << 16), (tokens, hidden, vocab)
+        assert size(desc(tokens=tokens, hidden=hidden, vocab=vocab, x_stride=hidden, weight_stride=hidden, dx=None)) <= logits * 1.04 + 2 * tokens * hidden + 24 * tokens + (1 << 16)
