@@ -31,8 +31,8 @@ int ntops_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, 
 /* One AdamW step over `count` tensors, all of one set of types:
  *   g = grad * *grad_scale;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   param = param (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * in fp32, every operation rounded by itself; param is rounded once to its type, and once more to copy_dtype into `copy`
- * where one is given.  bits 32: exp_avg and exp_avg_sq are fp32 m and v.  bits 8: exp_avg holds E4M3 codes of m and exp_avg_sq
+ * in fp32, every operation rounded by itself; the new value is rounded once to the type of param, and, by itself, to copy_dtype
+ * into `copy` where one is given.  bits 32: exp_avg and exp_avg_sq are fp32 m and v.  bits 8: exp_avg holds E4M3 codes of m and exp_avg_sq
  * those of sqrt(v); every NTOPS_ADAMW_BLOCK elements (counted from the tensor's start, the last block may be short) share a
  * scale (value = code / scale), the power of two that brings the largest finite magnitude of the block into (224, 448]; codes are
  * rounded stochastically with 16 bits hashed from the element's index and `seed`, a root above zero never to zero, and a value

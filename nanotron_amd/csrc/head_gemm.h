@@ -46,7 +46,10 @@ constexpr bool keeps(int epilogue) { return epilogue >= kSoftmax; }
 // are at the cost of the kernels behind.  So they are left there where K is long, or where the kernel behind finds them there.  us, through / left:
 //   logits, with the pass over their rows: 4096 tokens, 4096 hidden, 128000 labels 3535 / 3475; 2048, 4096, 32000 452 / 440; 4096, 2048,
 //   50000 810 / 832; 766, 1024, 50001 133 / 130 and 4 more in the product behind; a step of 256, 2048, 50000 294 / 285
+//   logits of 4096 tokens, 50000 labels at 40, 50, 56 and 64 K-tiles 949 / 980, 1121 / 1115, 1209 / 1204, 1357 / 1340; of 128000 at 56 3190 / 3100
 //   weight gradients: 128000 x 4096 of 4096 tokens 3294 / 3212; 50001 x 1024 of 766 93 / 93 and 10 more in the kernels behind
+//   50000 x 4096 at 24, 40, 56 and 64 K-tiles 528 / 543, 825 / 837, 1088 / 1106, 1262 / 1274; 128000 x 3584 at 64 2815 / 2792
+// So logits turn at about 48 K-tiles, weight gradients at 64 or behind, by their size; one bound for both costs either 3 % at most.
 constexpr int kLongK = 64;                                // K-tiles
 constexpr int64_t kFoundBytes = (int64_t)64 << 20;        // exponentials
 

@@ -196,7 +196,8 @@ Head head(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore
     return h;
 }
 
-// the gradients times what arrives from above, of type `to`
+// The gradients times what arrives from above, of type `to`.  bf16 ones are rounded a second time here unless that is a power of two,
+// by 2^-8 of their value at most: held in fp32 until now they would take twice the memory and the way to it.
 void scale(Tensor* const (&t)[2], const Tensor& factor, at::ScalarType to) {
     ntops_scale_tensor d[2];
     int n = 0, from = -1;

@@ -17,7 +17,9 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, labels: torch.Te
 
     reduction "mean" or "sum": a float32 scalar.  Both gradients are made in the forward call, where the softmax is at
     hand (three products in all, no recomputation), and handed to autograd once: a second backward through the same loss
-    raises RuntimeError.  "none": the float32 losses of the tokens, without gradients (ValueError if any are wanted).
+    raises RuntimeError.  bfloat16 gradients are rounded there, and a second time by a factor from above that is no power of
+    two (a loss divided by three accumulated batches); float16 ones are fp32 until then.  "none": the float32 losses of the
+    tokens, without gradients (ValueError if any are wanted).
 
     Memory beside the gradients, freed when the call returns: 2 bytes a logit for at most 2 GiB worth of tokens at a time, sums
     of the gradient of x in fp32 (4 bytes an element, at most 2 GiB at a time, or 256 MiB where there are few tokens), a copy of

@@ -18,7 +18,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     on one device.  Arithmetic is fp32; a 16-bit parameter is rounded to nearest once a step.  grad_scale (one float32 on the
     device: a clipping factor, the inverse of a loss scale) multiplies every gradient.  lr and step are part of the launch: a
     captured graph repeats them.  copies: for each parameter a tensor
-    (or None) that receives its new value in that tensor's type, as the 16-bit weights beside fp32 masters."""
+    (or None) that receives its new value, rounded from fp32 to that tensor's type, as the 16-bit weights beside fp32 masters."""
     _ops.host.adamw(params, grads, exp_avgs, exp_avg_sqs, None, None, copies, lr, betas[0], betas[1], eps, weight_decay, step, 0, grad_scale)
 
 
