@@ -4,7 +4,7 @@
 // the registers of the threads that read it (a 16-byte piece a thread up to 1024 threads), so that the mean
 // and then the variance about it, a sum of squared differences and not a difference of squares, cost no second read, nor does
 // what the mean was off by.
-// 16384 rows of 8192 bf16: forward 109 us, 537 MB at 4.9 TB/s, backward 159 to 168 us, 823 MB at 4.9 to 5.2; 4096 rows of
+// 16384 rows of 8192 bf16: forward 105 to 116 us, 537 MB at 4.6 to 5.1 TB/s, backward 159 to 168 us, 823 MB at 4.9 to 5.2; 4096 rows of
 // 4096 16 and 21 us; one row of 4096 2.5 us.
 #include "ops_common.h"
 
@@ -55,7 +55,7 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float2* at) {
 template <int D, int W, int TPR, int VPT>
 __global__ __launch_bounds__(forward_block(TPR)) void layer_norm_forward_kernel(const Norm n) {
     constexpr int kBlock = forward_block(TPR), VE = 16 / size_of(D);
-    __shared__ float2 sums[2][kBlock / 64];
+    __shared__ float2 sums[3][kBlock / 64];
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * (kBlock / TPR) + threadIdx.x / TPR;
     const bool live = row < n.rows;   // (rows that share a block share its barriers)
@@ -86,29 +86,47 @@ __global__ __launch_bounds__(forward_block(TPR)) void layer_norm_forward_kernel(
         for (int e = 0; e < VE; ++e) sum += v[k][e];   // (zeros behind the row's end)
     }
     row_sums<TPR>(sum, none, sums[0]);
-    // This mean may be an ulp or two off, of which rstd makes 0.02 in a row of 1000.1s.  The differences' own mean, summed beside their
-    // squares, is what is missing; divided and not multiplied, so that equal differences leave nothing.  (16384 rows of 8192:
-    // 105.0 us without, 108.8 so)
-    const float over = 1.0f / (float)n.cols, about = sum * over;
-    float var = 0.0f, rest = 0.0f;
+    const float over = 1.0f / (float)n.cols;
+    float mean = sum * over, var = 0.0f;
+    none = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int c = (t + k * TPR) * VE;
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-            const float d = c + e < n.cols ? v[k][e] - about : 0.0f;
+            const float d = c + e < n.cols ? v[k][e] - mean : 0.0f;
             v[k][e] = d;
             var += d * d;
-            rest += d;
         }
     }
-    row_sums<TPR>(var, rest, sums[1]);
-    rest /= (float)n.cols;
-    var = var * over - rest * rest;   // (next to nothing is taken away)
-    const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + n.eps);
+    row_sums<TPR>(var, none, sums[1]);
+    var *= over;
+    // The mean may be an ulp or two off, of which rstd makes 0.02 in a row of 1000.1s.  In rows whose mean is more than 16 deviations
+    // it is corrected by the differences' own mean, divided and not multiplied, so that equal differences leave nothing; in others it
+    // is good to 2^-15 of a deviation.  (For every row, beside the squares, it took 109 us instead of 105 for 16384 rows of 8192, and
+    // 280 instead of 214 for 8192 of 32768, whose registers it overran; so, 112 and 218 where all rows are such, 105 and 214 where none is.)
+    bool far = mean * mean > 256.0f * var;
+    if constexpr (TPR > 64 && kBlock > TPR) far = __syncthreads_or(far);   // (rows that share barriers take them together)
+    if (far) {
+        float rest = 0.0f;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) rest += v[k][e];   // (zeros behind the row's end)
+        row_sums<TPR>(rest, none, sums[2]);
+        rest /= (float)n.cols;
+        mean += rest;
+        var -= rest * rest;
+        var = var < 0.0f ? 0.0f : var;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) v[k][e] -= rest;
+    }
+    const float rstd = 1.0f / sqrtf(var + n.eps);
     if (!live) return;
     if (t == 0 && n.mean) {
-        n.mean[row] = about + rest;
+        n.mean[row] = mean;
         n.rstd[row] = rstd;
     }
 #pragma unroll
@@ -119,7 +137,7 @@ __global__ __launch_bounds__(forward_block(TPR)) void layer_norm_forward_kernel(
         float y[VE];
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-            y[e] = (v[k][e] - rest) * rstd;
+            y[e] = v[k][e] * rstd;
             if (n.weight) y[e] *= w[k][e];
             if (n.bias) y[e] += b[k][e];
         }

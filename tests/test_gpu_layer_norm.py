@@ -321,3 +321,18 @@ def test_weight_gradient_of_rows_that_cancel():
     xh = torch.where(torch.arange(cols - 1, device=DEV) % 2 == 0, -1.0, 1.0).double() / (1 + 1e-5) ** 0.5
     # (4 additions, and the product's own rounding of the two large ones, which are alike and cancel)
     assert ((dw[:-1] - (rows - 2) * xh).abs() <= 4 * 8 + 1e-3).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(11, 200), (7, 1000), (9, 1500), (6, 4000), (5, 8192), (4, 16384)])
+def test_rows_far_from_zero(rows, cols):
+    """Every other row 1000 deviations from zero, beside ordinary ones.  There the mean's own error is taken out: a difference is exact
+    or off by u, the rest of the mean by 32 u of a deviation, rstd by 36 u."""
+    x, w, b, dy = inputs(rows, cols, torch.float32, torch.float32, seed=cols)
+    x[::2] += 1000.0
+    want, bound = exact(x, w, b, dy, 1e-5)
+    y = layer_norm(x, w, b)
+    near(y, want[0], bound[0], torch.float32, "y")
+    xd = x.double()
+    xh = (xd - xd.mean(-1, keepdim=True)) * (xd.var(-1, unbiased=False, keepdim=True) + 1e-5).rsqrt()
+    far = U32 * (32 + 40 * xh.abs()) * w.double().abs() + 2 * U32 * (xh * w.double()).abs() + U32 * want[0].abs()
+    near(y[::2], want[0][::2], far[::2], torch.float32, "y of the rows far from zero")
