@@ -81,7 +81,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         try:
             self._check(self.param_groups[-1])
-        except ValueError:
+        except Exception:   # (a TypeError of the comparisons among them)
             self.param_groups.pop()
             raise
 

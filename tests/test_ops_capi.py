@@ -233,3 +233,11 @@ def test_workspace_of_many_tokens_of_few_labels():
         d = desc(tokens=tokens, hidden=hidden, vocab=vocab, x_stride=hidden, weight_stride=hidden)
         assert size(d) <= logits * 1.04 + dx + 2 * tokens * hidden + 24 * tokens + (1 << 16), (tokens, hidden, vocab)
         assert size(desc(tokens=tokens, hidden=hidden, vocab=vocab, x_stride=hidden, weight_stride=hidden, dx=None)) <= logits * 1.04 + 2 * tokens * hidden + 24 * tokens + (1 << 16)
+
+
+def test_a_group_of_wrong_types_is_not_added():
+    o = AdamW([torch.nn.Parameter(torch.ones(4))])
+    for kw in (dict(copies=iter([None])), dict(lr="high"), dict(betas=0.9)):
+        with pytest.raises(TypeError):
+            o.add_param_group(dict(params=[torch.nn.Parameter(torch.ones(4))], **kw))
+        assert len(o.param_groups) == 1
