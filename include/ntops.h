@@ -1,6 +1,6 @@
 /* ntops — C ABI of the operators that stand beside the FP8 linears in a training step (MI355X, gfx950): layer
- * normalisation, the vocabulary projection with its softmax cross entropy, and AdamW over many tensors.  They live in the
- * same library as the entry points of ntfp8.h and follow its conventions: device pointers owned by the caller, nothing
+ * normalisation, the norms around a block with its gate and residual, rotary positions, attention, the vocabulary projection with
+ * its softmax cross entropy, and AdamW over many tensors.  They live in the same library as the entry points of ntfp8.h and follow its conventions: device pointers owned by the caller, nothing
  * allocated, freed or synchronised, argument errors returned as NTFP8_ERR_* before anything is launched, element types
  * NTFP8_F32 / NTFP8_F16 / NTFP8_BF16, `stream` a hipStream_t.  Row strides are in elements. */
 #ifndef NTOPS_H
@@ -100,6 +100,112 @@ typedef struct ntops_scale_tensor {
     int64_t n;
 } ntops_scale_tensor;
 int ntops_scale(const ntops_scale_tensor* tensors, int count, int x_dtype, const float* factor, int out_dtype, void* stream);
+
+/* Root-mean-square norms around a block, over rows of `cols` elements (16384 at most of a 16-bit x, 8192 of fp32):
+ *   p = x / rms(x) * post_weight, or x where post_weight is NULL;  rms(x) = root(mean(x^2) + eps)
+ *   h = residual_scale * residual + gate * p, rounded to residual_dtype;  y = h / rms(h) * weight of the rounded h, rounded to x_dtype
+ * in fp32.  residual NULL: the norm alone, y = x / rms(x) * weight, without post_weight, gate and h.  x, y: x_dtype; residual, h:
+ * residual_dtype (fp32, or x_dtype); weight, post_weight [cols] (each may be NULL) and a channel's gate [cols]: w_dtype (fp32, or x_dtype).
+ * gate_kind NTOPS_GATE_NONE, NTOPS_GATE_CHANNEL, or NTOPS_GATE_ELEMENT (a gate of x_dtype for every element, rows gate_stride apart).
+ * y and h are dense; rows of x and residual lie x_stride and residual_stride elements apart.  first and second [rows] fp32 receive 1 / rms
+ * of x (where post_weight is given) and of h for a backward pass; both NULL if none follows. */
+#define NTOPS_GATE_NONE 0
+#define NTOPS_GATE_CHANNEL 1
+#define NTOPS_GATE_ELEMENT 2
+typedef struct ntops_rms_norm_desc {
+    const void* x;
+    const void* residual;
+    const void* gate;
+    const void* weight;
+    const void* post_weight;
+    int64_t rows, cols, x_stride, residual_stride, gate_stride;
+    int x_dtype, residual_dtype, w_dtype, gate_kind;
+    float eps, residual_scale;
+    void* y;
+    void* h;
+    float* first;
+    float* second;
+} ntops_rms_norm_desc;
+int ntops_rms_norm_forward(const ntops_rms_norm_desc* d, void* stream);
+
+/* Gradients of the above from dy (type of x) and dh (type of h), either of which may be NULL (nothing arrives there), rows dy_stride and
+ * dh_stride apart.  Of the desc: x, gate, weights, h (NULL: there was no residual), first, second, strides, types, eps and
+ * residual_scale; y and residual are not read.  dx (dense, type of x), dresidual (dense, type of h), dweight, dpost_weight (w_dtype) and dgate (as the
+ * gate; dense) may each be NULL.  Sums over rows are made in fp32 within a workgroup and in 64 bits over them, in an order that
+ * depends on the sizes alone.  scratch: ntops_rms_norm_scratch(...) bytes, 16-byte aligned, for the gradients that are such sums. */
+typedef struct ntops_rms_norm_grads {
+    const void* dy;
+    const void* dh;
+    int64_t dy_stride, dh_stride;
+    void* dx;
+    void* dresidual;
+    void* dgate;
+    void* dweight;
+    void* dpost_weight;
+    void* scratch;
+} ntops_rms_norm_grads;
+int64_t ntops_rms_norm_scratch(const ntops_rms_norm_desc* d);
+int ntops_rms_norm_backward(const ntops_rms_norm_desc* d, const ntops_rms_norm_grads* g, void* stream);
+
+/* Rotary positions: the first 2 * pairs elements of every head of q and k are turned, pair i by angle = position * frequencies[i]:
+ *   (a, b) -> (a cos - b sin, b cos + a sin) * scale;  `inverse`: by -angle (what a backward pass does with the gradients)
+ * a and b lie side by side (`interleaved`) or `pairs` elements apart; elements behind 2 * pairs are copied.  Angles are made in 64 bits, sines,
+ * cosines and products in fp32.  q [tokens][heads][head_dim] with q_stride elements between tokens and q_head between heads, k likewise; k (or q) may be NULL
+ * with kv_heads (heads) 0.  q_out and k_out are dense.  Token t is at positions[t mod position_count] (int32 or int64, by
+ * position_bits).  head_dim <= 2048, heads + kv_heads <= 16384. */
+typedef struct ntops_rotary_desc {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    int64_t tokens, q_stride, q_head, k_stride, k_head;
+    int heads, kv_heads, head_dim, pairs, dtype;
+    const void* positions;
+    int64_t position_count;
+    int position_bits;
+    const double* frequencies;   /* [pairs] radians a position */
+    int interleaved, inverse;
+    float scale;
+} ntops_rotary_desc;
+int ntops_rotary(const ntops_rotary_desc* d, void* stream);
+
+/* Attention: out = softmax(scale q k^T) v, a head of q each; heads of q share those of k and v (heads a multiple of kv_heads, head h
+ * reads kv head h / (heads / kv_heads)).  Rows of tokens: q [q_rows][heads][head_dim], k and v [k_rows][kv_heads][head_dim], elements
+ * between rows q_stride, k_stride, v_stride, between heads q_head, k_head, v_head, all multiples of 8, on 16-byte boundaries.
+ * Sequences: packed, sequence s being rows cu_q[s] .. cu_q[s + 1] - 1 of q and cu_k[s] .. cu_k[s + 1] - 1 of k and v (device
+ * memory, int32 [sequences + 1], not decreasing; offsets outside the rows that there are count as the nearest inside); or cu_q and cu_k NULL, `sequences` of equal
+ * lengths q_rows / sequences and k_rows / sequences, q_batch, k_batch, v_batch elements apart.
+ * causal: row i of a sequence of n queries and m keys sees the keys 0 .. m - n + i, so that the last rows of both belong together.  A
+ * row that sees no key, and a row of q that belongs to no sequence, is 0, and so are its gradients; what is in rows of k and v
+ * that a row does not see, NaN say, does not reach it.
+ * head_dim <= 128, a multiple of 8; scale > 0; dtype NTFP8_BF16 or NTFP8_F16.  Scores, maxima, sums and outputs are fp32 until the one rounding of
+ * out; the softmax's numerators are rounded to dtype for the product with v.  out is dense; lse [heads][q_rows] fp32 (base 2) is what a
+ * backward pass needs, NULL if none follows.  q_rows * heads and k_rows * kv_heads at most 2^27.
+ * workspace: ntops_attention_workspace(d, backward) bytes, aligned to 256.
+ * Backward: dq, dk, dv (dense, dtype, each may be NULL) from dout (strides as q's) and the q, k, v, out and lse of the forward call.
+ * The same inputs give the same bits.  fp16: p and ds are kept with powers of two on them, so that gradients below its normal range survive. */
+typedef struct ntops_attention_desc {
+    const void* q;
+    const void* k;
+    const void* v;
+    int64_t q_stride, k_stride, v_stride, q_head, k_head, v_head, q_batch, k_batch, v_batch;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    int64_t sequences, q_rows, k_rows;
+    int heads, kv_heads, head_dim, dtype, causal;
+    float scale;
+    void* out;
+    float* lse;
+    void* workspace;
+    const void* dout;
+    int64_t do_stride, do_head, do_batch;
+    void* dq;
+    void* dk;
+    void* dv;
+} ntops_attention_desc;
+int64_t ntops_attention_workspace(const ntops_attention_desc* d, int backward);
+int ntops_attention_forward(const ntops_attention_desc* d, void* stream);
+int ntops_attention_backward(const ntops_attention_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

@@ -41,6 +41,38 @@ class ScaleTensor(ctypes.Structure):
     _fields_ = [("x", _vp), ("out", _vp), ("n", _i64)]
 
 
+class RmsNormDesc(ctypes.Structure):
+    """`ntops_rms_norm_desc` of include/ntops.h."""
+    _fields_ = [("x", _vp), ("residual", _vp), ("gate", _vp), ("weight", _vp), ("post_weight", _vp), ("rows", _i64),
+                ("cols", _i64), ("x_stride", _i64), ("residual_stride", _i64), ("gate_stride", _i64), ("x_dtype", _i),
+                ("residual_dtype", _i), ("w_dtype", _i), ("gate_kind", _i), ("eps", _f), ("residual_scale", _f), ("y", _vp),
+                ("h", _vp), ("first", _vp), ("second", _vp)]
+
+
+class RmsNormGrads(ctypes.Structure):
+    """`ntops_rms_norm_grads` of include/ntops.h."""
+    _fields_ = [("dy", _vp), ("dh", _vp), ("dy_stride", _i64), ("dh_stride", _i64), ("dx", _vp), ("dresidual", _vp),
+                ("dgate", _vp), ("dweight", _vp), ("dpost_weight", _vp), ("scratch", _vp)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """`ntops_rotary_desc` of include/ntops.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("q_out", _vp), ("k_out", _vp), ("tokens", _i64), ("q_stride", _i64), ("q_head", _i64),
+                ("k_stride", _i64), ("k_head", _i64), ("heads", _i), ("kv_heads", _i), ("head_dim", _i), ("pairs", _i),
+                ("dtype", _i), ("positions", _vp), ("position_count", _i64), ("position_bits", _i), ("frequencies", _vp),
+                ("interleaved", _i), ("inverse", _i), ("scale", _f)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """`ntops_attention_desc` of include/ntops.h."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64),
+                ("q_head", _i64), ("k_head", _i64), ("v_head", _i64), ("q_batch", _i64), ("k_batch", _i64), ("v_batch", _i64),
+                ("cu_q", _vp), ("cu_k", _vp), ("sequences", _i64), ("q_rows", _i64), ("k_rows", _i64), ("heads", _i),
+                ("kv_heads", _i), ("head_dim", _i), ("dtype", _i), ("causal", _i), ("scale", _f), ("out", _vp), ("lse", _vp),
+                ("workspace", _vp), ("dout", _vp), ("do_stride", _i64), ("do_head", _i64), ("do_batch", _i64), ("dq", _vp),
+                ("dk", _vp), ("dv", _vp)]
+
+
 SIGNATURES = {
     "ntops_layer_norm_forward": (_i, [_vp, _i, _i64, _i64, _i64, _vp, _vp, _i, _f, _vp, _vp, _vp, _vp]),
     "ntops_layer_norm_scratch": (_i64, [_i, _i64, _i64]),
@@ -51,6 +83,13 @@ SIGNATURES = {
     "ntops_linear_cross_entropy_piece": (_i64, [_i64]),
     "ntops_linear_cross_entropy_workspace": (_i64, [_c.POINTER(LinearCrossEntropyDesc)]),
     "ntops_linear_cross_entropy": (_i, [_c.POINTER(LinearCrossEntropyDesc), _vp]),
+    "ntops_rms_norm_forward": (_i, [_c.POINTER(RmsNormDesc), _vp]),
+    "ntops_rms_norm_scratch": (_i64, [_c.POINTER(RmsNormDesc)]),
+    "ntops_rms_norm_backward": (_i, [_c.POINTER(RmsNormDesc), _c.POINTER(RmsNormGrads), _vp]),
+    "ntops_rotary": (_i, [_c.POINTER(RotaryDesc), _vp]),
+    "ntops_attention_workspace": (_i64, [_c.POINTER(AttentionDesc), _i]),
+    "ntops_attention_forward": (_i, [_c.POINTER(AttentionDesc), _vp]),
+    "ntops_attention_backward": (_i, [_c.POINTER(AttentionDesc), _vp]),
     "ntops_scale": (_i, [_c.POINTER(ScaleTensor), _i, _i, _vp, _i, _vp]),
 }
 for _name, (_res, _args) in SIGNATURES.items():

@@ -29,7 +29,7 @@ OPSCALL = os.path.join(HERE, "_opscall.so")
 PROFILING_DIR = os.path.join(HERE, "profiling")
 LIB_STAMPS = os.path.join(PROFILING_DIR, "libntfp8_stamps.so")
 SOURCES = ["quant.hip", "gemm.hip", "gemm_mid.hip", "gemm_few.hip", "gemm_any.hip", "capi.hip",
-           "layer_norm.hip", "adamw.hip", "head.hip", "ops_capi.hip"]
+           "layer_norm.hip", "rms_norm.hip", "rotary.hip", "attention.hip", "attention_backward.hip", "attention_launch.hip", "adamw.hip", "head.hip", "ops_capi.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",

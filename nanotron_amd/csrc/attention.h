@@ -1,0 +1,252 @@
+// What the attention kernels share: the spans that workgroups serve, tiles of rows in LDS and their fragments, products and stores.
+//
+// Every product is taken so that the 32 rows that a wave owns (queries, or keys in the pass for dk and dv) are the columns of
+// V_MFMA_F32_32X32X16's result, one a lane: a row's maximum, sum, logsumexp and limit of a mask are then one register, its
+// scores lie in that lane and lane ^ 32, and the scores, rounded to 16 bits, are the second operand of the next product as they
+// lie: its 16 places of k are taken in the order in which the result registers hold them, 4 h + j and 8 + 4 h + j of half
+// wave h, and the other operand, transposed out of LDS four rows at a time, is read in that order too.
+#pragma once
+#include "gemm_common.h"
+#include "ops_common.h"
+
+namespace ntfp8 {
+
+typedef __bf16 v8bf_attn __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h_attn __attribute__((ext_vector_type(8)));
+typedef int v2i_attn __attribute__((ext_vector_type(2)));
+
+constexpr int kAttnStep = 64;               // rows of a tile in LDS
+constexpr int kAttnWaves = 4;
+constexpr uint32_t kNowhere = 0xfffffff0u;  // past every descriptor: reads as zeros
+constexpr float kLog2E = 1.44269504088896340736f;
+
+// A run of rows of one sequence that a workgroup owns, and the other side's rows that belong to it
+struct AttnTask {
+    int own, rows;     // first row (counted over all sequences), and how many
+    int other, len;    // first row of the other side's sequence, and its length
+    int at, seq;       // first row within its sequence
+    int shift;         // own queries: row i sees the keys 0 .. shift + i; own keys: key i is seen by the queries shift + i and behind
+    int pad;
+};
+
+struct AttnArgs {
+    const void *q, *k, *v, *dout;
+    int64_t q_stride, k_stride, v_stride, do_stride;   // elements between rows,
+    int64_t q_head, k_head, v_head, do_head;           // heads
+    int64_t q_batch, k_batch, v_batch, do_batch;       // and sequences of equal lengths
+    const AttnTask* tasks;                             // or NULL: `sequences` of q_len and k_len rows
+    int64_t tiles;
+    int sequences, q_len, k_len;
+    int64_t q_rows, k_rows;
+    int heads, kv_heads, group, dim, causal;
+    float c;           // scale * log2(e)
+    float scale;
+    void* out;
+    const void* o;     // backward: the output of the forward pass
+    float* lse;        // [heads][q_rows], base 2; +infinity for a row that sees nothing
+    float* delta;      // [heads][q_rows]
+    uint32_t* most;    // fp16 gradients: bits of the largest magnitudes in dout and v
+    void *dq, *dk, *dv;
+    int splits;        // runs that the keys of a tile are cut into ...
+    float* part;       // ... and their results before they are joined: [split][q_rows][heads][dim], then
+    float2* part_ml;   // [split][q_rows][heads] maximum (base 2) and sum
+};
+
+// the task of tile `t`; the longest come first
+__device__ __forceinline__ AttnTask attn_task(const AttnArgs& A, int t, int tile_rows, bool keys) {
+    if (A.tasks) {
+        AttnTask r = A.tasks[t];
+        r.rows = __builtin_amdgcn_readfirstlane(r.rows);
+        r.own = __builtin_amdgcn_readfirstlane(r.own);
+        r.other = __builtin_amdgcn_readfirstlane(r.other);
+        r.len = __builtin_amdgcn_readfirstlane(r.len);
+        r.at = __builtin_amdgcn_readfirstlane(r.at);
+        r.seq = __builtin_amdgcn_readfirstlane(r.seq);
+        r.shift = __builtin_amdgcn_readfirstlane(r.shift);
+        return r;
+    }
+    const int own_len = keys ? A.k_len : A.q_len, len = keys ? A.q_len : A.k_len;
+    const int per = (own_len + tile_rows - 1) / tile_rows, rank = t / A.sequences, seq = t - rank * A.sequences;
+    const int at = (keys ? rank : per - 1 - rank) * tile_rows;
+    return {seq * own_len + at, min(tile_rows, own_len - at), seq * len, len, at, seq, keys ? at - (A.k_len - A.q_len) : at + A.k_len - A.q_len, 0};
+}
+// element offset of a run of rows: packed ones are counted over all sequences, others within theirs
+__device__ __forceinline__ int64_t attn_rows(const AttnArgs& A, int64_t packed, int seq, int at, int64_t stride, int64_t batch) {
+    return A.tasks ? packed * stride : seq * batch + at * stride;
+}
+
+template <int T>
+__device__ __forceinline__ v16f mfma_attn(v4i rows, v4i cols, v16f c) {   // result: row (register) of `rows`, column (lane) of `cols`
+    if constexpr (T == NTFP8_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf_attn, rows), __builtin_bit_cast(v8bf_attn, cols), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h_attn, rows), __builtin_bit_cast(v8h_attn, cols), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f zeros16() { return (v16f){0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 64 rows of DP elements in LDS, 16-byte chunks swizzled so that neither 8 rows' reads of one chunk nor the transposing reads of 4
+// rows' 64 bytes meet in a bank
+template <int DP>
+struct AttnTile {
+    static constexpr int kPitch = DP <= 64 ? 128 : 256, kBytes = kAttnStep * kPitch, kLoads = kBytes / 1024 / kAttnWaves;
+    static __device__ __forceinline__ int swizzle(int row) {
+        if constexpr (kPitch == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+        else return (row & 3) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
+    }
+    // loads: 1 KB a wave each, straight into LDS
+    struct Source {
+        const char* base;
+        int64_t row_bytes;
+        uint32_t off[kLoads];
+        int dim;
+        __device__ __forceinline__ void init(const void* p, int64_t elements, int64_t stride, int dim_, int wave, int lane) {
+            base = static_cast<const char*>(p) + 2 * elements;
+            row_bytes = 2 * stride;
+            dim = dim_;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int byte = ((i * kAttnWaves + wave) * 64 + lane) * 16, row = byte / kPitch, chunk = (byte % kPitch >> 4) ^ swizzle(row);
+                off[i] = chunk * 8 < dim ? (uint32_t)row * (uint32_t)row_bytes + chunk * 16 : kNowhere;
+            }
+        }
+        // rows first .. first + 63 of `len`, those behind it as zeros
+        __device__ __forceinline__ void load(uint8_t* stage, int first, int len, int wave) const {
+            const int rows = min(kAttnStep, len - first);
+            const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)row_bytes + 2u * dim : 0u;
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (int64_t)first * row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) lds_load16(r, (lds_ptr)(uintptr_t)(stage + (i * kAttnWaves + wave) * 1024), off[i], 0);
+        }
+    };
+    // fragments: 32 rows by 16 elements as they lie, and 16 rows by 32 elements transposed
+    int plain, plain_turn, across, across_turn;
+    __device__ __forceinline__ void init(int lane) {
+        const int row = lane & 31, h = lane >> 5, u = lane & 15, first = 4 * h + (u >> 2);
+        plain = row * kPitch;
+        plain_turn = (h ^ swizzle(row)) << 4;
+        across = first * kPitch + (u & 1) * 8;
+        across_turn = ((((lane >> 4) & 1) * 2 + ((u & 3) >> 1)) ^ swizzle(first)) << 4;
+    }
+    // rows 32 b .., elements 16 k ..
+    __device__ __forceinline__ v4i rows(const uint8_t* stage, int b, int k) const {
+        return *reinterpret_cast<const v4i*>(stage + plain + ((k << 5) ^ plain_turn) + b * 32 * kPitch);
+    }
+    // elements 32 e .. of the rows 16 s .., in the order of the result registers
+    __device__ __forceinline__ v4i columns(uint8_t* stage, int s, int e) const {
+        typedef short v4s __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) v4s* tr_ptr;
+        const int lo = across + ((e << 6) ^ across_turn) + s * 16 * kPitch, hi = (across + ((e << 6) ^ across_turn ^ 16)) + (s * 16 + 8) * kPitch;
+        const v2i_attn a = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[lo]));
+        const v2i_attn b = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[hi]));
+        return (v4i){a.x, a.y, b.x, b.y};
+    }
+};
+
+// 32 rows of global memory as the second operand: row `row` of each lane, 16 elements a fragment.  `live`: the row exists
+template <int DP>
+__device__ __forceinline__ void load_own(v4i (&f)[DP / 16], const void* p, int64_t element, int dim, bool live, int lane) {
+    const char* const at = static_cast<const char*>(p) + 2 * element;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+        const int e = 16 * k + 8 * (lane >> 5);
+        f[k] = live && e < dim ? *reinterpret_cast<const v4i*>(at + 2 * e) : (v4i){0, 0, 0, 0};
+    }
+}
+// 8 result registers (16 places of k) as a fragment of the second operand
+template <int T>
+__device__ __forceinline__ v4i pack_scores(const v16f& s, int first) {
+    return (v4i){(int)pack_pair<T>(s[first], s[first + 1]), (int)pack_pair<T>(s[first + 2], s[first + 3]), (int)pack_pair<T>(s[first + 4], s[first + 5]),
+                 (int)pack_pair<T>(s[first + 6], s[first + 7])};
+}
+// the place in its block of 32 of a result register
+__device__ __forceinline__ int place_of(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+
+// Whether a stage holds a value that is not finite, in any of its first `rows` rows
+template <int T, int DP>
+__device__ __forceinline__ bool attn_not_finite(const uint8_t* stage, int rows, int lane) {
+    float nan = 0.0f;
+    for (int at = lane * 16; at < rows * AttnTile<DP>::kPitch; at += 1024) {
+        const v4i x = *reinterpret_cast<const v4i*>(stage + at);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            float lo, hi;
+            unpack_pair<T>((uint32_t)x[w], lo, hi);
+            nan = __builtin_fmaf(lo, 0.0f, nan);
+            nan = __builtin_fmaf(hi, 0.0f, nan);
+        }
+    }
+    return __any(nan != nan);
+}
+// acc (elements by own rows) += columns of a stage's rows 16 s .. * scores
+template <int T, int DP>
+__device__ __forceinline__ void add_columns(v16f (&acc)[DP / 32], const AttnTile<DP>& tile, uint8_t* stage, int s, v4i scores) {
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) acc[e] = mfma_attn<T>(tile.columns(stage, s, e), scores, acc[e]);
+}
+// The same over the 16 kScores rows of a stage that holds values which are not finite, under a mask: a score of zero times such a value would
+// reach the rows that do not count it (a padded row, a token to come), so the stage's rows go one at a time, and only into the
+// rows that count them: `counts(i)`, this lane's row counts row i.
+template <int T, int DP, int kScores, typename F>
+__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const AttnTile<DP>& tile, uint8_t* stage, const v4i (&scores)[kScores], F&& counts, int lane) {
+#pragma unroll 1
+    for (int i = 0; i < 16 * kScores; ++i) {
+        const int s = i >> 4, j = (i & 3) + ((i >> 3) & 1) * 4;   // its place in the fragments of half wave (i >> 2) & 1
+        const bool mine = (lane >> 5) == ((i >> 2) & 1), take = counts(i);
+        v4i c = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < kScores; ++k) c |= scores[k] & (s == k ? -1 : 0);   // (a choice of one of them would put them all into memory)
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) {
+            v4i f = tile.columns(stage, s, e);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) f[w] = mine && (j >> 1) == w ? (j & 1 ? f[w] & (int)0xffff0000 : f[w] & 0xffff) : 0;
+            const v16f d = mfma_attn<T>(f, c, zeros16());
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[e][r] += take ? d[r] : 0.0f;
+        }
+    }
+}
+
+// acc * factor as one row a lane, rounded to T: 16 bytes a lane and store.  p: the row's first element
+template <int T, int DP>
+__device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float factor, void* p, int64_t element, int dim, bool live, int lane) {
+    char* const at = static_cast<char*>(p) + 2 * element;
+    const int h = lane >> 5;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            float v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] = acc[e][8 * s + r] * factor;
+            uint32_t a0 = pack_pair<T>(v[0], v[1]), a1 = pack_pair<T>(v[2], v[3]), b0 = pack_pair<T>(v[4], v[5]), b1 = pack_pair<T>(v[6], v[7]);
+            swap_halves(a0, b0);
+            swap_halves(a1, b1);
+            const int first = 32 * e + 16 * s + 8 * h;
+            if (live && first < dim) *reinterpret_cast<v4i*>(at + 2 * first) = (v4i){(int)a0, (int)a1, (int)b0, (int)b1};
+        }
+}
+
+// max of a lane and its counterpart of the other half wave
+__device__ __forceinline__ float both_max(float v) {
+    uint32_t x = __float_as_uint(v), y = x;
+    swap_halves(x, y);
+    return fmaxf(__uint_as_float(x), __uint_as_float(y));
+}
+__device__ __forceinline__ float both_sum(float v) {
+    uint32_t x = __float_as_uint(v), y = x;
+    swap_halves(x, y);
+    return __uint_as_float(x) + __uint_as_float(y);
+}
+
+// calls f with the type and the head's size rounded up to what the kernels are built for
+template <typename F>
+int with_attn(int dtype, int dim, F&& f) {
+    using std::integral_constant;
+    auto by_dim = [&](auto t) { 
+        if (dim <= 64) return f(t, integral_constant<int, 64>{});
+        return dim <= 96 ? f(t, integral_constant<int, 96>{}) : f(t, integral_constant<int, 128>{});
+    };
+    return dtype == NTFP8_BF16 ? by_dim(integral_constant<int, NTFP8_BF16>{}) : by_dim(integral_constant<int, NTFP8_F16>{});
+}
+
+}  // namespace ntfp8

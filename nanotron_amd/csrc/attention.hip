@@ -1,0 +1,467 @@
+// Attention, forward: out = softmax(scale q k^T) v over sequences of any lengths, heads of queries sharing heads of keys.
+#include "attention.h"
+
+namespace ntfp8 {
+namespace {
+
+// ------------------------------------------------------------------------------------------------ tasks
+// The tiles of packed sequences, heaviest first: two lists, of queries (block 0) and of keys (block 1, where asked for).  Offsets are clamped to
+// the rows that there are, so that none of them, whatever it holds, leads out of a tensor; rows before the first sequence and
+// behind the last one get tasks that see nothing, which write zeros.
+constexpr int kPlanThreads = 1024, kBuckets = 256;
+struct Plan {
+    const int* cu_q;
+    const int* cu_k;
+    int sequences;
+    int q_rows, k_rows, causal;
+    int q_tile, k_tile, q_tasks, k_tasks;   // rows a tile, tasks there is room for
+    AttnTask* q_list;
+    AttnTask* k_list;
+};
+
+__global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(const Plan P) {
+    __shared__ int count[kBuckets], total;
+    const bool keys = blockIdx.x == 1;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int tile = keys ? P.k_tile : P.q_tile, own_rows = keys ? P.k_rows : P.q_rows, most = keys ? P.k_tasks : P.q_tasks;
+    const int* const own_cu = keys ? P.cu_k : P.cu_q;
+    const int* const other_cu = keys ? P.cu_q : P.cu_k;
+    const int other_rows = keys ? P.q_rows : P.k_rows;
+    AttnTask* const list = keys ? P.k_list : P.q_list;
+    int unit = 1;   // of cost, so that the longest possible one falls into the last bucket
+    while (other_rows / unit >= kBuckets) unit *= 2;
+    for (int i = threadIdx.x; i < kBuckets; i += kPlanThreads) count[i] = 0;
+    if (threadIdx.x == 0) total = 0;
+    __syncthreads();
+    auto clamped = [](int v, int most_) { return min(max(v, 0), most_); };
+    auto each = [&](auto&& f) {
+        for (int s = wave; s < P.sequences + 2; s += kPlanThreads / 64) {
+            int a, len, b = 0, seen = 0;
+            if (s < P.sequences) {
+                a = clamped(own_cu[s], own_rows);
+                len = max(0, clamped(own_cu[s + 1], own_rows) - a);
+                b = clamped(other_cu[s], other_rows);
+                seen = max(0, clamped(other_cu[s + 1], other_rows) - b);
+            } else if (s == P.sequences) {
+                a = 0;
+                len = clamped(own_cu[0], own_rows);
+            } else {
+                a = clamped(own_cu[P.sequences], own_rows);
+                len = own_rows - a;
+            }
+            for (int at = lane * tile; at < len; at += 64 * tile) {
+                AttnTask t = {a + at, min(tile, len - at), b, seen, at, s, keys ? at - (len - seen) : at + seen - len, 0};
+                int cost = seen;
+                if (P.causal) cost = keys ? seen - max(0, t.shift) : t.shift + t.rows;
+                f(t, min(max(cost, 0) / unit, kBuckets - 1));
+            }
+        }
+    };
+    each([&](const AttnTask&, int bucket) { atomicAdd(&count[bucket], 1); });
+    __syncthreads();
+    // where each bucket begins, the heaviest in front
+    if (wave == 0) {
+        int held[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            held[i] = count[kBuckets - 1 - (4 * lane + i)];
+            sum += held[i];
+        }
+        int before = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(before, d);
+            if (lane >= d) before += o;
+        }
+        if (lane == 63) total = before;
+        before -= sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            count[kBuckets - 1 - (4 * lane + i)] = before;
+            before += held[i];
+        }
+    }
+    __syncthreads();
+    each([&](const AttnTask& t, int bucket) {
+        const int at = atomicAdd(&count[bucket], 1);   // (the order within a bucket reaches no result)
+        if (at < most) list[at] = t;
+    });
+    for (int i = total + threadIdx.x; i < most; i += kPlanThreads) list[i] = {0, 0, 0, 0, 0, 0, 0, 0};
+}
+
+// ------------------------------------------------------------------------------------------------ prompts
+// A workgroup owns 128 QB queries of one head, a wave 32 QB of them, and walks their keys 64 at a time: scores of 64 keys by 32
+// queries, the running maximum and sum, and the product with the values, into out^T [elements][queries].  Tiles of keys and
+// values travel straight into LDS, the next pair while this one is worked on.
+template <int T, int DP, int QB>
+__global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_forward_kernel(const AttnArgs A) {
+    typedef AttnTile<DP> Tile;
+    __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * Tile::kBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // heads that share keys go to one XCD: workgroups are dealt to the eight in turn
+    const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
+    const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
+    const AttnTask task = attn_task(A, t, 128 * QB, false);
+    if (task.rows <= 0) return;
+    const int64_t q0 = attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head;
+    const int64_t k0 = attn_rows(A, task.other, task.seq, 0, A.k_stride, A.k_batch) + kv * A.k_head;
+    const int64_t v0 = attn_rows(A, task.other, task.seq, 0, A.v_stride, A.v_batch) + kv * A.v_head;
+    const int end = A.causal ? min(max(task.shift + task.rows, 0), task.len) : task.len;
+    int first = 0, steps = (end + kAttnStep - 1) / kAttnStep;
+    if (A.splits > 1) {
+        const int each = (steps + A.splits - 1) / A.splits;
+        first = blockIdx.y * each;
+        steps = max(0, min(steps - first, each));
+    }
+    Tile tile;
+    tile.init(lane);
+    typename Tile::Source ks, vs;
+    ks.init(A.k, k0, A.k_stride, A.dim, wave, lane);
+    vs.init(A.v, v0, A.v_stride, A.dim, wave, lane);
+    if (steps > 0) {
+        ks.load(sk, first * kAttnStep, task.len, wave);
+        vs.load(sv, first * kAttnStep, task.len, wave);
+    }
+    const int row0 = wave * 32 * QB + (lane & 31);   // of block 0
+    v4i q[QB][DP / 16];
+    v16f out[QB][DP / 32];
+    float top[QB], sum[QB];   // maximum (of scores times c) and this half wave's sum
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int row = row0 + 32 * b;
+        load_own<DP>(q[b], A.q, q0 + row * A.q_stride, A.dim, row < task.rows, lane);
+        top[b] = -__builtin_inff();
+        sum[b] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e) out[b][e] = zeros16();
+    }
+    for (int j = 0; j < steps; ++j) {
+        const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wg_barrier();
+        if (j + 1 < steps) {
+            ks.load(sk + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
+            vs.load(sv + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
+        }
+        const int lead = task.shift + wave * 32 * QB;   // the last key that the wave's first row sees
+        if (A.causal && key0 > lead + 32 * QB - 1) continue;   // (uniform in the wave; barriers are met at the loop's head)
+        v16f s[QB][2];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) s[b][0] = s[b][1] = zeros16();
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            const v4i f0 = tile.rows(sk + stage, 0, k), f1 = tile.rows(sk + stage, 1, k);
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                s[b][0] = mfma_attn<T>(f0, q[b][k], s[b][0]);
+                s[b][1] = mfma_attn<T>(f1, q[b][k], s[b][1]);
+            }
+        }
+        const bool masked = key0 + kAttnStep > task.len || (A.causal && key0 + kAttnStep - 1 > lead);
+        if (masked) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const int last = (A.causal ? min(task.len - 1, lead + 32 * b + (lane & 31)) : task.len - 1) - key0;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (32 * g + place_of(r, lane) > last) s[b][g][r] = -__builtin_inff();
+            }
+        }
+        v4i p[QB][4];   // of 16 keys each
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            float most = s[b][0][0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) most = fmaxf(most, s[b][0][r]);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][1][r]);
+            most = both_max(most) * A.c;
+            // The exponentials are taken below a maximum that is raised only once a row's has grown by more than 2^8 (what is
+            // kept in 16 bits loses nothing by that): rescaling the outputs is 64 multiplications a lane
+            if (__any(most > top[b] + 8.0f)) {
+                const float now = fmaxf(top[b], most);
+                const float by = now == top[b] ? 1.0f : exp2_fast(top[b] - now);
+                sum[b] *= by;
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e) out[b][e] *= by;
+                top[b] = now;
+            }
+            const float below = top[b] == -__builtin_inff() ? 0.0f : top[b];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[b][g][r] = exp2_fast(__builtin_fmaf(s[b][g][r], A.c, -below));
+                    sum[b] += s[b][g][r];
+                }
+                p[b][2 * g] = pack_scores<T>(s[b][g], 0);
+                p[b][2 * g + 1] = pack_scores<T>(s[b][g], 8);
+            }
+        }
+        if (masked && attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const int last = (A.causal ? min(task.len - 1, lead + 32 * b + (lane & 31)) : task.len - 1) - key0;
+                add_columns_singly<T, DP, 4>(out[b], tile, sv + stage, p[b], [&](int i) { return i <= last; }, lane);
+            }
+            continue;
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) {
+                const v4i f = tile.columns(sv + stage, g, e);
+#pragma unroll
+                for (int b = 0; b < QB; ++b) out[b][e] = mfma_attn<T>(f, p[b][g], out[b][e]);
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int row = row0 + 32 * b;
+        const bool live = row < task.rows;
+        const float all = both_sum(sum[b]);
+        const int64_t at = (int64_t)task.own + row;
+        if (A.splits > 1) {
+            if (!live) continue;
+            const int64_t to = ((int64_t)blockIdx.y * A.q_rows + at) * A.heads + head;
+            if (lane < 32) A.part_ml[to] = make_float2(top[b], all);
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * e + 8 * g + 4 * (lane >> 5);
+                    if (d < A.dim) *reinterpret_cast<v4f*>(A.part + to * A.dim + d) = (v4f){out[b][e][4 * g], out[b][e][4 * g + 1], out[b][e][4 * g + 2], out[b][e][4 * g + 3]};
+                }
+            continue;
+        }
+        store_rows<T, DP>(out[b], all > 0.0f || all != all ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane);
+        if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = all > 0.0f || all != all ? top[b] + log2f(all) : __builtin_inff();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ few queries
+// Where the queries of a group of heads are 32 rows or fewer (a token, or a few, of every sequence) the keys are the work: the rows
+// (head in its group, query) share them, every wave takes keys of its own, 32 at a time through LDS of its own without a
+// barrier, and the waves' results are joined at the end; workgroups' (`splits` of a sequence) by a second launch.
+constexpr int kFewStep = 32, kFewRows = 32;
+template <int T, int DP>
+__global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const AttnArgs A) {
+    typedef AttnTile<DP> Tile;
+    constexpr int kBytes = Tile::kBytes / 2, kLoads = kBytes / 1024, kStages = 2;
+    __shared__ __attribute__((aligned(1024))) uint8_t sk[kAttnWaves][kStages * kBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t sv[kAttnWaves][kStages * kBytes];
+    __shared__ float2 ml[kAttnWaves][kFewRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int seq = blockIdx.x / A.kv_heads, kv = blockIdx.x - seq * A.kv_heads;
+    const int n = A.q_len, rows = A.group * n;
+    // this lane's row: query `token` of head `head`
+    const int row = lane & 31, inside = row / n, token = row - inside * n, head = kv * A.group + inside;
+    const bool live = row < rows;
+    const int64_t q0 = seq * A.q_batch + token * A.q_stride + head * A.q_head;
+    const int len = A.k_len, steps_all = (len + kFewStep - 1) / kFewStep, runs = A.splits * kAttnWaves, run = blockIdx.y * kAttnWaves + wave;
+    const int each = (steps_all + runs - 1) / runs, first = run * each, steps = max(0, min(steps_all - first, each));
+    const int last_row = A.causal ? len - n + token : len - 1;   // the last key that this row sees
+    const int first_last = A.causal ? len - n : len - 1;         // and the row that sees least
+    Tile tile;
+    tile.init(lane);
+    const char* const kp = static_cast<const char*>(A.k) + 2 * (seq * A.k_batch + kv * A.k_head);
+    const char* const vp = static_cast<const char*>(A.v) + 2 * (seq * A.v_batch + kv * A.v_head);
+    const int64_t kb = 2 * A.k_stride, vb = 2 * A.v_stride;
+    uint32_t koff[kLoads], voff[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int byte = (i * 64 + lane) * 16, r = byte / Tile::kPitch, chunk = (byte % Tile::kPitch >> 4) ^ Tile::swizzle(r);
+        koff[i] = chunk * 8 < A.dim ? (uint32_t)r * (uint32_t)kb + chunk * 16 : kNowhere;
+        voff[i] = chunk * 8 < A.dim ? (uint32_t)r * (uint32_t)vb + chunk * 16 : kNowhere;
+    }
+    // (a step behind the last is all zeros: every step is the same number of loads)
+    auto load = [&](int j) {
+        const int key = (first + j) * kFewStep, count = j < steps ? min(kFewStep, len - key) : 0;
+        const uint32_t kbytes = count > 0 ? (uint32_t)(count - 1) * (uint32_t)kb + 2u * A.dim : 0u, vbytes = count > 0 ? (uint32_t)(count - 1) * (uint32_t)vb + 2u * A.dim : 0u;
+        const __amdgpu_buffer_rsrc_t rk = make_rsrc(kp + (count > 0 ? key * kb : 0), (uint32_t)__builtin_amdgcn_readfirstlane((int)kbytes));
+        const __amdgpu_buffer_rsrc_t rv = make_rsrc(vp + (count > 0 ? key * vb : 0), (uint32_t)__builtin_amdgcn_readfirstlane((int)vbytes));
+        uint8_t* const k = sk[wave] + (j & 1) * kBytes;
+        uint8_t* const v = sv[wave] + (j & 1) * kBytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) lds_load16(rk, (lds_ptr)(uintptr_t)(k + i * 1024), koff[i], 0);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) lds_load16(rv, (lds_ptr)(uintptr_t)(v + i * 1024), voff[i], 0);
+    };
+    v4i q[DP / 16];
+    load_own<DP>(q, A.q, q0, A.dim, live, lane);
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) asm volatile("" : "+v"(q[k]));   // (here, in front of the loads that are counted below)
+    if (steps > 0) {
+        load(0);
+        load(1);
+    }
+    v16f out[DP / 32];
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) out[e] = zeros16();
+    float top = -__builtin_inff(), sum = 0.0f;
+    for (int j = 0; j < steps; ++j) {
+        const int key0 = (first + j) * kFewStep;
+        uint8_t* const k = sk[wave] + (j & 1) * kBytes;
+        uint8_t* const v = sv[wave] + (j & 1) * kBytes;
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");   // all but the step requested since
+        v16f s = zeros16();
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i) s = mfma_attn<T>(tile.rows(k, 0, i), q[i], s);
+        const bool masked = key0 + kFewStep - 1 > min(len - 1, first_last);
+        const int last = min(len - 1, last_row) - key0;
+        if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (place_of(r, lane) > last) s[r] = -__builtin_inff();
+        }
+        float most = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) most = fmaxf(most, s[r]);
+        most = both_max(most) * A.c;
+        if (__any(most > top + 8.0f)) {
+            const float now = fmaxf(top, most), by = now == top ? 1.0f : exp2_fast(top - now);
+            sum *= by;
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e) out[e] *= by;
+            top = now;
+        }
+        const float below = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, -below));
+            sum += s[r];
+        }
+        const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)};
+        if (masked && attn_not_finite<T, DP>(v, kFewStep, lane)) {
+            add_columns_singly<T, DP, 2>(out, tile, v, p, [&](int i) { return i <= last; }, lane);
+        } else {
+            add_columns<T, DP>(out, tile, v, 0, p[0]);
+            add_columns<T, DP>(out, tile, v, 1, p[1]);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage has been read
+        __builtin_amdgcn_sched_barrier(0);
+        load(j + 2);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last requests write zeros into stages nobody reads again)
+    sum = both_sum(sum);
+    if (lane < kFewRows) ml[wave][lane] = make_float2(top, sum);
+    __syncthreads();
+    float all_top = -__builtin_inff(), all_sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) all_top = fmaxf(all_top, ml[w][row].x);
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) {
+        const float2 o = ml[w][row];
+        if (o.x != -__builtin_inff() || o.y != 0.0f) all_sum += o.y * (o.x == all_top ? 1.0f : exp2_fast(o.x - all_top));
+    }
+    const float mine = top == -__builtin_inff() ? (sum != sum ? 1.0f : 0.0f) : top == all_top ? 1.0f : exp2_fast(top - all_top);
+    // the waves' outputs, [element][row], added up through LDS in the order of the waves
+    constexpr int kPitch = kFewRows + 1;
+    float* const at = reinterpret_cast<float*>(&sk[0][0]);
+    static_assert(sizeof(sk) >= sizeof(float) * DP * kPitch, "");
+    for (int w = 0; w < kAttnWaves; ++w) {
+        if (w == wave) {
+#pragma unroll
+            for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float* const o = at + (32 * e + place_of(r, lane)) * kPitch + row;
+                    const float x = mine == 0.0f ? 0.0f : out[e][r] * mine;
+                    *o = w == 0 ? x : *o + x;
+                }
+        }
+        __syncthreads();
+    }
+    // 8 threads a row
+    const int r = threadIdx.x >> 3;
+    if (r < rows) {
+        const int in = r / n, tok = r - in * n, hd = kv * A.group + in;
+        const int64_t out_row = (int64_t)seq * n + tok;
+        float m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) m = fmaxf(m, ml[w][r].x);
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; ++w) {
+            const float2 o = ml[w][r];
+            if (o.x != -__builtin_inff() || o.y != 0.0f) l += o.y * (o.x == m ? 1.0f : exp2_fast(o.x - m));
+        }
+        if (A.splits > 1) {
+            const int64_t to = ((int64_t)blockIdx.y * A.q_rows + out_row) * A.heads + hd;
+            if ((threadIdx.x & 7) == 0) A.part_ml[to] = make_float2(m, l);
+            for (int d = (threadIdx.x & 7) * 8; d < A.dim; d += 64)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) A.part[to * A.dim + d + i] = at[(d + i) * kPitch + r];
+        } else {
+            const float by = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            for (int d = (threadIdx.x & 7) * 8; d < A.dim; d += 64) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = at[(d + i) * kPitch + r] * by;
+                store_piece<T, 8>(A.out, (out_row * A.heads + hd) * A.dim + d, x);
+            }
+            if (A.lse && (threadIdx.x & 7) == 0) A.lse[hd * A.q_rows + out_row] = l > 0.0f || l != l ? m + log2f(l) : __builtin_inff();
+        }
+    }
+}
+
+// The splits' results joined: a row of one head in 16 lanes, 8 elements each
+template <int T>
+__global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
+    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const int d = (threadIdx.x & 15) * 8;
+    if (row >= A.q_rows * A.heads) return;
+    const int64_t pitch = A.q_rows * A.heads;
+    float top = -__builtin_inff(), sum = 0.0f, x[8] = {};
+    for (int s = 0; s < A.splits; ++s) top = fmaxf(top, A.part_ml[s * pitch + row].x);
+    for (int s = 0; s < A.splits; ++s) {
+        const float2 o = A.part_ml[s * pitch + row];
+        if (o.x == -__builtin_inff() && o.y == 0.0f) continue;
+        const float by = o.x == top ? 1.0f : exp2_fast(o.x - top);
+        sum += o.y * by;
+        if (d < A.dim) {
+            const v4f* const p = reinterpret_cast<const v4f*>(A.part + (s * pitch + row) * A.dim + d);
+            const v4f a = p[0], b = p[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] += a[i] * by;
+                x[4 + i] += b[i] * by;
+            }
+        }
+    }
+    const bool any = sum > 0.0f || sum != sum;
+    if (d < A.dim) {
+        const float over = any ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= over;
+        store_piece<T, 8>(A.out, row * A.dim + d, x);
+    }
+    if (A.lse && d == 0) A.lse[(row % A.heads) * A.q_rows + row / A.heads] = any ? top + log2f(sum) : __builtin_inff();
+}
+
+}  // namespace
+
+// ------------------------------------------------------------------------------------------------ launches
+int run_attention_plan(const int* cu_q, const int* cu_k, int sequences, int q_rows, int k_rows, int causal, int q_tile, int k_tile, int q_tasks, int k_tasks,
+                       AttnTask* q_list, AttnTask* k_list, hipStream_t st) {
+    const Plan p = {cu_q, cu_k, sequences, q_rows, k_rows, causal, q_tile, k_tile, q_tasks, k_tasks, q_list, k_list};
+    attention_plan_kernel<<<k_list ? 2 : 1, kPlanThreads, 0, st>>>(p);
+    return launch_status();
+}
+
+int run_attention_forward_kernels(const AttnArgs& A, int dtype, int q_blocks, bool few, hipStream_t st) {
+    return with_attn(dtype, A.dim, [&](auto t, auto d) {
+        constexpr int T = decltype(t)::value, DP = decltype(d)::value;
+        const dim3 grid((unsigned)(few ? (int64_t)A.sequences * A.kv_heads : A.tiles * A.heads), (unsigned)A.splits);
+        if (few) attention_few_kernel<T, DP><<<grid, 64 * kAttnWaves, 0, st>>>(A);
+        else if (q_blocks == 1) attention_forward_kernel<T, DP, 1><<<grid, 64 * kAttnWaves, 0, st>>>(A);
+        else attention_forward_kernel<T, DP, 2><<<grid, 64 * kAttnWaves, 0, st>>>(A);
+        if (const int rc = launch_status(); rc != NTFP8_OK || A.splits <= 1) return rc;
+        attention_join_kernel<T><<<(unsigned)((A.q_rows * A.heads * 16 + 255) / 256), 256, 0, st>>>(A);
+        return launch_status();
+    });
+}
+
+}  // namespace ntfp8

@@ -1,0 +1,263 @@
+// Attention, backward.  With p = exp2(c q k^T - lse) and delta = sum over elements of dout out, a row each:
+//   dv = p^T dout,  ds = p (dout v^T - delta),  dq = scale ds k,  dk = scale ds^T q
+// One kernel owns queries and makes dq, one owns keys and makes dk and dv; both make the scores again, seven products where five
+// would do, so that every sum is made in one place and order: no atomics, the same bits for the same inputs.
+//
+// fp16: ds is a gradient and may be smaller than that type's normal numbers, and p in a long row is.  p is kept times 2^8, ds
+// times the power of two that the largest magnitudes of dout and v allow it without overflow.
+#include "attention.h"
+
+namespace ntfp8 {
+namespace {
+
+constexpr float kLiftP = 8.0f;
+// what ds is multiplied by beyond p's lift: |dout v^T - delta| is at most 2 dim |dout| |v|, brought to 2^15 with the lift
+template <int T>
+__device__ __forceinline__ float gradient_lift(const AttnArgs& A) {
+    if constexpr (T == NTFP8_BF16) return 1.0f;
+    const float most = 2.0f * A.dim * __uint_as_float(A.most[0]) * __uint_as_float(A.most[1]);
+    if (!(most > 0.0f) || most > 1e30f || most < 1e-30f) return 1.0f;
+    const int e = (int)(__float_as_uint(most) >> 23) - 127;   // 2^e <= most < 2^(e + 1)
+    return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
+}
+
+__global__ void attention_clear_kernel(uint32_t* p) { p[threadIdx.x] = 0u; }
+
+// delta, 16 lanes a row; blocks behind those of the rows of dout read v, for its largest magnitude
+template <int T>
+__global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, const int* cu_q, const int* cu_k, int64_t q_blocks) {
+    const bool values = blockIdx.x >= q_blocks;
+    const int64_t item = ((int64_t)(values ? blockIdx.x - q_blocks : blockIdx.x) * 256 + threadIdx.x) >> 4;
+    const int heads = values ? A.kv_heads : A.heads, own_len = values ? A.k_len : A.q_len;
+    const int64_t rows = values ? A.k_rows : A.q_rows, row = item / heads;
+    const int head = (int)(item - row * heads), d = (threadIdx.x & 15) * 8;
+    const int* const cu = values ? cu_k : cu_q;
+    bool live = row < rows;
+    if (live && cu) live = row >= cu[0] && row < cu[A.sequences];   // rows of no sequence may hold anything
+    float x[8] = {}, y[8] = {}, sum = 0.0f;
+    if (live && d < A.dim) {
+        const int seq = A.tasks ? 0 : (int)(row / own_len);
+        const int64_t at = A.tasks ? row : row - (int64_t)seq * own_len;
+        const int64_t stride = values ? A.v_stride : A.do_stride, batch = values ? A.v_batch : A.do_batch, apart = values ? A.v_head : A.do_head;
+        unpack<T, 8>(load_piece<T, 8>(values ? A.v : A.dout, seq * batch + at * stride + head * apart + d), x);
+        if (!values) unpack<T, 8>(load_piece<T, 8>(A.o, (row * heads + head) * A.dim + d), y);
+    }
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        sum += x[i] * y[i];
+        const uint32_t size = __float_as_uint(x[i]) & 0x7fffffffu;
+        most = max(most, size < kInfBits ? size : 0u);   // (what is not finite spoils its own sequence, whatever the others are lifted by)
+    }
+#pragma unroll
+    for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
+    if (!values && row < rows && d == 0) A.delta[head * A.q_rows + row] = live ? sum : 0.0f;
+    if constexpr (T == NTFP8_F16) {
+        most = wave_most(most);
+        if ((threadIdx.x & 63) == 0 && most) atomicMax(&A.most[values], most);   // (a maximum: the order changes nothing)
+    }
+}
+
+// dq of 128 queries of one head, 32 a wave
+template <int T, int DP>
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const AttnArgs A) {
+    typedef AttnTile<DP> Tile;
+    __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * Tile::kBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
+    const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
+    const AttnTask task = attn_task(A, t, 128, false);
+    if (task.rows <= 0) return;
+    const int64_t k0 = attn_rows(A, task.other, task.seq, 0, A.k_stride, A.k_batch) + kv * A.k_head;
+    const int64_t v0 = attn_rows(A, task.other, task.seq, 0, A.v_stride, A.v_batch) + kv * A.v_head;
+    const int end = A.causal ? min(max(task.shift + task.rows, 0), task.len) : task.len, steps = (end + kAttnStep - 1) / kAttnStep;
+    Tile tile;
+    tile.init(lane);
+    typename Tile::Source ks, vs;
+    ks.init(A.k, k0, A.k_stride, A.dim, wave, lane);
+    vs.init(A.v, v0, A.v_stride, A.dim, wave, lane);
+    if (steps > 0) {
+        ks.load(sk, 0, task.len, wave);
+        vs.load(sv, 0, task.len, wave);
+    }
+    const int row = wave * 32 + (lane & 31);
+    const bool live = row < task.rows;
+    v4i q[DP / 16], g[DP / 16];
+    load_own<DP>(q, A.q, attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head + row * A.q_stride, A.dim, live, lane);
+    load_own<DP>(g, A.dout, attn_rows(A, task.own, task.seq, task.at, A.do_stride, A.do_batch) + head * A.do_head + row * A.do_stride, A.dim, live, lane);
+    const int64_t at = (int64_t)task.own + row;
+    const float lse = live ? A.lse[head * A.q_rows + at] : __builtin_inff(), delta = live ? A.delta[head * A.q_rows + at] : 0.0f;
+    const float lift = gradient_lift<T>(A);
+    v16f dq[DP / 32];
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) dq[e] = zeros16();
+    for (int j = 0; j < steps; ++j) {
+        const int key0 = j * kAttnStep, stage = (j & 1) * Tile::kBytes;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wg_barrier();
+        if (j + 1 < steps) {
+            ks.load(sk + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
+            vs.load(sv + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
+        }
+        const int lead = task.shift + wave * 32;
+        if (A.causal && key0 > lead + 31) continue;
+        const bool masked = key0 + kAttnStep > task.len || (A.causal && key0 + kAttnStep - 1 > lead);
+        const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0;
+        v4i p[4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            v16f s = zeros16(), d = zeros16();
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                s = mfma_attn<T>(tile.rows(sk + stage, b, k), q[k], s);
+                d = mfma_attn<T>(tile.rows(sv + stage, b, k), g[k], d);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, -lse)) * ((d[r] - delta) * lift);
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = 32 * b + place_of(r, lane) > last ? 0.0f : s[r];
+            }
+            p[2 * b] = pack_scores<T>(s, 0);
+            p[2 * b + 1] = pack_scores<T>(s, 8);
+        }
+        if (masked && attn_not_finite<T, DP>(sk + stage, kAttnStep, lane)) {
+            add_columns_singly<T, DP, 4>(dq, tile, sk + stage, p, [&](int i) { return i <= last; }, lane);
+            continue;
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) add_columns<T, DP>(dq, tile, sk + stage, s, p[s]);
+    }
+    store_rows<T, DP>(dq, A.scale / lift, A.dq, (at * A.heads + head) * A.dim, A.dim, live, lane);
+}
+
+// dk and dv of 128 keys of one head of keys, 32 a wave: over the heads of queries that share it, and their queries 64 at a time
+template <int T, int DP>
+__global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_dkv_kernel(const AttnArgs A) {
+    typedef AttnTile<DP> Tile;
+    __shared__ __attribute__((aligned(1024))) uint8_t sq[2 * Tile::kBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t sg[2 * Tile::kBytes];
+    __shared__ __attribute__((aligned(1024))) float rows_of[2][2][kAttnStep];   // lse and delta
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int t = blockIdx.x / A.kv_heads, kv = blockIdx.x - t * A.kv_heads;
+    const AttnTask task = attn_task(A, t, 128, true);
+    if (task.rows <= 0) return;
+    const int begin = A.causal ? max(0, task.shift) / kAttnStep : 0, per = max(0, (task.len + kAttnStep - 1) / kAttnStep - begin), steps = per * A.group;
+    Tile tile;
+    tile.init(lane);
+    typename Tile::Source qs, gs;
+    qs.init(A.q, attn_rows(A, task.other, task.seq, 0, A.q_stride, A.q_batch) + (int64_t)kv * A.group * A.q_head, A.q_stride, A.dim, wave, lane);
+    gs.init(A.dout, attn_rows(A, task.other, task.seq, 0, A.do_stride, A.do_batch) + (int64_t)kv * A.group * A.do_head, A.do_stride, A.dim, wave, lane);
+    const float* stats = (wave == 0 ? A.lse : A.delta) + kv * A.group * A.q_rows + task.other;
+    const char *const q_base = qs.base, *const g_base = gs.base;
+    auto load = [&](int j, int stage) {
+        const int head = j / per, first = (begin + j - head * per) * kAttnStep;
+        qs.base = q_base + 2 * (head * A.q_head);
+        gs.base = g_base + 2 * (head * A.do_head);
+        qs.load(sq + stage * Tile::kBytes, first, task.len, wave);
+        gs.load(sg + stage * Tile::kBytes, first, task.len, wave);
+        if (wave < 2) {
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(stats + head * A.q_rows + first, (uint32_t)__builtin_amdgcn_readfirstlane(min(kAttnStep, task.len - first) * 4));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(uintptr_t)&rows_of[stage][wave][0], 4, lane * 4, 0, 0, 0);
+        }
+    };
+    if (steps > 0) load(0, 0);
+    const int row = wave * 32 + (lane & 31);
+    const bool live = row < task.rows;
+    v4i k[DP / 16], v[DP / 16];
+    load_own<DP>(k, A.k, attn_rows(A, task.own, task.seq, task.at, A.k_stride, A.k_batch) + kv * A.k_head + row * A.k_stride, A.dim, live, lane);
+    load_own<DP>(v, A.v, attn_rows(A, task.own, task.seq, task.at, A.v_stride, A.v_batch) + kv * A.v_head + row * A.v_stride, A.dim, live, lane);
+    constexpr float kUp = T == NTFP8_F16 ? kLiftP : 0.0f, kDown = T == NTFP8_F16 ? 1.0f / 256.0f : 1.0f;
+    const float lift = gradient_lift<T>(A), down = lift * kDown;
+    v16f dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) dk[e] = dv[e] = zeros16();
+    for (int j = 0; j < steps; ++j) {
+        const int stage = j & 1, row0 = (begin + j % per) * kAttnStep;
+        uint8_t *const qa = sq + stage * Tile::kBytes, *const ga = sg + stage * Tile::kBytes;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wg_barrier();
+        if (j + 1 < steps) load(j + 1, stage ^ 1);
+        const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
+        if (A.causal && row0 + kAttnStep - 1 < lead) continue;
+        const bool masked = row0 + kAttnStep > task.len || (A.causal && row0 < lead + 31);
+        const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
+        v4i p[4], ds[4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            v16f s = zeros16(), d = zeros16();
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                s = mfma_attn<T>(tile.rows(qa, b, i), k[i], s);
+                d = mfma_attn<T>(tile.rows(ga, b, i), v[i], d);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const v4f lse = *reinterpret_cast<const v4f*>(&rows_of[stage][0][32 * b + 8 * n + 4 * (lane >> 5)]);
+                const v4f delta = *reinterpret_cast<const v4f*>(&rows_of[stage][1][32 * b + 8 * n + 4 * (lane >> 5)]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 4 * n + i;
+                    s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, kUp - lse[i]));
+                    d[r] = s[r] * ((d[r] - delta[i]) * down);
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 32 * b + place_of(r, lane);
+                    const bool in = i >= from && i < to;
+                    s[r] = in ? s[r] : 0.0f;
+                    d[r] = in ? d[r] : 0.0f;
+                }
+            }
+            p[2 * b] = pack_scores<T>(s, 0);
+            p[2 * b + 1] = pack_scores<T>(s, 8);
+            ds[2 * b] = pack_scores<T>(d, 0);
+            ds[2 * b + 1] = pack_scores<T>(d, 8);
+        }
+        const auto counts = [&](int i) { return i >= from && i < to; };
+        if (masked && (attn_not_finite<T, DP>(ga, kAttnStep, lane) || attn_not_finite<T, DP>(qa, kAttnStep, lane))) {
+            add_columns_singly<T, DP, 4>(dv, tile, ga, p, counts, lane);
+            add_columns_singly<T, DP, 4>(dk, tile, qa, ds, counts, lane);
+            continue;
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            add_columns<T, DP>(dv, tile, ga, s, p[s]);
+            add_columns<T, DP>(dk, tile, qa, s, ds[s]);
+        }
+    }
+    const int64_t to = (((int64_t)task.own + row) * A.kv_heads + kv) * A.dim;
+    if (A.dv) store_rows<T, DP>(dv, kDown, A.dv, to, A.dim, live, lane);
+    if (A.dk) store_rows<T, DP>(dk, A.scale / lift, A.dk, to, A.dim, live, lane);
+}
+
+}  // namespace
+
+int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, int64_t k_tiles, const int* cu_q, const int* cu_k, int dtype, hipStream_t st) {
+    return with_attn(dtype, A.dim, [&](auto t, auto d) {
+        constexpr int T = decltype(t)::value, DP = decltype(d)::value;
+        const int64_t q_blocks = (A.q_rows * A.heads + 15) / 16, v_blocks = T == NTFP8_F16 ? (A.k_rows * A.kv_heads + 15) / 16 : 0;
+        if (T == NTFP8_F16) {
+            attention_clear_kernel<<<1, 2, 0, st>>>(A.most);
+            if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+        }
+        attention_delta_kernel<T><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(A, cu_q, cu_k, q_blocks);
+        if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+        if (A.dk || A.dv) {
+            AttnArgs K = A;
+            K.tasks = k_tasks;
+            attention_dkv_kernel<T, DP><<<(unsigned)(k_tiles * A.kv_heads), 64 * kAttnWaves, 0, st>>>(K);
+            if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+        }
+        if (A.dq) {
+            attention_dq_kernel<T, DP><<<(unsigned)(A.tiles * A.heads), 64 * kAttnWaves, 0, st>>>(A);
+            if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+        }
+        return (int)NTFP8_OK;
+    });
+}
+
+}  // namespace ntfp8

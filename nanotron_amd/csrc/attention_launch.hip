@@ -1,0 +1,125 @@
+// Attention: which kernels a call takes, how the work is cut, and what lies where in the workspace.
+#include "attention.h"
+
+namespace ntfp8 {
+
+int run_attention_plan(const int* cu_q, const int* cu_k, int sequences, int q_rows, int k_rows, int causal, int q_tile, int k_tile, int q_tasks, int k_tasks,
+                       AttnTask* q_list, AttnTask* k_list, hipStream_t st);
+int run_attention_forward_kernels(const AttnArgs& A, int dtype, int q_blocks, bool few, hipStream_t st);
+int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, int64_t k_tiles, const int* cu_q, const int* cu_k, int dtype, hipStream_t st);
+
+namespace {
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+// tiles of `tile` rows: exactly of equal sequences, at most of packed ones (each may end in part of one, and so may the rows of none)
+int64_t tiles_of(const ntops_attention_desc& d, int64_t rows, int64_t tile) {
+    if (d.cu_q) return rows / tile + d.sequences + 2;
+    return d.sequences * ((rows / d.sequences + tile - 1) / tile);
+}
+
+struct Choice {
+    bool few;
+    int q_blocks, splits;
+    int64_t tiles;
+};
+Choice choose(const ntops_attention_desc& d) {
+    const int64_t cus = cu_count(), q_len = d.q_rows / d.sequences, k_len = d.k_rows / d.sequences;   // (of packed ones, on average)
+    Choice c = {};
+    c.splits = 1;
+    c.few = !d.cu_q && d.heads / d.kv_heads * q_len <= 32 && d.sequences * d.kv_heads <= ((int64_t)1 << 22);
+    if (c.few) {
+        const int64_t units = d.sequences * d.kv_heads;
+        c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len / 256));
+        return c;
+    }
+    c.q_blocks = 1;
+    c.tiles = tiles_of(d, d.q_rows, 128 * c.q_blocks);
+    const int64_t groups = c.tiles * d.heads, room = 2 * cus;
+    if (groups < room) c.splits = (int)std::max<int64_t>(1, std::min(room / groups, k_len / 512));
+    return c;
+}
+
+struct Layout {
+    int64_t q_tasks, k_tasks, part, part_ml, delta, most, bytes;
+};
+Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, int64_t q_tiles, int64_t k_tiles) {
+    Layout l = {};
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += up(bytes, 256);
+        return here;
+    };
+    l.q_tasks = take(d.cu_q ? q_tiles * (int64_t)sizeof(AttnTask) : 0);
+    if (backward) {
+        l.k_tasks = take(d.cu_q ? k_tiles * (int64_t)sizeof(AttnTask) : 0);
+        l.delta = take(d.q_rows * d.heads * 4);
+        l.most = take(8);
+    } else if (c.splits > 1) {
+        l.part = take(c.splits * d.q_rows * d.heads * d.head_dim * 4);
+        l.part_ml = take(c.splits * d.q_rows * d.heads * 8);
+    }
+    l.bytes = at;
+    return l;
+}
+
+AttnArgs args_of(const ntops_attention_desc& d) {
+    AttnArgs a = {};
+    a.q = d.q, a.k = d.k, a.v = d.v, a.dout = d.dout;
+    a.q_stride = d.q_stride, a.k_stride = d.k_stride, a.v_stride = d.v_stride, a.do_stride = d.do_stride;
+    a.q_head = d.q_head, a.k_head = d.k_head, a.v_head = d.v_head, a.do_head = d.do_head;
+    a.q_batch = d.q_batch, a.k_batch = d.k_batch, a.v_batch = d.v_batch, a.do_batch = d.do_batch;
+    a.sequences = (int)d.sequences, a.q_len = (int)(d.q_rows / d.sequences), a.k_len = (int)(d.k_rows / d.sequences);
+    a.q_rows = d.q_rows, a.k_rows = d.k_rows;
+    a.heads = d.heads, a.kv_heads = d.kv_heads, a.group = d.heads / d.kv_heads, a.dim = d.head_dim, a.causal = d.causal;
+    a.c = d.scale * kLog2E, a.scale = d.scale;
+    a.out = d.out, a.o = d.out, a.lse = d.lse, a.dq = d.dq, a.dk = d.dk, a.dv = d.dv, a.splits = 1;
+    return a;
+}
+
+}  // namespace
+
+// What a launch has to hold: workgroups, and threads, in 32 bits
+bool attention_fits(const ntops_attention_desc& d) {
+    constexpr int64_t kMost = (int64_t)1 << 23;
+    return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, 128) * d.heads <= kMost && tiles_of(d, d.k_rows, 128) * d.kv_heads <= kMost;
+}
+
+int64_t attention_workspace(const ntops_attention_desc& d, bool backward) {
+    const Choice c = choose(d);
+    return layout_of(d, backward, c, backward ? tiles_of(d, d.q_rows, 128) : c.tiles, tiles_of(d, d.k_rows, 128)).bytes;
+}
+
+int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
+    const Choice c = choose(d);
+    const Layout l = layout_of(d, false, c, c.tiles, 0);
+    char* const ws = static_cast<char*>(d.workspace);
+    AttnArgs a = args_of(d);
+    a.tiles = c.tiles, a.splits = c.splits;
+    if (c.splits > 1) a.part = reinterpret_cast<float*>(ws + l.part), a.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+    if (d.cu_q) {
+        AttnTask* const list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
+        a.tasks = list;
+        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, 128 * c.q_blocks, 0, (int)c.tiles, 0, list, nullptr, st)) return rc;
+    }
+    return run_attention_forward_kernels(a, d.dtype, c.q_blocks, c.few, st);
+}
+
+int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
+    AttnArgs a = args_of(d);
+    a.tiles = tiles_of(d, d.q_rows, 128);
+    const int64_t k_tiles = tiles_of(d, d.k_rows, 128);
+    const Layout l = layout_of(d, true, {}, a.tiles, k_tiles);
+    char* const ws = static_cast<char*>(d.workspace);
+    a.delta = reinterpret_cast<float*>(ws + l.delta), a.most = reinterpret_cast<uint32_t*>(ws + l.most);
+    AttnTask* k_list = nullptr;
+    if (d.cu_q) {
+        AttnTask* const q_list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
+        k_list = reinterpret_cast<AttnTask*>(ws + l.k_tasks);
+        a.tasks = q_list;
+        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, 128, 128, (int)a.tiles, (int)k_tiles, q_list, k_list, st)) return rc;
+    }
+    return run_attention_backward_kernels(a, k_list, k_tiles, d.cu_q, d.cu_k, d.dtype, st);
+}
+
+}  // namespace ntfp8

@@ -17,6 +17,15 @@ int run_adamw_unpack(const void* codes, const float* scale, int64_t n, float* ou
 int64_t head_piece(int64_t vocab);
 int64_t head_workspace(const ntops_linear_cross_entropy_desc& d);
 int run_head(const ntops_linear_cross_entropy_desc& d, hipStream_t st);
+int64_t rms_norm_most_cols(int dtype);
+int rms_norm_blocks(int dtype, int64_t rows, int64_t cols);
+int run_rms_norm_forward(const ntops_rms_norm_desc& d, hipStream_t st);
+int run_rms_norm_backward(const ntops_rms_norm_desc& d, const ntops_rms_norm_grads& g, hipStream_t st);
+int run_rotary(const ntops_rotary_desc& d, hipStream_t st);
+bool attention_fits(const ntops_attention_desc& d);
+int64_t attention_workspace(const ntops_attention_desc& d, bool backward);
+int run_attention_forward(const ntops_attention_desc& d, hipStream_t st);
+int run_attention_backward(const ntops_attention_desc& d, hipStream_t st);
 int run_scale(const ntops_scale_tensor* t, int count, int x_dtype, const float* factor, int out_dtype, hipStream_t st);
 
 namespace {
@@ -51,6 +60,95 @@ int check_head(const ntops_linear_cross_entropy_desc& d) {
     if (!rows_ok(d.tokens, d.hidden, d.x_stride) || !rows_ok(d.vocab, d.hidden, d.weight_stride)) return NTFP8_ERR_SIZE;
     if ((d.dx || d.dweight) && d.grad_dtype != d.x_dtype && d.grad_dtype != NTFP8_F32) return NTFP8_ERR_ENUM;
     return NTFP8_OK;
+}
+
+struct Range {
+    const void* p;
+    int64_t bytes;
+};
+// whether an output lies over an input, or over another output
+template <size_t I, size_t O>
+bool collide(const Range (&in)[I], const Range (&out)[O]) {
+    for (size_t i = 0; i < O; ++i) {
+        for (const Range& r : in)
+            if (overlap(r.p, r.bytes, out[i].p, out[i].bytes)) return true;
+        for (size_t j = 0; j < i; ++j)
+            if (overlap(out[j].p, out[j].bytes, out[i].p, out[i].bytes)) return true;
+    }
+    return false;
+}
+
+int check_rms_norm(const ntops_rms_norm_desc& d) {
+    if (!dtype_ok(d.x_dtype) || (d.residual_dtype != NTFP8_F32 && d.residual_dtype != d.x_dtype) || (d.w_dtype != NTFP8_F32 && d.w_dtype != d.x_dtype) ||
+        d.gate_kind < NTOPS_GATE_NONE || d.gate_kind > NTOPS_GATE_ELEMENT)
+        return NTFP8_ERR_ENUM;
+    if (!rows_ok(d.rows, d.cols, d.x_stride) || (d.residual && !rows_ok(d.rows, d.cols, d.residual_stride)) ||
+        (d.gate_kind == NTOPS_GATE_ELEMENT && !rows_ok(d.rows, d.cols, d.gate_stride)))
+        return NTFP8_ERR_SIZE;
+    if (d.cols > rms_norm_most_cols(d.x_dtype) || !(d.eps >= 0.0f) || !(d.residual_scale == d.residual_scale)) return NTFP8_ERR_UNSUPPORTED;
+    if (d.gate_kind != NTOPS_GATE_NONE && !d.gate) return NTFP8_ERR_NULL;
+    const size_t xs = size_of(d.x_dtype), rs = size_of(d.residual_dtype), ws = size_of(d.w_dtype);
+    if (!aligned(d.x, xs) || !aligned(d.residual, rs) || !aligned(d.gate, d.gate_kind == NTOPS_GATE_ELEMENT ? xs : ws) || !aligned(d.weight, ws) ||
+        !aligned(d.post_weight, ws) || !aligned(d.y, xs) || !aligned(d.h, rs) || !aligned(d.first, 4) || !aligned(d.second, 4))
+        return NTFP8_ERR_ALIGN;
+    return NTFP8_OK;
+}
+
+// elements between a tensor's first and behind its last
+int64_t reach(int64_t rows, int64_t stride, int64_t heads, int64_t head, int64_t dim) { return (rows - 1) * stride + (heads - 1) * head + dim; }
+
+int check_rotary(const ntops_rotary_desc& d) {
+    if (!dtype_ok(d.dtype) || (d.position_bits != 32 && d.position_bits != 64)) return NTFP8_ERR_ENUM;
+    if (d.heads < 0 || d.kv_heads < 0 || (d.heads > 0 && (!d.q || !d.q_out)) || (d.kv_heads > 0 && (!d.k || !d.k_out)) || !d.positions || !d.frequencies) return NTFP8_ERR_NULL;
+    if (d.tokens <= 0 || d.tokens > 0x7fffffff || d.heads + d.kv_heads < 1 || d.heads + d.kv_heads > 16384 || d.head_dim < 1 || d.pairs < 1 || 2 * d.pairs > d.head_dim ||
+        d.position_count < 1)
+        return NTFP8_ERR_SIZE;
+    constexpr int64_t kMost = (int64_t)1 << 31;   // elements from token to token and from head to head
+    for (const int64_t v : {d.q_stride, d.q_head, d.k_stride, d.k_head})
+        if (v < 0 || v > kMost) return NTFP8_ERR_SIZE;
+    if (d.head_dim > 2048 || !(d.scale == d.scale)) return NTFP8_ERR_UNSUPPORTED;
+    const size_t s = size_of(d.dtype);
+    if (!aligned(d.q, s) || !aligned(d.k, s) || !aligned(d.q_out, s) || !aligned(d.k_out, s) || !aligned(d.positions, d.position_bits / 8) || !aligned(d.frequencies, 8))
+        return NTFP8_ERR_ALIGN;
+    const int64_t b = (int64_t)s;
+    const Range in[] = {{d.heads ? d.q : nullptr, reach(d.tokens, d.q_stride, d.heads, d.q_head, d.head_dim) * b},
+                        {d.kv_heads ? d.k : nullptr, reach(d.tokens, d.k_stride, d.kv_heads, d.k_head, d.head_dim) * b},
+                        {d.positions, d.position_count * d.position_bits / 8},
+                        {d.frequencies, 8 * d.pairs}};
+    const Range out[] = {{d.heads ? d.q_out : nullptr, d.tokens * d.heads * d.head_dim * b}, {d.kv_heads ? d.k_out : nullptr, d.tokens * d.kv_heads * d.head_dim * b}};
+    return collide(in, out) ? NTFP8_ERR_ALIAS : NTFP8_OK;
+}
+
+int check_attention_sizes(const ntops_attention_desc& d) {
+    if (d.dtype != NTFP8_BF16 && d.dtype != NTFP8_F16) return NTFP8_ERR_ENUM;
+    constexpr int64_t kMost = (int64_t)1 << 27;
+    if (d.heads < 1 || d.kv_heads < 1 || d.heads % d.kv_heads != 0 || d.head_dim < 8 || d.sequences < 1 || d.sequences > kMost || d.q_rows < 1 || d.k_rows < 0 ||
+        d.q_rows > kMost / d.heads || d.k_rows > kMost / d.kv_heads)
+        return NTFP8_ERR_SIZE;
+    if ((d.cu_q == nullptr) != (d.cu_k == nullptr)) return NTFP8_ERR_NULL;
+    if (!d.cu_q && (d.q_rows % d.sequences != 0 || d.k_rows % d.sequences != 0)) return NTFP8_ERR_SIZE;
+    if (d.head_dim > 128 || d.head_dim % 8 != 0) return NTFP8_ERR_UNSUPPORTED;
+    return attention_fits(d) ? NTFP8_OK : NTFP8_ERR_SIZE;
+}
+
+int check_attention(const ntops_attention_desc& d) {
+    if (const int rc = check_attention_sizes(d)) return rc;
+    if (!d.q || (d.k_rows > 0 && (!d.k || !d.v)) || !d.out || !d.workspace) return NTFP8_ERR_NULL;
+    if (!(d.scale > 0.0f) || d.scale > 1e30f) return NTFP8_ERR_UNSUPPORTED;
+    // (64 rows of a tile lie within 2^31 bytes)
+    for (const int64_t v : {d.q_stride, d.k_stride, d.v_stride, d.do_stride})
+        if (v < 0 || v > ((int64_t)1 << 24) || v % 8 != 0) return NTFP8_ERR_SIZE;
+    for (const int64_t v : {d.q_head, d.k_head, d.v_head, d.do_head, d.q_batch, d.k_batch, d.v_batch, d.do_batch})
+        if (v < 0 || v > kMostElements || v % 8 != 0) return NTFP8_ERR_SIZE;
+    for (const void* p : {d.q, d.k, d.v, d.dout, (const void*)d.out, (const void*)d.dq, (const void*)d.dk, (const void*)d.dv})
+        if (!aligned(p, 16)) return NTFP8_ERR_ALIGN;
+    return aligned(d.lse, 4) && aligned(d.cu_q, 4) && aligned(d.cu_k, 4) && aligned(d.workspace, 256) ? NTFP8_OK : NTFP8_ERR_ALIGN;
+}
+// bytes of a tensor of a call, from its first element on
+int64_t attention_reach(const ntops_attention_desc& d, int64_t rows, int64_t heads, int64_t stride, int64_t head, int64_t batch) {
+    if (rows == 0) return 0;
+    const int64_t each = d.cu_q ? rows : rows / d.sequences;
+    return 2 * (reach(each, stride, heads, head, d.head_dim) + (d.cu_q ? 0 : (d.sequences - 1) * batch));
 }
 
 }  // namespace
@@ -145,20 +243,105 @@ int ntops_linear_cross_entropy(const ntops_linear_cross_entropy_desc* d, void* s
     if (!aligned(d->x, 2) || !aligned(d->weight, 2) || !aligned(d->labels, 8) || !aligned(d->losses, 4) || !aligned(d->loss, 4) || !aligned(d->dx, 16) ||
         !aligned(d->dweight, 16) || !aligned(d->workspace, 256))
         return NTFP8_ERR_ALIGN;
-    struct Range {
-        const void* p;
-        int64_t bytes;
-    };
     const int64_t gs = size_of(d->grad_dtype == NTFP8_F32 ? NTFP8_F32 : d->x_dtype);
     const Range in[] = {{d->x, span(d->tokens, d->hidden, d->x_stride, d->x_dtype)}, {d->weight, span(d->vocab, d->hidden, d->weight_stride, d->x_dtype)}, {d->labels, 8 * d->tokens}};
     const Range out[] = {{d->losses, 4 * d->tokens}, {d->loss, 4}, {d->dx, d->tokens * d->hidden * gs}, {d->dweight, d->vocab * d->hidden * gs}, {d->workspace, head_workspace(*d)}};
-    for (int i = 0; i < 5; ++i) {
-        for (const Range& r : in)
-            if (overlap(r.p, r.bytes, out[i].p, out[i].bytes)) return NTFP8_ERR_ALIAS;
-        for (int j = 0; j < i; ++j)
-            if (overlap(out[j].p, out[j].bytes, out[i].p, out[i].bytes)) return NTFP8_ERR_ALIAS;
-    }
+    if (collide(in, out)) return NTFP8_ERR_ALIAS;
     return run_head(*d, static_cast<hipStream_t>(stream));
+}
+
+int ntops_rms_norm_forward(const ntops_rms_norm_desc* d, void* stream) {
+    if (!d || !d->x || !d->y || (d->residual == nullptr) != (d->h == nullptr)) return NTFP8_ERR_NULL;
+    if (d->residual ? (d->second == nullptr && d->first != nullptr) : (d->post_weight || d->gate_kind != NTOPS_GATE_NONE)) return NTFP8_ERR_NULL;
+    if (d->second && d->post_weight && !d->first) return NTFP8_ERR_NULL;
+    if (const int rc = check_rms_norm(*d)) return rc;
+    if (!d->residual && d->residual_dtype != d->x_dtype) return NTFP8_ERR_ENUM;
+    const int64_t n = d->rows * d->cols, xs = size_of(d->x_dtype), rs = size_of(d->residual_dtype), wb = d->cols * size_of(d->w_dtype);
+    const bool element = d->gate_kind == NTOPS_GATE_ELEMENT;
+    const Range in[] = {{d->x, span(d->rows, d->cols, d->x_stride, d->x_dtype)},
+                        {d->residual, span(d->rows, d->cols, d->residual_stride, d->residual_dtype)},
+                        {d->gate_kind ? d->gate : nullptr, element ? span(d->rows, d->cols, d->gate_stride, d->x_dtype) : wb},
+                        {d->weight, wb},
+                        {d->post_weight, wb}};
+    const Range out[] = {{d->y, n * xs}, {d->h, n * rs}, {d->first, 4 * d->rows}, {d->second, 4 * d->rows}};
+    if (collide(in, out)) return NTFP8_ERR_ALIAS;
+    return run_rms_norm_forward(*d, static_cast<hipStream_t>(stream));
+}
+
+int64_t ntops_rms_norm_scratch(const ntops_rms_norm_desc* d) {
+    if (!d || check_rms_norm(*d) != NTFP8_OK) return 0;
+    return (int64_t)rms_norm_blocks(d->x_dtype, d->rows, d->cols) * (d->post_weight || d->gate_kind ? 3 : 1) * d->cols * 4;
+}
+
+int ntops_rms_norm_backward(const ntops_rms_norm_desc* d, const ntops_rms_norm_grads* g, void* stream) {
+    if (!d || !g || !d->x || !d->second || (d->post_weight && !d->first) || (!g->dy && !g->dh)) return NTFP8_ERR_NULL;
+    if (!d->h && (d->post_weight || d->gate_kind != NTOPS_GATE_NONE || g->dh || g->dresidual)) return NTFP8_ERR_NULL;
+    if ((g->dweight && !d->weight) || (g->dpost_weight && !d->post_weight) || (g->dgate && d->gate_kind == NTOPS_GATE_NONE)) return NTFP8_ERR_NULL;
+    if (!g->dx && !g->dresidual && !g->dgate && !g->dweight && !g->dpost_weight) return NTFP8_ERR_NULL;
+    if ((g->dweight || g->dpost_weight || (g->dgate && d->gate_kind == NTOPS_GATE_CHANNEL)) && !g->scratch) return NTFP8_ERR_NULL;
+    if (const int rc = check_rms_norm(*d)) return rc;
+    if (!d->h && d->residual_dtype != d->x_dtype) return NTFP8_ERR_ENUM;
+    if ((g->dy && !rows_ok(d->rows, d->cols, g->dy_stride)) || (g->dh && !rows_ok(d->rows, d->cols, g->dh_stride))) return NTFP8_ERR_SIZE;
+    const bool element = d->gate_kind == NTOPS_GATE_ELEMENT;
+    const size_t xs = size_of(d->x_dtype), rs = size_of(d->residual_dtype), ws = size_of(d->w_dtype);
+    if (!aligned(g->dy, xs) || !aligned(g->dh, rs) || !aligned(g->dx, xs) || !aligned(g->dresidual, rs) || !aligned(g->dgate, element ? xs : ws) || !aligned(g->dweight, ws) ||
+        !aligned(g->dpost_weight, ws) || !aligned(g->scratch, 16))
+        return NTFP8_ERR_ALIGN;
+    const int64_t n = d->rows * d->cols, wb = d->cols * (int64_t)ws;
+    const Range in[] = {{d->x, span(d->rows, d->cols, d->x_stride, d->x_dtype)},
+                        {d->h, n * (int64_t)rs},
+                        {d->gate_kind ? d->gate : nullptr, element ? span(d->rows, d->cols, d->gate_stride, d->x_dtype) : wb},
+                        {d->weight, wb},
+                        {d->post_weight, wb},
+                        {d->first, 4 * d->rows},
+                        {d->second, 4 * d->rows},
+                        {g->dy, span(d->rows, d->cols, g->dy_stride, d->x_dtype)},
+                        {g->dh, span(d->rows, d->cols, g->dh_stride, d->residual_dtype)}};
+    const Range out[] = {{g->dx, n * (int64_t)xs}, {g->dresidual, n * (int64_t)rs}, {g->dgate, element ? n * (int64_t)xs : wb}, {g->dweight, wb}, {g->dpost_weight, wb},
+                         {g->scratch, g->scratch ? ntops_rms_norm_scratch(d) : 0}};
+    if (collide(in, out)) return NTFP8_ERR_ALIAS;
+    return run_rms_norm_backward(*d, *g, static_cast<hipStream_t>(stream));
+}
+
+int ntops_rotary(const ntops_rotary_desc* d, void* stream) {
+    if (!d) return NTFP8_ERR_NULL;
+    if (const int rc = check_rotary(*d)) return rc;
+    return run_rotary(*d, static_cast<hipStream_t>(stream));
+}
+
+int64_t ntops_attention_workspace(const ntops_attention_desc* d, int backward) {
+    return d && check_attention_sizes(*d) == NTFP8_OK ? std::max<int64_t>(256, attention_workspace(*d, backward != 0)) : 0;
+}
+
+int ntops_attention_forward(const ntops_attention_desc* d, void* stream) {
+    if (!d) return NTFP8_ERR_NULL;
+    if (const int rc = check_attention(*d)) return rc;
+    const int64_t cu = d->cu_q ? 4 * (d->sequences + 1) : 0;
+    const Range in[] = {{d->q, attention_reach(*d, d->q_rows, d->heads, d->q_stride, d->q_head, d->q_batch)},
+                        {d->k, attention_reach(*d, d->k_rows, d->kv_heads, d->k_stride, d->k_head, d->k_batch)},
+                        {d->v, attention_reach(*d, d->k_rows, d->kv_heads, d->v_stride, d->v_head, d->v_batch)},
+                        {d->cu_q, cu},
+                        {d->cu_k, cu}};
+    const Range out[] = {{d->out, 2 * d->q_rows * d->heads * d->head_dim}, {d->lse, 4 * d->q_rows * d->heads}, {d->workspace, attention_workspace(*d, false)}};
+    if (collide(in, out)) return NTFP8_ERR_ALIAS;
+    return run_attention_forward(*d, static_cast<hipStream_t>(stream));
+}
+
+int ntops_attention_backward(const ntops_attention_desc* d, void* stream) {
+    if (!d || !d->dout || !d->lse || (!d->dq && !d->dk && !d->dv)) return NTFP8_ERR_NULL;
+    if (const int rc = check_attention(*d)) return rc;
+    const int64_t cu = d->cu_q ? 4 * (d->sequences + 1) : 0, qb = 2 * d->q_rows * d->heads * d->head_dim, kb = 2 * d->k_rows * d->kv_heads * d->head_dim;
+    const Range in[] = {{d->q, attention_reach(*d, d->q_rows, d->heads, d->q_stride, d->q_head, d->q_batch)},
+                        {d->k, attention_reach(*d, d->k_rows, d->kv_heads, d->k_stride, d->k_head, d->k_batch)},
+                        {d->v, attention_reach(*d, d->k_rows, d->kv_heads, d->v_stride, d->v_head, d->v_batch)},
+                        {d->dout, attention_reach(*d, d->q_rows, d->heads, d->do_stride, d->do_head, d->do_batch)},
+                        {d->out, qb},
+                        {d->lse, 4 * d->q_rows * d->heads},
+                        {d->cu_q, cu},
+                        {d->cu_k, cu}};
+    const Range out[] = {{d->dq, qb}, {d->dk, kb}, {d->dv, kb}, {d->workspace, attention_workspace(*d, true)}};
+    if (collide(in, out)) return NTFP8_ERR_ALIAS;
+    return run_attention_backward(*d, static_cast<hipStream_t>(stream));
 }
 
 int ntops_scale(const ntops_scale_tensor* tensors, int count, int x_dtype, const float* factor, int out_dtype, void* stream) {

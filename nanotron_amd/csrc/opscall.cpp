@@ -161,6 +161,447 @@ Tensor layer_norm(const Tensor& x, const std::optional<Tensor>& weight, const st
     return norm_forward(x, w, b, eps, false).y;
 }
 
+// ---------------------------------------------------------------------------------------------- norms around a block
+bool floats(const Tensor& t, const Tensor& x) { return t.scalar_type() == at::kFloat || t.scalar_type() == x.scalar_type(); }
+Tensor dense_like(const Tensor& t) { return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)); }
+
+struct Norms {
+    Rows x, residual, gate;
+    Tensor w, pw, y, h, stats;   // stats: 1 / rms of the rows of x and, behind them, of h
+};
+// what both passes hand to the library
+ntops_rms_norm_desc norms_desc(const Norms& n, const Tensor& x, const Tensor& residual, const Tensor& gate, double eps, double scale) {
+    ntops_rms_norm_desc d = {};
+    d.x = n.x.t.data_ptr(), d.rows = n.x.rows, d.cols = n.x.cols, d.x_stride = n.x.stride;
+    d.x_dtype = code_of(x, "x"), d.residual_dtype = residual.defined() ? code_of(residual, "residual") : d.x_dtype;
+    d.gate_kind = !gate.defined() ? NTOPS_GATE_NONE : gate.dim() == 1 ? NTOPS_GATE_CHANNEL : NTOPS_GATE_ELEMENT;
+    d.gate = at_or_null(n.gate.t), d.gate_stride = n.gate.stride;
+    d.weight = at_or_null(n.w), d.post_weight = at_or_null(n.pw);
+    const Tensor& one = n.w.defined() ? n.w : n.pw.defined() ? n.pw : n.gate.t;
+    d.w_dtype = n.w.defined() || n.pw.defined() || d.gate_kind == NTOPS_GATE_CHANNEL ? code_of(one, "weight") : d.x_dtype;
+    d.eps = (float)eps, d.residual_scale = (float)scale;
+    if (n.stats.defined()) {
+        d.second = n.stats.data_ptr<float>() + n.x.rows;
+        if (n.pw.defined()) d.first = n.stats.data_ptr<float>();
+    }
+    return d;
+}
+Tensor contiguous(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+Norms norms_of(const Tensor& x, const Tensor& gate, const Tensor& w, const Tensor& pw) {
+    Norms n;
+    n.x = rows_of(x);
+    n.w = contiguous(w), n.pw = contiguous(pw);
+    if (gate.defined()) n.gate = gate.dim() == 1 ? Rows{gate.contiguous(), 1, gate.size(0), gate.size(0)} : rows_of(gate);
+    return n;
+}
+Norms norms_forward(const Tensor& x, const Tensor& residual, const Tensor& w, const Tensor& pw, const Tensor& gate, double eps, double scale, bool keep) {
+    Norms n = norms_of(x, gate, w, pw);
+    n.y = dense_like(x);
+    if (residual.defined()) n.h = dense_like(residual);
+    if (keep) n.stats = at::empty({2, n.x.rows}, x.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+    if (x.numel() == 0) return n;
+    ntops_rms_norm_desc d = norms_desc(n, x, residual, gate, eps, scale);
+    if (residual.defined()) {
+        n.residual = rows_of(residual);
+        d.residual = n.residual.t.data_ptr(), d.residual_stride = n.residual.stride, d.h = n.h.data_ptr();
+    }
+    d.y = n.y.data_ptr();
+    call(ntops_rms_norm_forward(&d, stream_of(x)), "ntops_rms_norm_forward");
+    return n;
+}
+
+enum { kWantX = 1, kWantResidual = 2, kWantWeight = 4, kWantPost = 8, kWantGate = 16 };
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    // outputs: y, and h where there is a residual
+    static variable_list forward(AutogradContext* ctx, const Variable& x, const std::optional<Tensor>& residual_, const std::optional<Tensor>& weight, const std::optional<Tensor>& post,
+                                 const std::optional<Tensor>& gate_, double eps, double scale, int64_t want) {
+        const Tensor residual = residual_.value_or(Tensor()), w = weight.value_or(Tensor()), pw = post.value_or(Tensor()), gate = gate_.value_or(Tensor());
+        Guard guard(x.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Norms n = norms_forward(x, residual, w, pw, gate, eps, scale, true);
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["want"] = want;
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["scale"] = scale;
+        // x itself is read again where a norm or a gate stands behind it, or where it is what the one norm reads
+        const bool again = !residual.defined() || pw.defined() || gate.defined();
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["type"] = (int64_t)x.scalar_type();
+        ctx->save_for_backward({again ? (n.x.t.is_same(x) ? x : n.x.t) : Tensor(), n.h, w, pw, gate, n.stats});
+        if (!residual.defined()) return {n.y};
+        return {n.y, n.h};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("rms_norm");
+        const variable_list s = ctx->get_saved_variables();
+        const Variable &x_ = s[0], &h = s[1], &w = s[2], &pw = s[3], &gate = s[4];
+        const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
+        const int64_t want = ctx->saved_data["want"].toInt();
+        if (!dy.defined() && !dh.defined()) return variable_list(8);
+        const Tensor& some = dy.defined() ? dy : dh;
+        Guard guard(some.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        // the type of x is that of y; where x is not kept (a residual, no norm and no gate) its shape is that of h
+        const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const auto xo = some.options().dtype(type).memory_format(at::MemoryFormat::Contiguous);
+        const bool residual = h.defined();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        Tensor dx, dr, dw, dpw, dgate;
+        // one gradient serves both where they are equal
+        const bool same = residual && !pw.defined() && !gate.defined() && scale == 1.0 && h.scalar_type() == type;
+        if ((want & kWantX) || (same && (want & kWantResidual))) dx = at::empty(shape, xo);
+        if ((want & kWantResidual) && !same) dr = dense_like(h);
+        if (want & kWantWeight) dw = dense_like(w);
+        if (want & kWantPost) dpw = dense_like(pw);
+        if (want & kWantGate) dgate = dense_like(gate);
+        const auto given = [&] { return variable_list{want & kWantX ? dx : Tensor(), same && (want & kWantResidual) ? dx : dr, dw, dpw, dgate, Tensor(), Tensor(), Tensor()}; };
+        if (c10::multiply_integers(shape) == 0) {
+            for (Tensor* t : {&dw, &dpw, &dgate})
+                if (t->defined()) t->zero_();
+            return given();
+        }
+        const Tensor x = x_.defined() ? x_ : h;   // (not read where it was not kept)
+        Norms n = norms_of(x, gate, w, pw);
+        n.stats = s[5];
+        ntops_rms_norm_desc d = norms_desc(n, x, h, gate, ctx->saved_data["eps"].toDouble(), scale);
+        d.x_dtype = type == at::kFloat ? NTFP8_F32 : type == at::kHalf ? NTFP8_F16 : NTFP8_BF16;
+        if (!w.defined() && !pw.defined() && d.gate_kind != NTOPS_GATE_CHANNEL) d.w_dtype = d.x_dtype;
+        d.h = at_or_null(h);
+        ntops_rms_norm_grads g = {};
+        Rows gy, gh;
+        if (dy.defined()) {
+            gy = rows_of(dy.scalar_type() == type ? dy : dy.to(type));
+            g.dy = gy.t.data_ptr(), g.dy_stride = gy.stride;
+        }
+        if (dh.defined()) {
+            gh = rows_of(dh.scalar_type() == h.scalar_type() ? dh : dh.to(h.scalar_type()));
+            g.dh = gh.t.data_ptr(), g.dh_stride = gh.stride;
+        }
+        g.dx = at_or_null(dx), g.dresidual = at_or_null(dr), g.dgate = at_or_null(dgate), g.dweight = at_or_null(dw), g.dpost_weight = at_or_null(dpw);
+        Tensor scratch;
+        if (dw.defined() || dpw.defined() || (dgate.defined() && d.gate_kind == NTOPS_GATE_CHANNEL)) {
+            scratch = at::empty({ntops_rms_norm_scratch(&d)}, some.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+            g.scratch = scratch.data_ptr();
+        }
+        call(ntops_rms_norm_backward(&d, &g, stream_of(some)), "ntops_rms_norm_backward");
+        return given();
+    }
+};
+
+// y, and h where there is a residual
+std::vector<Tensor> rms_norm(const Tensor& x, const std::optional<Tensor>& residual_, const std::optional<Tensor>& weight, const std::optional<Tensor>& post, const std::optional<Tensor>& gate_,
+                             double eps, double scale) {
+    const Tensor residual = residual_.value_or(Tensor()), w = weight.value_or(Tensor()), pw = post.value_or(Tensor()), gate = gate_.value_or(Tensor());
+    on_gpu(x, "x");
+    code_of(x, "x");
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0, "x must have a last dimension to normalise over, got shape ", x.sizes());
+    const int64_t cols = x.size(-1), most = x.scalar_type() == at::kFloat ? 8192 : 16384;
+    TORCH_CHECK_VALUE(cols <= most, "x may have ", most, " columns at most as ", x.scalar_type(), ", got ", cols);
+    if (residual.defined()) {
+        same_device(residual, x, "residual");
+        code_of(residual, "residual");
+        TORCH_CHECK_VALUE(residual.sizes() == x.sizes(), "residual must have the shape of x, ", x.sizes(), ", got ", residual.sizes());
+        TORCH_CHECK_TYPE(floats(residual, x), "residual must be float32 or of the type of x (", x.scalar_type(), "), got ", residual.scalar_type());
+    }
+    Tensor first;   // the vectors have one type
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(w, "weight"), std::pair<const Tensor&, const char*>(pw, "post_weight"), std::pair<const Tensor&, const char*>(gate, "gate")}) {
+        if (!t.defined()) continue;
+        same_device(t, x, name);
+        code_of(t, name);
+        if (&t == &gate && t.dim() != 1) {
+            TORCH_CHECK_VALUE(t.sizes() == x.sizes(), "gate must have shape [", cols, "] or that of x, ", x.sizes(), ", got ", t.sizes());
+            TORCH_CHECK_TYPE(t.scalar_type() == x.scalar_type(), "a gate for every element must be of the type of x (", x.scalar_type(), "), got ", t.scalar_type());
+            continue;
+        }
+        TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == cols, name, " must have shape [", cols, "], got ", t.sizes());
+        TORCH_CHECK_TYPE(floats(t, x), name, " must be float32 or of the type of x (", x.scalar_type(), "), got ", t.scalar_type());
+        TORCH_CHECK_TYPE(!first.defined() || first.scalar_type() == t.scalar_type(), "weight, post_weight and a channel's gate must have one type");
+        first = t;
+    }
+    TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative");
+    TORCH_CHECK_VALUE(std::isfinite(scale), "residual_scale must be finite");
+    for (const Tensor* t : {&x, &residual, &w, &pw, &gate}) no_tangent(*t, "rms_norm");
+    int64_t want = 0;
+    const auto wants = [&](const Tensor& t, int64_t bit) { want |= t.defined() && t.requires_grad() ? bit : 0; };
+    wants(x, kWantX), wants(residual, kWantResidual), wants(w, kWantWeight), wants(pw, kWantPost), wants(gate, kWantGate);
+    if (at::GradMode::is_enabled() && want) return RmsNorm::apply(x, residual_, weight, post, gate_, eps, scale, want);
+    Guard guard(x.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Norms n = norms_forward(x, residual, w, pw, gate, eps, scale, false);
+    if (!residual.defined()) return {n.y};
+    return {n.y, n.h};
+}
+
+// ---------------------------------------------------------------------------------------------- rotary positions
+// x [..., heads, dim] as tokens a fixed distance apart
+struct Heads {
+    Tensor t;
+    int64_t tokens = 0, heads = 0, dim = 0, stride = 0, head = 0;
+};
+Heads heads_of(const Tensor& x) {
+    const int64_t n = x.dim();
+    Heads r{x, 0, x.size(-2), x.size(-1), 0, 0};
+    r.tokens = r.heads && r.dim ? x.numel() / (r.heads * r.dim) : 0;
+    bool walks = x.stride(-1) == 1 || r.dim == 1;
+    int64_t stride = r.heads * r.dim, size = 1;
+    for (int64_t i = n - 3; i >= 0 && walks; --i) {   // dimensions of one element have any stride
+        if (x.size(i) == 1) continue;
+        if (size == 1) stride = x.stride(i);
+        else walks = x.stride(i) == stride * size;
+        size *= x.size(i);
+    }
+    if (!walks) {
+        r.t = x.contiguous();
+        stride = r.heads * r.dim;
+    }
+    r.stride = stride;
+    r.head = r.heads > 1 ? r.t.stride(-2) : r.dim;
+    return r;
+}
+
+struct Turn {
+    Tensor positions, frequencies;
+    bool interleaved;
+    double scale;
+};
+// both outputs, undefined where the input is
+std::pair<Tensor, Tensor> rotate(const Tensor& q, const Tensor& k, const Turn& t, bool inverse) {
+    std::pair<Tensor, Tensor> out;
+    Heads qh, kh;
+    ntops_rotary_desc d = {};
+    const Tensor& some = q.defined() ? q : k;
+    if (q.defined()) {
+        out.first = dense_like(q);
+        qh = heads_of(q);
+        d.q = qh.t.data_ptr(), d.q_out = out.first.data_ptr(), d.q_stride = qh.stride, d.q_head = qh.head, d.heads = (int)qh.heads;
+    }
+    if (k.defined()) {
+        out.second = dense_like(k);
+        kh = heads_of(k);
+        d.k = kh.t.data_ptr(), d.k_out = out.second.data_ptr(), d.k_stride = kh.stride, d.k_head = kh.head, d.kv_heads = (int)kh.heads;
+    }
+    d.tokens = q.defined() ? qh.tokens : kh.tokens;
+    if (d.tokens == 0) return out;
+    d.head_dim = (int)some.size(-1), d.pairs = (int)t.frequencies.numel(), d.dtype = code_of(some, "q");
+    d.positions = t.positions.data_ptr(), d.position_count = t.positions.numel(), d.position_bits = t.positions.scalar_type() == at::kLong ? 64 : 32;
+    d.frequencies = t.frequencies.const_data_ptr<double>(), d.interleaved = t.interleaved, d.inverse = inverse, d.scale = (float)t.scale;
+    call(ntops_rotary(&d, stream_of(some)), "ntops_rotary");
+    return out;
+}
+struct Rotary : torch::autograd::Function<Rotary> {
+    static variable_list forward(AutogradContext* ctx, const Variable& q, const std::optional<Tensor>& k_, const Tensor& positions, const Tensor& frequencies, bool interleaved, double scale,
+                                 bool gq, bool gk) {
+        const Tensor k = k_.value_or(Tensor());
+        Guard guard(q.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Turn t{positions.contiguous(), frequencies.contiguous(), interleaved, scale};
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({t.positions, t.frequencies});
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["want"] = (int64_t)(gq | gk << 1);
+        ctx->saved_data["type"] = (int64_t)q.scalar_type();
+        auto out = rotate(q, k, t, false);
+        if (!k.defined()) return {out.first};
+        if (!gq) ctx->mark_non_differentiable({out.first});
+        if (!gk) ctx->mark_non_differentiable({out.second});
+        return {out.first, out.second};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("rotary");
+        const variable_list s = ctx->get_saved_variables();
+        const int64_t want = ctx->saved_data["want"].toInt();
+        const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const auto arrived = [&](size_t i) {
+            if (!(want >> i & 1) || i >= grads.size() || !grads[i].defined()) return Tensor();
+            return grads[i].scalar_type() == type ? grads[i] : grads[i].to(type);
+        };
+        const Tensor dq = arrived(0), dk = arrived(1);
+        if (!dq.defined() && !dk.defined()) return variable_list(8);
+        Guard guard((dq.defined() ? dq : dk).device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Turn t{s[0], s[1], ctx->saved_data["interleaved"].toBool(), ctx->saved_data["scale"].toDouble()};
+        const auto out = rotate(dq, dk, t, true);
+        return {out.first, out.second, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// the rotated q, and k where one is given
+std::vector<Tensor> rotary(const Tensor& q, const std::optional<Tensor>& k_, const Tensor& positions, const Tensor& frequencies, bool interleaved, double scale) {
+    const Tensor k = k_.value_or(Tensor());
+    on_gpu(q, "q");
+    code_of(q, "q");
+    TORCH_CHECK_VALUE(q.dim() >= 2 && q.size(-1) > 0 && q.size(-2) > 0, "q must have shape [..., heads, head_dim], got ", q.sizes());
+    const auto lead = q.sizes().slice(0, q.dim() - 2);
+    if (k.defined()) {
+        same_device(k, q, "k");
+        TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "k must be of the type of q (", q.scalar_type(), "), got ", k.scalar_type());
+        TORCH_CHECK_VALUE(k.dim() == q.dim() && k.sizes().slice(0, k.dim() - 2) == lead && k.size(-1) == q.size(-1) && k.size(-2) > 0, "k must have the shape of q but for its heads, ",
+                          q.sizes(), ", got ", k.sizes());
+    }
+    TORCH_CHECK_VALUE(q.size(-1) <= 2048 && q.size(-2) + (k.defined() ? k.size(-2) : 0) <= 16384, "head_dim may be 2048 at most and heads of q and k 16384, got ", q.sizes());
+    same_device(positions, q, "positions");
+    TORCH_CHECK_TYPE(positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt, "positions must be int64 or int32, got ", positions.scalar_type());
+    TORCH_CHECK_VALUE(positions.dim() <= (int64_t)lead.size() && positions.sizes() == lead.slice(lead.size() - positions.dim()),
+                      "positions must have the last of the dimensions of q in front of its heads, ", lead, ", got ", positions.sizes());
+    same_device(frequencies, q, "frequencies");
+    TORCH_CHECK_TYPE(frequencies.scalar_type() == at::kDouble, "frequencies must be float64 (angles of far positions need it), got ", frequencies.scalar_type());
+    TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.numel() >= 1 && 2 * frequencies.numel() <= q.size(-1),
+                      "frequencies must have shape [pairs], two elements of a head of ", q.size(-1), " each, got ", frequencies.sizes());
+    TORCH_CHECK_VALUE(!frequencies.requires_grad(), "frequencies get no gradient: detach them");
+    TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
+    for (const Tensor* t : {&q, &k}) no_tangent(*t, "rotary");
+    const bool gq = q.requires_grad(), gk = k.defined() && k.requires_grad();
+    if (at::GradMode::is_enabled() && (gq || gk)) return Rotary::apply(q, k_, positions, frequencies, interleaved, scale, gq, gk);
+    Guard guard(q.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    const auto out = rotate(q, k, Turn{positions.contiguous(), frequencies.contiguous(), interleaved, scale}, false);
+    if (!k.defined()) return {out.first};
+    return {out.first, out.second};
+}
+
+// ---------------------------------------------------------------------------------------------- attention
+// x [rows, heads, dim] or [sequences, rows, heads, dim] as the kernels walk it, copied where they cannot
+struct Attended {
+    Tensor t;
+    int64_t row = 0, head = 0, batch = 0;
+};
+Attended attended(const Tensor& x) {
+    const auto walks = [](const Tensor& t) {
+        if (t.numel() == 0) return true;
+        const int64_t n = t.dim();
+        if (t.stride(n - 1) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+        for (int64_t i = 0; i < n - 1; ++i)
+            if (t.size(i) > 1 && (t.stride(i) % 8 != 0 || t.stride(i) < 0 || t.stride(i) > ((int64_t)1 << (i == n - 3 ? 24 : 45)))) return false;
+        return true;
+    };
+    Attended a;
+    a.t = walks(x) ? x : x.contiguous();
+    if (!walks(a.t)) a.t = a.t.clone(at::MemoryFormat::Contiguous);   // (a dense view that begins off a 16-byte boundary)
+    const int64_t n = a.t.dim(), dim = a.t.size(-1);
+    const auto stride = [&](int64_t i) { return a.t.size(i) > 1 ? a.t.stride(i) : dim; };
+    a.head = stride(n - 2), a.row = stride(n - 3), a.batch = n == 4 ? stride(0) : 0;
+    return a;
+}
+struct Sequences {
+    Tensor q, k;   // cu_seqlens, or undefined
+    double scale;
+    bool causal;
+};
+ntops_attention_desc attention_desc(const Attended& q, const Attended& k, const Attended& v, const Sequences& s) {
+    ntops_attention_desc d = {};
+    const bool batch = q.t.dim() == 4;
+    d.q = q.t.data_ptr(), d.k = k.t.data_ptr(), d.v = v.t.data_ptr();
+    d.q_stride = q.row, d.k_stride = k.row, d.v_stride = v.row, d.q_head = q.head, d.k_head = k.head, d.v_head = v.head;
+    d.q_batch = q.batch, d.k_batch = k.batch, d.v_batch = v.batch;
+    d.heads = (int)q.t.size(-2), d.kv_heads = (int)k.t.size(-2), d.head_dim = (int)q.t.size(-1), d.dtype = code_of(q.t, "q");
+    d.sequences = batch ? q.t.size(0) : s.q.defined() ? s.q.numel() - 1 : 1;
+    d.q_rows = batch ? q.t.size(0) * q.t.size(1) : q.t.size(0), d.k_rows = batch ? k.t.size(0) * k.t.size(1) : k.t.size(0);
+    if (s.q.defined()) d.cu_q = s.q.const_data_ptr<int32_t>(), d.cu_k = s.k.const_data_ptr<int32_t>();
+    d.causal = s.causal, d.scale = (float)s.scale;
+    return d;
+}
+Tensor attention_room(ntops_attention_desc& d, bool backward, const Tensor& like) {
+    const int64_t bytes = ntops_attention_workspace(&d, backward);
+    Tensor ws = at::empty({bytes + 256}, like.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+    d.workspace = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws.data_ptr()) + 255) / 256 * 256);
+    return ws;
+}
+// out, and lse where a backward pass follows
+std::pair<Tensor, Tensor> attention_forward(const Attended& q, const Attended& k, const Attended& v, const Sequences& s, bool keep) {
+    std::pair<Tensor, Tensor> r;
+    r.first = dense_like(q.t);
+    ntops_attention_desc d = attention_desc(q, k, v, s);
+    if (keep) r.second = at::empty({d.heads, d.q_rows}, q.t.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
+    if (q.t.numel() == 0) return r;
+    d.out = r.first.data_ptr(), d.lse = keep ? r.second.data_ptr<float>() : nullptr;
+    const Tensor ws = attention_room(d, false, q.t);
+    call(ntops_attention_forward(&d, stream_of(q.t)), "ntops_attention_forward");
+    return r;
+}
+struct Attention : torch::autograd::Function<Attention> {
+    static Variable forward(AutogradContext* ctx, const Variable& q, const Variable& k, const Variable& v, const std::optional<Tensor>& cu_q, const std::optional<Tensor>& cu_k, bool causal,
+                            double scale, bool gq, bool gk, bool gv) {
+        Guard guard(q.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Sequences s{contiguous(cu_q.value_or(Tensor())), contiguous(cu_k.value_or(Tensor())), scale, causal};
+        const Attended a = attended(q), b = attended(k), c = attended(v);
+        const auto r = attention_forward(a, b, c, s, true);
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["want"] = (int64_t)(gq | gk << 1 | gv << 2);
+        // (what was copied is kept as the copy)
+        ctx->save_for_backward({a.t.is_same(q) ? q : a.t, b.t.is_same(k) ? k : b.t, c.t.is_same(v) ? v : c.t, s.q, s.k, r.first, r.second});
+        return r.first;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        once("attention");
+        const variable_list saved = ctx->get_saved_variables();
+        if (!grads[0].defined()) return variable_list(10);
+        const Variable &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[5];
+        Guard guard(q.device());
+        at::AutoDispatchBelowADInplaceOrView below;
+        const int64_t want = ctx->saved_data["want"].toInt();
+        Tensor dq, dk, dv;
+        if (want & 1) dq = dense_like(q);
+        if (want & 2) dk = dense_like(k);
+        if (want & 4) dv = dense_like(v);
+        const variable_list given = {dq, dk, dv, Variable(), Variable(), Variable(), Variable(), Variable(), Variable(), Variable()};
+        if (q.numel() == 0 || k.numel() == 0) {   // no pair of a query and a key
+            for (Tensor* t : {&dq, &dk, &dv})
+                if (t->defined()) t->zero_();
+            return given;
+        }
+        const Sequences s{saved[3], saved[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool()};
+        const Attended g = attended(grads[0].scalar_type() == q.scalar_type() ? grads[0] : grads[0].to(q.scalar_type()));
+        ntops_attention_desc d = attention_desc(attended(q), attended(k), attended(v), s);
+        d.out = out.data_ptr(), d.lse = saved[6].data_ptr<float>();
+        d.dout = g.t.data_ptr(), d.do_stride = g.row, d.do_head = g.head, d.do_batch = g.batch;
+        d.dq = at_or_null(dq), d.dk = at_or_null(dk), d.dv = at_or_null(dv);
+        const Tensor ws = attention_room(d, true, q);
+        call(ntops_attention_backward(&d, stream_of(q)), "ntops_attention_backward");
+        return given;
+    }
+};
+
+Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& cu_q, const std::optional<Tensor>& cu_k_, bool causal, const std::optional<double>& scale_) {
+    on_gpu(q, "q");
+    TORCH_CHECK_TYPE(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "q must be bfloat16 or float16, got ", q.scalar_type());
+    TORCH_CHECK_VALUE(q.dim() == 3 || q.dim() == 4, "q must have shape [tokens, heads, head_dim] or [batch, tokens, heads, head_dim], got ", q.sizes());
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(k, "k"), std::pair<const Tensor&, const char*>(v, "v")}) {
+        same_device(t, q, name);
+        TORCH_CHECK_TYPE(t.scalar_type() == q.scalar_type(), name, " must be of the type of q (", q.scalar_type(), "), got ", t.scalar_type());
+        TORCH_CHECK_VALUE(t.dim() == q.dim() && t.sizes() == k.sizes() && t.size(-1) == q.size(-1) && (q.dim() == 3 || t.size(0) == q.size(0)),
+                          "k and v must have one shape, that of q but for tokens and heads: ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+    }
+    const int64_t heads = q.size(-2), kv_heads = k.size(-2), dim = q.size(-1);
+    TORCH_CHECK_VALUE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "the heads of q must be a multiple of those of k, got ", heads, " and ", kv_heads);
+    TORCH_CHECK_VALUE(dim > 0 && dim <= 128 && dim % 8 == 0, "head_dim must be a multiple of 8 and 128 at most, got ", dim);
+    TORCH_CHECK_VALUE(!cu_k_ || cu_q, "cu_seqlens_k needs cu_seqlens");
+    std::optional<Tensor> cu_k = cu_k_;
+    if (cu_q) {
+        TORCH_CHECK_VALUE(q.dim() == 3, "cu_seqlens goes with packed q of shape [tokens, heads, head_dim], got ", q.sizes());
+        if (!cu_k) {
+            TORCH_CHECK_VALUE(q.size(0) == k.size(0), "q and k have ", q.size(0), " and ", k.size(0), " tokens: give cu_seqlens_k too");
+            cu_k = cu_q;
+        }
+        for (const auto& [t, name] : {std::pair<const Tensor&, const char*>(*cu_q, "cu_seqlens"), std::pair<const Tensor&, const char*>(*cu_k, "cu_seqlens_k")}) {
+            same_device(t, q, name);
+            TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ", t.scalar_type());
+            TORCH_CHECK_VALUE(t.dim() == 1 && t.numel() >= 2 && t.numel() == cu_q->numel(), name, " must have shape [sequences + 1], got ", t.sizes());
+        }
+    }
+    const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)dim);
+    TORCH_CHECK_VALUE(scale > 0 && scale <= 1e30, "scale must be positive, got ", scale);
+    for (const Tensor* t : {&q, &k, &v}) no_tangent(*t, "attention");
+    const bool gq = q.requires_grad(), gk = k.requires_grad(), gv = v.requires_grad();
+    if (at::GradMode::is_enabled() && (gq || gk || gv)) return Attention::apply(q, k, v, cu_q, cu_k, causal, scale, gq, gk, gv);
+    Guard guard(q.device());
+    at::AutoDispatchBelowADInplaceOrView below;
+    return attention_forward(attended(q), attended(k), attended(v), Sequences{contiguous(cu_q.value_or(Tensor())), contiguous(cu_k.value_or(Tensor())), scale, causal}, false).first;
+}
+
 // ---------------------------------------------------------------------------------------------- cross entropy
 struct Head {
     Tensor loss, losses, dx, dw;
@@ -388,6 +829,9 @@ Tensor adamw_unpack(const Tensor& codes, const Tensor& scale) {
 
 PYBIND11_MODULE(_opscall, m) {
     m.def("layer_norm", &layer_norm);
+    m.def("rms_norm", &rms_norm);
+    m.def("rotary", &rotary);
+    m.def("attention", &attention);
     m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("adamw", &adamw);
     m.def("adamw_unpack", &adamw_unpack);

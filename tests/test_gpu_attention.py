@@ -1,0 +1,437 @@
+"""Attention against its formulas in 64 bits.
+
+Tolerances, with u = 2^-8 (bf16) or 2^-11 (fp16), half a step of what is rounded to 16 bits, and w = 2^-24.  A score is a sum of D products in fp32:
+off by (D + 4) w c sum|q||k| in the exponent, and exponential, maximum and logarithm bring 16 w each way, so the softmax p and what it is
+divided by are off by e = 2 (D + 4) w c max sum|q||k| + (n + 64) w relative, n keys being added up.  The numerators are rounded once for the
+product: out is off by (u + e) p|v|, and u |out| for its own rounding.  dv by (u + e) p^T|dout| and its rounding.  delta is made of the rounded
+out: off by |dout| (what out is off by); dout v^T by D w |dout||v|; ds = p (..) by p times both and (u + 2 e) |ds|, of which dq and dk are
+sums with |k| and |q|, n more w for adding up.  fp16 has a smallest step besides, 2^-25 half of it: of p, kept below its row's maximum times 2^8 at most
+(forward) or times 2^8 (backward), and of ds, kept times 2^14 / (4 D max|dout| max|v|) at least.  And fp32's normal numbers end at 2^-126: a p or ds
+below that may count as 0 (a score 90 standard deviations below its row's maximum has such a p, and its key, if no other row attends to it, a gradient
+of that size)."""
+import math
+
+import pytest
+import torch
+
+from nanotron_amd.nn import attention
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+W = 2.0 ** -24
+
+
+def exact_one(q, k, v, do, scale, causal, u, tiny):
+    """One head of one sequence, [rows, dim] in 64 bits: (out, dq, dk, dv) and what each may be off by before its own rounding."""
+    n, m, d = q.shape[0], k.shape[0], q.shape[1]
+    s = q @ k.t() * scale
+    seen = torch.ones(n, m, dtype=torch.bool, device=q.device)
+    if causal:
+        seen = torch.arange(m, device=q.device)[None] <= torch.arange(m - n, m, device=q.device)[:, None]
+    any_ = seen.any(-1, keepdim=True)
+    s = s.masked_fill(~seen, -math.inf)
+    p = torch.where(any_, torch.softmax(torch.where(any_, s, 0.0), -1), 0.0).masked_fill(~seen, 0.0)
+    qk = ((q.abs() @ k.abs().t()).masked_fill(~seen, 0.0).amax(-1, keepdim=True) if m else torch.zeros(n, 1, device=q.device, dtype=q.dtype)) * scale
+    e = 2 * (d + 4) * W * 1.45 * qk + (m + 64) * W
+    o = p @ v
+    low = 2.0 ** -126 * seen.double()
+    step = tiny * seen.double() + low   # of a numerator, beside the sum, which is 1 or more
+    eo = (u + e) * (p @ v.abs()) + step @ v.abs()
+    dv = p.t() @ do
+    edv = ((u + e) * p + tiny / 256 * seen.double() + low).t() @ do.abs()
+    dp = do @ v.t()
+    delta = (do * o).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    off = d * W * (do.abs() @ v.abs().t()) + (do.abs() * (eo + u * (o.abs() + eo) + d * W * o.abs())).sum(-1, keepdim=True)
+    lift = 2.0 ** 14 / (4 * d * max(1e-30, do.abs().max().item() if n else 0) * max(1e-30, v.abs().max().item() if m else 0))
+    eds = p * off + (u + 2 * e) * ds.abs() + tiny * seen.double() / lift + low * (1 + dp.abs() + delta.abs())
+    more = (max(n, m) + 8) * W
+    return (o, ds @ k * scale, ds.t() @ q * scale, dv), (eo, (eds + more * ds.abs()) @ k.abs() * scale, (eds + more * ds.abs()).t() @ q.abs() * scale, edv + more * p.t() @ do.abs())
+
+
+def exact(q, k, v, do, lengths, causal=True, scale=None):
+    """q [tokens, heads, dim] and the others; lengths: (queries, keys) of the sequences, end to end."""
+    u, tiny = U[q.dtype], 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    group = q.shape[1] // k.shape[1]
+    args = [t.double() for t in (q, k, v, do)]
+    want, bound = ([torch.zeros(t.shape, dtype=torch.float64, device=t.device) for t in (q, q, k, v)] for _ in range(2))
+    a = b = 0
+    for n, m in lengths:
+        if n and m:
+            for h in range(q.shape[1]):
+                j = h // group
+                r, x = exact_one(args[0][a:a + n, h], args[1][b:b + m, j], args[2][b:b + m, j], args[3][a:a + n, h], scale, causal, u, tiny)
+                for t, y in ((want, r), (bound, x)):
+                    t[0][a:a + n, h] += y[0]
+                    t[1][a:a + n, h] += y[1]
+                    t[2][b:b + m, j] += y[2]
+                    t[3][b:b + m, j] += y[3]
+        a, b = a + n, b + m
+    return want, bound
+
+
+def near(got, want, bound, name):
+    u = U[got.dtype]
+    tiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}[got.dtype]
+    assert torch.isfinite(got).all(), name
+    off = (got.double() - want).abs()
+    limit = bound + u * (want.abs() + bound) + tiny
+    worst = (off / limit.clamp_min(1e-300)).max().item() if off.numel() else 0.0
+    assert worst <= 1.0, f"{name}: {worst:.2f} times what it may be off"
+
+
+def inputs(tokens, heads, kv_heads, dim, dtype, keys=None, seed=0, gradient=0.1):
+    g = torch.Generator().manual_seed(seed)
+    keys = tokens if keys is None else keys
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(*shape, generator=g) * std).to(dtype).to(DEV)
+
+    return normal(tokens, heads, dim, std=1.5), normal(keys, kv_heads, dim), normal(keys, kv_heads, dim), normal(tokens, heads, dim, std=gradient)
+
+
+def offsets(lengths, which=0):
+    at = [0]
+    for x in lengths:
+        at.append(at[-1] + (x[which] if isinstance(x, tuple) else x))
+    return torch.tensor(at, dtype=torch.int32, device=DEV)
+
+
+def step(q, k, v, do, **kw):
+    q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+    out = attention(q, k, v, **kw)
+    return (out.detach(), *torch.autograd.grad(out, (q, k, v), do))
+
+
+def check(q, k, v, do, lengths, causal=True, scale=None, **kw):
+    got = step(q, k, v, do, causal=causal, scale=scale, **kw)
+    want, bound = exact(q, k, v, do, lengths, causal, scale)
+    for o, a, e, n in zip(got, want, bound, ("out", "dq", "dk", "dv")):
+        assert o.shape == a.shape and o.dtype == q.dtype and o.is_contiguous()
+        near(o, a, e, n)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128, 8, 72, 96, 104])
+@pytest.mark.parametrize("causal", [True, False])
+def test_one_sequence(dtype, dim, causal):
+    q, k, v, do = inputs(333, 4, 2, dim, dtype)
+    check(q, k, v, do, [(333, 333)], causal)
+
+
+@pytest.mark.parametrize("length", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257])
+def test_lengths(length):
+    q, k, v, do = inputs(length, 2, 1, 64, torch.bfloat16, seed=length)
+    check(q, k, v, do, [(length, length)])
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 8), (8, 2), (8, 1), (6, 3), (5, 1)])
+def test_heads(heads, kv_heads):
+    q, k, v, do = inputs(150, heads, kv_heads, 64, torch.bfloat16)
+    check(q, k, v, do, [(150, 150)])
+
+
+PACKED = [[1], [5, 7, 1, 0, 3], [0, 0, 200], [200, 0, 0], [64, 64, 64], [128, 1, 127, 130], [1] * 70, [300, 17, 1, 90]]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths", PACKED)
+def test_packed(lengths, causal):
+    n = sum(lengths)
+    q, k, v, do = inputs(n, 4, 2, 128, torch.bfloat16, seed=n)
+    check(q, k, v, do, [(x, x) for x in lengths], causal, cu_seqlens=offsets(lengths))
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths", [[(3, 70), (1, 1), (40, 40)], [(70, 3), (5, 200), (0, 9), (9, 0), (130, 129)], [(1, 300)], [(300, 1)], [(0, 4), (4, 0)]])
+def test_more_or_fewer_keys(lengths, causal):
+    """Causal rows in front of the first key see nothing: 0, and no gradient."""
+    n, m = (sum(x[i] for x in lengths) for i in range(2))
+    q, k, v, do = inputs(n, 4, 2, 64, torch.bfloat16, keys=m, seed=m)
+    got = check(q, k, v, do, lengths, causal, cu_seqlens=offsets(lengths), cu_seqlens_k=offsets(lengths, 1))
+    a = 0
+    for x, y in lengths:
+        if causal and x > y:
+            assert not got[0][a:a + x - y].any() and not got[1][a:a + x - y].any()
+        a += x
+
+
+@pytest.mark.parametrize("tokens,keys", [(1, 1), (1, 7), (1, 300), (1, 5000), (3, 1000), (8, 8), (8, 33), (9, 1), (17, 900), (100, 3000), (65, 64)])
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 80)])
+def test_batches(tokens, keys, dtype, dim):
+    """A batch of equal lengths, fewer or more rows than one tile, keys the first part of a cache."""
+    b, heads, kv = 3, 8, 2
+    g = torch.Generator().manual_seed(tokens + keys)
+    q = (1.5 * torch.randn(b, tokens, heads, dim, generator=g)).to(dtype).to(DEV)
+    k, v = ((torch.randn(b, keys + 5, kv, dim, generator=g)).to(dtype).to(DEV)[:, :keys] for _ in range(2))
+    do = torch.randn(b, tokens, heads, dim, generator=g).mul_(0.1).to(dtype).to(DEV)
+    got = step(q, k, v, do)
+    flat = [t.reshape(-1, *t.shape[2:]) for t in (q, k, v, do)]
+    want, bound = exact(*flat, [(tokens, keys)] * b)
+    for o, a, e, n in zip(got, want, bound, ("out", "dq", "dk", "dv")):
+        near(o.flatten(0, 1), a, e, n)
+    with torch.no_grad():
+        assert torch.equal(attention(q, k, v), got[0])
+
+
+def test_many_sequences_of_a_batch():
+    q = torch.randn(200, 1, 4, 64, device=DEV).bfloat16()
+    k, v = (torch.randn(200, 40, 1, 64, device=DEV).bfloat16() for _ in range(2))
+    want, bound = exact(*(t.flatten(0, 1) for t in (q, k, v, q)), [(1, 40)] * 200)
+    with torch.no_grad():
+        near(attention(q, k, v).flatten(0, 1), want[0], bound[0], "out")
+
+
+def test_long_rows():
+    q, k, v, do = inputs(3000, 2, 1, 128, torch.bfloat16)
+    check(q, k, v, do, [(3000, 3000)])
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.01, 7.5])
+def test_scales(scale):
+    q, k, v, do = inputs(200, 2, 2, 64, torch.bfloat16)
+    check(q, k, v, do, [(200, 200)], scale=scale)
+
+
+def test_large_scores():
+    """Scores of hundreds: the softmax is a choice of one key, and nothing overflows."""
+    q, k, v, do = inputs(300, 2, 1, 128, torch.bfloat16)
+    check(q * 16, k * 4, v, do, [(300, 300)])
+    # in rising order, so that the running maximum is raised again and again
+    order = (q[:, 0].float() @ k[:, 0].float().t()).sum(0).argsort()
+    check(q * 16, k[order].contiguous(), v[order].contiguous(), do, [(300, 300)], causal=False)
+
+
+@pytest.mark.parametrize("gradient", [1e-6, 1e-3, 100.0])
+def test_small_and_large_gradients_of_fp16(gradient):
+    q, k, v, do = inputs(700, 2, 1, 64, torch.float16, gradient=gradient)
+    check(q, k, v, do, [(700, 700)])
+
+
+def test_strided_views():
+    """Parts of one linear's output, heads in front of tokens, rows that repeat."""
+    qkv = torch.randn(260, 12, 64, device=DEV).bfloat16()
+    do = torch.randn(260, 8, 64, device=DEV).bfloat16()
+    parts = qkv[:, :8], qkv[:, 8:10], qkv[:, 10:]
+    check(*parts, do, [(260, 260)])
+    dense = [t.contiguous() for t in parts]
+    turned = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in dense]
+    for a, b in zip(step(*dense, do), step(*turned, do.transpose(0, 1).contiguous().transpose(0, 1))):
+        assert torch.equal(a, b)
+    # off 16-byte boundaries, an odd distance apart: copied
+    odd = [torch.nn.functional.pad(t, (1, 2))[..., 1:-2] for t in dense]
+    assert all(t.stride(1) == 67 for t in odd)
+    for a, b in zip(step(*dense, do), step(*odd, do)):
+        assert torch.equal(a, b)
+    one = dense[1][:1].expand(260, 2, 64)
+    check(dense[0], one, one, do, [(260, 260)])
+
+
+def test_gradient_that_is_broadcast():
+    q, k, v, _ = inputs(130, 4, 2, 64, torch.bfloat16)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    a = torch.autograd.grad(attention(*leaves).sum(), leaves)
+    b = torch.autograd.grad(attention(*leaves), leaves, torch.ones_like(q))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    attention(*leaves).float().square().sum().backward()
+    assert all(t.grad is not None and torch.isfinite(t.grad).all() for t in leaves)
+
+
+@pytest.mark.parametrize("leaf", [0, 1, 2])
+def test_one_gradient_at_a_time(leaf):
+    q, k, v, do = inputs(140, 4, 2, 64, torch.bfloat16)
+    every = step(q, k, v, do)
+    t = (q, k, v)[leaf].requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(attention(q, k, v), t, do)[0], every[leaf + 1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_what_is_not_seen_does_not_arrive(dtype, bad):
+    """NaN and infinities in rows of no sequence, in the sequence behind, and in tokens to come."""
+    lengths, pad = [100, 90, 60], 40
+    n = sum(lengths)
+    q, k, v, do = inputs(n, 4, 2, 64, dtype, seed=3)
+    clean = step(q, k, v, do, cu_seqlens=offsets(lengths))
+    spoilt = [torch.cat([t, torch.full((pad, *t.shape[1:]), bad, dtype=dtype, device=DEV)]) for t in (q, k, v, do)]
+    got = step(*spoilt, cu_seqlens=offsets(lengths))
+    for a, b, name in zip(got, clean, ("out", "dq", "dk", "dv")):
+        assert torch.equal(a[:n], b), name
+        assert not a[n:].any(), name
+    # sequence 1 spoilt: 0 and 2 are as they were
+    for which in range(4):
+        args = [t.clone() for t in (q, k, v, do)]
+        args[which][100:190] = bad
+        for a, b in zip(step(*args, cu_seqlens=offsets(lengths)), clean):
+            assert torch.equal(a[:100], b[:100]) and torch.equal(a[190:], b[190:])
+    # a token to come: rows in front of it are as they were, forward
+    for at in (99, 50, 33, 64):
+        for which in (1, 2):
+            args = [t.clone() for t in (q, k, v)]
+            args[which][at] = bad
+            with torch.no_grad():
+                out = attention(*args, cu_seqlens=offsets(lengths))
+            assert torch.isfinite(out[:at]).all()
+            near(out[:at], clean[0][:at].double(), (clean[0][:at].double().abs() + 1e-3) * 4 * U[dtype], "rows in front")
+            assert not torch.isfinite(out[at]).any() or which == 1
+            assert torch.equal(out[100:], clean[0][100:])
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 3])
+def test_gradients_beside_a_bad_row(which):
+    """A row that is not finite spoils the gradients that the formula says, in its tile too, and no others: keys behind a bad query see nothing of it,
+    nor do queries in front of a bad key."""
+    n, at = 64, 20
+    q, k, v, do = inputs(n, 1, 1, 64, torch.bfloat16, seed=4)
+    clean = step(q, k, v, do)
+    args = [t.clone() for t in (q, k, v, do)]
+    args[which][at] = math.nan
+    got = step(*args)
+    if which in (0, 3):   # a query: its own dq, and dk and dv of the keys that it sees
+        assert torch.isfinite(got[1][:at]).all() and torch.isfinite(got[1][at + 1:]).all()
+        for g, c in zip(got[2:], clean[2:]):
+            assert torch.isfinite(g[at + 1:]).all()
+            near(g[at + 1:], c[at + 1:].double(), (c[at + 1:].double().abs() + 1e-3) * 4 * U[g.dtype], "keys behind")
+    else:                 # a key: dq of the queries that see it
+        assert torch.isfinite(got[1][:at]).all()
+        near(got[1][:at], clean[1][:at].double(), (clean[1][:at].double().abs() + 1e-3) * 4 * U[q.dtype], "queries in front")
+
+
+def test_offsets_that_are_wrong_stay_inside():
+    """Offsets behind the rows that there are, or below zero, count as the nearest inside; rows of no sequence are zeros."""
+    q, k, v, do = inputs(100, 2, 1, 64, torch.bfloat16)
+    cu = torch.tensor([-5, 40, 1000], dtype=torch.int32, device=DEV)
+    for a, b in zip(step(q, k, v, do, cu_seqlens=cu), step(q, k, v, do, cu_seqlens=offsets([40, 60]))):
+        assert torch.equal(a, b)
+    cu = torch.tensor([30, 60, 80], dtype=torch.int32, device=DEV)
+    got = step(q, k, v, do, cu_seqlens=cu)
+    inner = step(*(t[30:80].contiguous() for t in (q, k, v, do)), cu_seqlens=offsets([30, 20]))
+    for a, b in zip(got, inner):
+        assert not a[:30].any() and not a[80:].any() and torch.equal(a[30:80], b)
+
+
+def test_nothing_to_do():
+    q, k, v, do = inputs(0, 4, 2, 64, torch.bfloat16, keys=5)
+    got = step(q, k, v, do)
+    assert got[0].shape == (0, 4, 64) and not got[2].any() and not got[3].any()
+    q, k, v, do = inputs(6, 4, 2, 64, torch.bfloat16, keys=0)
+    got = step(q, k, v, do)
+    assert not got[0].any() and not got[1].any() and got[2].shape == (0, 2, 64)
+    e = torch.zeros(0, 3, 4, 64, device=DEV, dtype=torch.bfloat16)
+    assert attention(e, e, e).shape == e.shape
+
+
+def test_same_bits_again():
+    q, k, v, do = inputs(900, 8, 2, 128, torch.bfloat16)
+    cu = offsets([400, 37, 463])
+    first = step(q, k, v, do, cu_seqlens=cu)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, step(q, k, v, do, cu_seqlens=cu)))
+
+
+def test_gradient_against_differences():
+    """The forward pass in 64 bits, differenced: an independent statement of the gradients, which the kernels' then meet within 16-bit rounding."""
+    q, k, v, do = inputs(9, 2, 1, 16, torch.float16)
+    got = step(q, k, v, do)[1:]
+    full = [t.double() for t in (q, k, v)]
+
+    def value(q, k, v):
+        x = torch.einsum("ihd,jd->hij", q.cpu(), k[:, 0].cpu()) / 4.0
+        x = x.masked_fill(torch.ones(9, 9).triu(1).bool(), -math.inf)
+        return (torch.einsum("hij,jd->ihd", torch.softmax(x, -1), v[:, 0].cpu()) * do.double().cpu()).sum().item()
+
+    h = 1e-5
+    for i, g in enumerate(got):
+        flat = full[i].view(-1)
+        for at in range(0, flat.numel(), 7):
+            keep = flat[at].item()
+            flat[at] = keep + h
+            up = value(*full)
+            flat[at] = keep - h
+            down = value(*full)
+            flat[at] = keep
+            assert abs((up - down) / (2 * h) - g.view(-1)[at].item()) < 4e-3 * g.abs().max().item() + 1e-6
+
+
+def test_graph_replays():
+    """Captured forward and backward, replayed with other inputs and eager calls between."""
+    q, k, v, do = inputs(500, 4, 2, 64, torch.float16)
+    cu = offsets([200, 300])
+    static = [t.clone() for t in (q, k, v, do)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static, cu_seqlens=cu)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*static, cu_seqlens=cu)
+    for seed, lengths in ((5, [200, 300]), (6, [499, 1]), (7, [0, 500])):
+        fresh = inputs(500, 4, 2, 64, torch.float16, seed=seed)
+        for a, b in zip(static, fresh):
+            a.copy_(b)
+        cu.copy_(offsets(lengths))   # other lengths too: the device reads them
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(*fresh, cu_seqlens=offsets(lengths))
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), seed
+
+
+def test_two_graphs_of_one_token_over_a_cache():
+    q = torch.randn(2, 1, 8, 128, device=DEV).bfloat16()
+    cache = torch.randn(2, 4096, 2, 128, device=DEV).bfloat16()
+    with torch.no_grad():
+        graphs, outs = [], []
+        for n in (4000, 1500):
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                attention(q, cache[:, :n], cache[:, :n])
+            torch.cuda.current_stream().wait_stream(side)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(attention(q, cache[:, :n], cache[:, :n]))
+            graphs.append(g)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for _ in range(3):
+            torch.cuda.synchronize()
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+            torch.cuda.synchronize()
+            for n, o in zip((4000, 1500), outs):
+                assert torch.equal(o, attention(q, cache[:, :n], cache[:, :n]))
+            q.normal_()
+
+
+def test_another_stream():
+    q, k, v, do = inputs(400, 4, 2, 64, torch.bfloat16)
+    want = step(q, k, v, do)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step(q, k, v, do)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals():
+    q, k, v, do = inputs(10, 4, 2, 64, torch.bfloat16)
+    cu = offsets([4, 6])
+    for e, args, kw in (
+            (TypeError, (q.float(), k.float(), v.float()), {}), (TypeError, (q, k.half(), v), {}), (ValueError, (q, k, v[:5]), {}),
+            (ValueError, (q[:, :3], k, v), {}), (ValueError, (q[..., :60], k[..., :60], v[..., :60]), {}), (ValueError, (q[0], k[0], v[0]), {}),
+            (ValueError, (q, k, v), dict(scale=0.0)), (ValueError, (q, k, v), dict(scale=-1.0)), (TypeError, (q, k, v), dict(cu_seqlens=cu.long())),
+            (ValueError, (q, k, v), dict(cu_seqlens=cu[:1])), (ValueError, (q, k, v), dict(cu_seqlens_k=cu)), (ValueError, (q, k, v), dict(cu_seqlens=cu.cpu())),
+            (ValueError, (q, k, v), dict(cu_seqlens=cu, cu_seqlens_k=offsets([10]))), (ValueError, (q[:5], k, v), dict(cu_seqlens=cu)),
+            (ValueError, (q[None], k[None], v[None]), dict(cu_seqlens=cu)), (ValueError, (torch.zeros(2, 2, 136, device=DEV, dtype=torch.bfloat16),) * 3, {}),
+            (ValueError, (q[:, :0], k, v), {}), (ValueError, (q.cpu(), k, v), {})):
+        with pytest.raises(e):
+            attention(*args, **kw)
+    leaf = q.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(attention(leaf, k, v).sum(), leaf, create_graph=True)
