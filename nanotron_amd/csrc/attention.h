@@ -17,6 +17,8 @@ typedef int v2i_attn __attribute__((ext_vector_type(2)));
 
 constexpr int kAttnStep = 64;               // rows of a tile in LDS
 constexpr int kAttnWaves = 4;
+constexpr int kAttnKeyWaves = 8;            // of the kernel that owns keys, and its keys
+constexpr int kAttnKeys = 32 * kAttnKeyWaves;
 constexpr uint32_t kNowhere = 0xfffffff0u;  // past every descriptor: reads as zeros
 constexpr float kLog2E = 1.44269504088896340736f;
 
@@ -87,13 +89,15 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 // rows' 64 bytes meet in a bank
 template <int DP>
 struct AttnTile {
-    static constexpr int kPitch = DP <= 64 ? 128 : 256, kBytes = kAttnStep * kPitch, kLoads = kBytes / 1024 / kAttnWaves;
+    static constexpr int kPitch = DP <= 64 ? 128 : 256, kBytes = kAttnStep * kPitch;
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (kPitch == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
         else return (row & 3) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
     }
-    // loads: 1 KB a wave each, straight into LDS
+    // loads: 1 KB a wave each, straight into LDS, by kWaves waves
+    template <int kWaves = kAttnWaves>
     struct Source {
+        static constexpr int kLoads = kBytes / 1024 / kWaves;
         const char* base;
         int64_t row_bytes;
         uint32_t off[kLoads];
@@ -104,7 +108,7 @@ struct AttnTile {
             dim = dim_;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int byte = ((i * kAttnWaves + wave) * 64 + lane) * 16, row = byte / kPitch, chunk = (byte % kPitch >> 4) ^ swizzle(row);
+                const int byte = ((i * kWaves + wave) * 64 + lane) * 16, row = byte / kPitch, chunk = (byte % kPitch >> 4) ^ swizzle(row);
                 off[i] = chunk * 8 < dim ? (uint32_t)row * (uint32_t)row_bytes + chunk * 16 : kNowhere;
             }
         }
@@ -114,7 +118,7 @@ struct AttnTile {
             const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)row_bytes + 2u * dim : 0u;
             const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (int64_t)first * row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) lds_load16(r, (lds_ptr)(uintptr_t)(stage + (i * kAttnWaves + wave) * 1024), off[i], 0);
+            for (int i = 0; i < kLoads; ++i) lds_load16(r, (lds_ptr)(uintptr_t)(stage + (i * kWaves + wave) * 1024), off[i], 0);
         }
     };
     // fragments: 32 rows by 16 elements as they lie, and 16 rows by 32 elements transposed
@@ -137,6 +141,24 @@ struct AttnTile {
         const int lo = across + ((e << 6) ^ across_turn) + s * 16 * kPitch, hi = (across + ((e << 6) ^ across_turn ^ 16)) + (s * 16 + 8) * kPitch;
         const v2i_attn a = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[lo]));
         const v2i_attn b = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[hi]));
+        return (v4i){a.x, a.y, b.x, b.y};
+    }
+    // The same of the stage that begins at byte `at` of an array, for kernels without registers to keep each fragment's address in: one
+    // exclusive or a read, which the compiler is kept from doing once and for all
+    __device__ __forceinline__ v4i rows_anew(const uint8_t* array, int at, int b, int k) const {
+        int off = (at + plain + plain_turn) ^ (k << 5);
+        asm volatile("" : "+v"(off));
+        return *reinterpret_cast<const v4i*>(array + off + b * 32 * kPitch);
+    }
+    __device__ __forceinline__ v4i columns_anew(uint8_t* array, int at, int s, int e) const {
+        typedef short v4s __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) v4s* tr_ptr;
+        int lo = (at + across + across_turn) ^ (e << 6);
+        asm volatile("" : "+v"(lo));
+        int hi = lo ^ 16;
+        asm volatile("" : "+v"(hi));
+        const v2i_attn a = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&array[lo + s * 16 * kPitch]));
+        const v2i_attn b = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&array[hi + (s * 16 + 8) * kPitch]));
         return (v4i){a.x, a.y, b.x, b.y};
     }
 };
@@ -182,21 +204,21 @@ __device__ __forceinline__ void add_columns(v16f (&acc)[DP / 32], const AttnTile
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) acc[e] = mfma_attn<T>(tile.columns(stage, s, e), scores, acc[e]);
 }
-// The same over the 16 kScores rows of a stage that holds values which are not finite, under a mask: a score of zero times such a value would
+// The same over 16 kScores rows, from 16 s0 on, of a stage that holds values which are not finite, under a mask: a score of zero times such a value would
 // reach the rows that do not count it (a padded row, a token to come), so the stage's rows go one at a time, and only into the
 // rows that count them: `counts(i)`, this lane's row counts row i.
 template <int T, int DP, int kScores, typename F>
-__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const AttnTile<DP>& tile, uint8_t* stage, const v4i (&scores)[kScores], F&& counts, int lane) {
+__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const AttnTile<DP>& tile, uint8_t* stage, int s0, const v4i (&scores)[kScores], F&& counts, int lane) {
 #pragma unroll 1
     for (int i = 0; i < 16 * kScores; ++i) {
         const int s = i >> 4, j = (i & 3) + ((i >> 3) & 1) * 4;   // its place in the fragments of half wave (i >> 2) & 1
-        const bool mine = (lane >> 5) == ((i >> 2) & 1), take = counts(i);
+        const bool mine = (lane >> 5) == ((i >> 2) & 1), take = counts(16 * s0 + i);
         v4i c = {0, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < kScores; ++k) c |= scores[k] & (s == k ? -1 : 0);   // (a choice of one of them would put them all into memory)
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) {
-            v4i f = tile.columns(stage, s, e);
+            v4i f = tile.columns(stage, s0 + s, e);
 #pragma unroll
             for (int w = 0; w < 4; ++w) f[w] = mine && (j >> 1) == w ? (j & 1 ? f[w] & (int)0xffff0000 : f[w] & 0xffff) : 0;
             const v16f d = mfma_attn<T>(f, c, zeros16());

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
     }
     Tile tile;
     tile.init(lane);
-    typename Tile::Source ks, vs;
+    typename Tile::template Source<> ks, vs;
     ks.init(A.k, k0, A.k_stride, A.dim, wave, lane);
     vs.init(A.v, v0, A.v_stride, A.dim, wave, lane);
     if (steps > 0) {
@@ -136,7 +136,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
 #pragma unroll
         for (int e = 0; e < DP / 32; ++e) out[b][e] = zeros16();
     }
-    for (int j = 0; j < steps; ++j) {
+    // One tile of keys.  kMasked: some rows of the workgroup may not see all of them
+    auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked_)::value;
         const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         wg_barrier();
@@ -145,7 +147,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
             vs.load(sv + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
         }
         const int lead = task.shift + wave * 32 * QB;   // the last key that the wave's first row sees
-        if (A.causal && key0 > lead + 32 * QB - 1) continue;   // (uniform in the wave; barriers are met at the loop's head)
+        if (kMasked && A.causal && key0 > lead + 32 * QB - 1) return;   // (uniform in the wave)
         v16f s[QB][2];
 #pragma unroll
         for (int b = 0; b < QB; ++b) s[b][0] = s[b][1] = zeros16();
@@ -158,11 +160,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
                 s[b][1] = mfma_attn<T>(f1, q[b][k], s[b][1]);
             }
         }
-        const bool masked = key0 + kAttnStep > task.len || (A.causal && key0 + kAttnStep - 1 > lead);
-        if (masked) {
+        auto last_of = [&](int b) { return (A.causal ? min(task.len - 1, lead + 32 * b + (lane & 31)) : task.len - 1) - key0; };   // the last key of the tile that a row sees
+        if constexpr (kMasked) {
 #pragma unroll
             for (int b = 0; b < QB; ++b) {
-                const int last = (A.causal ? min(task.len - 1, lead + 32 * b + (lane & 31)) : task.len - 1) - key0;
+                const int last = last_of(b);
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
 #pragma unroll
@@ -201,13 +203,15 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
                 p[b][2 * g + 1] = pack_scores<T>(s[b][g], 8);
             }
         }
-        if (masked && attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
+        if constexpr (kMasked) {
+            if (attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
 #pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                const int last = (A.causal ? min(task.len - 1, lead + 32 * b + (lane & 31)) : task.len - 1) - key0;
-                add_columns_singly<T, DP, 4>(out[b], tile, sv + stage, p[b], [&](int i) { return i <= last; }, lane);
+                for (int b = 0; b < QB; ++b) {
+                    const int last = last_of(b);
+                    add_columns_singly<T, DP, 4>(out[b], tile, sv + stage, 0, p[b], [&](int i) { return i <= last; }, lane);
+                }
+                return;
             }
-            continue;
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -217,7 +221,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
 #pragma unroll
                 for (int b = 0; b < QB; ++b) out[b][e] = mfma_attn<T>(f, p[b][g], out[b][e]);
             }
-    }
+    };
+    // tiles that every row sees whole, then the others
+    const int whole = min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, clear = max(0, min(whole - first, steps));
+    int j = 0;
+    for (; j < clear; ++j) step(j, std::false_type{});
+    for (; j < steps; ++j) step(j, std::true_type{});
 #pragma unroll
     for (int b = 0; b < QB; ++b) {
         const int row = row0 + 32 * b;
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         }
         const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)};
         if (masked && attn_not_finite<T, DP>(v, kFewStep, lane)) {
-            add_columns_singly<T, DP, 2>(out, tile, v, p, [&](int i) { return i <= last; }, lane);
+            add_columns_singly<T, DP, 2>(out, tile, v, 0, p, [&](int i) { return i <= last; }, lane);
         } else {
             add_columns<T, DP>(out, tile, v, 0, p[0]);
             add_columns<T, DP>(out, tile, v, 1, p[1]);

@@ -53,8 +53,10 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
     for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
     if (!values && row < rows && d == 0) A.delta[head * A.q_rows + row] = live ? sum : 0.0f;
     if constexpr (T == NTFP8_F16) {
+        // (a maximum: the order changes nothing; and few find themselves above what is there already)
         most = wave_most(most);
-        if ((threadIdx.x & 63) == 0 && most) atomicMax(&A.most[values], most);   // (a maximum: the order changes nothing)
+        uint32_t* const at = &A.most[values];
+        if ((threadIdx.x & 63) == 0 && most > __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(at, most);
     }
 }
 
@@ -74,7 +76,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
     const int end = A.causal ? min(max(task.shift + task.rows, 0), task.len) : task.len, steps = (end + kAttnStep - 1) / kAttnStep;
     Tile tile;
     tile.init(lane);
-    typename Tile::Source ks, vs;
+    typename Tile::template Source<> ks, vs;
     ks.init(A.k, k0, A.k_stride, A.dim, wave, lane);
     vs.init(A.v, v0, A.v_stride, A.dim, wave, lane);
     if (steps > 0) {
@@ -92,7 +94,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
     v16f dq[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) dq[e] = zeros16();
-    for (int j = 0; j < steps; ++j) {
+    // One tile of keys.  kMasked: some rows of the workgroup may not see all of them
+    auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked_)::value;
         const int key0 = j * kAttnStep, stage = (j & 1) * Tile::kBytes;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         wg_barrier();
@@ -100,9 +104,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
             ks.load(sk + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
             vs.load(sv + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
         }
-        const int lead = task.shift + wave * 32;
-        if (A.causal && key0 > lead + 31) continue;
-        const bool masked = key0 + kAttnStep > task.len || (A.causal && key0 + kAttnStep - 1 > lead);
+        const int lead = task.shift + wave * 32;   // the last key that the wave's first row sees
+        if (kMasked && A.causal && key0 > lead + 31) return;   // (uniform in the wave)
         const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0;
         v4i p[4];
 #pragma unroll
@@ -115,44 +118,57 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, -lse)) * ((d[r] - delta) * lift);
-            if (masked) {
+            if constexpr (kMasked) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 32 * b + place_of(r, lane) > last ? 0.0f : s[r];
             }
             p[2 * b] = pack_scores<T>(s, 0);
             p[2 * b + 1] = pack_scores<T>(s, 8);
         }
-        if (masked && attn_not_finite<T, DP>(sk + stage, kAttnStep, lane)) {
-            add_columns_singly<T, DP, 4>(dq, tile, sk + stage, p, [&](int i) { return i <= last; }, lane);
-            continue;
+        if constexpr (kMasked) {
+            if (attn_not_finite<T, DP>(sk + stage, kAttnStep, lane)) {
+                add_columns_singly<T, DP, 4>(dq, tile, sk + stage, 0, p, [&](int i) { return i <= last; }, lane);
+                return;
+            }
         }
 #pragma unroll
         for (int s = 0; s < 4; ++s) add_columns<T, DP>(dq, tile, sk + stage, s, p[s]);
-    }
+    };
+    // tiles that every row sees whole, then the others
+    const int clear = max(0, min(min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, steps));
+    int j = 0;
+    for (; j < clear; ++j) step(j, std::false_type{});
+    for (; j < steps; ++j) step(j, std::true_type{});
     store_rows<T, DP>(dq, A.scale / lift, A.dq, (at * A.heads + head) * A.dim, A.dim, live, lane);
 }
 
-// dk and dv of 128 keys of one head of keys, 32 a wave: over the heads of queries that share it, and their queries 64 at a time
+// dk and dv of 256 keys of one head of keys, 32 a wave: over the heads of queries that share it, and their queries 64 at a time.  A wave holds
+// its keys and both sums in registers, 160 of the 256 that two waves a SIMD have; its values stay in LDS.
 template <int T, int DP>
-__global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_dkv_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(const AttnArgs A) {
     typedef AttnTile<DP> Tile;
     __shared__ __attribute__((aligned(1024))) uint8_t sq[2 * Tile::kBytes];
     __shared__ __attribute__((aligned(1024))) uint8_t sg[2 * Tile::kBytes];
+    __shared__ __attribute__((aligned(1024))) uint8_t sv[kAttnKeyWaves / 2 * Tile::kBytes];
     __shared__ __attribute__((aligned(1024))) float rows_of[2][2][kAttnStep];   // lse and delta
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = blockIdx.x / A.kv_heads, kv = blockIdx.x - t * A.kv_heads;
-    const AttnTask task = attn_task(A, t, 128, true);
+    const AttnTask task = attn_task(A, t, kAttnKeys, true);
     if (task.rows <= 0) return;
     const int begin = A.causal ? max(0, task.shift) / kAttnStep : 0, per = max(0, (task.len + kAttnStep - 1) / kAttnStep - begin), steps = per * A.group;
     Tile tile;
     tile.init(lane);
-    typename Tile::Source qs, gs;
+    typename Tile::template Source<kAttnKeyWaves> qs, gs, vs;
     qs.init(A.q, attn_rows(A, task.other, task.seq, 0, A.q_stride, A.q_batch) + (int64_t)kv * A.group * A.q_head, A.q_stride, A.dim, wave, lane);
     gs.init(A.dout, attn_rows(A, task.other, task.seq, 0, A.do_stride, A.do_batch) + (int64_t)kv * A.group * A.do_head, A.do_stride, A.dim, wave, lane);
     const float* stats = (wave == 0 ? A.lse : A.delta) + kv * A.group * A.q_rows + task.other;
     const char *const q_base = qs.base, *const g_base = gs.base;
+    // Tiles of a head's queries: first those whose rows all see all keys of the workgroup, then the ones in front of and behind these
+    const int front = A.causal ? min(max(0, (task.shift + task.rows - 1 + kAttnStep - 1) / kAttnStep - begin), per) : 0;
+    const int whole = max(0, min(task.len / kAttnStep - begin, per) - front);
+    auto row_of = [&](int i) { return (begin + (i < whole ? front + i : i < whole + front ? i - whole : i)) * kAttnStep; };
     auto load = [&](int j, int stage) {
-        const int head = j / per, first = (begin + j - head * per) * kAttnStep;
+        const int head = j / per, first = row_of(j - head * per);
         qs.base = q_base + 2 * (head * A.q_head);
         gs.base = g_base + 2 * (head * A.do_head);
         qs.load(sq + stage * Tile::kBytes, first, task.len, wave);
@@ -162,35 +178,43 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_dkv_kernel(const
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(uintptr_t)&rows_of[stage][wave][0], 4, lane * 4, 0, 0, 0);
         }
     };
-    if (steps > 0) load(0, 0);
+    vs.init(A.v, attn_rows(A, task.own, task.seq, task.at, A.v_stride, A.v_batch) + kv * A.v_head, A.v_stride, A.dim, wave, lane);
+    if (steps > 0) {
+#pragma unroll
+        for (int i = 0; i < kAttnKeyWaves / 2; ++i) vs.load(sv + i * Tile::kBytes, i * kAttnStep, task.rows, wave);
+        load(0, 0);
+    }
+    const int mine = wave * 32 * Tile::kPitch;
     const int row = wave * 32 + (lane & 31);
     const bool live = row < task.rows;
-    v4i k[DP / 16], v[DP / 16];
+    v4i k[DP / 16];
     load_own<DP>(k, A.k, attn_rows(A, task.own, task.seq, task.at, A.k_stride, A.k_batch) + kv * A.k_head + row * A.k_stride, A.dim, live, lane);
-    load_own<DP>(v, A.v, attn_rows(A, task.own, task.seq, task.at, A.v_stride, A.v_batch) + kv * A.v_head + row * A.v_stride, A.dim, live, lane);
     constexpr float kUp = T == NTFP8_F16 ? kLiftP : 0.0f, kDown = T == NTFP8_F16 ? 1.0f / 256.0f : 1.0f;
     const float lift = gradient_lift<T>(A), down = lift * kDown;
     v16f dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) dk[e] = dv[e] = zeros16();
-    for (int j = 0; j < steps; ++j) {
-        const int stage = j & 1, row0 = (begin + j % per) * kAttnStep;
+    // One tile of queries of one head.  kMasked: some of its rows may not see all the workgroup's keys
+    auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
+        constexpr bool kMasked = decltype(masked_)::value;
+        const int row0 = row_of(j % per), stage = j & 1, at = stage * Tile::kBytes;
         uint8_t *const qa = sq + stage * Tile::kBytes, *const ga = sg + stage * Tile::kBytes;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         wg_barrier();
         if (j + 1 < steps) load(j + 1, stage ^ 1);
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
-        if (A.causal && row0 + kAttnStep - 1 < lead) continue;
-        const bool masked = row0 + kAttnStep > task.len || (A.causal && row0 < lead + 31);
+        if (kMasked && A.causal && row0 + kAttnStep - 1 < lead) return;
         const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
-        v4i p[4], ds[4];
+        bool singly = false;
+        if constexpr (kMasked) singly = attn_not_finite<T, DP>(ga, kAttnStep, lane) || attn_not_finite<T, DP>(qa, kAttnStep, lane);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
+            __builtin_amdgcn_sched_barrier(0);
             v16f s = zeros16(), d = zeros16();
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                s = mfma_attn<T>(tile.rows(qa, b, i), k[i], s);
-                d = mfma_attn<T>(tile.rows(ga, b, i), v[i], d);
+                s = mfma_attn<T>(tile.rows_anew(sq, at, b, i), k[i], s);
+                d = mfma_attn<T>(tile.rows_anew(sg, at, b, i), tile.rows_anew(sv, mine, 0, i), d);
             }
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
@@ -203,7 +227,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_dkv_kernel(const
                     d[r] = s[r] * ((d[r] - delta[i]) * down);
                 }
             }
-            if (masked) {
+            if constexpr (kMasked) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int i = 32 * b + place_of(r, lane);
@@ -212,22 +236,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_dkv_kernel(const
                     d[r] = in ? d[r] : 0.0f;
                 }
             }
-            p[2 * b] = pack_scores<T>(s, 0);
-            p[2 * b + 1] = pack_scores<T>(s, 8);
-            ds[2 * b] = pack_scores<T>(d, 0);
-            ds[2 * b + 1] = pack_scores<T>(d, 8);
-        }
-        const auto counts = [&](int i) { return i >= from && i < to; };
-        if (masked && (attn_not_finite<T, DP>(ga, kAttnStep, lane) || attn_not_finite<T, DP>(qa, kAttnStep, lane))) {
-            add_columns_singly<T, DP, 4>(dv, tile, ga, p, counts, lane);
-            add_columns_singly<T, DP, 4>(dk, tile, qa, ds, counts, lane);
-            continue;
-        }
+            __builtin_amdgcn_sched_barrier(0);
+            const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)}, ds[2] = {pack_scores<T>(d, 0), pack_scores<T>(d, 8)};
+            if constexpr (kMasked) {
+                if (singly) {
+                    const auto counts = [&](int i) { return i >= from && i < to; };
+                    add_columns_singly<T, DP, 2>(dv, tile, ga, 2 * b, p, counts, lane);
+                    add_columns_singly<T, DP, 2>(dk, tile, qa, 2 * b, ds, counts, lane);
+                    continue;
+                }
+            }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            add_columns<T, DP>(dv, tile, ga, s, p[s]);
-            add_columns<T, DP>(dk, tile, qa, s, ds[s]);
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < DP / 32; ++e) {
+                    dv[e] = mfma_attn<T>(tile.columns_anew(sg, at, 2 * b + h, e), p[h], dv[e]);
+                    dk[e] = mfma_attn<T>(tile.columns_anew(sq, at, 2 * b + h, e), ds[h], dk[e]);
+                }
         }
+    };
+    for (int j = 0; j < steps;) {
+        const int head_end = j + per;
+        for (const int end = j + whole; j < end; ++j) step(j, std::false_type{});
+        for (; j < head_end; ++j) step(j, std::true_type{});
     }
     const int64_t to = (((int64_t)task.own + row) * A.kv_heads + kv) * A.dim;
     if (A.dv) store_rows<T, DP>(dv, kDown, A.dv, to, A.dim, live, lane);
@@ -249,7 +280,7 @@ int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, i
         if (A.dk || A.dv) {
             AttnArgs K = A;
             K.tasks = k_tasks;
-            attention_dkv_kernel<T, DP><<<(unsigned)(k_tiles * A.kv_heads), 64 * kAttnWaves, 0, st>>>(K);
+            attention_dkv_kernel<T, DP><<<(unsigned)(k_tiles * A.kv_heads), 64 * kAttnKeyWaves, 0, st>>>(K);
             if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
         }
         if (A.dq) {

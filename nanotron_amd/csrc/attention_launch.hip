@@ -82,12 +82,12 @@ AttnArgs args_of(const ntops_attention_desc& d) {
 // What a launch has to hold: workgroups, and threads, in 32 bits
 bool attention_fits(const ntops_attention_desc& d) {
     constexpr int64_t kMost = (int64_t)1 << 23;
-    return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, 128) * d.heads <= kMost && tiles_of(d, d.k_rows, 128) * d.kv_heads <= kMost;
+    return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, 128) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
 }
 
 int64_t attention_workspace(const ntops_attention_desc& d, bool backward) {
     const Choice c = choose(d);
-    return layout_of(d, backward, c, backward ? tiles_of(d, d.q_rows, 128) : c.tiles, tiles_of(d, d.k_rows, 128)).bytes;
+    return layout_of(d, backward, c, backward ? tiles_of(d, d.q_rows, 128) : c.tiles, tiles_of(d, d.k_rows, kAttnKeys)).bytes;
 }
 
 int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
@@ -108,7 +108,7 @@ int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
 int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
     AttnArgs a = args_of(d);
     a.tiles = tiles_of(d, d.q_rows, 128);
-    const int64_t k_tiles = tiles_of(d, d.k_rows, 128);
+    const int64_t k_tiles = tiles_of(d, d.k_rows, kAttnKeys);
     const Layout l = layout_of(d, true, {}, a.tiles, k_tiles);
     char* const ws = static_cast<char*>(d.workspace);
     a.delta = reinterpret_cast<float*>(ws + l.delta), a.most = reinterpret_cast<uint32_t*>(ws + l.most);
@@ -117,7 +117,7 @@ int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
         AttnTask* const q_list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
         k_list = reinterpret_cast<AttnTask*>(ws + l.k_tasks);
         a.tasks = q_list;
-        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, 128, 128, (int)a.tiles, (int)k_tiles, q_list, k_list, st)) return rc;
+        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, 128, kAttnKeys, (int)a.tiles, (int)k_tiles, q_list, k_list, st)) return rc;
     }
     return run_attention_backward_kernels(a, k_list, k_tiles, d.cu_q, d.cu_k, d.dtype, st);
 }
