@@ -17,7 +17,7 @@ typedef int v2i_attn __attribute__((ext_vector_type(2)));
 
 constexpr int kAttnStep = 64;               // rows of a tile in LDS
 constexpr int kAttnWaves = 4;
-constexpr int kAttnKeyWaves = 8;            // of the kernel that owns keys, and its keys
+constexpr int kAttnKeyWaves = 4, kAttnKeyStep = 32;   // of the kernel that owns keys: its waves, the rows of its tiles of queries, and its keys
 constexpr int kAttnKeys = 32 * kAttnKeyWaves;
 constexpr uint32_t kNowhere = 0xfffffff0u;  // past every descriptor: reads as zeros
 constexpr float kLog2E = 1.44269504088896340736f;
@@ -52,6 +52,9 @@ struct AttnArgs {
     int splits;        // runs that the keys of a tile are cut into ...
     float* part;       // ... and their results before they are joined: [split][q_rows][heads][dim], then
     float2* part_ml;   // [split][q_rows][heads] maximum (base 2) and sum
+    // dk and dv: runs that the queries of a tile of keys are cut into, and their sums before they are added up: [split][dk, dv][k_rows][kv_heads][dim]
+    int k_splits;
+    float* k_part;
 };
 
 // the task of tile `t`; the longest come first
@@ -85,11 +88,11 @@ __device__ __forceinline__ v16f mfma_attn(v4i rows, v4i cols, v16f c) {   // res
 __device__ __forceinline__ v16f zeros16() { return (v16f){0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0}; }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// 64 rows of DP elements in LDS, 16-byte chunks swizzled so that neither 8 rows' reads of one chunk nor the transposing reads of 4
+// kRows rows of DP elements in LDS, 16-byte chunks swizzled so that neither 8 rows' reads of one chunk nor the transposing reads of 4
 // rows' 64 bytes meet in a bank
-template <int DP>
+template <int DP, int kRows = kAttnStep>
 struct AttnTile {
-    static constexpr int kPitch = DP <= 64 ? 128 : 256, kBytes = kAttnStep * kPitch;
+    static constexpr int kPitch = DP <= 64 ? 128 : 256, kBytes = kRows * kPitch;
     static __device__ __forceinline__ int swizzle(int row) {
         if constexpr (kPitch == 128) return ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
         else return (row & 3) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
@@ -112,9 +115,9 @@ struct AttnTile {
                 off[i] = chunk * 8 < dim ? (uint32_t)row * (uint32_t)row_bytes + chunk * 16 : kNowhere;
             }
         }
-        // rows first .. first + 63 of `len`, those behind it as zeros
+        // rows first .. of `len`, those behind it as zeros
         __device__ __forceinline__ void load(uint8_t* stage, int first, int len, int wave) const {
-            const int rows = min(kAttnStep, len - first);
+            const int rows = min(kRows, len - first);
             const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)row_bytes + 2u * dim : 0u;
             const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (int64_t)first * row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
 #pragma unroll
@@ -207,8 +210,8 @@ __device__ __forceinline__ void add_columns(v16f (&acc)[DP / 32], const AttnTile
 // The same over 16 kScores rows, from 16 s0 on, of a stage that holds values which are not finite, under a mask: a score of zero times such a value would
 // reach the rows that do not count it (a padded row, a token to come), so the stage's rows go one at a time, and only into the
 // rows that count them: `counts(i)`, this lane's row counts row i.
-template <int T, int DP, int kScores, typename F>
-__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const AttnTile<DP>& tile, uint8_t* stage, int s0, const v4i (&scores)[kScores], F&& counts, int lane) {
+template <int T, int DP, int kScores, typename Tile, typename F>
+__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const Tile& tile, uint8_t* stage, int s0, const v4i (&scores)[kScores], F&& counts, int lane) {
 #pragma unroll 1
     for (int i = 0; i < 16 * kScores; ++i) {
         const int s = i >> 4, j = (i & 3) + ((i >> 3) & 1) * 4;   // its place in the fragments of half wave (i >> 2) & 1

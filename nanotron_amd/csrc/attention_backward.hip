@@ -146,16 +146,17 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
 // its keys and both sums in registers, 160 of the 256 that two waves a SIMD have; its values stay in LDS.
 template <int T, int DP>
 __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(const AttnArgs A) {
-    typedef AttnTile<DP> Tile;
+    typedef AttnTile<DP, kAttnKeyStep> Tile;
     __shared__ __attribute__((aligned(1024))) uint8_t sq[2 * Tile::kBytes];
     __shared__ __attribute__((aligned(1024))) uint8_t sg[2 * Tile::kBytes];
-    __shared__ __attribute__((aligned(1024))) uint8_t sv[kAttnKeyWaves / 2 * Tile::kBytes];
-    __shared__ __attribute__((aligned(1024))) float rows_of[2][2][kAttnStep];   // lse and delta
+    __shared__ __attribute__((aligned(1024))) uint8_t sv[kAttnKeys / kAttnKeyStep * Tile::kBytes];
+    __shared__ __attribute__((aligned(1024))) float rows_of[2][2][64];   // lse and delta (a wave loads 64)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x / A.kv_heads, kv = blockIdx.x - t * A.kv_heads;
+    const int run = blockIdx.x / A.kv_heads, kv = blockIdx.x - run * A.kv_heads, t = run / A.k_splits, split = run - t * A.k_splits;
     const AttnTask task = attn_task(A, t, kAttnKeys, true);
     if (task.rows <= 0) return;
-    const int begin = A.causal ? max(0, task.shift) / kAttnStep : 0, per = max(0, (task.len + kAttnStep - 1) / kAttnStep - begin), steps = per * A.group;
+    const int begin = A.causal ? max(0, task.shift) / kAttnKeyStep : 0, per = max(0, (task.len + kAttnKeyStep - 1) / kAttnKeyStep - begin);
+    const int each = (per * A.group + A.k_splits - 1) / A.k_splits, step0 = min(split * each, per * A.group), steps = min(step0 + each, per * A.group);
     Tile tile;
     tile.init(lane);
     typename Tile::template Source<kAttnKeyWaves> qs, gs, vs;
@@ -164,9 +165,9 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
     const float* stats = (wave == 0 ? A.lse : A.delta) + kv * A.group * A.q_rows + task.other;
     const char *const q_base = qs.base, *const g_base = gs.base;
     // Tiles of a head's queries: first those whose rows all see all keys of the workgroup, then the ones in front of and behind these
-    const int front = A.causal ? min(max(0, (task.shift + task.rows - 1 + kAttnStep - 1) / kAttnStep - begin), per) : 0;
-    const int whole = max(0, min(task.len / kAttnStep - begin, per) - front);
-    auto row_of = [&](int i) { return (begin + (i < whole ? front + i : i < whole + front ? i - whole : i)) * kAttnStep; };
+    const int front = A.causal ? min(max(0, (task.shift + task.rows - 1 + kAttnKeyStep - 1) / kAttnKeyStep - begin), per) : 0;
+    const int whole = max(0, min(task.len / kAttnKeyStep - begin, per) - front);
+    auto row_of = [&](int i) { return (begin + (i < whole ? front + i : i < whole + front ? i - whole : i)) * kAttnKeyStep; };
     auto load = [&](int j, int stage) {
         const int head = j / per, first = row_of(j - head * per);
         qs.base = q_base + 2 * (head * A.q_head);
@@ -174,15 +175,15 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
         qs.load(sq + stage * Tile::kBytes, first, task.len, wave);
         gs.load(sg + stage * Tile::kBytes, first, task.len, wave);
         if (wave < 2) {
-            const __amdgpu_buffer_rsrc_t r = make_rsrc(stats + head * A.q_rows + first, (uint32_t)__builtin_amdgcn_readfirstlane(min(kAttnStep, task.len - first) * 4));
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(stats + head * A.q_rows + first, (uint32_t)__builtin_amdgcn_readfirstlane(min(kAttnKeyStep, task.len - first) * 4));
             __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(uintptr_t)&rows_of[stage][wave][0], 4, lane * 4, 0, 0, 0);
         }
     };
     vs.init(A.v, attn_rows(A, task.own, task.seq, task.at, A.v_stride, A.v_batch) + kv * A.v_head, A.v_stride, A.dim, wave, lane);
-    if (steps > 0) {
+    if (step0 < steps) {
 #pragma unroll
-        for (int i = 0; i < kAttnKeyWaves / 2; ++i) vs.load(sv + i * Tile::kBytes, i * kAttnStep, task.rows, wave);
-        load(0, 0);
+        for (int i = 0; i < kAttnKeys / kAttnKeyStep; ++i) vs.load(sv + i * Tile::kBytes, i * kAttnKeyStep, task.rows, wave);
+        load(step0, step0 & 1);
     }
     const int mine = wave * 32 * Tile::kPitch;
     const int row = wave * 32 + (lane & 31);
@@ -203,12 +204,12 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
         wg_barrier();
         if (j + 1 < steps) load(j + 1, stage ^ 1);
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
-        if (kMasked && A.causal && row0 + kAttnStep - 1 < lead) return;
+        if (kMasked && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
         const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
         bool singly = false;
-        if constexpr (kMasked) singly = attn_not_finite<T, DP>(ga, kAttnStep, lane) || attn_not_finite<T, DP>(qa, kAttnStep, lane);
+        if constexpr (kMasked) singly = attn_not_finite<T, DP>(ga, kAttnKeyStep, lane) || attn_not_finite<T, DP>(qa, kAttnKeyStep, lane);
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kAttnKeyStep / 32; ++b) {
             __builtin_amdgcn_sched_barrier(0);
             v16f s = zeros16(), d = zeros16();
 #pragma unroll
@@ -255,14 +256,55 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
                 }
         }
     };
-    for (int j = 0; j < steps;) {
-        const int head_end = j + per;
-        for (const int end = j + whole; j < end; ++j) step(j, std::false_type{});
-        for (; j < head_end; ++j) step(j, std::true_type{});
+    for (int j = step0; j < steps;) {
+        const int i = j % per;
+        for (const int end = min(steps, j + whole - i); j < end; ++j) step(j, std::false_type{});
+        for (const int end = min(steps, j + per - max(i, whole)); j < end; ++j) step(j, std::true_type{});
     }
     const int64_t to = (((int64_t)task.own + row) * A.kv_heads + kv) * A.dim;
+    const float dk_by = A.scale / lift;
+    if (A.k_splits > 1) {
+        if (!live) return;
+        const int64_t all = A.k_rows * A.kv_heads * A.dim;
+        float* const part = A.k_part + 2 * split * all + to;
+#pragma unroll
+        for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * e + 8 * g + 4 * (lane >> 5);
+                if (d >= A.dim) continue;
+                v4f x, y;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = dk[e][4 * g + i] * dk_by;
+                    y[i] = dv[e][4 * g + i] * kDown;
+                }
+                *reinterpret_cast<v4f*>(part + d) = x;
+                *reinterpret_cast<v4f*>(part + all + d) = y;
+            }
+        return;
+    }
     if (A.dv) store_rows<T, DP>(dv, kDown, A.dv, to, A.dim, live, lane);
-    if (A.dk) store_rows<T, DP>(dk, A.scale / lift, A.dk, to, A.dim, live, lane);
+    if (A.dk) store_rows<T, DP>(dk, dk_by, A.dk, to, A.dim, live, lane);
+}
+
+// The runs' sums added up, in their order: 8 elements a thread, dk and dv side by side
+template <int T>
+__global__ __launch_bounds__(256) void attention_add_kernel(const AttnArgs A) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8, all = A.k_rows * A.kv_heads * A.dim;
+    void* const out = blockIdx.y ? A.dv : A.dk;
+    if (at >= all || !out) return;
+    float x[8] = {};
+    const float* p = A.k_part + blockIdx.y * all + at;
+    for (int s = 0; s < A.k_splits; ++s, p += 2 * all) {
+        const v4f a = *reinterpret_cast<const v4f*>(p), b = *reinterpret_cast<const v4f*>(p + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] += a[i];
+            x[4 + i] += b[i];
+        }
+    }
+    store_piece<T, 8>(out, at, x);
 }
 
 }  // namespace
@@ -280,8 +322,12 @@ int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, i
         if (A.dk || A.dv) {
             AttnArgs K = A;
             K.tasks = k_tasks;
-            attention_dkv_kernel<T, DP><<<(unsigned)(k_tiles * A.kv_heads), 64 * kAttnKeyWaves, 0, st>>>(K);
+            attention_dkv_kernel<T, DP><<<(unsigned)(k_tiles * A.kv_heads * A.k_splits), 64 * kAttnKeyWaves, 0, st>>>(K);
             if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+            if (A.k_splits > 1) {
+                attention_add_kernel<T><<<dim3((unsigned)((A.k_rows * A.kv_heads * A.dim + 2047) / 2048), 2), 256, 0, st>>>(A);
+                if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+            }
         }
         if (A.dq) {
             attention_dq_kernel<T, DP><<<(unsigned)(A.tiles * A.heads), 64 * kAttnWaves, 0, st>>>(A);

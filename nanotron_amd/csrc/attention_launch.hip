@@ -39,8 +39,15 @@ Choice choose(const ntops_attention_desc& d) {
     return c;
 }
 
+// Runs that the queries of a tile of keys are cut into.  Two workgroups a CU have room; where tiles and heads of keys are fewer than twice as many, each
+// is cut, but into no less than 32 steps where it is longest.
+int key_splits(const ntops_attention_desc& d) {
+    const int64_t units = tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads, steps = (d.q_rows / d.sequences + kAttnKeyStep - 1) / kAttnKeyStep * (d.heads / d.kv_heads);
+    return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 32));
+}
+
 struct Layout {
-    int64_t q_tasks, k_tasks, part, part_ml, delta, most, bytes;
+    int64_t q_tasks, k_tasks, part, part_ml, delta, most, k_part, bytes;
 };
 Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, int64_t q_tiles, int64_t k_tiles) {
     Layout l = {};
@@ -55,6 +62,8 @@ Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, 
         l.k_tasks = take(d.cu_q ? k_tiles * (int64_t)sizeof(AttnTask) : 0);
         l.delta = take(d.q_rows * d.heads * 4);
         l.most = take(8);
+        const int splits = key_splits(d);
+        if (splits > 1) l.k_part = take(2 * splits * d.k_rows * d.kv_heads * d.head_dim * 4);
     } else if (c.splits > 1) {
         l.part = take(c.splits * d.q_rows * d.heads * d.head_dim * 4);
         l.part_ml = take(c.splits * d.q_rows * d.heads * 8);
@@ -112,6 +121,7 @@ int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
     const Layout l = layout_of(d, true, {}, a.tiles, k_tiles);
     char* const ws = static_cast<char*>(d.workspace);
     a.delta = reinterpret_cast<float*>(ws + l.delta), a.most = reinterpret_cast<uint32_t*>(ws + l.most);
+    a.k_splits = key_splits(d), a.k_part = reinterpret_cast<float*>(ws + l.k_part);
     AttnTask* k_list = nullptr;
     if (d.cu_q) {
         AttnTask* const q_list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
