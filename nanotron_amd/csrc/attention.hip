@@ -367,68 +367,63 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         if (o.x != -__builtin_inff() || o.y != 0.0f) all_sum += o.y * (o.x == all_top ? 1.0f : exp2_fast(o.x - all_top));
     }
     const float mine = top == -__builtin_inff() ? (sum != sum ? 1.0f : 0.0f) : top == all_top ? 1.0f : exp2_fast(top - all_top);
-    // the waves' outputs, [element][row], added up through LDS in the order of the waves
-    constexpr int kPitch = kFewRows + 1;
+    // the waves' outputs, [wave][element][row] in the stages that they no longer need, added up in the order of the waves
     float* const at = reinterpret_cast<float*>(&sk[0][0]);
-    static_assert(sizeof(sk) >= sizeof(float) * DP * kPitch, "");
-    for (int w = 0; w < kAttnWaves; ++w) {
-        if (w == wave) {
+    static_assert(sizeof(sk[0]) >= sizeof(float) * 64 * kFewRows && sizeof(sk) + sizeof(sv) >= sizeof(float) * kAttnWaves * DP * kFewRows, "");
+    // (64 elements a wave in the stages of keys, the others in those of values)
+    float* const over = reinterpret_cast<float*>(&sv[0][0]);
 #pragma unroll
-            for (int e = 0; e < DP / 32; ++e)
+    for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float* const o = at + (32 * e + place_of(r, lane)) * kPitch + row;
-                    const float x = mine == 0.0f ? 0.0f : out[e][r] * mine;
-                    *o = w == 0 ? x : *o + x;
-                }
+        for (int r = 0; r < 16; ++r) {
+            float* const to = e < 2 ? at : over;
+            to[(wave * 64 + 32 * (e & 1) + place_of(r, lane)) * kFewRows + row] = mine == 0.0f ? 0.0f : out[e][r] * mine;
         }
-        __syncthreads();
-    }
-    // 8 threads a row
-    const int r = threadIdx.x >> 3;
+    __syncthreads();
+    // 8 threads a row, 8 elements at a time
+    const int r = threadIdx.x & 31;
     if (r < rows) {
         const int in = r / n, tok = r - in * n, hd = kv * A.group + in;
         const int64_t out_row = (int64_t)seq * n + tok;
-        float m = -__builtin_inff(), l = 0.0f;
+        const int64_t to = ((int64_t)blockIdx.y * A.q_rows + out_row) * A.heads + hd;
+        const float by = A.splits > 1 ? 1.0f : all_sum > 0.0f || all_sum != all_sum ? 1.0f / all_sum : 0.0f;
+        for (int d = (threadIdx.x >> 5) * 8; d < A.dim; d += 64) {
+            const float* const from = d < 64 ? at : over;
+            float x[8] = {};
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) m = fmaxf(m, ml[w][r].x);
+            for (int w = 0; w < kAttnWaves; ++w)
 #pragma unroll
-        for (int w = 0; w < kAttnWaves; ++w) {
-            const float2 o = ml[w][r];
-            if (o.x != -__builtin_inff() || o.y != 0.0f) l += o.y * (o.x == m ? 1.0f : exp2_fast(o.x - m));
+                for (int i = 0; i < 8; ++i) x[i] += from[(w * 64 + (d & 63) + i) * kFewRows + r];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= by;
+            if (A.splits > 1) store_piece<NTFP8_F32, 8>(A.part, to * A.dim + d, x);
+            else store_piece<T, 8>(A.out, (out_row * A.heads + hd) * A.dim + d, x);
         }
-        if (A.splits > 1) {
-            const int64_t to = ((int64_t)blockIdx.y * A.q_rows + out_row) * A.heads + hd;
-            if ((threadIdx.x & 7) == 0) A.part_ml[to] = make_float2(m, l);
-            for (int d = (threadIdx.x & 7) * 8; d < A.dim; d += 64)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) A.part[to * A.dim + d + i] = at[(d + i) * kPitch + r];
-        } else {
-            const float by = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            for (int d = (threadIdx.x & 7) * 8; d < A.dim; d += 64) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = at[(d + i) * kPitch + r] * by;
-                store_piece<T, 8>(A.out, (out_row * A.heads + hd) * A.dim + d, x);
-            }
-            if (A.lse && (threadIdx.x & 7) == 0) A.lse[hd * A.q_rows + out_row] = l > 0.0f || l != l ? m + log2f(l) : __builtin_inff();
+        if (threadIdx.x < kFewRows) {
+            if (A.splits > 1) A.part_ml[to] = make_float2(all_top, all_sum);
+            else if (A.lse) A.lse[hd * A.q_rows + out_row] = all_sum > 0.0f || all_sum != all_sum ? all_top + log2f(all_sum) : __builtin_inff();
         }
     }
 }
 
-// The splits' results joined: a row of one head in 16 lanes, 8 elements each
+// The splits' results joined: a row of one head is a wave's, 16 lanes of 8 elements by four runs of splits
 template <int T>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
-    const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-    const int d = (threadIdx.x & 15) * 8;
-    if (row >= A.q_rows * A.heads) return;
-    const int64_t pitch = A.q_rows * A.heads;
-    float top = -__builtin_inff(), sum = 0.0f, x[8] = {};
-    for (int s = 0; s < A.splits; ++s) top = fmaxf(top, A.part_ml[s * pitch + row].x);
-    for (int s = 0; s < A.splits; ++s) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), pitch = A.q_rows * A.heads;
+    if (row >= pitch) return;   // (whole waves)
+    const int lane = threadIdx.x & 63, d = (lane & 15) * 8, run = lane >> 4;
+    // every lane's splits, one after another: their largest maximum first
+    float top = -__builtin_inff();
+    for (int s = lane; s < A.splits; s += 64) top = fmaxf(top, A.part_ml[s * pitch + row].x);
+#pragma unroll
+    for (int m = 32; m >= 1; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
+    float sum = 0.0f, x[8] = {};
+#pragma unroll 4
+    for (int s = run; s < A.splits; s += 4) {
         const float2 o = A.part_ml[s * pitch + row];
-        if (o.x == -__builtin_inff() && o.y == 0.0f) continue;
-        const float by = o.x == top ? 1.0f : exp2_fast(o.x - top);
+        // (an empty split, of which nothing counts; not one whose sum is NaN)
+        const bool none = o.x == -__builtin_inff() && o.y == 0.0f;
+        const float by = none ? 0.0f : o.x == top ? 1.0f : exp2_fast(o.x - top);
         sum += o.y * by;
         if (d < A.dim) {
             const v4f* const p = reinterpret_cast<const v4f*>(A.part + (s * pitch + row) * A.dim + d);
@@ -440,6 +435,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
             }
         }
     }
+#pragma unroll
+    for (int m = 16; m <= 32; m *= 2) {
+        sum += __shfl_xor(sum, m);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += __shfl_xor(x[i], m);
+    }
+    if (run != 0) return;
     const bool any = sum > 0.0f || sum != sum;
     if (d < A.dim) {
         const float over = any ? 1.0f / sum : 0.0f;
@@ -468,7 +470,7 @@ int run_attention_forward_kernels(const AttnArgs& A, int dtype, int q_blocks, bo
         else if (q_blocks == 1) attention_forward_kernel<T, DP, 1><<<grid, 64 * kAttnWaves, 0, st>>>(A);
         else attention_forward_kernel<T, DP, 2><<<grid, 64 * kAttnWaves, 0, st>>>(A);
         if (const int rc = launch_status(); rc != NTFP8_OK || A.splits <= 1) return rc;
-        attention_join_kernel<T><<<(unsigned)((A.q_rows * A.heads * 16 + 255) / 256), 256, 0, st>>>(A);
+        attention_join_kernel<T><<<(unsigned)((A.q_rows * A.heads + 3) / 4), 256, 0, st>>>(A);
         return launch_status();
     });
 }

@@ -15,13 +15,14 @@ constexpr float kLiftP = 8.0f;
 template <int T>
 __device__ __forceinline__ float gradient_lift(const AttnArgs& A) {
     if constexpr (T == NTFP8_BF16) return 1.0f;
-    const float most = 2.0f * A.dim * __uint_as_float(A.most[0]) * __uint_as_float(A.most[1]);
+    const uint32_t* const at = A.most + (threadIdx.x & 63) * kMostLine;
+    const float most = 2.0f * A.dim * __uint_as_float(wave_most(at[0])) * __uint_as_float(wave_most(at[64 * kMostLine]));
     if (!(most > 0.0f) || most > 1e30f || most < 1e-30f) return 1.0f;
     const int e = (int)(__float_as_uint(most) >> 23) - 127;   // 2^e <= most < 2^(e + 1)
     return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
 }
 
-__global__ void attention_clear_kernel(uint32_t* p) { p[threadIdx.x] = 0u; }
+__global__ void attention_clear_kernel(uint32_t* p) { p[threadIdx.x * kMostLine] = 0u; }
 
 // delta, 16 lanes a row; blocks behind those of the rows of dout read v, for its largest magnitude
 template <int T>
@@ -53,10 +54,9 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
     for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
     if (!values && row < rows && d == 0) A.delta[head * A.q_rows + row] = live ? sum : 0.0f;
     if constexpr (T == NTFP8_F16) {
-        // (a maximum: the order changes nothing; and few find themselves above what is there already)
+        // (a maximum: the order changes nothing.  64 lines, or the blocks' atomics wait for each other: 56 us for 36000 rows on one, 8 so)
         most = wave_most(most);
-        uint32_t* const at = &A.most[values];
-        if ((threadIdx.x & 63) == 0 && most > __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) atomicMax(at, most);
+        if ((threadIdx.x & 63) == 0 && most) atomicMax(&A.most[((values ? 64 : 0) + blockIdx.x % 64) * kMostLine], most);
     }
 }
 
@@ -314,7 +314,7 @@ int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, i
         constexpr int T = decltype(t)::value, DP = decltype(d)::value;
         const int64_t q_blocks = (A.q_rows * A.heads + 15) / 16, v_blocks = T == NTFP8_F16 ? (A.k_rows * A.kv_heads + 15) / 16 : 0;
         if (T == NTFP8_F16) {
-            attention_clear_kernel<<<1, 2, 0, st>>>(A.most);
+            attention_clear_kernel<<<1, 128, 0, st>>>(A.most);
             if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
         }
         attention_delta_kernel<T><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(A, cu_q, cu_k, q_blocks);

@@ -40,10 +40,11 @@ Choice choose(const ntops_attention_desc& d) {
 }
 
 // Runs that the queries of a tile of keys are cut into.  Two workgroups a CU have room; where tiles and heads of keys are fewer than twice as many, each
-// is cut, but into no less than 32 steps where it is longest.
+// is cut, but into no less than 16 steps where it is longest (of packed sequences, where one is twice as long as their average).
 int key_splits(const ntops_attention_desc& d) {
-    const int64_t units = tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads, steps = (d.q_rows / d.sequences + kAttnKeyStep - 1) / kAttnKeyStep * (d.heads / d.kv_heads);
-    return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 32));
+    const int64_t rows = std::min(d.q_rows, d.q_rows / d.sequences * (d.cu_q && d.sequences > 1 ? 2 : 1));
+    const int64_t units = tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads, steps = (rows + kAttnKeyStep - 1) / kAttnKeyStep * (d.heads / d.kv_heads);
+    return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 16));
 }
 
 struct Layout {
@@ -61,7 +62,7 @@ Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, 
     if (backward) {
         l.k_tasks = take(d.cu_q ? k_tiles * (int64_t)sizeof(AttnTask) : 0);
         l.delta = take(d.q_rows * d.heads * 4);
-        l.most = take(8);
+        l.most = take(d.dtype == NTFP8_F16 ? 128 * kMostLine * 4 : 0);
         const int splits = key_splits(d);
         if (splits > 1) l.k_part = take(2 * splits * d.k_rows * d.kv_heads * d.head_dim * 4);
     } else if (c.splits > 1) {
