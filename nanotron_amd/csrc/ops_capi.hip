@@ -18,7 +18,7 @@ int64_t head_piece(int64_t vocab);
 int64_t head_workspace(const ntops_linear_cross_entropy_desc& d);
 int run_head(const ntops_linear_cross_entropy_desc& d, hipStream_t st);
 int64_t rms_norm_most_cols(int dtype);
-int rms_norm_blocks(int dtype, int64_t rows, int64_t cols);
+int rms_norm_blocks(int dtype, int64_t rows, int64_t cols, bool full);
 int run_rms_norm_forward(const ntops_rms_norm_desc& d, hipStream_t st);
 int run_rms_norm_backward(const ntops_rms_norm_desc& d, const ntops_rms_norm_grads& g, hipStream_t st);
 int run_rotary(const ntops_rotary_desc& d, hipStream_t st);
@@ -270,7 +270,8 @@ int ntops_rms_norm_forward(const ntops_rms_norm_desc* d, void* stream) {
 
 int64_t ntops_rms_norm_scratch(const ntops_rms_norm_desc* d) {
     if (!d || check_rms_norm(*d) != NTFP8_OK) return 0;
-    return (int64_t)rms_norm_blocks(d->x_dtype, d->rows, d->cols) * (d->post_weight || d->gate_kind ? 3 : 1) * d->cols * 4;
+    const bool full = d->post_weight || d->gate_kind;
+    return (int64_t)rms_norm_blocks(d->x_dtype, d->rows, d->cols, full) * (full ? 3 : 1) * d->cols * 4;
 }
 
 int ntops_rms_norm_backward(const ntops_rms_norm_desc* d, const ntops_rms_norm_grads* g, void* stream) {

@@ -10,7 +10,8 @@ namespace ntfp8 {
 namespace {
 
 constexpr int forward_block(int tpr) { return tpr < 256 ? 256 : tpr; }
-constexpr int backward_block(int tpr) { return tpr <= 128 ? 512 : 1024; }
+// backward: rows enough to fill a CU; with a norm behind the block or a gate half the threads, which then have registers for its vectors
+constexpr int backward_block(int tpr, bool full) { return tpr == 1024 || (tpr >= 256 && !full) ? 1024 : 512; }
 constexpr int kMostPieces = 2;   // 16-byte pieces of a row of x that a thread holds
 enum Gate { kNoGate = 0, kChannelGate = 1, kElementGate = 2 };
 constexpr int kVectors = 3;      // gradients that are summed over rows: weight, post_weight, a channel's gate
@@ -143,8 +144,9 @@ __global__ __launch_bounds__(forward_block(TPR)) void rms_norm_forward_kernel(co
 // groups of a block are added through LDS, and each block leaves one row of sums a vector for vector_sums_kernel.
 // kFull: there is a norm behind the block, or a gate.
 template <int D, int R, bool kFull, int TPR, int VPT>
-__global__ __launch_bounds__(backward_block(TPR)) void rms_norm_backward_kernel(const Norms n) {
-    constexpr int kBlock = backward_block(TPR), kGroups = kBlock / TPR, VE = 16 / size_of(D), kSums = kFull ? kVectors : 1;
+__global__ __launch_bounds__(backward_block(TPR, kFull)) void rms_norm_backward_kernel(const Norms n) {
+    constexpr int kBlock = backward_block(TPR, kFull), kGroups = kBlock / TPR, VE = 16 / size_of(D), kSums = kFull ? kVectors : 1;
+    constexpr bool kHold = VPT == 1;
     __shared__ float sums[2][2][kBlock / 64];
     __shared__ float other[kGroups > 1 ? kBlock / 2 * VPT * VE : 1];
     const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
@@ -156,33 +158,62 @@ __global__ __launch_bounds__(backward_block(TPR)) void rms_norm_backward_kernel(
         for (int k = 0; k < VPT; ++k)
 #pragma unroll
             for (int e = 0; e < VE; ++e) total[s][k][e] = 0.0f;
+    // the vectors, kept where there are registers for them
+    float held[kHold ? kSums : 1][VE];
+    if constexpr (kHold) {
+        if (n.weight) vector_piece<D, VE>(n.weight, n.w_dtype, t * VE, n.cols, held[0]);
+        if constexpr (kFull) {
+            if (n.post_weight) vector_piece<D, VE>(n.post_weight, n.w_dtype, t * VE, n.cols, held[1]);
+            if (n.gate_kind == kChannelGate) vector_piece<D, VE>(n.gate, n.w_dtype, t * VE, n.cols, held[2]);
+        }
+    }
+    auto vector = [&](int which, const void* p, int k, float (&w)[VE]) {
+        if constexpr (kHold) {
+#pragma unroll
+            for (int e = 0; e < VE; ++e) w[e] = held[kFull ? which : 0][e];
+        } else {
+            vector_piece<D, VE>(p, n.w_dtype, (t + k * TPR) * VE, n.cols, w);
+        }
+    };
+    struct Row {
+        Piece<D, VE> dy[VPT], x[VPT], gate[VPT];
+        Piece<R, VE> h[VPT], dh[VPT];
+        float first, second;
+    };
+    auto read = [&](Row& r, int64_t row) {
+        const bool live = row < n.rows;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int c = (t + k * TPR) * VE, left = live && c < n.cols ? n.cols - c : 0;
+            r.h[k] = load_piece<R, VE>(n.h, row * n.residual_stride + c, left);
+            r.dy[k] = load_piece<D, VE>(n.dy, row * n.dy_stride + c, n.dy ? left : 0);
+            r.dh[k] = load_piece<R, VE>(n.dh, row * n.dh_stride + c, n.dh ? left : 0);
+            if constexpr (kFull) {
+                r.x[k] = load_piece<D, VE>(n.x, row * n.x_stride + c, left);
+                if (n.gate_kind == kElementGate) r.gate[k] = load_piece<D, VE>(n.gate, row * n.gate_stride + c, left);
+            }
+        }
+        r.second = live ? n.second[row] : 0.0f;
+        r.first = kFull && live && n.post_weight ? n.first[row] : 0.0f;
+    };
     const int64_t step = (int64_t)gridDim.x * kGroups;
     int64_t row = (int64_t)blockIdx.x * kGroups + group;
+    Row now;
     int turn = 0;
     // (the same number of turns for every group: the barriers are the block's)
     for (int64_t at = (int64_t)blockIdx.x * kGroups; at < n.rows; at += step, row += step, turn ^= 1) {
         const bool live = row < n.rows;
-        Piece<D, VE> dy[VPT], x[VPT], gate[VPT];
-        Piece<R, VE> h[VPT], dh[VPT];
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-            const int c = (t + k * TPR) * VE, left = live && c < n.cols ? n.cols - c : 0;
-            h[k] = load_piece<R, VE>(n.h, row * n.residual_stride + c, left);
-            dy[k] = load_piece<D, VE>(n.dy, row * n.dy_stride + c, n.dy ? left : 0);
-            dh[k] = load_piece<R, VE>(n.dh, row * n.dh_stride + c, n.dh ? left : 0);
-            if constexpr (kFull) {
-                x[k] = load_piece<D, VE>(n.x, row * n.x_stride + c, left);
-                if (n.gate_kind == kElementGate) gate[k] = load_piece<D, VE>(n.gate, row * n.gate_stride + c, left);
-            }
-        }
-        const float second = live ? n.second[row] : 0.0f, first = kFull && live && n.post_weight ? n.first[row] : 0.0f;
+        read(now, row);
+        const Piece<D, VE>(&dy)[VPT] = now.dy, (&x)[VPT] = now.x, (&gate)[VPT] = now.gate;
+        const Piece<R, VE>(&h)[VPT] = now.h, (&dh)[VPT] = now.dh;
+        const float first = now.first, second = now.second;
         float a[VPT][VE], s = 0.0f;   // g
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             float hv[VE], w[VE];
             unpack<R, VE>(h[k], hv);
             unpack<D, VE>(dy[k], a[k]);
-            if (n.weight) vector_piece<D, VE>(n.weight, n.w_dtype, (t + k * TPR) * VE, n.cols, w);
+            if (n.weight) vector(0, n.weight, k, w);
 #pragma unroll
             for (int e = 0; e < VE; ++e) {
                 const float nv = hv[e] * second;
@@ -210,13 +241,13 @@ __global__ __launch_bounds__(backward_block(TPR)) void rms_norm_backward_kernel(
                 float u[VE], pw[VE], g[VE];
                 unpack<D, VE>(x[k], u);
                 if (n.post_weight) {
-                    vector_piece<D, VE>(n.post_weight, n.w_dtype, c, n.cols, pw);
+                    vector(1, n.post_weight, k, pw);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) u[e] *= first;
                 }
                 if (n.gate_kind != kNoGate) {
                     if (n.gate_kind == kElementGate) unpack<D, VE>(gate[k], g);
-                    else vector_piece<D, VE>(n.gate, n.w_dtype, c, n.cols, g);
+                    else vector(2, n.gate, k, g);
 #pragma unroll
                     for (int e = 0; e < VE; ++e) {
                         o[e] = a[k][e] * (n.post_weight ? u[e] * pw[e] : u[e]);
@@ -337,10 +368,10 @@ int pieces_of(int dtype, int64_t cols) { return (int)((cols * size_of(dtype) + 1
 
 int64_t rms_norm_most_cols(int dtype) { return 1024 * kMostPieces * 16 / size_of(dtype); }
 
-int rms_norm_blocks(int dtype, int64_t rows, int64_t cols) {
+int rms_norm_blocks(int dtype, int64_t rows, int64_t cols, bool full) {
     return by_width(pieces_of(dtype, cols), [&](auto tpr, auto) {
-        constexpr int kBlock = backward_block(decltype(tpr)::value), kGroups = kBlock / decltype(tpr)::value;
-        return (int)std::min<int64_t>((rows + kGroups - 1) / kGroups, (int64_t)cu_count() * (1024 / kBlock));
+        const int block = backward_block(decltype(tpr)::value, full), groups = block / decltype(tpr)::value;
+        return (int)std::min<int64_t>((rows + groups - 1) / groups, (int64_t)cu_count() * (full ? 1 : 1024 / block));
     });
 }
 
@@ -375,7 +406,7 @@ int run_rms_norm_forward(const ntops_rms_norm_desc& d, hipStream_t st) {
 int run_rms_norm_backward(const ntops_rms_norm_desc& d, const ntops_rms_norm_grads& g, hipStream_t st) {
     const bool full = d.post_weight || d.gate_kind != kNoGate;
     const bool vectors = g.dweight || g.dpost_weight || (g.dgate && d.gate_kind == kChannelGate);
-    const int blocks = rms_norm_blocks(d.x_dtype, d.rows, d.cols);
+    const int blocks = rms_norm_blocks(d.x_dtype, d.rows, d.cols, full);
     Norms n = {};
     n.rows = d.rows, n.cols = (int)d.cols, n.w_dtype = d.w_dtype, n.eps = d.eps, n.scale = d.residual_scale;
     n.x = d.x, n.x_stride = d.x_stride, n.gate = d.gate, n.gate_kind = d.gate_kind, n.gate_stride = d.gate_stride;
@@ -389,8 +420,8 @@ int run_rms_norm_backward(const ntops_rms_norm_desc& d, const ntops_rms_norm_gra
         return with_residual<decltype(t)::value>(d.residual_dtype, [&](auto r) {
             return by_width(pieces_of(d.x_dtype, d.cols), [&](auto tpr, auto vpt) {
                 constexpr int D = decltype(t)::value, R = decltype(r)::value, TPR = decltype(tpr)::value, VPT = decltype(vpt)::value;
-                if (full) rms_norm_backward_kernel<D, R, true, TPR, VPT><<<blocks, backward_block(TPR), 0, st>>>(n);
-                else rms_norm_backward_kernel<D, R, false, TPR, VPT><<<blocks, backward_block(TPR), 0, st>>>(n);
+                if (full) rms_norm_backward_kernel<D, R, true, TPR, VPT><<<blocks, backward_block(TPR, true), 0, st>>>(n);
+                else rms_norm_backward_kernel<D, R, false, TPR, VPT><<<blocks, backward_block(TPR, false), 0, st>>>(n);
                 return launch_status();
             });
         });

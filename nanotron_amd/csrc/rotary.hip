@@ -8,7 +8,7 @@
 namespace ntfp8 {
 namespace {
 
-constexpr int kThreads = 256, kUnits = 4;   // threads of a workgroup, pieces of work a thread holds at once
+constexpr int kThreads = 256, kTurns = 4;   // threads of a workgroup, and pieces of work of each, about
 constexpr int kMostPairs = 1024;            // sines and cosines in LDS
 
 struct Rotary {
@@ -77,11 +77,10 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary R) {
         u.from = u.to + a;
         u.to += b;
     };
-    // what is read first is asked for before the angles are worked out
-    Unit unit[kUnits];
-#pragma unroll
-    for (int k = 0; k < kUnits; ++k)
-        if ((int)threadIdx.x + k * kThreads < total) read(unit[k], threadIdx.x + k * kThreads);
+    // What is read first is asked for before the angles are worked out.  One piece of work at a time: the registers of two or four
+    // halve or quarter the waves on a CU, whose loads overlap (16381 tokens, 40 heads of 128: 73, 82, 88 us)
+    Unit unit;
+    if ((int)threadIdx.x < total) read(unit, threadIdx.x);
     for (int i = threadIdx.x; i < tokens * R.pairs; i += kThreads) {
         const int token = over(i, R.pairs, R.magic_pairs);
         int64_t p = R.first_token + token0 + token;
@@ -123,15 +122,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(const Rotary R) {
         store_piece<D, VE>(R.out[u.which], u.from, p, u.first);
         store_piece<D, VE>(R.out[u.which], u.to, q, u.second);
     };
-    for (int base = 0; base < total; base += kUnits * kThreads) {
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-            const int i = base + (int)threadIdx.x + k * kThreads;
-            if (i < total) {
-                if (base) read(unit[k], i);
-                write(unit[k]);
-            }
-        }
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        if (i != (int)threadIdx.x) read(unit, i);
+        write(unit);
     }
 }
 
@@ -151,8 +144,8 @@ int run_rotary(const ntops_rotary_desc& d, hipStream_t st) {
     r.positions = d.positions, r.position_count = d.position_count, r.position_bits = d.position_bits;
     r.frequencies = d.frequencies, r.interleaved = d.interleaved, r.inverse = d.inverse, r.scale = d.scale;
     const int heads = d.heads + d.kv_heads;
-    // a workgroup's tokens: about kUnits pieces of work a thread, and no more angles than LDS has room for
-    r.tokens_a_block = std::max(1, std::min(kUnits * kThreads / (heads * r.units), kMostPairs / d.pairs));
+    // a workgroup's tokens: about kTurns pieces of work a thread, and no more angles than LDS has room for
+    r.tokens_a_block = std::max(1, std::min(kTurns * kThreads / (heads * r.units), kMostPairs / d.pairs));
     r.magic_heads = magic_of_count(heads), r.magic_units = magic_of_count(r.units), r.magic_pairs = magic_of_count(d.pairs);
     // (a launch takes fewer than 2^32 threads)
     const int64_t most = (int64_t)r.tokens_a_block << 23;
