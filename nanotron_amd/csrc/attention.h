@@ -46,8 +46,8 @@ struct AttnArgs {
     float scale;
     void* out;
     const void* o;     // backward: the output of the forward pass
-    float* lse;        // [heads][q_rows], base 2; +infinity for a row that sees nothing
-    float* delta;      // [heads][q_rows]
+    float* lse;        // [heads][q_rows] minus the logarithm of a row's sum of exponentials, in units of q k^T; minus infinity for a row that sees nothing
+    float* delta;      // [heads][q_rows] minus the sum of dout out
     uint32_t* most;    // fp16 gradients: bits of the largest magnitudes in dout and v, [2][64] a line each
     void *dq, *dk, *dv;
     int splits;        // runs that the keys of a tile are cut into ...
@@ -263,6 +263,10 @@ __device__ __forceinline__ float both_sum(float v) {
     swap_halves(x, y);
     return __uint_as_float(x) + __uint_as_float(y);
 }
+
+// what is kept of a row's maximum (base 2) and sum for the backward pass, and whether it sees anything
+__device__ __forceinline__ bool attn_any(float sum) { return sum > 0.0f || sum != sum; }
+__device__ __forceinline__ float attn_lse(const AttnArgs& A, float top, float sum) { return attn_any(sum) ? -(top + log2f(sum)) / A.c : -__builtin_inff(); }
 
 // calls f with the type and the head's size rounded up to what the kernels are built for
 template <typename F>

@@ -246,8 +246,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
                 }
             continue;
         }
-        store_rows<T, DP>(out[b], all > 0.0f || all != all ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane);
-        if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = all > 0.0f || all != all ? top[b] + log2f(all) : __builtin_inff();
+        store_rows<T, DP>(out[b], attn_any(all) ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane);
+        if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = attn_lse(A, top[b], all);
     }
 }
 
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         const int in = r / n, tok = r - in * n, hd = kv * A.group + in;
         const int64_t out_row = (int64_t)seq * n + tok;
         const int64_t to = ((int64_t)blockIdx.y * A.q_rows + out_row) * A.heads + hd;
-        const float by = A.splits > 1 ? 1.0f : all_sum > 0.0f || all_sum != all_sum ? 1.0f / all_sum : 0.0f;
+        const float by = A.splits > 1 ? 1.0f : attn_any(all_sum) ? 1.0f / all_sum : 0.0f;
         for (int d = (threadIdx.x >> 5) * 8; d < A.dim; d += 64) {
             const float* const from = d < 64 ? at : over;
             float x[8] = {};
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         }
         if (threadIdx.x < kFewRows) {
             if (A.splits > 1) A.part_ml[to] = make_float2(all_top, all_sum);
-            else if (A.lse) A.lse[hd * A.q_rows + out_row] = all_sum > 0.0f || all_sum != all_sum ? all_top + log2f(all_sum) : __builtin_inff();
+            else if (A.lse) A.lse[hd * A.q_rows + out_row] = attn_lse(A, all_top, all_sum);
         }
     }
 }
@@ -442,14 +442,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
         for (int i = 0; i < 8; ++i) x[i] += __shfl_xor(x[i], m);
     }
     if (run != 0) return;
-    const bool any = sum > 0.0f || sum != sum;
     if (d < A.dim) {
-        const float over = any ? 1.0f / sum : 0.0f;
+        const float over = attn_any(sum) ? 1.0f / sum : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= over;
         store_piece<T, 8>(A.out, row * A.dim + d, x);
     }
-    if (A.lse && d == 0) A.lse[(row % A.heads) * A.q_rows + row / A.heads] = any ? top + log2f(sum) : __builtin_inff();
+    if (A.lse && d == 0) A.lse[(row % A.heads) * A.q_rows + row / A.heads] = attn_lse(A, top, sum);
 }
 
 }  // namespace

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
     }
 #pragma unroll
     for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
-    if (!values && row < rows && d == 0) A.delta[head * A.q_rows + row] = live ? sum : 0.0f;
+    if (!values && row < rows && d == 0) A.delta[head * A.q_rows + row] = live ? -sum : 0.0f;
     if constexpr (T == NTFP8_F16) {
         // (a maximum: the order changes nothing.  64 lines, or the blocks' atomics wait for each other: 56 us for 36000 rows on one, 8 so)
         most = wave_most(most);
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
     load_own<DP>(q, A.q, attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head + row * A.q_stride, A.dim, live, lane);
     load_own<DP>(g, A.dout, attn_rows(A, task.own, task.seq, task.at, A.do_stride, A.do_batch) + head * A.do_head + row * A.do_stride, A.dim, live, lane);
     const int64_t at = (int64_t)task.own + row;
-    const float lse = live ? A.lse[head * A.q_rows + at] : __builtin_inff(), delta = live ? A.delta[head * A.q_rows + at] : 0.0f;
+    const float lse = live ? A.lse[head * A.q_rows + at] * A.c : -__builtin_inff(), delta = live ? A.delta[head * A.q_rows + at] : 0.0f;
     const float lift = gradient_lift<T>(A);
     v16f dq[DP / 32];
 #pragma unroll
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
                 d = mfma_attn<T>(tile.rows(sv + stage, b, k), g[k], d);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, -lse)) * ((d[r] - delta) * lift);
+            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, lse)) * ((d[r] + delta) * lift);
             if constexpr (kMasked) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = 32 * b + place_of(r, lane) > last ? 0.0f : s[r];
@@ -190,8 +190,8 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
     const bool live = row < task.rows;
     v4i k[DP / 16];
     load_own<DP>(k, A.k, attn_rows(A, task.own, task.seq, task.at, A.k_stride, A.k_batch) + kv * A.k_head + row * A.k_stride, A.dim, live, lane);
-    constexpr float kUp = T == NTFP8_F16 ? kLiftP : 0.0f, kDown = T == NTFP8_F16 ? 1.0f / 256.0f : 1.0f;
-    const float lift = gradient_lift<T>(A), down = lift * kDown;
+    constexpr float kDown = T == NTFP8_F16 ? 1.0f / 256.0f : 1.0f;   // 2^-kLiftP
+    const float lift = gradient_lift<T>(A), down = lift * kDown, up = kLiftP / A.c;
     v16f dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) dk[e] = dv[e] = zeros16();
@@ -206,54 +206,73 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
         if (kMasked && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
         const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
-        bool singly = false;
-        if constexpr (kMasked) singly = attn_not_finite<T, DP>(ga, kAttnKeyStep, lane) || attn_not_finite<T, DP>(qa, kAttnKeyStep, lane);
+        // s and d begin at what is subtracted from them.  Fragments are read one product ahead: held back by the registers that they take,
+        // the compiler reads each in front of its product and waits, 0.39 of the MFMA slots used instead of XX
+        v16f s, d;
 #pragma unroll
-        for (int b = 0; b < kAttnKeyStep / 32; ++b) {
-            __builtin_amdgcn_sched_barrier(0);
-            v16f s = zeros16(), d = zeros16();
+        for (int n = 0; n < 4; ++n) {
+            const v4f x = *reinterpret_cast<const v4f*>(&rows_of[stage][0][8 * n + 4 * (lane >> 5)]), y = *reinterpret_cast<const v4f*>(&rows_of[stage][1][8 * n + 4 * (lane >> 5)]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[4 * n + i] = T == NTFP8_F16 ? x[i] + up : x[i];
+                d[4 * n + i] = y[i];
+            }
+        }
+        {
+            v4i fq[2], fg[2], fv[2];
+            auto fetch = [&](int i) {
+                fq[i & 1] = tile.rows_anew(sq, at, 0, i);
+                fg[i & 1] = tile.rows_anew(sg, at, 0, i);
+                fv[i & 1] = tile.rows_anew(sv, mine, 0, i);
+            };
+            fetch(0);
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
-                s = mfma_attn<T>(tile.rows_anew(sq, at, b, i), k[i], s);
-                d = mfma_attn<T>(tile.rows_anew(sg, at, b, i), tile.rows_anew(sv, mine, 0, i), d);
+                if (i + 1 < DP / 16) fetch(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
+                s = mfma_attn<T>(fq[i & 1], k[i], s);
+                d = mfma_attn<T>(fg[i & 1], fv[i & 1], d);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        }
+        v4i fa[2], fb[2];
+        auto fetch = [&](int x) {   // of the products with rows 16 (x / (DP / 32)) .., elements 32 (x mod (DP / 32)) ..
+            fa[x & 1] = tile.columns_anew(sg, at, x / (DP / 32), x % (DP / 32));
+            fb[x & 1] = tile.columns_anew(sq, at, x / (DP / 32), x % (DP / 32));
+        };
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const v4f lse = *reinterpret_cast<const v4f*>(&rows_of[stage][0][32 * b + 8 * n + 4 * (lane >> 5)]);
-                const v4f delta = *reinterpret_cast<const v4f*>(&rows_of[stage][1][32 * b + 8 * n + 4 * (lane >> 5)]);
+        for (int r = 0; r < 16; ++r) {
+            s[r] = exp2_fast(s[r] * A.c);
+            d[r] = T == NTFP8_F16 ? s[r] * (d[r] * down) : s[r] * d[r];
+        }
+        if constexpr (kMasked) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 4 * n + i;
-                    s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, kUp - lse[i]));
-                    d[r] = s[r] * ((d[r] - delta[i]) * down);
-                }
+            for (int r = 0; r < 16; ++r) {
+                const int i = place_of(r, lane);
+                const bool in = i >= from && i < to;
+                s[r] = in ? s[r] : 0.0f;
+                d[r] = in ? d[r] : 0.0f;
             }
-            if constexpr (kMasked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = 32 * b + place_of(r, lane);
-                    const bool in = i >= from && i < to;
-                    s[r] = in ? s[r] : 0.0f;
-                    d[r] = in ? d[r] : 0.0f;
-                }
+        }
+        const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)}, ds[2] = {pack_scores<T>(d, 0), pack_scores<T>(d, 8)};
+        if constexpr (kMasked) {
+            if (attn_not_finite<T, DP>(ga, kAttnKeyStep, lane) || attn_not_finite<T, DP>(qa, kAttnKeyStep, lane)) {
+                const auto counts = [&](int i) { return i >= from && i < to; };
+                add_columns_singly<T, DP, 2>(dv, tile, ga, 0, p, counts, lane);
+                add_columns_singly<T, DP, 2>(dk, tile, qa, 0, ds, counts, lane);
+                return;
             }
+        }
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+            if (x + 1 < DP / 16) fetch(x + 1);
             __builtin_amdgcn_sched_barrier(0);
-            const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)}, ds[2] = {pack_scores<T>(d, 0), pack_scores<T>(d, 8)};
-            if constexpr (kMasked) {
-                if (singly) {
-                    const auto counts = [&](int i) { return i >= from && i < to; };
-                    add_columns_singly<T, DP, 2>(dv, tile, ga, 2 * b, p, counts, lane);
-                    add_columns_singly<T, DP, 2>(dk, tile, qa, 2 * b, ds, counts, lane);
-                    continue;
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int e = 0; e < DP / 32; ++e) {
-                    dv[e] = mfma_attn<T>(tile.columns_anew(sg, at, 2 * b + h, e), p[h], dv[e]);
-                    dk[e] = mfma_attn<T>(tile.columns_anew(sq, at, 2 * b + h, e), ds[h], dk[e]);
-                }
+            const int e = x % (DP / 32), h = x / (DP / 32);
+            dv[e] = mfma_attn<T>(fa[x & 1], p[h], dv[e]);
+            dk[e] = mfma_attn<T>(fb[x & 1], ds[h], dk[e]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     for (int j = step0; j < steps;) {

@@ -134,7 +134,7 @@ int check_attention_sizes(const ntops_attention_desc& d) {
 int check_attention(const ntops_attention_desc& d) {
     if (const int rc = check_attention_sizes(d)) return rc;
     if (!d.q || (d.k_rows > 0 && (!d.k || !d.v)) || !d.out || !d.workspace) return NTFP8_ERR_NULL;
-    if (!(d.scale > 0.0f) || d.scale > 1e30f) return NTFP8_ERR_UNSUPPORTED;
+    if (!(d.scale >= 1e-30f) || d.scale > 1e30f) return NTFP8_ERR_UNSUPPORTED;
     // (64 rows of a tile lie within 2^31 bytes)
     for (const int64_t v : {d.q_stride, d.k_stride, d.v_stride, d.do_stride})
         if (v < 0 || v > ((int64_t)1 << 24) || v % 8 != 0) return NTFP8_ERR_SIZE;

@@ -593,7 +593,7 @@ Tensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const std::o
         }
     }
     const double scale = scale_ ? *scale_ : 1.0 / std::sqrt((double)dim);
-    TORCH_CHECK_VALUE(scale > 0 && scale <= 1e30, "scale must be positive, got ", scale);
+    TORCH_CHECK_VALUE(scale >= 1e-30 && scale <= 1e30, "scale must be positive (1e-30 to 1e30), got ", scale);
     for (const Tensor* t : {&q, &k, &v}) no_tangent(*t, "attention");
     const bool gq = q.requires_grad(), gk = k.requires_grad(), gv = v.requires_grad();
     if (at::GradMode::is_enabled() && (gq || gk || gv)) return Attention::apply(q, k, v, cu_q, cu_k, causal, scale, gq, gk, gv);
