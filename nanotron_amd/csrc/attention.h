@@ -16,7 +16,7 @@ typedef _Float16 v8h_attn __attribute__((ext_vector_type(8)));
 typedef int v2i_attn __attribute__((ext_vector_type(2)));
 
 constexpr int kAttnStep = 64;               // rows of a tile in LDS
-constexpr int kAttnWaves = 4;
+constexpr int kAttnWaves = 4, kAttnQueries = 32 * kAttnWaves;   // of the kernels that own queries
 constexpr int kAttnKeyWaves = 4, kAttnKeyStep = 32;   // of the kernel that owns keys: its waves, the rows of its tiles of queries, and its keys
 constexpr int kAttnKeys = 32 * kAttnKeyWaves;
 constexpr uint32_t kNowhere = 0xfffffff0u;  // past every descriptor: reads as zeros

@@ -90,11 +90,12 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(const Plan
 }
 
 // ------------------------------------------------------------------------------------------------ prompts
-// A workgroup owns 128 QB queries of one head, a wave 32 QB of them, and walks their keys 64 at a time: scores of 64 keys by 32
+// A workgroup owns 128 queries of one head, a wave 32 of them, and walks their keys 64 at a time: scores of 64 keys by 32
 // queries, the running maximum and sum, and the product with the values, into out^T [elements][queries].  Tiles of keys and
-// values travel straight into LDS, the next pair while this one is worked on.
-template <int T, int DP, int QB>
-__global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_forward_kernel(const AttnArgs A) {
+// values travel straight into LDS.  The scores of the next tile are made while the exponentials of this one are: products and
+// arithmetic then share a wave's time.
+template <int T, int DP>
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(const AttnArgs A) {
     typedef AttnTile<DP> Tile;
     __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * Tile::kBytes];
     __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
     // heads that share keys go to one XCD: workgroups are dealt to the eight in turn
     const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
     const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
-    const AttnTask task = attn_task(A, t, 128 * QB, false);
+    const AttnTask task = attn_task(A, t, kAttnQueries, false);
     if (task.rows <= 0) return;
     const int64_t q0 = attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head;
     const int64_t k0 = attn_rows(A, task.other, task.seq, 0, A.k_stride, A.k_batch) + kv * A.k_head;
@@ -119,136 +120,163 @@ __global__ __launch_bounds__(64 * kAttnWaves, QB == 1 ? 2 : 1) void attention_fo
     typename Tile::template Source<> ks, vs;
     ks.init(A.k, k0, A.k_stride, A.dim, wave, lane);
     vs.init(A.v, v0, A.v_stride, A.dim, wave, lane);
+    if (steps > 0) ks.load(sk, first * kAttnStep, task.len, wave);
+    const int row = wave * 32 + (lane & 31);
+    const bool live = row < task.rows;
+    v4i q[DP / 16];
+    load_own<DP>(q, A.q, q0 + row * A.q_stride, A.dim, live, lane);
+    v16f out[DP / 32], s[2];
+    float top = -__builtin_inff(), sum = 0.0f;   // maximum (of scores times c) and this half wave's sum
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) out[e] = zeros16();
+    auto scores = [&](const uint8_t* keys, v16f (&to)[2]) __attribute__((always_inline)) {
+        to[0] = to[1] = zeros16();
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+            to[0] = mfma_attn<T>(tile.rows(keys, 0, k), q[k], to[0]);
+            to[1] = mfma_attn<T>(tile.rows(keys, 1, k), q[k], to[1]);
+        }
+    };
     if (steps > 0) {
-        ks.load(sk, first * kAttnStep, task.len, wave);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wg_barrier();
+        ks.load(sk + Tile::kBytes, (first + 1) * kAttnStep, task.len, wave);   // (behind the last key: zeros)
         vs.load(sv, first * kAttnStep, task.len, wave);
+        scores(sk, s);
     }
-    const int row0 = wave * 32 * QB + (lane & 31);   // of block 0
-    v4i q[QB][DP / 16];
-    v16f out[QB][DP / 32];
-    float top[QB], sum[QB];   // maximum (of scores times c) and this half wave's sum
+    const int lead = task.shift + wave * 32;                                            // the last key that the wave's first row sees
+    const int last_key = A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1;   // and that this lane's does
+    // a row's maximum of a tile's scores, in two chains
+    auto largest = [&]() __attribute__((always_inline)) {
+        float x = s[0][0], y = s[1][0];
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        const int row = row0 + 32 * b;
-        load_own<DP>(q[b], A.q, q0 + row * A.q_stride, A.dim, row < task.rows, lane);
-        top[b] = -__builtin_inff();
-        sum[b] = 0.0f;
+        for (int r = 1; r < 16; ++r) {
+            x = fmaxf(x, s[0][r]);
+            y = fmaxf(y, s[1][r]);
+        }
+        return both_max(fmaxf(x, y)) * A.c;
+    };
+    // The exponentials are taken below a maximum that is raised only once a row's has grown by more than 2^8 (what is
+    // kept in 16 bits loses nothing by that): rescaling the outputs is 64 multiplications a lane
+    auto raise = [&](float most) __attribute__((always_inline)) {
+        if (__any(most > top + 8.0f)) {
+            const float now = fmaxf(top, most);
+            const float by = now == top ? 1.0f : exp2_fast(top - now);
+            sum *= by;
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e) out[b][e] = zeros16();
-    }
-    // One tile of keys.  kMasked: some rows of the workgroup may not see all of them
-    auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
-        constexpr bool kMasked = decltype(masked_)::value;
-        const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes;
+            for (int e = 0; e < DP / 32; ++e) out[e] *= by;
+            top = now;
+        }
+        return top == -__builtin_inff() ? 0.0f : top;
+    };
+    // exponentials of 4 scores, from register r of block g on
+    auto exponentials = [&](int g, int r, float below) __attribute__((always_inline)) {
+        float x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = s[g][r + i] = exp2_fast(__builtin_fmaf(s[g][r + i], A.c, -below));
+        sum += (x[0] + x[1]) + (x[2] + x[3]);
+    };
+    // One tile of keys that every row of the workgroup sees whole, with another behind it.  A wave issues one instruction after another, so their
+    // order is set here: between two products of 32 cycles each what is done beside them, and fragments read two pairs of products ahead.
+    float most = steps > 0 ? largest() : 0.0f;
+    auto whole_step = [&](int j) __attribute__((always_inline)) {
+        const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes, other = Tile::kBytes - stage;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        wg_barrier();
+        ks.load(sk + stage, key0 + 2 * kAttnStep, task.len, wave);
+        vs.load(sv + other, key0 + kAttnStep, task.len, wave);
+        const float below = raise(most);
+        constexpr int kPairs = DP / 16;   // of products of the next scores
+        v4i fk[3][2], p[4];
+        v16f next[2] = {zeros16(), zeros16()};
+        auto fetch = [&](int k) __attribute__((always_inline)) {
+            fk[k % 3][0] = tile.rows(sk + other, 0, k);
+            fk[k % 3][1] = tile.rows(sk + other, 1, k);
+        };
+        v4i fv[4];
+        auto fetch_v = [&](int x) __attribute__((always_inline)) { fv[x & 3] = tile.columns(sv + stage, x / (DP / 32), x % (DP / 32)); };
+        fetch(0);
+        fetch(1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+            next[0] = mfma_attn<T>(fk[k % 3][0], q[k], next[0]);
+            if (k + 2 < kPairs) fetch(k + 2);
+            else fetch_v(k + 2 - kPairs);
+            // the k-th share of 8 quadruples of exponentials
+#pragma unroll
+            for (int n = k * 8 / kPairs; n < (k + 1) * 8 / kPairs; ++n) exponentials(n / 4, n % 4 * 4, below);
+            __builtin_amdgcn_sched_barrier(0);
+            next[1] = mfma_attn<T>(fk[k % 3][1], q[k], next[1]);
+#pragma unroll
+            for (int n = k * 8 / kPairs; n < (k + 1) * 8 / kPairs; ++n)
+                if (n % 2 == 1) p[n / 2] = pack_scores<T>(s[n / 4], n % 4 == 1 ? 0 : 8);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        s[0] = next[0];
+        s[1] = next[1];
+#pragma unroll
+        for (int x = 0; x < DP / 8; ++x) {
+            if (x + 2 < DP / 8) fetch_v(x + 2);
+            out[x % (DP / 32)] = mfma_attn<T>(fv[x & 3], p[x / (DP / 32)], out[x % (DP / 32)]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        most = largest();
+    };
+    // Any tile: rows that do not see all of it, or nothing behind it
+    auto step = [&](int j) __attribute__((always_inline)) {
+        const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes, other = Tile::kBytes - stage, last = last_key - key0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         wg_barrier();
         if (j + 1 < steps) {
-            ks.load(sk + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
-            vs.load(sv + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
+            ks.load(sk + stage, key0 + 2 * kAttnStep, task.len, wave);
+            vs.load(sv + other, key0 + kAttnStep, task.len, wave);
         }
-        const int lead = task.shift + wave * 32 * QB;   // the last key that the wave's first row sees
-        if (kMasked && A.causal && key0 > lead + 32 * QB - 1) return;   // (uniform in the wave)
-        v16f s[QB][2];
+        if (A.causal && key0 > lead + 31) return;   // (uniform in the wave; so are the tiles behind this one)
 #pragma unroll
-        for (int b = 0; b < QB; ++b) s[b][0] = s[b][1] = zeros16();
+        for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-            const v4i f0 = tile.rows(sk + stage, 0, k), f1 = tile.rows(sk + stage, 1, k);
+            for (int r = 0; r < 16; ++r)
+                if (32 * g + place_of(r, lane) > last) s[g][r] = -__builtin_inff();
+        const float below = raise(largest());
+        v4i p[4];   // of 16 keys each
 #pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                s[b][0] = mfma_attn<T>(f0, q[b][k], s[b][0]);
-                s[b][1] = mfma_attn<T>(f1, q[b][k], s[b][1]);
-            }
+        for (int g = 0; g < 2; ++g) {
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) exponentials(g, r, below);
+            p[2 * g] = pack_scores<T>(s[g], 0);
+            p[2 * g + 1] = pack_scores<T>(s[g], 8);
         }
-        auto last_of = [&](int b) { return (A.causal ? min(task.len - 1, lead + 32 * b + (lane & 31)) : task.len - 1) - key0; };   // the last key of the tile that a row sees
-        if constexpr (kMasked) {
+        if (attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
+            add_columns_singly<T, DP, 4>(out, tile, sv + stage, 0, p, [&](int i) { return i <= last; }, lane);
+        } else {
 #pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                const int last = last_of(b);
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (32 * g + place_of(r, lane) > last) s[b][g][r] = -__builtin_inff();
-            }
+            for (int g = 0; g < 4; ++g) add_columns<T, DP>(out, tile, sv + stage, g, p[g]);
         }
-        v4i p[QB][4];   // of 16 keys each
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            float most = s[b][0][0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) most = fmaxf(most, s[b][0][r]);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][1][r]);
-            most = both_max(most) * A.c;
-            // The exponentials are taken below a maximum that is raised only once a row's has grown by more than 2^8 (what is
-            // kept in 16 bits loses nothing by that): rescaling the outputs is 64 multiplications a lane
-            if (__any(most > top[b] + 8.0f)) {
-                const float now = fmaxf(top[b], most);
-                const float by = now == top[b] ? 1.0f : exp2_fast(top[b] - now);
-                sum[b] *= by;
-#pragma unroll
-                for (int e = 0; e < DP / 32; ++e) out[b][e] *= by;
-                top[b] = now;
-            }
-            const float below = top[b] == -__builtin_inff() ? 0.0f : top[b];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    s[b][g][r] = exp2_fast(__builtin_fmaf(s[b][g][r], A.c, -below));
-                    sum[b] += s[b][g][r];
-                }
-                p[b][2 * g] = pack_scores<T>(s[b][g], 0);
-                p[b][2 * g + 1] = pack_scores<T>(s[b][g], 8);
-            }
-        }
-        if constexpr (kMasked) {
-            if (attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
-#pragma unroll
-                for (int b = 0; b < QB; ++b) {
-                    const int last = last_of(b);
-                    add_columns_singly<T, DP, 4>(out[b], tile, sv + stage, 0, p[b], [&](int i) { return i <= last; }, lane);
-                }
-                return;
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int e = 0; e < DP / 32; ++e) {
-                const v4i f = tile.columns(sv + stage, g, e);
-#pragma unroll
-                for (int b = 0; b < QB; ++b) out[b][e] = mfma_attn<T>(f, p[b][g], out[b][e]);
-            }
+        if (j + 1 < steps) scores(sk + other, s);
     };
-    // tiles that every row sees whole, then the others
-    const int whole = min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, clear = max(0, min(whole - first, steps));
+    // tiles that every row sees whole, then the others and the last
+    const int whole = min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, clear = min(whole - first, steps - 1);
     int j = 0;
-    for (; j < clear; ++j) step(j, std::false_type{});
-    for (; j < steps; ++j) step(j, std::true_type{});
+    for (; j < clear; ++j) whole_step(j);
+    for (; j < steps; ++j) step(j);
+    const float all = both_sum(sum);
+    const int64_t at = (int64_t)task.own + row;
+    if (A.splits > 1) {
+        if (!live) return;
+        const int64_t to = ((int64_t)blockIdx.y * A.q_rows + at) * A.heads + head;
+        if (lane < 32) A.part_ml[to] = make_float2(top, all);
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        const int row = row0 + 32 * b;
-        const bool live = row < task.rows;
-        const float all = both_sum(sum[b]);
-        const int64_t at = (int64_t)task.own + row;
-        if (A.splits > 1) {
-            if (!live) continue;
-            const int64_t to = ((int64_t)blockIdx.y * A.q_rows + at) * A.heads + head;
-            if (lane < 32) A.part_ml[to] = make_float2(top[b], all);
+        for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
-            for (int e = 0; e < DP / 32; ++e)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int d = 32 * e + 8 * g + 4 * (lane >> 5);
-                    if (d < A.dim) *reinterpret_cast<v4f*>(A.part + to * A.dim + d) = (v4f){out[b][e][4 * g], out[b][e][4 * g + 1], out[b][e][4 * g + 2], out[b][e][4 * g + 3]};
-                }
-            continue;
-        }
-        store_rows<T, DP>(out[b], attn_any(all) ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane);
-        if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = attn_lse(A, top[b], all);
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * e + 8 * g + 4 * (lane >> 5);
+                if (d < A.dim) *reinterpret_cast<v4f*>(A.part + to * A.dim + d) = (v4f){out[e][4 * g], out[e][4 * g + 1], out[e][4 * g + 2], out[e][4 * g + 3]};
+            }
+        return;
     }
+    store_rows<T, DP>(out, attn_any(all) ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane);
+    if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = attn_lse(A, top, all);
 }
 
 // ------------------------------------------------------------------------------------------------ few queries
@@ -461,13 +489,12 @@ int run_attention_plan(const int* cu_q, const int* cu_k, int sequences, int q_ro
     return launch_status();
 }
 
-int run_attention_forward_kernels(const AttnArgs& A, int dtype, int q_blocks, bool few, hipStream_t st) {
+int run_attention_forward_kernels(const AttnArgs& A, int dtype, bool few, hipStream_t st) {
     return with_attn(dtype, A.dim, [&](auto t, auto d) {
         constexpr int T = decltype(t)::value, DP = decltype(d)::value;
         const dim3 grid((unsigned)(few ? (int64_t)A.sequences * A.kv_heads : A.tiles * A.heads), (unsigned)A.splits);
         if (few) attention_few_kernel<T, DP><<<grid, 64 * kAttnWaves, 0, st>>>(A);
-        else if (q_blocks == 1) attention_forward_kernel<T, DP, 1><<<grid, 64 * kAttnWaves, 0, st>>>(A);
-        else attention_forward_kernel<T, DP, 2><<<grid, 64 * kAttnWaves, 0, st>>>(A);
+        else attention_forward_kernel<T, DP><<<grid, 64 * kAttnWaves, 0, st>>>(A);
         if (const int rc = launch_status(); rc != NTFP8_OK || A.splits <= 1) return rc;
         attention_join_kernel<T><<<(unsigned)((A.q_rows * A.heads + 3) / 4), 256, 0, st>>>(A);
         return launch_status();

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
     const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
-    const AttnTask task = attn_task(A, t, 128, false);
+    const AttnTask task = attn_task(A, t, kAttnQueries, false);
     if (task.rows <= 0) return;
     const int64_t k0 = attn_rows(A, task.other, task.seq, 0, A.k_stride, A.k_batch) + kv * A.k_head;
     const int64_t v0 = attn_rows(A, task.other, task.seq, 0, A.v_stride, A.v_batch) + kv * A.v_head;

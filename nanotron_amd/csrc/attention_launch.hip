@@ -5,7 +5,7 @@ namespace ntfp8 {
 
 int run_attention_plan(const int* cu_q, const int* cu_k, int sequences, int q_rows, int k_rows, int causal, int q_tile, int k_tile, int q_tasks, int k_tasks,
                        AttnTask* q_list, AttnTask* k_list, hipStream_t st);
-int run_attention_forward_kernels(const AttnArgs& A, int dtype, int q_blocks, bool few, hipStream_t st);
+int run_attention_forward_kernels(const AttnArgs& A, int dtype, bool few, hipStream_t st);
 int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, int64_t k_tiles, const int* cu_q, const int* cu_k, int dtype, hipStream_t st);
 
 namespace {
@@ -19,7 +19,7 @@ int64_t tiles_of(const ntops_attention_desc& d, int64_t rows, int64_t tile) {
 
 struct Choice {
     bool few;
-    int q_blocks, splits;
+    int splits;
     int64_t tiles;
 };
 Choice choose(const ntops_attention_desc& d) {
@@ -32,8 +32,7 @@ Choice choose(const ntops_attention_desc& d) {
         c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len / 256));
         return c;
     }
-    c.q_blocks = 1;
-    c.tiles = tiles_of(d, d.q_rows, 128 * c.q_blocks);
+    c.tiles = tiles_of(d, d.q_rows, kAttnQueries);
     const int64_t groups = c.tiles * d.heads, room = 2 * cus;
     if (groups < room) c.splits = (int)std::max<int64_t>(1, std::min(room / groups, k_len / 512));
     return c;
@@ -92,12 +91,12 @@ AttnArgs args_of(const ntops_attention_desc& d) {
 // What a launch has to hold: workgroups, and threads, in 32 bits
 bool attention_fits(const ntops_attention_desc& d) {
     constexpr int64_t kMost = (int64_t)1 << 23;
-    return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, 128) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
+    return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
 }
 
 int64_t attention_workspace(const ntops_attention_desc& d, bool backward) {
     const Choice c = choose(d);
-    return layout_of(d, backward, c, backward ? tiles_of(d, d.q_rows, 128) : c.tiles, tiles_of(d, d.k_rows, kAttnKeys)).bytes;
+    return layout_of(d, backward, c, backward ? tiles_of(d, d.q_rows, kAttnQueries) : c.tiles, tiles_of(d, d.k_rows, kAttnKeys)).bytes;
 }
 
 int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
@@ -110,14 +109,14 @@ int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
     if (d.cu_q) {
         AttnTask* const list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
         a.tasks = list;
-        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, 128 * c.q_blocks, 0, (int)c.tiles, 0, list, nullptr, st)) return rc;
+        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, kAttnQueries, 0, (int)c.tiles, 0, list, nullptr, st)) return rc;
     }
-    return run_attention_forward_kernels(a, d.dtype, c.q_blocks, c.few, st);
+    return run_attention_forward_kernels(a, d.dtype, c.few, st);
 }
 
 int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
     AttnArgs a = args_of(d);
-    a.tiles = tiles_of(d, d.q_rows, 128);
+    a.tiles = tiles_of(d, d.q_rows, kAttnQueries);
     const int64_t k_tiles = tiles_of(d, d.k_rows, kAttnKeys);
     const Layout l = layout_of(d, true, {}, a.tiles, k_tiles);
     char* const ws = static_cast<char*>(d.workspace);
@@ -128,7 +127,7 @@ int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
         AttnTask* const q_list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
         k_list = reinterpret_cast<AttnTask*>(ws + l.k_tasks);
         a.tasks = q_list;
-        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, 128, kAttnKeys, (int)a.tiles, (int)k_tiles, q_list, k_list, st)) return rc;
+        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, kAttnQueries, kAttnKeys, (int)a.tiles, (int)k_tiles, q_list, k_list, st)) return rc;
     }
     return run_attention_backward_kernels(a, k_list, k_tiles, d.cu_q, d.cu_k, d.dtype, st);
 }
