@@ -147,18 +147,20 @@ struct AttnTile {
         const v2i_attn b = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&stage[hi]));
         return (v4i){a.x, a.y, b.x, b.y};
     }
-    // The same of the stage that begins at byte `at` of an array, for kernels without registers to keep each fragment's address in: one
-    // exclusive or a read, which the compiler is kept from doing once and for all
+    // The same of the stage that begins at byte `at` of an array, for kernels without registers to keep each fragment's address in: an
+    // exclusive or and an addition a read, which the compiler is kept from doing once and for all
     __device__ __forceinline__ v4i rows_anew(const uint8_t* array, int at, int b, int k) const {
-        int off = (at + plain + plain_turn) ^ (k << 5);
+        int off = (plain + plain_turn) ^ (k << 5);
         asm volatile("" : "+v"(off));
+        off += at;
         return *reinterpret_cast<const v4i*>(array + off + b * 32 * kPitch);
     }
     __device__ __forceinline__ v4i columns_anew(uint8_t* array, int at, int s, int e) const {
         typedef short v4s __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) v4s* tr_ptr;
-        int lo = (at + across + across_turn) ^ (e << 6);
+        int lo = (across + across_turn) ^ (e << 6);
         asm volatile("" : "+v"(lo));
+        lo += at;
         int hi = lo ^ 16;
         asm volatile("" : "+v"(hi));
         const v2i_attn a = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)&array[lo + s * 16 * kPitch]));
@@ -208,28 +210,54 @@ __device__ __forceinline__ void add_columns(v16f (&acc)[DP / 32], const AttnTile
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) acc[e] = mfma_attn<T>(tile.columns(stage, s, e), scores, acc[e]);
 }
-// The same over 16 kScores rows, from 16 s0 on, of a stage that holds values which are not finite, under a mask: a score of zero times such a value would
+// The same over the 16 kScores rows of a stage that holds values which are not finite, under a mask: a score of zero times such a value would
 // reach the rows that do not count it (a padded row, a token to come), so the stage's rows go one at a time, and only into the
-// rows that count them: `counts(i)`, this lane's row counts row i.
-template <int T, int DP, int kScores, typename Tile, typename F>
-__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const Tile& tile, uint8_t* stage, int s0, const v4i (&scores)[kScores], F&& counts, int lane) {
+// rows that count them: this lane's row counts the rows from .. to - 1.  A function of its own, which finds the sums in memory: beside the loops of
+// the kernels it would take the registers that they live from (240 of 256 in the forward pass with it, 102 spilled, 450 TFLOP/s for 990).
+template <int DP, int kScores>
+struct AttnSingly {
+    v16f acc[DP / 32];
+    v4i scores[kScores];
+};
+template <int T, int DP, int kScores, int kRows>
+__device__ __attribute__((noinline)) void attn_add_singly(AttnSingly<DP, kScores>* w, uint32_t stage, int from, int to) {
+    typedef short v4s __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) v4s* tr_ptr;
+    typedef AttnTile<DP, kRows> Tile;
+    const int lane = threadIdx.x & 63;
+    Tile tile;
+    tile.init(lane);
 #pragma unroll 1
-    for (int i = 0; i < 16 * kScores; ++i) {
-        const int s = i >> 4, j = (i & 3) + ((i >> 3) & 1) * 4;   // its place in the fragments of half wave (i >> 2) & 1
-        const bool mine = (lane >> 5) == ((i >> 2) & 1), take = counts(16 * s0 + i);
-        v4i c = {0, 0, 0, 0};
+    for (int e = 0; e < DP / 32; ++e) {
+        v16f acc = w->acc[e];
+#pragma unroll 1
+        for (int i = 0; i < 16 * kScores; ++i) {
+            const int s = i >> 4, j = (i & 3) + ((i >> 3) & 1) * 4;   // its place in the fragments of half wave (i >> 2) & 1
+            const bool mine = (lane >> 5) == ((i >> 2) & 1), take = i >= from && i < to;
+            const uint32_t lo = stage + ((tile.across + tile.across_turn) ^ (e << 6)) + s * 16 * Tile::kPitch;
+            const uint32_t hi = stage + ((tile.across + tile.across_turn) ^ (e << 6) ^ 16) + (s * 16 + 8) * Tile::kPitch;
+            const v2i_attn a = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(uintptr_t)lo));
+            const v2i_attn b = __builtin_bit_cast(v2i_attn, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr)(uintptr_t)hi));
+            v4i f = {a.x, a.y, b.x, b.y};
 #pragma unroll
-        for (int k = 0; k < kScores; ++k) c |= scores[k] & (s == k ? -1 : 0);   // (a choice of one of them would put them all into memory)
+            for (int k = 0; k < 4; ++k) f[k] = mine && (j >> 1) == k ? (j & 1 ? f[k] & (int)0xffff0000 : f[k] & 0xffff) : 0;
+            const v16f d = mfma_attn<T>(f, w->scores[s], zeros16());
 #pragma unroll
-        for (int e = 0; e < DP / 32; ++e) {
-            v4i f = tile.columns(stage, s0 + s, e);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) f[w] = mine && (j >> 1) == w ? (j & 1 ? f[w] & (int)0xffff0000 : f[w] & 0xffff) : 0;
-            const v16f d = mfma_attn<T>(f, c, zeros16());
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[e][r] += take ? d[r] : 0.0f;
+            for (int r = 0; r < 16; ++r) acc[r] += take ? d[r] : 0.0f;
         }
+        w->acc[e] = acc;
     }
+}
+template <int T, int DP, int kScores, typename Tile>
+__device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const Tile&, uint8_t* stage, const v4i (&scores)[kScores], int from, int to) {
+    AttnSingly<DP, kScores> w;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) w.acc[e] = acc[e];
+#pragma unroll
+    for (int k = 0; k < kScores; ++k) w.scores[k] = scores[k];
+    attn_add_singly<T, DP, kScores, Tile::kBytes / Tile::kPitch>(&w, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)stage, from, to);
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) acc[e] = w.acc[e];
 }
 
 // acc * factor as one row a lane, rounded to T: 16 bytes a lane and store.  p: the row's first element

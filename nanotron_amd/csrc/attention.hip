@@ -248,7 +248,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(c
             p[2 * g + 1] = pack_scores<T>(s[g], 8);
         }
         if (attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
-            add_columns_singly<T, DP, 4>(out, tile, sv + stage, 0, p, [&](int i) { return i <= last; }, lane);
+            add_columns_singly<T, DP, 4>(out, tile, sv + stage, p, 0, last + 1);
         } else {
 #pragma unroll
             for (int g = 0; g < 4; ++g) add_columns<T, DP>(out, tile, sv + stage, g, p[g]);
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         }
         const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)};
         if (masked && attn_not_finite<T, DP>(v, kFewStep, lane)) {
-            add_columns_singly<T, DP, 2>(out, tile, v, 0, p, [&](int i) { return i <= last; }, lane);
+            add_columns_singly<T, DP, 2>(out, tile, v, p, 0, last + 1);
         } else {
             add_columns<T, DP>(out, tile, v, 0, p[0]);
             add_columns<T, DP>(out, tile, v, 1, p[1]);

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
         }
         if constexpr (kMasked) {
             if (attn_not_finite<T, DP>(sk + stage, kAttnStep, lane)) {
-                add_columns_singly<T, DP, 4>(dq, tile, sk + stage, 0, p, [&](int i) { return i <= last; }, lane);
+                add_columns_singly<T, DP, 4>(dq, tile, sk + stage, p, 0, last + 1);
                 return;
             }
         }
@@ -206,8 +206,7 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
         if (kMasked && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
         const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
-        // s and d begin at what is subtracted from them.  Fragments are read one product ahead: held back by the registers that they take,
-        // the compiler reads each in front of its product and waits, 0.39 of the MFMA slots used instead of XX
+        // s and d begin at what is subtracted from them
         v16f s, d;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -218,60 +217,69 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
                 d[4 * n + i] = y[i];
             }
         }
-        {
-            v4i fq[2], fg[2], fv[2];
-            auto fetch = [&](int i) {
-                fq[i & 1] = tile.rows_anew(sq, at, 0, i);
-                fg[i & 1] = tile.rows_anew(sg, at, 0, i);
-                fv[i & 1] = tile.rows_anew(sv, mine, 0, i);
-            };
-            fetch(0);
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                if (i + 1 < DP / 16) fetch(i + 1);
-                __builtin_amdgcn_sched_barrier(0);
-                s = mfma_attn<T>(fq[i & 1], k[i], s);
-                d = mfma_attn<T>(fg[i & 1], fv[i & 1], d);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        }
-        v4i fa[2], fb[2];
-        auto fetch = [&](int x) {   // of the products with rows 16 (x / (DP / 32)) .., elements 32 (x mod (DP / 32)) ..
-            fa[x & 1] = tile.columns_anew(sg, at, x / (DP / 32), x % (DP / 32));
-            fb[x & 1] = tile.columns_anew(sq, at, x / (DP / 32), x % (DP / 32));
+        // Four runs of products: scores, dout v^T, dv and dk.  Beside the second go the exponentials, beside the third what ds is made of; the
+        // fragments are read two products ahead.  A wave issues one instruction after another, so their order is set here.
+        constexpr int kProducts = DP / 16;   // of a run
+        v4i fq[3], fg[2], fv[2], p[2], ds[2];
+        auto fetch_q = [&](int i) __attribute__((always_inline)) { fq[i % 3] = tile.rows_anew(sq, at, 0, i); };
+        auto fetch_g = [&](int i) __attribute__((always_inline)) {
+            fg[i & 1] = tile.rows_anew(sg, at, 0, i);
+            fv[i & 1] = tile.rows_anew(sv, mine, 0, i);
         };
-        fetch(0);
-        __builtin_amdgcn_sched_barrier(0);
+        fetch_q(0);
+        fetch_q(1);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = exp2_fast(s[r] * A.c);
-            d[r] = T == NTFP8_F16 ? s[r] * (d[r] * down) : s[r] * d[r];
+        for (int i = 0; i < kProducts; ++i) {
+            if (i + 2 < kProducts) fetch_q(i + 2);
+            if (i + 1 == kProducts) fetch_g(0);
+            s = mfma_attn<T>(fq[i % 3], k[i], s);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (kMasked) {
+        auto counted = [&](float x, int r) __attribute__((always_inline)) {
+            if constexpr (!kMasked) return x;
+            const int i = place_of(r, lane);
+            return i >= from && i < to ? x : 0.0f;
+        };
+        v4i fa[3];
+        // fragment x of the products for dv, and those for dk behind them
+        auto fetch_a = [&](int x) __attribute__((always_inline)) { fa[x % 3] = tile.columns_anew(x < kProducts ? sg : sq, at, x % kProducts / (DP / 32), x % (DP / 32)); };
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = place_of(r, lane);
-                const bool in = i >= from && i < to;
-                s[r] = in ? s[r] : 0.0f;
-                d[r] = in ? d[r] : 0.0f;
+        for (int i = 0; i < kProducts; ++i) {
+            if (i + 1 < kProducts) fetch_g(i + 1);
+            if (i + 2 >= kProducts) fetch_a(i + 2 - kProducts);
+            d = mfma_attn<T>(fg[i & 1], fv[i & 1], d);
+#pragma unroll
+            for (int r = i * 16 / kProducts; r < (i + 1) * 16 / kProducts; ++r) {
+                s[r] = counted(exp2_fast(s[r] * A.c), r);
+                if (r % 8 == 7) p[r / 8] = pack_scores<T>(s, r - 7);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)}, ds[2] = {pack_scores<T>(d, 0), pack_scores<T>(d, 8)};
+        auto gradient = [&](int r) __attribute__((always_inline)) {
+            d[r] = counted(T == NTFP8_F16 ? s[r] * (d[r] * down) : s[r] * d[r], r);
+            if (r % 8 == 7) ds[r / 8] = pack_scores<T>(d, r - 7);
+        };
         if constexpr (kMasked) {
             if (attn_not_finite<T, DP>(ga, kAttnKeyStep, lane) || attn_not_finite<T, DP>(qa, kAttnKeyStep, lane)) {
-                const auto counts = [&](int i) { return i >= from && i < to; };
-                add_columns_singly<T, DP, 2>(dv, tile, ga, 0, p, counts, lane);
-                add_columns_singly<T, DP, 2>(dk, tile, qa, 0, ds, counts, lane);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) gradient(r);
+                add_columns_singly<T, DP, 2>(dv, tile, ga, p, from, to);
+                add_columns_singly<T, DP, 2>(dk, tile, qa, ds, from, to);
                 return;
             }
         }
 #pragma unroll
-        for (int x = 0; x < DP / 16; ++x) {
-            if (x + 1 < DP / 16) fetch(x + 1);
+        for (int x = 0; x < kProducts; ++x) {
+            fetch_a(x + 2);
+            dv[x % (DP / 32)] = mfma_attn<T>(fa[x % 3], p[x / (DP / 32)], dv[x % (DP / 32)]);
+#pragma unroll
+            for (int r = x * 16 / kProducts; r < (x + 1) * 16 / kProducts; ++r) gradient(r);
             __builtin_amdgcn_sched_barrier(0);
-            const int e = x % (DP / 32), h = x / (DP / 32);
-            dv[e] = mfma_attn<T>(fa[x & 1], p[h], dv[e]);
-            dk[e] = mfma_attn<T>(fb[x & 1], ds[h], dk[e]);
+        }
+#pragma unroll
+        for (int x = 0; x < kProducts; ++x) {
+            if (x + 2 < kProducts) fetch_a(kProducts + x + 2);
+            dk[x % (DP / 32)] = mfma_attn<T>(fa[(kProducts + x) % 3], ds[x / (DP / 32)], dk[x % (DP / 32)]);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
