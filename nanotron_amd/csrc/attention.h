@@ -20,7 +20,7 @@ constexpr int kAttnWaves = 4, kAttnQueries = 32 * kAttnWaves;   // of the kernel
 constexpr int kAttnKeyWaves = 4, kAttnKeyStep = 32;   // of the kernel that owns keys: its waves, the rows of its tiles of queries, and its keys
 constexpr int kAttnKeys = 32 * kAttnKeyWaves;
 constexpr uint32_t kNowhere = 0xfffffff0u;  // past every descriptor: reads as zeros
-constexpr int kMostLine = 32;                // words from one of AttnArgs::most to the next
+constexpr int kAttnMost = 1024;             // workgroups that look for the largest magnitudes, of dout and of v
 constexpr float kLog2E = 1.44269504088896340736f;
 
 // A run of rows of one sequence that a workgroup owns, and the other side's rows that belong to it
@@ -48,7 +48,8 @@ struct AttnArgs {
     const void* o;     // backward: the output of the forward pass
     float* lse;        // [heads][q_rows] minus the logarithm of a row's sum of exponentials, in units of q k^T; minus infinity for a row that sees nothing
     float* delta;      // [heads][q_rows] minus the sum of dout out
-    uint32_t* most;    // fp16 gradients: bits of the largest magnitudes in dout and v, [2][64] a line each
+    uint32_t* most;    // fp16 gradients: bits of the largest magnitudes in dout and v, of each workgroup that looked, [2][kAttnMost]
+    int most_q, most_v;   // and how many looked
     void *dq, *dk, *dv;
     int splits;        // runs that the keys of a tile are cut into ...
     float* part;       // ... and their results before they are joined: [split][q_rows][heads][dim], then

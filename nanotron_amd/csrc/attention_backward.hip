@@ -15,59 +15,64 @@ constexpr float kLiftP = 8.0f;
 template <int T>
 __device__ __forceinline__ float gradient_lift(const AttnArgs& A) {
     if constexpr (T == NTFP8_BF16) return 1.0f;
-    const uint32_t* const at = A.most + (threadIdx.x & 63) * kMostLine;
-    const float most = 2.0f * A.dim * __uint_as_float(wave_most(at[0])) * __uint_as_float(wave_most(at[64 * kMostLine]));
+    uint32_t q = 0, v = 0;
+    for (int i = threadIdx.x & 63; i < A.most_q; i += 64) q = max(q, A.most[i]);
+    for (int i = threadIdx.x & 63; i < A.most_v; i += 64) v = max(v, A.most[kAttnMost + i]);
+    const float most = 2.0f * A.dim * __uint_as_float(wave_most(q)) * __uint_as_float(wave_most(v));
     if (!(most > 0.0f) || most > 1e30f || most < 1e-30f) return 1.0f;
     const int e = (int)(__float_as_uint(most) >> 23) - 127;   // 2^e <= most < 2^(e + 1)
     return __uint_as_float((uint32_t)(127 + 14 - e) << 23);
 }
 
-__global__ void attention_clear_kernel(uint32_t* p) { p[threadIdx.x * kMostLine] = 0u; }
-
-// delta, 16 lanes a row; blocks behind those of the rows of dout read v, for its largest magnitude
+// delta, 16 lanes a row; the workgroups behind the first q_groups read v, for its largest magnitude.  Each leaves what it found in a place of
+// its own: no atomics, and nothing to clear before
 template <int T>
-__global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, const int* cu_q, const int* cu_k, int64_t q_blocks) {
-    const bool values = blockIdx.x >= q_blocks;
-    const int64_t item = ((int64_t)(values ? blockIdx.x - q_blocks : blockIdx.x) * 256 + threadIdx.x) >> 4;
+__global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, const int* cu_q, const int* cu_k, int q_groups) {
+    __shared__ uint32_t found[4];
+    const bool values = (int)blockIdx.x >= q_groups;
+    const int own = values ? blockIdx.x - q_groups : blockIdx.x, groups = values ? gridDim.x - q_groups : q_groups;
     const int heads = values ? A.kv_heads : A.heads, own_len = values ? A.k_len : A.q_len;
-    const int64_t rows = values ? A.k_rows : A.q_rows, row = item / heads;
-    const int head = (int)(item - row * heads), d = (threadIdx.x & 15) * 8;
+    const int64_t rows = values ? A.k_rows : A.q_rows;
+    const int d = (threadIdx.x & 15) * 8;
     const int* const cu = values ? cu_k : cu_q;
-    bool live = row < rows;
-    if (live && cu) live = row >= cu[0] && row < cu[A.sequences];   // rows of no sequence may hold anything
-    float x[8] = {}, y[8] = {}, sum = 0.0f;
-    if (live && d < A.dim) {
-        const int seq = A.tasks ? 0 : (int)(row / own_len);
-        const int64_t at = A.tasks ? row : row - (int64_t)seq * own_len;
-        const int64_t stride = values ? A.v_stride : A.do_stride, batch = values ? A.v_batch : A.do_batch, apart = values ? A.v_head : A.do_head;
-        unpack<T, 8>(load_piece<T, 8>(values ? A.v : A.dout, seq * batch + at * stride + head * apart + d), x);
-        if (!values) unpack<T, 8>(load_piece<T, 8>(A.o, (row * heads + head) * A.dim + d), y);
-    }
     uint32_t most = 0;
+    for (int64_t item = (int64_t)own * 16 + (threadIdx.x >> 4); item < rows * heads; item += (int64_t)groups * 16) {
+        const int64_t row = item / heads;
+        const int head = (int)(item - row * heads);
+        const bool live = !cu || (row >= cu[0] && row < cu[A.sequences]);   // rows of no sequence may hold anything
+        float x[8] = {}, y[8] = {}, sum = 0.0f;
+        if (live && d < A.dim) {
+            const int seq = A.tasks ? 0 : (int)(row / own_len);
+            const int64_t at = A.tasks ? row : row - (int64_t)seq * own_len;
+            const int64_t stride = values ? A.v_stride : A.do_stride, batch = values ? A.v_batch : A.do_batch, apart = values ? A.v_head : A.do_head;
+            unpack<T, 8>(load_piece<T, 8>(values ? A.v : A.dout, seq * batch + at * stride + head * apart + d), x);
+            if (!values) unpack<T, 8>(load_piece<T, 8>(A.o, (row * heads + head) * A.dim + d), y);
+        }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        sum += x[i] * y[i];
-        const uint32_t size = __float_as_uint(x[i]) & 0x7fffffffu;
-        most = max(most, size < kInfBits ? size : 0u);   // (what is not finite spoils its own sequence, whatever the others are lifted by)
+        for (int i = 0; i < 8; ++i) {
+            sum += x[i] * y[i];
+            const uint32_t size = __float_as_uint(x[i]) & 0x7fffffffu;
+            most = max(most, size < kInfBits ? size : 0u);   // (what is not finite spoils its own sequence, whatever the others are lifted by)
+        }
+#pragma unroll
+        for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
+        if (!values && d == 0) A.delta[head * A.q_rows + row] = live ? -sum : 0.0f;
     }
-#pragma unroll
-    for (int m = 1; m < 16; m *= 2) sum += __shfl_xor(sum, m);
-    if (!values && row < rows && d == 0) A.delta[head * A.q_rows + row] = live ? -sum : 0.0f;
     if constexpr (T == NTFP8_F16) {
-        // (a maximum: the order changes nothing.  64 lines, or the blocks' atomics wait for each other: 56 us for 36000 rows on one, 8 so)
         most = wave_most(most);
-        if ((threadIdx.x & 63) == 0 && most) atomicMax(&A.most[((values ? 64 : 0) + blockIdx.x % 64) * kMostLine], most);
+        if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = most;
+        __syncthreads();
+        if (threadIdx.x == 0) A.most[(values ? kAttnMost : 0) + own] = max(max(found[0], found[1]), max(found[2], found[3]));
     }
 }
 
 // dq of 128 queries of one head, 32 a wave
 template <int T, int DP>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const AttnArgs A) {
+__device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8_t* lds) {
     typedef AttnTile<DP> Tile;
-    __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * Tile::kBytes];
-    __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];
+    uint8_t *const sk = lds, *const sv = lds + 2 * Tile::kBytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
+    const int t = group / A.heads, pick = group - t * A.heads;
     const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
     const AttnTask task = attn_task(A, t, kAttnQueries, false);
     if (task.rows <= 0) return;
@@ -107,32 +112,66 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
         const int lead = task.shift + wave * 32;   // the last key that the wave's first row sees
         if (kMasked && A.causal && key0 > lead + 31) return;   // (uniform in the wave)
         const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0;
-        v4i p[4];
+        // Runs of products, of two blocks of 32 keys: scores and dout v^T of the one, of the other, then dq; beside each the arithmetic of the run
+        // before.  Fragments are read two products ahead.
+        constexpr int kProducts = DP / 16;   // of a run
+        v16f s[2], d[2];
+        v4i p[4], f[3];
+        // fragment x of the runs: keys, values, keys, values of the two blocks, then columns of the keys
+        auto fetch = [&](int x) __attribute__((always_inline)) {
+            const int run = x / kProducts, i = x % kProducts;
+            if (run < 4) f[x % 3] = tile.rows(run & 1 ? sv + stage : sk + stage, run >> 1, i);
+            else f[x % 3] = tile.columns(sk + stage, (x - 4 * kProducts) / (DP / 32), (x - 4 * kProducts) % (DP / 32));
+        };
+        auto run = [&](int which, auto&& beside) __attribute__((always_inline)) {
+            const int b = which >> 1;
+            v16f& to = which & 1 ? d[b] : s[b];
+            to = zeros16();
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            v16f s = zeros16(), d = zeros16();
+            for (int i = 0; i < kProducts; ++i) {
+                const int x = which * kProducts + i;
+                if (!kMasked || x + 2 < 4 * kProducts) fetch(x + 2);
+                to = mfma_attn<T>(f[x % 3], which & 1 ? g[i] : q[i], to);
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                s = mfma_attn<T>(tile.rows(sk + stage, b, k), q[k], s);
-                d = mfma_attn<T>(tile.rows(sv + stage, b, k), g[k], d);
+                for (int r = i * 16 / kProducts; r < (i + 1) * 16 / kProducts; ++r) beside(r);
+                __builtin_amdgcn_sched_barrier(0);
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(__builtin_fmaf(s[r], A.c, lse)) * ((d[r] + delta) * lift);
-            if constexpr (kMasked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = 32 * b + place_of(r, lane) > last ? 0.0f : s[r];
-            }
-            p[2 * b] = pack_scores<T>(s, 0);
-            p[2 * b + 1] = pack_scores<T>(s, 8);
-        }
+        };
+        auto exponential = [&](int b, int r) __attribute__((always_inline)) { s[b][r] = exp2_fast(__builtin_fmaf(s[b][r], A.c, lse)); };
+        auto gradient = [&](int b, int r) __attribute__((always_inline)) {
+            d[b][r] = s[b][r] * ((d[b][r] + delta) * lift);
+            if (kMasked && 32 * b + place_of(r, lane) > last) d[b][r] = 0.0f;
+            if (r % 8 == 7) p[2 * b + r / 8] = pack_scores<T>(d[b], r - 7);
+        };
+        fetch(0);
+        fetch(1);
+        run(0, [](int) {});
+        run(1, [&](int r) __attribute__((always_inline)) { exponential(0, r); });
+        run(2, [&](int r) __attribute__((always_inline)) { gradient(0, r); });
+        run(3, [&](int r) __attribute__((always_inline)) { exponential(1, r); });
         if constexpr (kMasked) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) gradient(1, r);
             if (attn_not_finite<T, DP>(sk + stage, kAttnStep, lane)) {
                 add_columns_singly<T, DP, 4>(dq, tile, sk + stage, p, 0, last + 1);
                 return;
             }
+            fetch(4 * kProducts);
+            fetch(4 * kProducts + 1);
         }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) add_columns<T, DP>(dq, tile, sk + stage, s, p[s]);
+        for (int i = 0; i < 2 * kProducts; ++i) {
+            const int x = 4 * kProducts + i;
+            if (i + 2 < 2 * kProducts) fetch(x + 2);
+            dq[i % (DP / 32)] = mfma_attn<T>(f[x % 3], p[i / (DP / 32)], dq[i % (DP / 32)]);
+            if constexpr (!kMasked) {
+                if (i < kProducts) {
+#pragma unroll
+                    for (int r = i * 16 / kProducts; r < (i + 1) * 16 / kProducts; ++r) gradient(1, r);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     // tiles that every row sees whole, then the others
     const int clear = max(0, min(min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, steps));
@@ -145,14 +184,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_dq_kernel(const 
 // dk and dv of 256 keys of one head of keys, 32 a wave: over the heads of queries that share it, and their queries 64 at a time.  A wave holds
 // its keys and both sums in registers, 160 of the 256 that two waves a SIMD have; its values stay in LDS.
 template <int T, int DP>
-__global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(const AttnArgs A) {
+__device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint8_t* lds) {
     typedef AttnTile<DP, kAttnKeyStep> Tile;
-    __shared__ __attribute__((aligned(1024))) uint8_t sq[2 * Tile::kBytes];
-    __shared__ __attribute__((aligned(1024))) uint8_t sg[2 * Tile::kBytes];
-    __shared__ __attribute__((aligned(1024))) uint8_t sv[kAttnKeys / kAttnKeyStep * Tile::kBytes];
-    __shared__ __attribute__((aligned(1024))) float rows_of[2][2][64];   // lse and delta (a wave loads 64)
+    uint8_t *const sq = lds, *const sg = lds + 2 * Tile::kBytes, *const sv = lds + 4 * Tile::kBytes;
+    float(*const rows_of)[2][64] = reinterpret_cast<float(*)[2][64]>(sv + kAttnKeys / kAttnKeyStep * Tile::kBytes);   // [stage]: lse and delta (a wave loads 64)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int run = blockIdx.x / A.kv_heads, kv = blockIdx.x - run * A.kv_heads, t = run / A.k_splits, split = run - t * A.k_splits;
+    const int run = group / A.kv_heads, kv = group - run * A.kv_heads, t = run / A.k_splits, split = run - t * A.k_splits;
     const AttnTask task = attn_task(A, t, kAttnKeys, true);
     if (task.rows <= 0) return;
     const int begin = A.causal ? max(0, task.shift) / kAttnKeyStep : 0, per = max(0, (task.len + kAttnKeyStep - 1) / kAttnKeyStep - begin);
@@ -315,6 +352,21 @@ __global__ __launch_bounds__(64 * kAttnKeyWaves, 2) void attention_dkv_kernel(co
     if (A.dk) store_rows<T, DP>(dk, dk_by, A.dk, to, A.dim, live, lane);
 }
 
+// Both in one launch, the workgroups of keys first: they have more to do each, and those of queries fill what they leave of the chip
+template <int T, int DP>
+__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_backward_kernel(const AttnArgs A, const AttnTask* k_tasks, int k_groups) {
+    static_assert(kAttnWaves == kAttnKeyWaves, "");
+    constexpr int kKeys = (4 + kAttnKeys / kAttnKeyStep) * AttnTile<DP, kAttnKeyStep>::kBytes + 1024, kQueries = 4 * AttnTile<DP>::kBytes;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeys > kQueries ? kKeys : kQueries];
+    if ((int)blockIdx.x < k_groups) {
+        AttnArgs K = A;
+        K.tasks = k_tasks;
+        attention_dkv<T, DP>(K, blockIdx.x, lds);
+    } else {
+        attention_dq<T, DP>(A, blockIdx.x - k_groups, lds);
+    }
+}
+
 // The runs' sums added up, in their order: 8 elements a thread, dk and dv side by side
 template <int T>
 __global__ __launch_bounds__(256) void attention_add_kernel(const AttnArgs A) {
@@ -339,25 +391,18 @@ __global__ __launch_bounds__(256) void attention_add_kernel(const AttnArgs A) {
 int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, int64_t k_tiles, const int* cu_q, const int* cu_k, int dtype, hipStream_t st) {
     return with_attn(dtype, A.dim, [&](auto t, auto d) {
         constexpr int T = decltype(t)::value, DP = decltype(d)::value;
-        const int64_t q_blocks = (A.q_rows * A.heads + 15) / 16, v_blocks = T == NTFP8_F16 ? (A.k_rows * A.kv_heads + 15) / 16 : 0;
-        if (T == NTFP8_F16) {
-            attention_clear_kernel<<<1, 128, 0, st>>>(A.most);
-            if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
-        }
-        attention_delta_kernel<T><<<(unsigned)(q_blocks + v_blocks), 256, 0, st>>>(A, cu_q, cu_k, q_blocks);
+        AttnArgs B = A;
+        const int64_t q_groups = (A.q_rows * A.heads + 15) / 16, v_groups = (A.k_rows * A.kv_heads + 15) / 16;
+        if (T == NTFP8_F16) B.most_q = (int)std::min<int64_t>(q_groups, kAttnMost), B.most_v = (int)std::min<int64_t>(v_groups, kAttnMost);
+        const int first = T == NTFP8_F16 ? B.most_q : (int)q_groups;
+        attention_delta_kernel<T><<<(unsigned)(first + B.most_v), 256, 0, st>>>(B, cu_q, cu_k, first);
         if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
-        if (A.dk || A.dv) {
-            AttnArgs K = A;
-            K.tasks = k_tasks;
-            attention_dkv_kernel<T, DP><<<(unsigned)(k_tiles * A.kv_heads * A.k_splits), 64 * kAttnKeyWaves, 0, st>>>(K);
-            if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
-            if (A.k_splits > 1) {
-                attention_add_kernel<T><<<dim3((unsigned)((A.k_rows * A.kv_heads * A.dim + 2047) / 2048), 2), 256, 0, st>>>(A);
-                if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
-            }
-        }
-        if (A.dq) {
-            attention_dq_kernel<T, DP><<<(unsigned)(A.tiles * A.heads), 64 * kAttnWaves, 0, st>>>(A);
+        const bool keys = A.dk || A.dv;
+        const int64_t k_groups = keys ? k_tiles * A.kv_heads * A.k_splits : 0;
+        attention_backward_kernel<T, DP><<<(unsigned)(k_groups + (A.dq ? A.tiles * A.heads : 0)), 64 * kAttnWaves, 0, st>>>(B, k_tasks, (int)k_groups);
+        if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
+        if (keys && A.k_splits > 1) {
+            attention_add_kernel<T><<<dim3((unsigned)((A.k_rows * A.kv_heads * A.dim + 2047) / 2048), 2), 256, 0, st>>>(A);
             if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
         }
         return (int)NTFP8_OK;

@@ -61,7 +61,7 @@ Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, 
     if (backward) {
         l.k_tasks = take(d.cu_q ? k_tiles * (int64_t)sizeof(AttnTask) : 0);
         l.delta = take(d.q_rows * d.heads * 4);
-        l.most = take(d.dtype == NTFP8_F16 ? 128 * kMostLine * 4 : 0);
+        l.most = take(d.dtype == NTFP8_F16 ? 2 * kAttnMost * 4 : 0);
         const int splits = key_splits(d);
         if (splits > 1) l.k_part = take(2 * splits * d.k_rows * d.kv_heads * d.head_dim * 4);
     } else if (c.splits > 1) {
@@ -90,7 +90,7 @@ AttnArgs args_of(const ntops_attention_desc& d) {
 
 // What a launch has to hold: workgroups, and threads, in 32 bits
 bool attention_fits(const ntops_attention_desc& d) {
-    constexpr int64_t kMost = (int64_t)1 << 23;
+    constexpr int64_t kMost = (int64_t)1 << 22;
     return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
 }
 
