@@ -181,7 +181,8 @@ int ntops_rotary(const ntops_rotary_desc* d, void* stream);
  * head_dim <= 128, a multiple of 8; scale 1e-30 to 1e30; dtype NTFP8_BF16 or NTFP8_F16.  Scores, maxima, sums and outputs are fp32 until the one rounding of
  * out; the softmax's numerators are rounded to dtype for the product with v.  out is dense; lse [heads][q_rows] fp32 (minus the logarithm of a row's
  * sum of exponentials, over scale) is what a backward pass needs, NULL if none follows.  q_rows * heads and k_rows * kv_heads at most 2^27.
- * workspace: ntops_attention_workspace(d, backward) bytes, aligned to 256.
+ * workspace: ntops_attention_workspace(d, backward) bytes, aligned to 256.  plan (packed sequences, may be NULL): ntops_attention_plan(d) bytes,
+ * aligned to 256, that a forward call fills and the backward call of the same sizes and offsets reads; without it each makes its own.
  * Backward: dq, dk, dv (dense, dtype, each may be NULL) from dout (strides as q's) and the q, k, v, out and lse of the forward call.
  * The same inputs give the same bits.  fp16: p and ds are kept with powers of two on them, so that gradients below its normal range survive. */
 typedef struct ntops_attention_desc {
@@ -197,6 +198,7 @@ typedef struct ntops_attention_desc {
     void* out;
     float* lse;
     void* workspace;
+    void* plan;
     const void* dout;
     int64_t do_stride, do_head, do_batch;
     void* dq;
@@ -204,6 +206,7 @@ typedef struct ntops_attention_desc {
     void* dv;
 } ntops_attention_desc;
 int64_t ntops_attention_workspace(const ntops_attention_desc* d, int backward);
+int64_t ntops_attention_plan(const ntops_attention_desc* d);
 int ntops_attention_forward(const ntops_attention_desc* d, void* stream);
 int ntops_attention_backward(const ntops_attention_desc* d, void* stream);
 

@@ -69,7 +69,7 @@ class AttentionDesc(ctypes.Structure):
                 ("q_head", _i64), ("k_head", _i64), ("v_head", _i64), ("q_batch", _i64), ("k_batch", _i64), ("v_batch", _i64),
                 ("cu_q", _vp), ("cu_k", _vp), ("sequences", _i64), ("q_rows", _i64), ("k_rows", _i64), ("heads", _i),
                 ("kv_heads", _i), ("head_dim", _i), ("dtype", _i), ("causal", _i), ("scale", _f), ("out", _vp), ("lse", _vp),
-                ("workspace", _vp), ("dout", _vp), ("do_stride", _i64), ("do_head", _i64), ("do_batch", _i64), ("dq", _vp),
+                ("workspace", _vp), ("plan", _vp), ("dout", _vp), ("do_stride", _i64), ("do_head", _i64), ("do_batch", _i64), ("dq", _vp),
                 ("dk", _vp), ("dv", _vp)]
 
 
@@ -88,6 +88,7 @@ SIGNATURES = {
     "ntops_rms_norm_backward": (_i, [_c.POINTER(RmsNormDesc), _c.POINTER(RmsNormGrads), _vp]),
     "ntops_rotary": (_i, [_c.POINTER(RotaryDesc), _vp]),
     "ntops_attention_workspace": (_i64, [_c.POINTER(AttentionDesc), _i]),
+    "ntops_attention_plan": (_i64, [_c.POINTER(AttentionDesc)]),
     "ntops_attention_forward": (_i, [_c.POINTER(AttentionDesc), _vp]),
     "ntops_attention_backward": (_i, [_c.POINTER(AttentionDesc), _vp]),
     "ntops_scale": (_i, [_c.POINTER(ScaleTensor), _i, _i, _vp, _i, _vp]),

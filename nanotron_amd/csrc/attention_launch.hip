@@ -46,10 +46,21 @@ int key_splits(const ntops_attention_desc& d) {
     return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 16));
 }
 
-struct Layout {
-    int64_t q_tasks, k_tasks, part, part_ml, delta, most, k_part, bytes;
+// Tasks of packed sequences: those of queries, and behind them those of keys
+struct Plan {
+    int64_t q_tiles, k_tiles, keys_at, bytes;
 };
-Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, int64_t q_tiles, int64_t k_tiles) {
+Plan plan_of(const ntops_attention_desc& d) {
+    Plan p = {tiles_of(d, d.q_rows, kAttnQueries), tiles_of(d, d.k_rows, kAttnKeys), 0, 0};
+    p.keys_at = up(p.q_tiles * (int64_t)sizeof(AttnTask), 256);
+    p.bytes = p.keys_at + up(p.k_tiles * (int64_t)sizeof(AttnTask), 256);
+    return p;
+}
+
+struct Layout {
+    int64_t plan, part, part_ml, delta, most, k_part, bytes;
+};
+Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c) {
     Layout l = {};
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
@@ -57,9 +68,8 @@ Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c, 
         at += up(bytes, 256);
         return here;
     };
-    l.q_tasks = take(d.cu_q ? q_tiles * (int64_t)sizeof(AttnTask) : 0);
+    l.plan = take(d.cu_q && !d.plan ? plan_of(d).bytes : 0);
     if (backward) {
-        l.k_tasks = take(d.cu_q ? k_tiles * (int64_t)sizeof(AttnTask) : 0);
         l.delta = take(d.q_rows * d.heads * 4);
         l.most = take(d.dtype == NTFP8_F16 ? 2 * kAttnMost * 4 : 0);
         const int splits = key_splits(d);
@@ -94,42 +104,51 @@ bool attention_fits(const ntops_attention_desc& d) {
     return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
 }
 
-int64_t attention_workspace(const ntops_attention_desc& d, bool backward) {
-    const Choice c = choose(d);
-    return layout_of(d, backward, c, backward ? tiles_of(d, d.q_rows, kAttnQueries) : c.tiles, tiles_of(d, d.k_rows, kAttnKeys)).bytes;
+int64_t attention_plan(const ntops_attention_desc& d) { return d.cu_q ? plan_of(d).bytes : 0; }
+
+int64_t attention_workspace(const ntops_attention_desc& d, bool backward) { return layout_of(d, backward, choose(d)).bytes; }
+
+namespace {
+// the tasks of a call's sequences at `at`; those of keys where a backward pass reads them
+int make_plan(const ntops_attention_desc& d, char* at, bool keys, hipStream_t st) {
+    const Plan p = plan_of(d);
+    return run_attention_plan(d.cu_q, d.cu_k, (int)d.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, kAttnQueries, kAttnKeys, (int)p.q_tiles, (int)p.k_tiles,
+                              reinterpret_cast<AttnTask*>(at), keys ? reinterpret_cast<AttnTask*>(at + p.keys_at) : nullptr, st);
 }
+}  // namespace
 
 int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
     const Choice c = choose(d);
-    const Layout l = layout_of(d, false, c, c.tiles, 0);
+    const Layout l = layout_of(d, false, c);
     char* const ws = static_cast<char*>(d.workspace);
     AttnArgs a = args_of(d);
     a.tiles = c.tiles, a.splits = c.splits;
     if (c.splits > 1) a.part = reinterpret_cast<float*>(ws + l.part), a.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
     if (d.cu_q) {
-        AttnTask* const list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
-        a.tasks = list;
-        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, kAttnQueries, 0, (int)c.tiles, 0, list, nullptr, st)) return rc;
+        char* const plan = d.plan ? static_cast<char*>(d.plan) : ws + l.plan;
+        a.tasks = reinterpret_cast<AttnTask*>(plan);
+        if (const int rc = make_plan(d, plan, d.plan != nullptr, st)) return rc;
     }
     return run_attention_forward_kernels(a, d.dtype, c.few, st);
 }
 
 int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
     AttnArgs a = args_of(d);
-    a.tiles = tiles_of(d, d.q_rows, kAttnQueries);
-    const int64_t k_tiles = tiles_of(d, d.k_rows, kAttnKeys);
-    const Layout l = layout_of(d, true, {}, a.tiles, k_tiles);
+    const Plan p = plan_of(d);
+    a.tiles = p.q_tiles;
+    const Layout l = layout_of(d, true, {});
     char* const ws = static_cast<char*>(d.workspace);
     a.delta = reinterpret_cast<float*>(ws + l.delta), a.most = reinterpret_cast<uint32_t*>(ws + l.most);
     a.k_splits = key_splits(d), a.k_part = reinterpret_cast<float*>(ws + l.k_part);
-    AttnTask* k_list = nullptr;
+    const AttnTask* k_list = nullptr;
     if (d.cu_q) {
-        AttnTask* const q_list = reinterpret_cast<AttnTask*>(ws + l.q_tasks);
-        k_list = reinterpret_cast<AttnTask*>(ws + l.k_tasks);
-        a.tasks = q_list;
-        if (const int rc = run_attention_plan(d.cu_q, d.cu_k, a.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, kAttnQueries, kAttnKeys, (int)a.tiles, (int)k_tiles, q_list, k_list, st)) return rc;
+        char* const plan = d.plan ? static_cast<char*>(d.plan) : ws + l.plan;
+        a.tasks = reinterpret_cast<AttnTask*>(plan);
+        k_list = reinterpret_cast<AttnTask*>(plan + p.keys_at);
+        if (!d.plan)
+            if (const int rc = make_plan(d, plan, true, st)) return rc;
     }
-    return run_attention_backward_kernels(a, k_list, k_tiles, d.cu_q, d.cu_k, d.dtype, st);
+    return run_attention_backward_kernels(a, k_list, p.k_tiles, d.cu_q, d.cu_k, d.dtype, st);
 }
 
 }  // namespace ntfp8

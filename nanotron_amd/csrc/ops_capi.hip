@@ -24,6 +24,7 @@ int run_rms_norm_backward(const ntops_rms_norm_desc& d, const ntops_rms_norm_gra
 int run_rotary(const ntops_rotary_desc& d, hipStream_t st);
 bool attention_fits(const ntops_attention_desc& d);
 int64_t attention_workspace(const ntops_attention_desc& d, bool backward);
+int64_t attention_plan(const ntops_attention_desc& d);
 int run_attention_forward(const ntops_attention_desc& d, hipStream_t st);
 int run_attention_backward(const ntops_attention_desc& d, hipStream_t st);
 int run_scale(const ntops_scale_tensor* t, int count, int x_dtype, const float* factor, int out_dtype, hipStream_t st);
@@ -142,7 +143,7 @@ int check_attention(const ntops_attention_desc& d) {
         if (v < 0 || v > kMostElements || v % 8 != 0) return NTFP8_ERR_SIZE;
     for (const void* p : {d.q, d.k, d.v, d.dout, (const void*)d.out, (const void*)d.dq, (const void*)d.dk, (const void*)d.dv})
         if (!aligned(p, 16)) return NTFP8_ERR_ALIGN;
-    return aligned(d.lse, 4) && aligned(d.cu_q, 4) && aligned(d.cu_k, 4) && aligned(d.workspace, 256) ? NTFP8_OK : NTFP8_ERR_ALIGN;
+    return aligned(d.lse, 4) && aligned(d.cu_q, 4) && aligned(d.cu_k, 4) && aligned(d.workspace, 256) && aligned(d.plan, 256) ? NTFP8_OK : NTFP8_ERR_ALIGN;
 }
 // bytes of a tensor of a call, from its first element on
 int64_t attention_reach(const ntops_attention_desc& d, int64_t rows, int64_t heads, int64_t stride, int64_t head, int64_t batch) {
@@ -314,6 +315,8 @@ int64_t ntops_attention_workspace(const ntops_attention_desc* d, int backward) {
     return d && check_attention_sizes(*d) == NTFP8_OK ? std::max<int64_t>(256, attention_workspace(*d, backward != 0)) : 0;
 }
 
+int64_t ntops_attention_plan(const ntops_attention_desc* d) { return d && check_attention_sizes(*d) == NTFP8_OK ? attention_plan(*d) : 0; }
+
 int ntops_attention_forward(const ntops_attention_desc* d, void* stream) {
     if (!d) return NTFP8_ERR_NULL;
     if (const int rc = check_attention(*d)) return rc;
@@ -323,7 +326,8 @@ int ntops_attention_forward(const ntops_attention_desc* d, void* stream) {
                         {d->v, attention_reach(*d, d->k_rows, d->kv_heads, d->v_stride, d->v_head, d->v_batch)},
                         {d->cu_q, cu},
                         {d->cu_k, cu}};
-    const Range out[] = {{d->out, 2 * d->q_rows * d->heads * d->head_dim}, {d->lse, 4 * d->q_rows * d->heads}, {d->workspace, attention_workspace(*d, false)}};
+    const Range out[] = {{d->out, 2 * d->q_rows * d->heads * d->head_dim}, {d->lse, 4 * d->q_rows * d->heads}, {d->workspace, attention_workspace(*d, false)},
+                         {d->plan, attention_plan(*d)}};
     if (collide(in, out)) return NTFP8_ERR_ALIAS;
     return run_attention_forward(*d, static_cast<hipStream_t>(stream));
 }
@@ -338,6 +342,7 @@ int ntops_attention_backward(const ntops_attention_desc* d, void* stream) {
                         {d->dout, attention_reach(*d, d->q_rows, d->heads, d->do_stride, d->do_head, d->do_batch)},
                         {d->out, qb},
                         {d->lse, 4 * d->q_rows * d->heads},
+                        {d->plan, attention_plan(*d)},
                         {d->cu_q, cu},
                         {d->cu_k, cu}};
     const Range out[] = {{d->dq, qb}, {d->dk, kb}, {d->dv, kb}, {d->workspace, attention_workspace(*d, true)}};

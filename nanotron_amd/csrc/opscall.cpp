@@ -508,14 +508,28 @@ Tensor attention_room(ntops_attention_desc& d, bool backward, const Tensor& like
     d.workspace = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws.data_ptr()) + 255) / 256 * 256);
     return ws;
 }
-// out, and lse where a backward pass follows
+// out, and where a backward pass follows what it needs: lse, and behind it (at a 256-byte boundary) the plan of packed sequences
+struct AttentionKept {
+    int64_t plan, bytes;
+    explicit AttentionKept(const ntops_attention_desc& d) : plan((d.heads * d.q_rows * 4 + 255) / 256 * 256), bytes(plan + ntops_attention_plan(&d)) {}
+    // (`kept` is 256 bytes longer: a tensor may begin anywhere)
+    void into(ntops_attention_desc& d, const Tensor& kept) const {
+        char* const at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(kept.data_ptr()) + 255) / 256 * 256);
+        d.lse = reinterpret_cast<float*>(at);
+        d.plan = d.cu_q ? at + plan : nullptr;
+    }
+};
 std::pair<Tensor, Tensor> attention_forward(const Attended& q, const Attended& k, const Attended& v, const Sequences& s, bool keep) {
     std::pair<Tensor, Tensor> r;
     r.first = dense_like(q.t);
-    ntops_attention_desc d = attention_desc(q, k, v, s);
-    if (keep) r.second = at::empty({d.heads, d.q_rows}, q.t.options().dtype(at::kFloat).memory_format(at::MemoryFormat::Contiguous));
     if (q.t.numel() == 0) return r;
-    d.out = r.first.data_ptr(), d.lse = keep ? r.second.data_ptr<float>() : nullptr;
+    ntops_attention_desc d = attention_desc(q, k, v, s);
+    d.out = r.first.data_ptr();
+    if (keep) {
+        const AttentionKept room(d);
+        r.second = at::empty({room.bytes + 256}, q.t.options().dtype(at::kByte).memory_format(at::MemoryFormat::Contiguous));
+        room.into(d, r.second);
+    }
     const Tensor ws = attention_room(d, false, q.t);
     call(ntops_attention_forward(&d, stream_of(q.t)), "ntops_attention_forward");
     return r;
@@ -556,7 +570,8 @@ struct Attention : torch::autograd::Function<Attention> {
         const Sequences s{saved[3], saved[4], ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool()};
         const Attended g = attended(grads[0].scalar_type() == q.scalar_type() ? grads[0] : grads[0].to(q.scalar_type()));
         ntops_attention_desc d = attention_desc(attended(q), attended(k), attended(v), s);
-        d.out = out.data_ptr(), d.lse = saved[6].data_ptr<float>();
+        d.out = out.data_ptr();
+        AttentionKept(d).into(d, saved[6]);
         d.dout = g.t.data_ptr(), d.do_stride = g.row, d.do_head = g.head, d.do_batch = g.batch;
         d.dq = at_or_null(dq), d.dk = at_or_null(dk), d.dv = at_or_null(dv);
         const Tensor ws = attention_room(d, true, q);
