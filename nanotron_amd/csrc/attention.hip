@@ -327,14 +327,12 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) lds_load16(rv, (lds_ptr)(uintptr_t)(v + i * 1024), voff[i], 0);
     };
-    v4i q[DP / 16];
-    load_own<DP>(q, A.q, q0, A.dim, live, lane);
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k) asm volatile("" : "+v"(q[k]));   // (here, in front of the loads that are counted below)
     if (steps > 0) {
         load(0);
         load(1);
     }
+    v4i q[DP / 16];   // (behind the first keys and values: what waits for it, waits for one trip to memory and not for two)
+    load_own<DP>(q, A.q, q0, A.dim, live, lane);
     v16f out[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) out[e] = zeros16();

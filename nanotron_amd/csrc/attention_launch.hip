@@ -29,7 +29,7 @@ Choice choose(const ntops_attention_desc& d) {
     c.few = !d.cu_q && d.heads / d.kv_heads * q_len <= 32 && d.sequences * d.kv_heads <= ((int64_t)1 << 22);
     if (c.few) {
         const int64_t units = d.sequences * d.kv_heads;
-        c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len / 256));
+        c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len / 128));
         return c;
     }
     c.tiles = tiles_of(d, d.q_rows, kAttnQueries);
