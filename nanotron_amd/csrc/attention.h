@@ -104,24 +104,24 @@ struct AttnTile {
     struct Source {
         static constexpr int kLoads = kBytes / 1024 / kWaves;
         const char* base;
-        int64_t row_bytes;
+        uint32_t row_bytes;   // (2^25 at most)
         uint32_t off[kLoads];
         int dim;
         __device__ __forceinline__ void init(const void* p, int64_t elements, int64_t stride, int dim_, int wave, int lane) {
             base = static_cast<const char*>(p) + 2 * elements;
-            row_bytes = 2 * stride;
+            row_bytes = (uint32_t)(2 * stride);
             dim = dim_;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int byte = ((i * kWaves + wave) * 64 + lane) * 16, row = byte / kPitch, chunk = (byte % kPitch >> 4) ^ swizzle(row);
-                off[i] = chunk * 8 < dim ? (uint32_t)row * (uint32_t)row_bytes + chunk * 16 : kNowhere;
+                off[i] = chunk * 8 < dim ? (uint32_t)row * row_bytes + chunk * 16 : kNowhere;
             }
         }
         // rows first .. of `len`, those behind it as zeros
         __device__ __forceinline__ void load(uint8_t* stage, int first, int len, int wave) const {
             const int rows = min(kRows, len - first);
-            const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * (uint32_t)row_bytes + 2u * dim : 0u;
-            const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (int64_t)first * row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
+            const uint32_t bytes = rows > 0 ? (uint32_t)(rows - 1) * row_bytes + 2u * dim : 0u;
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (uint64_t)(uint32_t)first * row_bytes, (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes));
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) lds_load16(r, (lds_ptr)(uintptr_t)(stage + (i * kWaves + wave) * 1024), off[i], 0);
         }
@@ -279,6 +279,13 @@ __device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float fac
             const int first = 32 * e + 16 * s + 8 * h;
             if (live && first < dim) *reinterpret_cast<v4i*>(at + 2 * first) = (v4i){(int)a0, (int)a1, (int)b0, (int)b1};
         }
+}
+
+// the lane's number, made anew where a register kept for it would be spilled
+__device__ __forceinline__ uint32_t lane_anew() {
+    uint32_t none = 0;
+    asm volatile("" : "+v"(none));
+    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none));
 }
 
 // max of a lane and its counterpart of the other half wave

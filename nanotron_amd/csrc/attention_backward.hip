@@ -199,28 +199,40 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
     typename Tile::template Source<kAttnKeyWaves> qs, gs, vs;
     qs.init(A.q, attn_rows(A, task.other, task.seq, 0, A.q_stride, A.q_batch) + (int64_t)kv * A.group * A.q_head, A.q_stride, A.dim, wave, lane);
     gs.init(A.dout, attn_rows(A, task.other, task.seq, 0, A.do_stride, A.do_batch) + (int64_t)kv * A.group * A.do_head, A.do_stride, A.dim, wave, lane);
-    const float* stats = (wave == 0 ? A.lse : A.delta) + kv * A.group * A.q_rows + task.other;
-    const char *const q_base = qs.base, *const g_base = gs.base;
     // Tiles of a head's queries: first those whose rows all see all keys of the workgroup, then the ones in front of and behind these
     const int front = A.causal ? min(max(0, (task.shift + task.rows - 1 + kAttnKeyStep - 1) / kAttnKeyStep - begin), per) : 0;
     const int whole = max(0, min(task.len / kAttnKeyStep - begin, per) - front);
     auto row_of = [&](int i) { return (begin + (i < whole ? front + i : i < whole + front ? i - whole : i)) * kAttnKeyStep; };
-    auto load = [&](int j, int stage) {
-        const int head = j / per, first = row_of(j - head * per);
-        qs.base = q_base + 2 * (head * A.q_head);
-        gs.base = g_base + 2 * (head * A.do_head);
+    // The tile that is loaded next, and its head's first rows: counted along, a division a step is as long as three of its products
+    int next_tile = per > 0 ? step0 % per : 0, next_row = 0;
+    const int64_t q_apart = 2 * A.q_head, g_apart = 2 * A.do_head;
+    {
+        const int head = per > 0 ? step0 / per : 0;
+        qs.base += head * q_apart;
+        gs.base += head * g_apart;
+    }
+    const float* stats = (wave == 0 ? A.lse : A.delta) + (kv * A.group + (per > 0 ? step0 / per : 0)) * A.q_rows + task.other;
+    auto load = [&](int stage) __attribute__((always_inline)) {
+        const int first = next_row = row_of(next_tile);
         qs.load(sq + stage * Tile::kBytes, first, task.len, wave);
         gs.load(sg + stage * Tile::kBytes, first, task.len, wave);
         if (wave < 2) {
-            const __amdgpu_buffer_rsrc_t r = make_rsrc(stats + head * A.q_rows + first, (uint32_t)__builtin_amdgcn_readfirstlane(min(kAttnKeyStep, task.len - first) * 4));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(uintptr_t)&rows_of[stage][wave][0], 4, lane * 4, 0, 0, 0);
+            const __amdgpu_buffer_rsrc_t r = make_rsrc(stats + first, (uint32_t)__builtin_amdgcn_readfirstlane(min(kAttnKeyStep, task.len - first) * 4));
+            // (a lane's offset from memory would be waited for behind the loads above, 800 cycles a step)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(uintptr_t)&rows_of[stage][wave][0], 4, lane_anew() * 4, 0, 0, 0);
+        }
+        if (++next_tile == per) {
+            next_tile = 0;
+            qs.base += q_apart;
+            gs.base += g_apart;
+            stats += A.q_rows;
         }
     };
     vs.init(A.v, attn_rows(A, task.own, task.seq, task.at, A.v_stride, A.v_batch) + kv * A.v_head, A.v_stride, A.dim, wave, lane);
     if (step0 < steps) {
 #pragma unroll
         for (int i = 0; i < kAttnKeys / kAttnKeyStep; ++i) vs.load(sv + i * Tile::kBytes, i * kAttnKeyStep, task.rows, wave);
-        load(step0, step0 & 1);
+        load(step0 & 1);
     }
     const int mine = wave * 32 * Tile::kPitch;
     const int row = wave * 32 + (lane & 31);
@@ -235,11 +247,11 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
     // One tile of queries of one head.  kMasked: some of its rows may not see all the workgroup's keys
     auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
         constexpr bool kMasked = decltype(masked_)::value;
-        const int row0 = row_of(j % per), stage = j & 1, at = stage * Tile::kBytes;
+        const int row0 = next_row, stage = j & 1, at = stage * Tile::kBytes;   // (its load was the last)
         uint8_t *const qa = sq + stage * Tile::kBytes, *const ga = sg + stage * Tile::kBytes;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         wg_barrier();
-        if (j + 1 < steps) load(j + 1, stage ^ 1);
+        if (j + 1 < steps) load(stage ^ 1);
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
         if (kMasked && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
         const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
