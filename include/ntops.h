@@ -181,6 +181,8 @@ int ntops_rotary(const ntops_rotary_desc* d, void* stream);
  * head_dim <= 128, a multiple of 8; scale 1e-30 to 1e30; dtype NTFP8_BF16 or NTFP8_F16.  Scores, maxima, sums and outputs are fp32 until the one rounding of
  * out; the softmax's numerators are rounded to dtype for the product with v.  out is dense; lse [heads][q_rows] fp32 (minus the logarithm of a row's
  * sum of exponentials, over scale) is what a backward pass needs, NULL if none follows.  q_rows * heads and k_rows * kv_heads at most 2^27.
+ * out_low (as out, a byte an element, aligned to 8; may be NULL): what a forward call's rounding of out left out, 8 more bits of
+ * significand, with which a backward call's dq and dk lose less.
  * workspace: ntops_attention_workspace(d, backward) bytes, aligned to 256.  plan (packed sequences, may be NULL): ntops_attention_plan(d) bytes,
  * aligned to 256, that a forward call fills and the backward call of the same sizes and offsets reads; without it each makes its own.
  * Backward: dq, dk, dv (dense, dtype, each may be NULL) from dout (strides as q's) and the q, k, v, out and lse of the forward call.
@@ -196,6 +198,7 @@ typedef struct ntops_attention_desc {
     int heads, kv_heads, head_dim, dtype, causal;
     float scale;
     void* out;
+    uint8_t* out_low;
     float* lse;
     void* workspace;
     void* plan;

@@ -68,7 +68,7 @@ class AttentionDesc(ctypes.Structure):
     _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _i64), ("k_stride", _i64), ("v_stride", _i64),
                 ("q_head", _i64), ("k_head", _i64), ("v_head", _i64), ("q_batch", _i64), ("k_batch", _i64), ("v_batch", _i64),
                 ("cu_q", _vp), ("cu_k", _vp), ("sequences", _i64), ("q_rows", _i64), ("k_rows", _i64), ("heads", _i),
-                ("kv_heads", _i), ("head_dim", _i), ("dtype", _i), ("causal", _i), ("scale", _f), ("out", _vp), ("lse", _vp),
+                ("kv_heads", _i), ("head_dim", _i), ("dtype", _i), ("causal", _i), ("scale", _f), ("out", _vp), ("out_low", _vp), ("lse", _vp),
                 ("workspace", _vp), ("plan", _vp), ("dout", _vp), ("do_stride", _i64), ("do_head", _i64), ("do_batch", _i64), ("dq", _vp),
                 ("dk", _vp), ("dv", _vp)]
 

@@ -46,6 +46,7 @@ struct AttnArgs {
     float scale;
     void* out;
     const void* o;     // backward: the output of the forward pass
+    uint8_t* low;      // of every element of out the 8 bits behind those that its rounding kept, where a backward pass follows (or NULL)
     float* lse;        // [heads][q_rows] minus the logarithm of a row's sum of exponentials, in units of q k^T; minus infinity for a row that sees nothing
     float* delta;      // [heads][q_rows] minus the sum of dout out
     uint32_t* most;    // fp16 gradients: bits of the largest magnitudes in dout and v, of each workgroup that looked, [2][kAttnMost]
@@ -261,9 +262,36 @@ __device__ __forceinline__ void add_columns_singly(v16f (&acc)[DP / 32], const T
     for (int e = 0; e < DP / 32; ++e) acc[e] = w.acc[e];
 }
 
+// What rounding x to T left out, as 8 more bits of significand: the difference of their bit patterns as fp32, in steps of 2^-8 of one of T's.
+// The backward pass subtracts the sum of dout out from every dout v^T; made of the rounded out alone it brings a fifth of dq's and dk's error.
+template <int T>
+constexpr int kLowShift = T == NTFP8_BF16 ? 8 : 5;
+template <int T>
+__device__ __forceinline__ uint32_t low_bits(float x, float rounded) {
+    const int r = (int)(__float_as_uint(x) - __float_as_uint(rounded));
+    const int code = max(-128, min(127, (r + (1 << (kLowShift<T> - 1))) >> kLowShift<T>));
+    return (__float_as_uint(rounded) & 0x7fffffffu) < kInfBits ? (uint32_t)code & 0xffu : 0u;
+}
+template <int T>
+__device__ __forceinline__ float with_low(float rounded, uint32_t code) {
+    return __uint_as_float(__float_as_uint(rounded) + (uint32_t)((int)(code << 24) >> 24 << kLowShift<T>));
+}
+// of 8 consecutive elements
+template <int T>
+__device__ __forceinline__ void store_low(uint8_t* low, int64_t element, const float (&x)[8]) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        float a, b;
+        unpack_pair<T>(pack_pair<T>(x[i], x[i + 1]), a, b);
+        w[i / 4] |= (low_bits<T>(x[i], a) | low_bits<T>(x[i + 1], b) << 8) << (i % 4 * 8);
+    }
+    *reinterpret_cast<v2i_attn*>(low + element) = (v2i_attn){(int)w[0], (int)w[1]};
+}
+
 // acc * factor as one row a lane, rounded to T: 16 bytes a lane and store.  p: the row's first element
 template <int T, int DP>
-__device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float factor, void* p, int64_t element, int dim, bool live, int lane) {
+__device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float factor, void* p, int64_t element, int dim, bool live, int lane, uint8_t* low = nullptr) {
     char* const at = static_cast<char*>(p) + 2 * element;
     const int h = lane >> 5;
 #pragma unroll
@@ -273,11 +301,20 @@ __device__ __forceinline__ void store_rows(const v16f (&acc)[DP / 32], float fac
             float v[8];
 #pragma unroll
             for (int r = 0; r < 8; ++r) v[r] = acc[e][8 * s + r] * factor;
-            uint32_t a0 = pack_pair<T>(v[0], v[1]), a1 = pack_pair<T>(v[2], v[3]), b0 = pack_pair<T>(v[4], v[5]), b1 = pack_pair<T>(v[6], v[7]);
-            swap_halves(a0, b0);
-            swap_halves(a1, b1);
+            // 8 elements in a row: the second four of this half wave for the first four of the other
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                uint32_t x = __float_as_uint(v[r]), y = __float_as_uint(v[4 + r]);
+                swap_halves(x, y);
+                v[r] = __uint_as_float(x);
+                v[4 + r] = __uint_as_float(y);
+            }
             const int first = 32 * e + 16 * s + 8 * h;
-            if (live && first < dim) *reinterpret_cast<v4i*>(at + 2 * first) = (v4i){(int)a0, (int)a1, (int)b0, (int)b1};
+            if (live && first < dim) {
+                *reinterpret_cast<v4i*>(at + 2 * first) =
+                    (v4i){(int)pack_pair<T>(v[0], v[1]), (int)pack_pair<T>(v[2], v[3]), (int)pack_pair<T>(v[4], v[5]), (int)pack_pair<T>(v[6], v[7])};
+                if (low) store_low<T>(low, element + first, v);
+            }
         }
 }
 

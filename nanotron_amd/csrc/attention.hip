@@ -275,7 +275,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(c
             }
         return;
     }
-    store_rows<T, DP>(out, attn_any(all) ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane);
+    store_rows<T, DP>(out, attn_any(all) ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane, A.low);
     if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = attn_lse(A, top, all);
 }
 
@@ -423,7 +423,10 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] *= by;
             if (A.splits > 1) store_piece<NTFP8_F32, 8>(A.part, to * A.dim + d, x);
-            else store_piece<T, 8>(A.out, (out_row * A.heads + hd) * A.dim + d, x);
+            else {
+                store_piece<T, 8>(A.out, (out_row * A.heads + hd) * A.dim + d, x);
+                if (A.low) store_low<T>(A.low, (out_row * A.heads + hd) * A.dim + d, x);
+            }
         }
         if (threadIdx.x < kFewRows) {
             if (A.splits > 1) A.part_ml[to] = make_float2(all_top, all_sum);
@@ -473,6 +476,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= over;
         store_piece<T, 8>(A.out, row * A.dim + d, x);
+        if (A.low) store_low<T>(A.low, row * A.dim + d, x);
     }
     if (A.lse && d == 0) A.lse[(row % A.heads) * A.q_rows + row / A.heads] = attn_lse(A, top, sum);
 }

@@ -46,7 +46,15 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
             const int64_t at = A.tasks ? row : row - (int64_t)seq * own_len;
             const int64_t stride = values ? A.v_stride : A.do_stride, batch = values ? A.v_batch : A.do_batch, apart = values ? A.v_head : A.do_head;
             unpack<T, 8>(load_piece<T, 8>(values ? A.v : A.dout, seq * batch + at * stride + head * apart + d), x);
-            if (!values) unpack<T, 8>(load_piece<T, 8>(A.o, (row * heads + head) * A.dim + d), y);
+            if (!values) {
+                const int64_t at_out = (row * heads + head) * A.dim + d;
+                unpack<T, 8>(load_piece<T, 8>(A.o, at_out), y);
+                if (A.low) {
+                    const v2i_attn low = *reinterpret_cast<const v2i_attn*>(A.low + at_out);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = with_low<T>(y[i], (uint32_t)low[i / 4] >> (i % 4 * 8));
+                }
+            }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {

@@ -92,7 +92,7 @@ AttnArgs args_of(const ntops_attention_desc& d) {
     a.q_rows = d.q_rows, a.k_rows = d.k_rows;
     a.heads = d.heads, a.kv_heads = d.kv_heads, a.group = d.heads / d.kv_heads, a.dim = d.head_dim, a.causal = d.causal;
     a.c = d.scale * kLog2E, a.scale = d.scale;
-    a.out = d.out, a.o = d.out, a.lse = d.lse, a.dq = d.dq, a.dk = d.dk, a.dv = d.dv, a.splits = 1;
+    a.out = d.out, a.o = d.out, a.low = d.out_low, a.lse = d.lse, a.dq = d.dq, a.dk = d.dk, a.dv = d.dv, a.splits = 1;
     return a;
 }
 

@@ -143,7 +143,7 @@ int check_attention(const ntops_attention_desc& d) {
         if (v < 0 || v > kMostElements || v % 8 != 0) return NTFP8_ERR_SIZE;
     for (const void* p : {d.q, d.k, d.v, d.dout, (const void*)d.out, (const void*)d.dq, (const void*)d.dk, (const void*)d.dv})
         if (!aligned(p, 16)) return NTFP8_ERR_ALIGN;
-    return aligned(d.lse, 4) && aligned(d.cu_q, 4) && aligned(d.cu_k, 4) && aligned(d.workspace, 256) && aligned(d.plan, 256) ? NTFP8_OK : NTFP8_ERR_ALIGN;
+    return aligned(d.lse, 4) && aligned(d.cu_q, 4) && aligned(d.cu_k, 4) && aligned(d.workspace, 256) && aligned(d.plan, 256) && aligned(d.out_low, 8) ? NTFP8_OK : NTFP8_ERR_ALIGN;
 }
 // bytes of a tensor of a call, from its first element on
 int64_t attention_reach(const ntops_attention_desc& d, int64_t rows, int64_t heads, int64_t stride, int64_t head, int64_t batch) {
@@ -327,7 +327,8 @@ int ntops_attention_forward(const ntops_attention_desc* d, void* stream) {
                         {d->cu_q, cu},
                         {d->cu_k, cu}};
     const Range out[] = {{d->out, 2 * d->q_rows * d->heads * d->head_dim}, {d->lse, 4 * d->q_rows * d->heads}, {d->workspace, attention_workspace(*d, false)},
-                         {d->plan, attention_plan(*d)}};
+                         {d->plan, attention_plan(*d)},
+                         {d->out_low, d->q_rows * d->heads * d->head_dim}};
     if (collide(in, out)) return NTFP8_ERR_ALIAS;
     return run_attention_forward(*d, static_cast<hipStream_t>(stream));
 }
@@ -343,6 +344,7 @@ int ntops_attention_backward(const ntops_attention_desc* d, void* stream) {
                         {d->out, qb},
                         {d->lse, 4 * d->q_rows * d->heads},
                         {d->plan, attention_plan(*d)},
+                        {d->out_low, d->q_rows * d->heads * d->head_dim},
                         {d->cu_q, cu},
                         {d->cu_k, cu}};
     const Range out[] = {{d->dq, qb}, {d->dk, kb}, {d->dv, kb}, {d->workspace, attention_workspace(*d, true)}};

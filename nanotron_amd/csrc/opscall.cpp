@@ -508,14 +508,17 @@ Tensor attention_room(ntops_attention_desc& d, bool backward, const Tensor& like
     d.workspace = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(ws.data_ptr()) + 255) / 256 * 256);
     return ws;
 }
-// out, and where a backward pass follows what it needs: lse, and behind it (at a 256-byte boundary) the plan of packed sequences
+// out, and where a backward pass follows what it needs: lse, the bits that out's rounding left out, and the plan of packed sequences, each on
+// a 256-byte boundary
 struct AttentionKept {
-    int64_t plan, bytes;
-    explicit AttentionKept(const ntops_attention_desc& d) : plan((d.heads * d.q_rows * 4 + 255) / 256 * 256), bytes(plan + ntops_attention_plan(&d)) {}
+    int64_t low, plan, bytes;
+    explicit AttentionKept(const ntops_attention_desc& d)
+        : low((d.heads * d.q_rows * 4 + 255) / 256 * 256), plan(low + (d.heads * d.q_rows * d.head_dim + 255) / 256 * 256), bytes(plan + ntops_attention_plan(&d)) {}
     // (`kept` is 256 bytes longer: a tensor may begin anywhere)
     void into(ntops_attention_desc& d, const Tensor& kept) const {
         char* const at = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(kept.data_ptr()) + 255) / 256 * 256);
         d.lse = reinterpret_cast<float*>(at);
+        d.out_low = reinterpret_cast<uint8_t*>(at + low);
         d.plan = d.cu_q ? at + plan : nullptr;
     }
 };

@@ -22,7 +22,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: 
 
     bfloat16 or float16, head_dim a multiple of 8 up to 128.  Products run on the matrix cores with fp32 sums; maxima and sums are fp32; the
     softmax's numerators, and in backward the scores' gradients, are rounded to the type of q for the products they go into.  Rows are read where they are
-    if they lie on 16-byte boundaries, else from a copy.  The same inputs give the same bits, forward and backward.  Memory beside results:
-    in training 8 bytes a query and head; with few queries partial results of fp32, freed on return.  ValueError / TypeError for what does not
+    if they lie on 16-byte boundaries, else from a copy.  The same inputs give the same bits, forward and backward.  Memory kept for
+    the backward pass beside q, k, v and the result: a byte an element of the result and 4 bytes a query and head; freed on return, where queries are few or keys
+    are in the backward pass, partial results of fp32.  ValueError / TypeError for what does not
     fit; differentiable once."""
     return _ops.host.attention(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale)

@@ -300,6 +300,21 @@ def test_gradients_beside_a_bad_row(which):
         near(got[1][:at], clean[1][:at].double(), (clean[1][:at].double().abs() + 1e-3) * 4 * U[q.dtype], "queries in front")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_lose_little_beyond_their_own_roundings(dtype):
+    """In the 2-norm a rounding of values of any significand costs 0.41 u (2 u / sqrt(12), and sqrt(1/2) for significands between 1 and 2).  dq and
+    dk are rounded, and so is ds: 0.58 u.  What else there is, out's own error in the subtracted sums first of all, is to be less than one
+    rounding: sqrt(3) 0.41 u = 0.71 u.  (With the sums made of the rounded out it is more in sequences as short as these.)"""
+    lengths = [7, 20, 33, 64, 15, 90, 41, 5]
+    n = sum(lengths)
+    q, k, v, do = inputs(n, 8, 4, 64, dtype, seed=11)
+    got = step(q, k, v, do, cu_seqlens=offsets(lengths))
+    want, _ = exact(q, k, v, do, [(x, x) for x in lengths])
+    for o, a, name in zip(got, want, ("out", "dq", "dk", "dv")):
+        off = ((o.double() - a).norm() / a.norm()).item()
+        assert off <= 3 ** 0.5 * 0.41 * U[dtype], (name, off / U[dtype])
+
+
 def test_offsets_that_are_wrong_stay_inside():
     """Offsets behind the rows that there are, or below zero, count as the nearest inside; rows of no sequence are zeros."""
     q, k, v, do = inputs(100, 2, 1, 64, torch.bfloat16)
