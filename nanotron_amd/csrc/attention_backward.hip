@@ -419,7 +419,9 @@ int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, i
         if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
         const bool keys = A.dk || A.dv;
         const int64_t k_groups = keys ? k_tiles * A.kv_heads * A.k_splits : 0;
-        attention_backward_kernel<T, DP><<<(unsigned)(k_groups + (A.dq ? A.tiles * A.heads : 0)), 64 * kAttnWaves, 0, st>>>(B, k_tasks, (int)k_groups);
+        const int64_t groups = k_groups + (A.dq ? A.tiles * A.heads : 0);
+        if (groups == 0) return (int)NTFP8_OK;   // (no keys, and dq not asked for)
+        attention_backward_kernel<T, DP><<<(unsigned)groups, 64 * kAttnWaves, 0, st>>>(B, k_tasks, (int)k_groups);
         if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
         if (keys && A.k_splits > 1) {
             attention_add_kernel<T><<<dim3((unsigned)((A.k_rows * A.kv_heads * A.dim + 2047) / 2048), 2), 256, 0, st>>>(A);

@@ -434,6 +434,70 @@ def test_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_a_cache_of_more_than_2_32_bytes():
+    """One new token, and a few, over 9 million keys: all of them 0 but some far ones, so the softmax is known in closed form."""
+    n, kv, dim = 9_000_000, 2, 128
+    k, v = (torch.zeros(1, n, kv, dim, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    assert k.numel() * 2 > 1 << 32
+    spots = torch.tensor([0, 5, 4_194_303, 4_194_304, 8_388_608, 8_500_001, n - 2], device=DEV)
+    g = torch.Generator().manual_seed(0)
+    k[:, spots] = torch.randn(1, len(spots), kv, dim, generator=g).mul_(2).bfloat16().to(DEV)
+    v[:, spots] = torch.randn(1, len(spots), kv, dim, generator=g).bfloat16().to(DEV)
+    for tokens in (1, 40):
+        q = torch.randn(1, tokens, 4, dim, generator=g).mul_(2).bfloat16().to(DEV)
+        with torch.no_grad():
+            out = attention(q, k, v, causal=False)
+        s = torch.einsum("ihd,jhd->hij", q[0].double().cpu(), k[0, spots].double().cpu().repeat_interleave(2, 1)) * dim ** -0.5
+        e = torch.exp(s)
+        total = e.sum(-1, keepdim=True) + (n - len(spots))
+        far = v[0, spots].double().cpu().repeat_interleave(2, 1)
+        want = torch.einsum("hij,jhd->ihd", e / total, far)
+        # numerators rounded to 16 bits, a sum of nine million ones in fp32 (runs of 2^20 at most, joined: 2^-4 of one in each addition's rounding)
+        bound = (U[q.dtype] + 2.0 ** -12) * torch.einsum("hij,jhd->ihd", e / total, far.abs())
+        near(out[0].cpu(), want, bound, f"{tokens} tokens")
+
+
+def test_rows_far_apart():
+    """Rows 2^24 elements apart, the last ones more than 2^32 bytes from the first."""
+    n, far = 140, 1 << 24
+    room = torch.zeros(n * far, device=DEV, dtype=torch.bfloat16)
+    assert room.numel() * 2 > 1 << 32
+    q, k, v, do = inputs(n, 4, 2, 64, torch.bfloat16)
+    at, views = 0, []
+    for t in (q, k, v, do):
+        view = room.as_strided(t.shape, (far, 64, 1), at)
+        view.copy_(t)
+        views.append(view)
+        at += 4096
+    for a, b in zip(step(*views), step(q, k, v, do)):
+        assert torch.equal(a, b)
+    # one step further apart: copied
+    room = torch.zeros(4 * (far + 8), device=DEV, dtype=torch.bfloat16)
+    view = room.as_strided((4, 4, 64), (far + 8, 64, 1), 0)
+    view.copy_(q[:4])
+    assert torch.equal(attention(view, k[:4], v[:4]), attention(q[:4], k[:4], v[:4]))
+
+
+def test_many_short_sequences():
+    """More sequences than a workgroup of the plan has threads."""
+    g = torch.Generator().manual_seed(1)
+    lengths = torch.randint(0, 4, (3000,), generator=g).tolist()
+    n = sum(lengths)
+    q, k, v, do = inputs(n, 2, 1, 64, torch.bfloat16)
+    got = step(q, k, v, do, cu_seqlens=offsets(lengths))
+    # one sequence under a mask of blocks is the same
+    owner = torch.repeat_interleave(torch.arange(3000), torch.tensor(lengths)).to(DEV)
+    at = torch.arange(n, device=DEV)
+    seen = (owner[:, None] == owner[None]) & (at[None] <= at[:, None])
+    leaves = [t.double().requires_grad_(True) for t in (q, k, v)]
+    p = torch.softmax((torch.einsum("ihd,jd->hij", leaves[0], leaves[1][:, 0]) * 0.125).masked_fill(~seen, -math.inf), -1)
+    want = torch.einsum("hij,jd->ihd", p, leaves[2][:, 0])
+    exact_ = (want.detach(), *torch.autograd.grad(want, leaves, do.double()))
+    for o, a, name in zip(got, exact_, ("out", "dq", "dk", "dv")):
+        # (sequences of three: the bound of a rounding of every operand, twice)
+        assert ((o.double() - a).norm() / a.norm()).item() < 4 * U[q.dtype], name
+
+
 def test_refusals():
     q, k, v, do = inputs(10, 4, 2, 64, torch.bfloat16)
     cu = offsets([4, 6])

@@ -127,6 +127,12 @@ def test_attention_workspaces():
     assert size(attend(q_rows=1 << 20, k_rows=1 << 20), 1) < (1 << 20) * 8 * 4 + 1024
     packed = dict(cu_q=0x6000000, cu_k=0x6000000, sequences=500)
     assert size(attend(q_rows=1 << 20, k_rows=1 << 20, **packed), 1) < (1 << 20) * 8 * 4 + 2 * 32 * (8192 + 502) + 2048
+    # no keys at all: nothing is divided by their tiles
+    for kw in (dict(), packed):
+        assert size(attend(k_rows=0, k=None, v=None, q_rows=500, **kw), 1) > 0 and size(attend(k_rows=0, q_rows=500, **kw), 0) > 0
+    plan = _ops.lib.ntops_attention_plan
+    assert plan(attend()) == 0 and plan(attend(q_rows=1 << 20, k_rows=1 << 20, **packed)) < 2 * 32 * (8192 + 502) + 1024
+    assert size(attend(q_rows=1 << 20, k_rows=1 << 20, plan=0x7000000, **packed), 1) < size(attend(q_rows=1 << 20, k_rows=1 << 20, **packed), 1)
     # partial results where there are few queries: never more than the chip has room for
     assert size(attend(q_rows=1, k_rows=1 << 20), 0) < 1 << 22
 
