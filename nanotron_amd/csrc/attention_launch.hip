@@ -39,11 +39,11 @@ Choice choose(const ntops_attention_desc& d) {
 }
 
 // Runs that the queries of a tile of keys are cut into.  Two workgroups a CU have room; where tiles and heads of keys are fewer than twice as many, each
-// is cut, but into no less than 16 steps where it is longest (of packed sequences, where one is twice as long as their average).
+// is cut, but into no less than 8 steps where it is longest (of packed sequences, where one is twice as long as their average).
 int key_splits(const ntops_attention_desc& d) {
     const int64_t rows = std::min(d.q_rows, d.q_rows / d.sequences * (d.cu_q && d.sequences > 1 ? 2 : 1));
     const int64_t units = std::max<int64_t>(1, tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads), steps = (rows + kAttnKeyStep - 1) / kAttnKeyStep * (d.heads / d.kv_heads);
-    return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 16));
+    return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 8));
 }
 
 // Tasks of packed sequences: those of queries, and behind them those of keys
