@@ -189,22 +189,37 @@ __device__ __forceinline__ v4i pack_scores(const v16f& s, int first) {
 }
 // the place in its block of 32 of a result register
 __device__ __forceinline__ int place_of(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+// and what is left of it without the lane's share, for comparisons with a bound that holds that share, once a tile: sixteen places made in front
+// of a loop are spilled, and waited for behind the loads of the next tile
+__device__ __forceinline__ constexpr int place_in_half(int r) { return 8 * (r >> 2) + (r & 3); }
 
-// Whether a stage holds a value that is not finite, in any of its first `rows` rows
-template <int T, int DP>
-__device__ __forceinline__ bool attn_not_finite(const uint8_t* stage, int rows, int lane) {
-    float nan = 0.0f;
-    for (int at = lane * 16; at < rows * AttnTile<DP>::kPitch; at += 1024) {
-        const v4i x = *reinterpret_cast<const v4i*>(stage + at);
+// Whether what a wave loaded of a stage (its pieces of 1 KB, see Source; all of them where kWaves is 1) holds a value that is not finite: the
+// largest magnitude of the pairs of 16 bits, in integers.  Where waves share a stage each looks at its own part, which its own wait has brought, and
+// leaves the answer in front of the barrier: every wave looking at the whole stage took three times as long as its products.
+template <int T, int DP, int kRows, int kWaves>
+__device__ __forceinline__ bool attn_not_finite(const uint8_t* stage, int wave, int lane) {
+    typedef unsigned short v2us __attribute__((ext_vector_type(2)));
+    constexpr int kLoads = AttnTile<DP, kRows>::kBytes / 1024 / kWaves;
+    v2us most = {0, 0};
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            float lo, hi;
-            unpack_pair<T>((uint32_t)x[w], lo, hi);
-            nan = __builtin_fmaf(lo, 0.0f, nan);
-            nan = __builtin_fmaf(hi, 0.0f, nan);
-        }
+    for (int i = 0; i < kLoads; ++i) {
+        const v4i x = *reinterpret_cast<const v4i*>(stage + (i * kWaves + wave) * 1024 + lane * 16);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(v2us, x[w] & 0x7fff7fff));
     }
-    return __any(nan != nan);
+    constexpr unsigned short kInf = T == NTFP8_BF16 ? 0x7f80 : 0x7c00;
+    return __any(most.x >= kInf || most.y >= kInf);
+}
+// A wave's answer for all of them, behind the next barrier, and theirs
+__device__ __forceinline__ void attn_tell(int (&odd)[kAttnWaves], int wave, bool mine) {
+    odd[wave] = mine;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ bool attn_any_wave(const int (&odd)[kAttnWaves]) {
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < kAttnWaves; ++w) any |= odd[w];
+    return __builtin_amdgcn_readfirstlane(any);
 }
 // acc (elements by own rows) += columns of a stage's rows 16 s .. * scores
 template <int T, int DP>

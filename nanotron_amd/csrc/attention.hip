@@ -99,6 +99,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(c
     typedef AttnTile<DP> Tile;
     __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * Tile::kBytes];
     __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];
+    __shared__ __attribute__((aligned(16))) int odd[2][kAttnWaves];   // [stage]: a wave's part of the values is not finite throughout
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // heads that share keys go to one XCD: workgroups are dealt to the eight in turn
     const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
@@ -223,21 +224,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(c
         }
         most = largest();
     };
-    // Any tile: rows that do not see all of it, or nothing behind it
-    auto step = [&](int j) __attribute__((always_inline)) {
-        const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes, other = Tile::kBytes - stage, last = last_key - key0;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        wg_barrier();
-        if (j + 1 < steps) {
-            ks.load(sk + stage, key0 + 2 * kAttnStep, task.len, wave);
-            vs.load(sv + other, key0 + kAttnStep, task.len, wave);
-        }
-        if (A.causal && key0 > lead + 31) return;   // (uniform in the wave; so are the tiles behind this one)
+    // The scores' tile under its mask, into the sums.  kSingly: it holds values which are not finite
+    auto masked = [&](int key0, uint8_t* values, auto singly_) __attribute__((always_inline)) {
+        const int last = last_key - key0, last_half = last - 4 * (lane >> 5);
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (32 * g + place_of(r, lane) > last) s[g][r] = -__builtin_inff();
+                if (32 * g + place_in_half(r) > last_half) s[g][r] = -__builtin_inff();
         const float below = raise(largest());
         v4i p[4];   // of 16 keys each
 #pragma unroll
@@ -247,12 +241,29 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(c
             p[2 * g] = pack_scores<T>(s[g], 0);
             p[2 * g + 1] = pack_scores<T>(s[g], 8);
         }
-        if (attn_not_finite<T, DP>(sv + stage, kAttnStep, lane)) {
-            add_columns_singly<T, DP, 4>(out, tile, sv + stage, p, 0, last + 1);
+        if constexpr (decltype(singly_)::value) {
+            add_columns_singly<T, DP, 4>(out, tile, values, p, 0, last + 1);
         } else {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) add_columns<T, DP>(out, tile, sv + stage, g, p[g]);
+            for (int g = 0; g < 4; ++g) add_columns<T, DP>(out, tile, values, g, p[g]);
         }
+    };
+    // Any tile: rows that do not see all of it, or nothing behind it.  One with values which are not finite is left for later (of the same tiles, for
+    // every wave): what such a tile needs would take registers from this loop
+    bool left = false;
+    auto step = [&](int j) __attribute__((always_inline)) {
+        const int key0 = (first + j) * kAttnStep, stage = (j & 1) * Tile::kBytes, other = Tile::kBytes - stage;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        attn_tell(odd[j & 1], wave, attn_not_finite<T, DP, kAttnStep, kAttnWaves>(sv + stage, wave, lane));
+        wg_barrier();
+        if (j + 1 < steps) {
+            ks.load(sk + stage, key0 + 2 * kAttnStep, task.len, wave);
+            vs.load(sv + other, key0 + kAttnStep, task.len, wave);
+        }
+        const bool later = attn_any_wave(odd[j & 1]);
+        left |= later;
+        if (A.causal && key0 > lead + 31) return;   // (uniform in the wave; so are the tiles behind this one)
+        if (!later) masked(key0, sv + stage, std::false_type{});
         if (j + 1 < steps) scores(sk + other, s);
     };
     // tiles that every row sees whole, then the others and the last
@@ -260,6 +271,21 @@ __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(c
     int j = 0;
     for (; j < clear; ++j) whole_step(j);
     for (; j < steps; ++j) step(j);
+    if (__builtin_expect(left, 0)) {
+        for (j = max(0, clear); j < steps; ++j) {
+            const int key0 = (first + j) * kAttnStep;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            wg_barrier();
+            ks.load(sk, key0, task.len, wave);
+            vs.load(sv, key0, task.len, wave);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            attn_tell(odd[j & 1], wave, attn_not_finite<T, DP, kAttnStep, kAttnWaves>(sv, wave, lane));
+            wg_barrier();
+            if (!attn_any_wave(odd[j & 1]) || (A.causal && key0 > lead + 31)) continue;
+            scores(sk, s);
+            masked(key0, sv, std::true_type{});
+        }
+    }
     const float all = both_sum(sum);
     const int64_t at = (int64_t)task.own + row;
     if (A.splits > 1) {
@@ -346,11 +372,11 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) s = mfma_attn<T>(tile.rows(k, 0, i), q[i], s);
         const bool masked = key0 + kFewStep - 1 > min(len - 1, first_last);
-        const int last = min(len - 1, last_row) - key0;
+        const int last = min(len - 1, last_row) - key0, last_half = last - 4 * (lane >> 5);
         if (masked) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (place_of(r, lane) > last) s[r] = -__builtin_inff();
+                if (place_in_half(r) > last_half) s[r] = -__builtin_inff();
         }
         float most = s[0];
 #pragma unroll
@@ -370,7 +396,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
             sum += s[r];
         }
         const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)};
-        if (masked && attn_not_finite<T, DP>(v, kFewStep, lane)) {
+        if (__builtin_expect(masked && attn_not_finite<T, DP, kFewStep, 1>(v, 0, lane), 0)) {
             add_columns_singly<T, DP, 2>(out, tile, v, p, 0, last + 1);
         } else {
             add_columns<T, DP>(out, tile, v, 0, p[0]);

@@ -74,11 +74,15 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
     }
 }
 
+// How a tile is taken: all its rows and keys see each other, or some do not, or these hold values that are not finite
+constexpr int kWhole = 0, kMasked = 1, kSingly = 2;
+
 // dq of 128 queries of one head, 32 a wave
 template <int T, int DP>
 __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8_t* lds) {
     typedef AttnTile<DP> Tile;
     uint8_t *const sk = lds, *const sv = lds + 2 * Tile::kBytes;
+    int(*const odd)[kAttnWaves] = reinterpret_cast<int(*)[kAttnWaves]>(lds + 4 * Tile::kBytes);   // [stage]: a wave's part of the keys is not finite throughout
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = group / A.heads, pick = group - t * A.heads;
     const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
@@ -107,19 +111,34 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
     v16f dq[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) dq[e] = zeros16();
-    // One tile of keys.  kMasked: some rows of the workgroup may not see all of them
-    auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
-        constexpr bool kMasked = decltype(masked_)::value;
-        const int key0 = j * kAttnStep, stage = (j & 1) * Tile::kBytes;
+    // One tile of keys.  kMasked: some rows of the workgroup may not see all of them.  One of those with keys which are not finite is left for
+    // later, see the forward pass, and then fetched by itself
+    bool left = false;
+    auto step = [&](int j, auto how_) __attribute__((always_inline)) {
+        constexpr int kHow = decltype(how_)::value;
+        constexpr bool kMask = kHow != kWhole;
+        const int key0 = j * kAttnStep, stage = kHow == kSingly ? 0 : (j & 1) * Tile::kBytes;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (kHow == kSingly) {
+            wg_barrier();
+            ks.load(sk, key0, task.len, wave);
+            vs.load(sv, key0, task.len, wave);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if constexpr (kMask) attn_tell(odd[j & 1], wave, attn_not_finite<T, DP, kAttnStep, kAttnWaves>(sk + stage, wave, lane));
         wg_barrier();
-        if (j + 1 < steps) {
+        if (kHow != kSingly && j + 1 < steps) {
             ks.load(sk + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
             vs.load(sv + Tile::kBytes - stage, key0 + kAttnStep, task.len, wave);
         }
+        if constexpr (kMask) {
+            const bool not_finite = attn_any_wave(odd[j & 1]);
+            left |= not_finite;
+            if (not_finite != (kHow == kSingly)) return;
+        }
         const int lead = task.shift + wave * 32;   // the last key that the wave's first row sees
-        if (kMasked && A.causal && key0 > lead + 31) return;   // (uniform in the wave)
-        const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0;
+        if (kMask && A.causal && key0 > lead + 31) return;   // (uniform in the wave)
+        const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0, last_half = last - 4 * (lane >> 5);
         // Runs of products, of two blocks of 32 keys: scores and dout v^T of the one, of the other, then dq; beside each the arithmetic of the run
         // before.  Fragments are read two products ahead.
         constexpr int kProducts = DP / 16;   // of a run
@@ -138,7 +157,7 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
                 const int x = which * kProducts + i;
-                if (!kMasked || x + 2 < 4 * kProducts) fetch(x + 2);
+                if (!kMask || x + 2 < 4 * kProducts) fetch(x + 2);
                 to = mfma_attn<T>(f[x % 3], which & 1 ? g[i] : q[i], to);
 #pragma unroll
                 for (int r = i * 16 / kProducts; r < (i + 1) * 16 / kProducts; ++r) beside(r);
@@ -148,7 +167,7 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
         auto exponential = [&](int b, int r) __attribute__((always_inline)) { s[b][r] = exp2_fast(__builtin_fmaf(s[b][r], A.c, lse)); };
         auto gradient = [&](int b, int r) __attribute__((always_inline)) {
             d[b][r] = s[b][r] * ((d[b][r] + delta) * lift);
-            if (kMasked && 32 * b + place_of(r, lane) > last) d[b][r] = 0.0f;
+            if (kMask && 32 * b + place_in_half(r) > last_half) d[b][r] = 0.0f;
             if (r % 8 == 7) p[2 * b + r / 8] = pack_scores<T>(d[b], r - 7);
         };
         fetch(0);
@@ -157,10 +176,10 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
         run(1, [&](int r) __attribute__((always_inline)) { exponential(0, r); });
         run(2, [&](int r) __attribute__((always_inline)) { gradient(0, r); });
         run(3, [&](int r) __attribute__((always_inline)) { exponential(1, r); });
-        if constexpr (kMasked) {
+        if constexpr (kMask) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) gradient(1, r);
-            if (attn_not_finite<T, DP>(sk + stage, kAttnStep, lane)) {
+            if constexpr (kHow == kSingly) {
                 add_columns_singly<T, DP, 4>(dq, tile, sk + stage, p, 0, last + 1);
                 return;
             }
@@ -172,7 +191,7 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
             const int x = 4 * kProducts + i;
             if (i + 2 < 2 * kProducts) fetch(x + 2);
             dq[i % (DP / 32)] = mfma_attn<T>(f[x % 3], p[i / (DP / 32)], dq[i % (DP / 32)]);
-            if constexpr (!kMasked) {
+            if constexpr (!kMask) {
                 if (i < kProducts) {
 #pragma unroll
                     for (int r = i * 16 / kProducts; r < (i + 1) * 16 / kProducts; ++r) gradient(1, r);
@@ -184,8 +203,10 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
     // tiles that every row sees whole, then the others
     const int clear = max(0, min(min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, steps));
     int j = 0;
-    for (; j < clear; ++j) step(j, std::false_type{});
-    for (; j < steps; ++j) step(j, std::true_type{});
+    for (; j < clear; ++j) step(j, std::integral_constant<int, kWhole>{});
+    for (; j < steps; ++j) step(j, std::integral_constant<int, kMasked>{});
+    if (__builtin_expect(left, 0))
+        for (j = clear; j < steps; ++j) step(j, std::integral_constant<int, kSingly>{});
     store_rows<T, DP>(dq, A.scale / lift, A.dq, (at * A.heads + head) * A.dim, A.dim, live, lane);
 }
 
@@ -196,6 +217,7 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
     typedef AttnTile<DP, kAttnKeyStep> Tile;
     uint8_t *const sq = lds, *const sg = lds + 2 * Tile::kBytes, *const sv = lds + 4 * Tile::kBytes;
     float(*const rows_of)[2][64] = reinterpret_cast<float(*)[2][64]>(sv + kAttnKeys / kAttnKeyStep * Tile::kBytes);   // [stage]: lse and delta (a wave loads 64)
+    int(*const odd)[kAttnKeyWaves] = reinterpret_cast<int(*)[kAttnKeyWaves]>(rows_of + 2);   // [stage]: a wave's part of the queries or gradients is not finite throughout
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int run = group / A.kv_heads, kv = group - run * A.kv_heads, t = run / A.k_splits, split = run - t * A.k_splits;
     const AttnTask task = attn_task(A, t, kAttnKeys, true);
@@ -205,21 +227,24 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
     Tile tile;
     tile.init(lane);
     typename Tile::template Source<kAttnKeyWaves> qs, gs, vs;
-    qs.init(A.q, attn_rows(A, task.other, task.seq, 0, A.q_stride, A.q_batch) + (int64_t)kv * A.group * A.q_head, A.q_stride, A.dim, wave, lane);
-    gs.init(A.dout, attn_rows(A, task.other, task.seq, 0, A.do_stride, A.do_batch) + (int64_t)kv * A.group * A.do_head, A.do_stride, A.dim, wave, lane);
+    qs.init(A.q, 0, A.q_stride, A.dim, wave, lane);
+    gs.init(A.dout, 0, A.do_stride, A.dim, wave, lane);
     // Tiles of a head's queries: first those whose rows all see all keys of the workgroup, then the ones in front of and behind these
     const int front = A.causal ? min(max(0, (task.shift + task.rows - 1 + kAttnKeyStep - 1) / kAttnKeyStep - begin), per) : 0;
     const int whole = max(0, min(task.len / kAttnKeyStep - begin, per) - front);
     auto row_of = [&](int i) { return (begin + (i < whole ? front + i : i < whole + front ? i - whole : i)) * kAttnKeyStep; };
     // The tile that is loaded next, and its head's first rows: counted along, a division a step is as long as three of its products
-    int next_tile = per > 0 ? step0 % per : 0, next_row = 0;
+    int next_tile = 0, next_row = 0;
     const int64_t q_apart = 2 * A.q_head, g_apart = 2 * A.do_head;
-    {
-        const int head = per > 0 ? step0 / per : 0;
-        qs.base += head * q_apart;
-        gs.base += head * g_apart;
-    }
-    const float* stats = (wave == 0 ? A.lse : A.delta) + (kv * A.group + (per > 0 ? step0 / per : 0)) * A.q_rows + task.other;
+    const float* stats = nullptr;
+    auto seek = [&](int j) __attribute__((always_inline)) {
+        const int in = per > 0 ? j / per : 0, head = kv * A.group + in;
+        next_tile = j - in * per;
+        qs.base = static_cast<const char*>(A.q) + 2 * (attn_rows(A, task.other, task.seq, 0, A.q_stride, A.q_batch) + head * A.q_head);
+        gs.base = static_cast<const char*>(A.dout) + 2 * (attn_rows(A, task.other, task.seq, 0, A.do_stride, A.do_batch) + head * A.do_head);
+        stats = (wave == 0 ? A.lse : A.delta) + head * A.q_rows + task.other;
+    };
+    seek(step0);
     auto load = [&](int stage) __attribute__((always_inline)) {
         const int first = next_row = row_of(next_tile);
         qs.load(sq + stage * Tile::kBytes, first, task.len, wave);
@@ -252,17 +277,32 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
     v16f dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) dk[e] = dv[e] = zeros16();
-    // One tile of queries of one head.  kMasked: some of its rows may not see all the workgroup's keys
-    auto step = [&](int j, auto masked_) __attribute__((always_inline)) {
-        constexpr bool kMasked = decltype(masked_)::value;
+    // One tile of queries of one head.  kMasked: some of its rows may not see all the workgroup's keys, and where it is not finite it is left for later
+    bool left = false;
+    auto step = [&](int j, auto how_) __attribute__((always_inline)) {
+        constexpr int kHow = decltype(how_)::value;
+        constexpr bool kMask = kHow != kWhole;
+        if constexpr (kHow == kSingly) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            wg_barrier();
+            seek(j);
+            load(j & 1);
+        }
         const int row0 = next_row, stage = j & 1, at = stage * Tile::kBytes;   // (its load was the last)
         uint8_t *const qa = sq + stage * Tile::kBytes, *const ga = sg + stage * Tile::kBytes;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (kMask)
+            attn_tell(odd[stage], wave, attn_not_finite<T, DP, kAttnKeyStep, kAttnKeyWaves>(qa, wave, lane) || attn_not_finite<T, DP, kAttnKeyStep, kAttnKeyWaves>(ga, wave, lane));
         wg_barrier();
-        if (j + 1 < steps) load(stage ^ 1);
+        if (kHow != kSingly && j + 1 < steps) load(stage ^ 1);
+        if constexpr (kMask) {
+            const bool not_finite = attn_any_wave(odd[stage]);
+            left |= not_finite;
+            if (not_finite != (kHow == kSingly)) return;
+        }
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
-        if (kMasked && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
-        const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0;   // rows of the tile that see this lane's key
+        if (kMask && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
+        const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0, half = 4 * (lane_anew() >> 5);   // rows of the tile that see this lane's key
         // s and d begin at what is subtracted from them
         v16f s, d;
 #pragma unroll
@@ -293,9 +333,8 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
             __builtin_amdgcn_sched_barrier(0);
         }
         auto counted = [&](float x, int r) __attribute__((always_inline)) {
-            if constexpr (!kMasked) return x;
-            const int i = place_of(r, lane);
-            return i >= from && i < to ? x : 0.0f;
+            if constexpr (!kMask) return x;
+            return place_in_half(r) >= from - half && place_in_half(r) < to - half ? x : 0.0f;
         };
         v4i fa[3];
         // fragment x of the products for dv, and those for dk behind them
@@ -316,10 +355,10 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
             d[r] = counted(T == NTFP8_F16 ? s[r] * (d[r] * down) : s[r] * d[r], r);
             if (r % 8 == 7) ds[r / 8] = pack_scores<T>(d, r - 7);
         };
-        if constexpr (kMasked) {
-            if (attn_not_finite<T, DP>(ga, kAttnKeyStep, lane) || attn_not_finite<T, DP>(qa, kAttnKeyStep, lane)) {
+        if constexpr (kMask) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) gradient(r);
+            for (int r = 0; r < 16; ++r) gradient(r);
+            if constexpr (kHow == kSingly) {
                 add_columns_singly<T, DP, 2>(dv, tile, ga, p, from, to);
                 add_columns_singly<T, DP, 2>(dk, tile, qa, ds, from, to);
                 return;
@@ -329,8 +368,10 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
         for (int x = 0; x < kProducts; ++x) {
             fetch_a(x + 2);
             dv[x % (DP / 32)] = mfma_attn<T>(fa[x % 3], p[x / (DP / 32)], dv[x % (DP / 32)]);
+            if constexpr (!kMask) {
 #pragma unroll
-            for (int r = x * 16 / kProducts; r < (x + 1) * 16 / kProducts; ++r) gradient(r);
+                for (int r = x * 16 / kProducts; r < (x + 1) * 16 / kProducts; ++r) gradient(r);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -342,9 +383,12 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
     };
     for (int j = step0; j < steps;) {
         const int i = j % per;
-        for (const int end = min(steps, j + whole - i); j < end; ++j) step(j, std::false_type{});
-        for (const int end = min(steps, j + per - max(i, whole)); j < end; ++j) step(j, std::true_type{});
+        for (const int end = min(steps, j + whole - i); j < end; ++j) step(j, std::integral_constant<int, kWhole>{});
+        for (const int end = min(steps, j + per - max(i, whole)); j < end; ++j) step(j, std::integral_constant<int, kMasked>{});
     }
+    if (__builtin_expect(left, 0))
+        for (int j = step0; j < steps; ++j)
+            if (j % per >= whole) step(j, std::integral_constant<int, kSingly>{});
     const int64_t to = (((int64_t)task.own + row) * A.kv_heads + kv) * A.dim;
     const float dk_by = A.scale / lift;
     if (A.k_splits > 1) {
@@ -376,7 +420,7 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
 template <int T, int DP>
 __global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_backward_kernel(const AttnArgs A, const AttnTask* k_tasks, int k_groups) {
     static_assert(kAttnWaves == kAttnKeyWaves, "");
-    constexpr int kKeys = (4 + kAttnKeys / kAttnKeyStep) * AttnTile<DP, kAttnKeyStep>::kBytes + 1024, kQueries = 4 * AttnTile<DP>::kBytes;
+    constexpr int kKeys = (4 + kAttnKeys / kAttnKeyStep) * AttnTile<DP, kAttnKeyStep>::kBytes + 1024 + 8 * kAttnKeyWaves, kQueries = 4 * AttnTile<DP>::kBytes + 8 * kAttnWaves;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeys > kQueries ? kKeys : kQueries];
     if ((int)blockIdx.x < k_groups) {
         AttnArgs K = A;
