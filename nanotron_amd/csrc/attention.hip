@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(const Plan
 // values travel straight into LDS.  The scores of the next tile are made while the exponentials of this one are: products and
 // arithmetic then share a wave's time.
 template <int T, int DP>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_forward_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attention_forward_kernel(const AttnArgs A) {
     typedef AttnTile<DP> Tile;
     __shared__ __attribute__((aligned(1024))) uint8_t sk[2 * Tile::kBytes];
     __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];

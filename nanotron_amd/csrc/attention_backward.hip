@@ -418,7 +418,7 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
 
 // Both in one launch, the workgroups of keys first: they have more to do each, and those of queries fill what they leave of the chip
 template <int T, int DP>
-__global__ __launch_bounds__(64 * kAttnWaves, 2) void attention_backward_kernel(const AttnArgs A, const AttnTask* k_tasks, int k_groups) {
+__global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attention_backward_kernel(const AttnArgs A, const AttnTask* k_tasks, int k_groups) {
     static_assert(kAttnWaves == kAttnKeyWaves, "");
     constexpr int kKeys = (4 + kAttnKeys / kAttnKeyStep) * AttnTile<DP, kAttnKeyStep>::kBytes + 1024 + 8 * kAttnKeyWaves, kQueries = 4 * AttnTile<DP>::kBytes + 8 * kAttnWaves;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kKeys > kQueries ? kKeys : kQueries];

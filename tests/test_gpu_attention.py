@@ -280,6 +280,60 @@ def test_what_is_not_seen_does_not_arrive(dtype, bad):
             assert torch.equal(out[100:], clean[0][100:])
 
 
+@pytest.mark.parametrize("dtype, dim, heads, kv_heads", [(torch.bfloat16, 128, 4, 2), (torch.float16, 80, 2, 2), (torch.float16, 64, 6, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_bad_values_in_several_tiles(dtype, dim, heads, kv_heads, causal):
+    """Values that are not finite, in tiles of several steps, reach the rows that see them and the elements that they are in; what they do not reach is
+    added up in another order, so that it may be off by roundings of what the sums hold on the way, not by more."""
+    lengths, rows = [333, 5, 270], (333 + 5 + 64, 333 + 5 + 200)
+    n, first = sum(lengths), 338
+    q, k, v, do = inputs(n, heads, kv_heads, dim, dtype, seed=8)
+    cu = offsets(lengths)
+    clean = step(q, k, v, do, cu_seqlens=cu, causal=causal)
+    u = U[dtype]
+
+    def same(got, name, at):
+        c = clean[("out", "dq", "dk", "dv").index(name)]
+        near(got[at], c[at].double(), (c[at].double().abs() + 1e-3 + 0.5 * (name != "out") * c.double().abs().max()) * 4 * u, name)
+
+    # a value: its element of the rows behind it, of the heads that share it; gradients of the rows in front of it
+    bad = v.clone()
+    bad[rows[0], 0, 5], bad[rows[1], kv_heads - 1, dim - 1] = math.inf, math.nan
+    out, dq, dk, dv = step(q, k, bad, do, cu_seqlens=cu, causal=causal)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    group = heads // kv_heads
+    hit[rows[0] if causal else first:, :group, 5] = True
+    hit[rows[1] if causal else first:, heads - group:, dim - 1] = True
+    assert torch.equal(~torch.isfinite(out), hit)
+    same(out, "out", ~hit)
+    same(dv[:first], "dv", slice(0, first))
+    if causal:
+        assert torch.isfinite(dq[:rows[0]]).all()
+        same(dq, "dq", slice(first, rows[0]))
+    # a gradient: its element of the values that it saw, in the heads' own
+    bad = do.clone()
+    bad[rows[0], 0, 3] = bad[rows[1], 0, 3] = math.nan
+    out, dq, dk, dv = step(q, k, v, bad, cu_seqlens=cu, causal=causal)
+    hit = torch.zeros(dv.shape, dtype=torch.bool, device=DEV)
+    hit[first:rows[1] + 1 if causal else n, 0, 3] = True
+    assert torch.equal(~torch.isfinite(dv), hit)
+    same(dv, "dv", ~hit)
+    hit = torch.zeros(dq.shape, dtype=torch.bool, device=DEV)
+    hit[rows[0], 0] = hit[rows[1], 0] = True
+    assert torch.equal(~torch.isfinite(dq), hit)
+    hit = torch.zeros(dk.shape, dtype=torch.bool, device=DEV)
+    hit[first:rows[1] + 1 if causal else n, 0] = True
+    assert torch.equal(~torch.isfinite(dk), hit)
+    # a key: the queries that see it
+    bad = k.clone()
+    bad[rows[1], 0, 7] = math.nan
+    out, dq, dk, dv = step(q, bad, v, do, cu_seqlens=cu, causal=causal)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    hit[rows[1] if causal else first:, :group] = True
+    assert torch.equal(~torch.isfinite(out), hit) and torch.equal(~torch.isfinite(dq), hit)
+    same(out, "out", ~hit)
+
+
 @pytest.mark.parametrize("which", [0, 1, 2, 3])
 def test_gradients_beside_a_bad_row(which):
     """A row that is not finite spoils the gradients that the formula says, in its tile too, and no others: keys behind a bad query see nothing of it,
