@@ -38,12 +38,14 @@ Choice choose(const ntops_attention_desc& d) {
     return c;
 }
 
-// Runs that the queries of a tile of keys are cut into.  Two workgroups a CU have room; where tiles and heads of keys are fewer than twice as many, each
-// is cut, but into no less than 8 steps where it is longest (of packed sequences, where one is twice as long as their average).
+// Runs that the queries of a tile of keys are cut into, so that there are workgroups of keys for two and a half a CU (two or three have room, those of queries
+// fill in), but none of less than 10 steps where it is longest (of packed sequences, where one is twice as long as their average).  Backward, us, 32 heads
+// of 128 over 8, for two, two and a half, three and four a CU: 1024 tokens 64, 65, 73, 91; 2048 160, 153, 161, 173; 4096 648, 474, 473, 485.  For
+// 8, 10 and 16 steps at least: 512 tokens of these heads 38, 40, 45; 1500 of 2 heads of 128 47, 45, 41; 1000 of 4 of 64 over one 29, 27, 27.
 int key_splits(const ntops_attention_desc& d) {
     const int64_t rows = std::min(d.q_rows, d.q_rows / d.sequences * (d.cu_q && d.sequences > 1 ? 2 : 1));
     const int64_t units = std::max<int64_t>(1, tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads), steps = (rows + kAttnKeyStep - 1) / kAttnKeyStep * (d.heads / d.kv_heads);
-    return (int)std::max<int64_t>(1, std::min(4 * cu_count() / units, steps / 8));
+    return (int)std::max<int64_t>(1, std::min(5 * cu_count() / 2 / units, steps / 10));
 }
 
 // Tasks of packed sequences: those of queries, and behind them those of keys
