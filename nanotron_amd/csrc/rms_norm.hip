@@ -4,13 +4,15 @@
 //
 // Bound by memory.  A row lives in the registers of the threads that read it, so that both norms cost one read; h is rounded to the type of
 // the residual stream before the second norm reads it, as the backward pass does, which has it from memory.
+// 16384 rows of 4096, bf16 with an fp32 residual stream, both norms and a gate: 805 MB forward in 160 us, 5.0 TB/s, 1208 MB backward in 245, 4.9 TB/s.
 #include "ops_common.h"
 
 namespace ntfp8 {
 namespace {
 
 constexpr int forward_block(int tpr) { return tpr < 256 ? 256 : tpr; }
-// backward: rows enough to fill a CU; with a norm behind the block or a gate half the threads, which then have registers for its vectors
+// backward: rows enough to fill a CU; with a norm behind the block or a gate half the threads, which then have registers for its vectors (both norms
+// and a gate, 16384 x 4096, forward and backward: 404 us, 431 with 1024 threads that read the vectors for every row)
 constexpr int backward_block(int tpr, bool full) { return tpr == 1024 || (tpr >= 256 && !full) ? 1024 : 512; }
 constexpr int kMostPieces = 2;   // 16-byte pieces of a row of x that a thread holds
 enum Gate { kNoGate = 0, kChannelGate = 1, kElementGate = 2 };

@@ -24,6 +24,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: 
     softmax's numerators, and in backward the scores' gradients, are rounded to the type of q for the products they go into.  Rows are read where they are
     if they lie on 16-byte boundaries, else from a copy.  The same inputs give the same bits, forward and backward.  Memory kept for
     the backward pass beside q, k, v and the result: a byte an element of the result and 4 bytes a query and head; freed on return, where queries are few or keys
-    are in the backward pass, partial results of fp32.  ValueError / TypeError for what does not
-    fit; differentiable once."""
+    are in the backward pass, partial results of fp32.  At most 2^27 queries times heads and keys times kv_heads, 2^24 elements from row to row, and
+    (rows / 128 + sequences + 2) * heads up to 2^22.  ValueError / TypeError for what does not fit, RuntimeError beyond these sizes; differentiable once."""
     return _ops.host.attention(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale)
