@@ -488,6 +488,20 @@ def test_another_stream():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_twice_backward_and_inference():
+    q, k, v, do = inputs(300, 4, 2, 80, torch.float16)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    cu = offsets([120, 0, 180])
+    out = attention(*leaves, cu_seqlens=cu)
+    first = torch.autograd.grad(out, leaves, do, retain_graph=True)
+    second = torch.autograd.grad(out, leaves, do)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    with torch.inference_mode():
+        assert torch.equal(attention(*leaves, cu_seqlens=cu), out)
+        few = attention(q[None, :1], k[None], v[None])
+    near(few[0], attention(q[None, :1].detach(), k[None].detach(), v[None].detach())[0].double(), 0.0 * few[0].double(), "one token")
+
+
 def test_a_cache_of_more_than_2_32_bytes():
     """One new token, and a few, over 9 million keys: all of them 0 but some far ones, so the softmax is known in closed form."""
     n, kv, dim = 9_000_000, 2, 128

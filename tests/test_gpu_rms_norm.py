@@ -240,6 +240,47 @@ def test_gradient_against_differences():
             assert abs((up - down) / 2e-5 - g.view(-1)[i].item()) < 1e-4 * (1 + g.abs().max().item())
 
 
+def test_more_than_2_32_bytes():
+    """A block of rows again and again: the same bits in every copy, and the vectors' gradients as many times the block's."""
+    copies, rows, cols = 140, 4000, 4096
+    s, dy, dh = inputs(rows, cols, torch.bfloat16, torch.bfloat16, torch.float32, True, "channel")
+    want = exact({k: v if v.dim() == 1 else v.double() for k, v in s.items()}, check(s, dy, dh)[1], dy, dh, 1.0)
+    one = check(s, dy, dh)
+    many = {k: v.repeat(copies, 1) if v.dim() == 2 else v for k, v in s.items()}
+    assert many["x"].numel() * 2 > 1 << 32
+    many = {k: v.requires_grad_(True) for k, v in many.items()}
+    y, h = residual_rms_norm(many["x"], many["residual"], many["weight"], post_weight=many["post_weight"], gate=many["gate"], eps=EPS)
+    grads = dict(zip(many, torch.autograd.grad((y, h), list(many.values()), (dy.repeat(copies, 1), dh.repeat(copies, 1)))))
+    for c in range(copies):
+        at = slice(c * rows, (c + 1) * rows)
+        assert torch.equal(y[at], one[0]) and torch.equal(h[at], one[1])
+        assert torch.equal(grads["x"][at], one[2]["x"]) and torch.equal(grads["residual"][at], one[2]["residual"])
+    for k in ("weight", "post_weight", "gate"):
+        # the bound of one block, whose sums are of copies times as many rows: a thread adds an eighth of the rows of a 256th of the chip, see exact()
+        near(grads[k], copies * want[k][0], copies * (want[k][1] * copies), k)
+
+
+def test_another_stream_and_twice_backward():
+    s, dy, dh = inputs(257, 640, torch.bfloat16, torch.float32, torch.float32, True, "channel")
+    s = {k: v.requires_grad_(True) for k, v in s.items()}
+
+    def run():
+        return residual_rms_norm(s["x"], s["residual"], s["weight"], post_weight=s["post_weight"], gate=s["gate"], eps=EPS)
+
+    want = run()
+    grads = torch.autograd.grad(want, list(s.values()), (dy, dh), retain_graph=True)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = run()
+        back = torch.autograd.grad(got, list(s.values()), (dy, dh))
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((*got, *back), (*want, *grads)))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, list(s.values()), (dy, dh)), grads))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(run(), want))
+
+
 def test_nothing_to_do():
     x = torch.zeros(0, 16, device=DEV, requires_grad=True)
     w = torch.ones(16, device=DEV, requires_grad=True)

@@ -134,6 +134,40 @@ def test_many_tokens():
     check(q, k, torch.arange(20011, device=DEV), f, scale=1.25)
 
 
+def test_more_than_2_32_bytes():
+    """A block of tokens again and again: every one of its copies turns to the same bits, forward and backward."""
+    copies, tokens, heads, dim = 280, 1000, 64, 128
+    f, _ = rotary_frequencies(dim, device=DEV)
+    block = torch.randn(tokens, heads, dim, device=DEV).bfloat16()
+    q = block.repeat(copies, 1, 1).requires_grad_(True)
+    assert q.numel() * 2 > 1 << 32
+    out = rotary(q, None, torch.arange(tokens, device=DEV).repeat(copies), f)[0]
+    (back,) = torch.autograd.grad(out, q, out.detach())
+    first = check(block, None, torch.arange(tokens, device=DEV), f)[0].detach()
+    for c in range(copies):
+        rows = slice(c * tokens, (c + 1) * tokens)
+        assert torch.equal(out[rows], first)
+        assert torch.equal(back[rows], back[:tokens])
+
+
+def test_another_stream_and_twice_backward():
+    f, _ = rotary_frequencies(64, device=DEV)
+    q, k = (torch.randn(500, h, 64, device=DEV).bfloat16().requires_grad_(True) for h in (4, 2))
+    at = torch.arange(500, device=DEV)
+    want = rotary(q, k, at, f)
+    grads = torch.autograd.grad(want, (q, k), [t.detach() for t in want], retain_graph=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = rotary(q, k, at, f)
+        back = torch.autograd.grad(got, (q, k), [t.detach() for t in got])
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((*got, *back), (*want, *grads)))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, (q, k), [t.detach() for t in want]), grads))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(rotary(q, k, at, f), want))
+
+
 def test_nothing_to_do():
     f, _ = rotary_frequencies(64, device=DEV)
     q = torch.zeros(0, 4, 64, device=DEV, requires_grad=True)
