@@ -374,16 +374,14 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
 #pragma unroll
     for (int e = 0; e < DP / 32; ++e) out[e] = zeros16();
     float top = -__builtin_inff(), sum = 0.0f;
-    for (int j = 0; j < steps; ++j) {
-        const int key0 = (first + j) * kFewStep;
+    // A step's scores and values into the sums.  kSingly: some rows do not see all of its values, which are not finite throughout
+    auto add = [&](int j, bool masked, auto singly_) __attribute__((always_inline)) {
         uint8_t* const k = sk[wave] + (j & 1) * kBytes;
         uint8_t* const v = sv[wave] + (j & 1) * kBytes;
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");   // all but the step requested since
         v16f s = zeros16();
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) s = mfma_attn<T>(tile.rows(k, 0, i), q[i], s);
-        const bool masked = key0 + kFewStep - 1 > min(len - 1, first_last);
-        const int last = min(len - 1, last_row) - key0, last_half = last - 4 * (lane >> 5);
+        const int last = min(len - 1, last_row) - (first + j) * kFewStep, last_half = last - 4 * (lane >> 5);
         if (masked) {
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -407,17 +405,34 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
             sum += s[r];
         }
         const v4i p[2] = {pack_scores<T>(s, 0), pack_scores<T>(s, 8)};
-        if (__builtin_expect(masked && attn_not_finite<T, DP, kFewStep, 1>(v, 0, lane), 0)) {
+        if constexpr (decltype(singly_)::value) {
             add_columns_singly<T, DP, 2>(out, tile, v, p, 0, last + 1);
         } else {
             add_columns<T, DP>(out, tile, v, 0, p[0]);
             add_columns<T, DP>(out, tile, v, 1, p[1]);
         }
+    };
+    auto masked_at = [&](int j) { return (first + j) * kFewStep + kFewStep - 1 > min(len - 1, first_last); };
+    bool left = false;   // a step for later, see above
+    for (int j = 0; j < steps; ++j) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kLoads) : "memory");   // all but the step requested since
+        const bool masked = masked_at(j);
+        if (masked && attn_not_finite<T, DP, kFewStep, 1>(sv[wave] + (j & 1) * kBytes, 0, lane)) left = true;
+        else add(j, masked, std::false_type{});
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the stage has been read
         __builtin_amdgcn_sched_barrier(0);
         load(j + 2);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (the last requests write zeros into stages nobody reads again)
+    if (__builtin_expect(left, 0)) {
+        for (int j = 0; j < steps; ++j) {
+            if (!masked_at(j)) continue;
+            load(j);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (attn_not_finite<T, DP, kFewStep, 1>(sv[wave] + (j & 1) * kBytes, 0, lane)) add(j, true, std::true_type{});
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
     sum = both_sum(sum);
     if (lane < kFewRows) ml[wave][lane] = make_float2(top, sum);
     __syncthreads();

@@ -334,6 +334,29 @@ def test_bad_values_in_several_tiles(dtype, dim, heads, kv_heads, causal):
     same(out, "out", ~hit)
 
 
+@pytest.mark.parametrize("dtype, dim", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 80)])
+@pytest.mark.parametrize("keys", [40, 700])
+def test_bad_values_behind_a_few_tokens(dtype, dim, keys):
+    """Six tokens of a batch over a cache whose last values are not finite: tokens in front of these see nothing of them."""
+    g = torch.Generator().manual_seed(keys)
+    q, k, v = (torch.randn(3, n, h, dim, generator=g).to(dtype).to(DEV) for n, h in ((6, 4), (keys, 2), (keys, 2)))
+    with torch.no_grad():
+        clean = attention(q, k, v)
+        bad = v.clone()
+        bad[1, keys - 3, 1, 4], bad[1, keys - 2, 0, 9] = math.inf, math.nan
+        out = attention(q, k, bad)
+        hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+        hit[1, 3:, 2:, 4] = True
+        hit[1, 4:, :2, 9] = True
+        assert torch.equal(~torch.isfinite(out), hit)
+        # (one score more or less in a sum, in another order)
+        near(out[~hit], clean[~hit].double(), (clean[~hit].double().abs() + v.double().abs().max()) * 4 * U[dtype], "elements beside")
+        bad = k.clone()
+        bad[2, keys - 1] = math.nan
+        out = attention(q, bad, v)
+        assert torch.isfinite(out[:2]).all() and torch.isfinite(out[2, :5]).all() and torch.isnan(out[2, 5]).all()
+
+
 @pytest.mark.parametrize("which", [0, 1, 2, 3])
 def test_gradients_beside_a_bad_row(which):
     """A row that is not finite spoils the gradients that the formula says, in its tile too, and no others: keys behind a bad query see nothing of it,
