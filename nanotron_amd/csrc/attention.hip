@@ -493,28 +493,44 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), pitch = A.q_rows * A.heads;
     if (row >= pitch) return;   // (whole waves)
     const int lane = threadIdx.x & 63, d = (lane & 15) * 8, run = lane >> 4;
-    // every lane's splits, one after another: their largest maximum first
+    // the first splits are asked for before the largest maximum is known: one trip to memory for two
+    constexpr int kAhead = 8;
+    float2 ml[kAhead];
+    v4f part[kAhead][2];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const int s = run + 4 * i;
+        ml[i] = make_float2(-__builtin_inff(), 0.0f);
+        part[i][0] = part[i][1] = (v4f){0, 0, 0, 0};
+        if (s >= A.splits) continue;
+        ml[i] = A.part_ml[s * pitch + row];
+        if (d >= A.dim) continue;
+        const v4f* const p = reinterpret_cast<const v4f*>(A.part + (s * pitch + row) * A.dim + d);
+        part[i][0] = p[0], part[i][1] = p[1];
+    }
+    // every lane's splits, one after another: their largest maximum
     float top = -__builtin_inff();
     for (int s = lane; s < A.splits; s += 64) top = fmaxf(top, A.part_ml[s * pitch + row].x);
 #pragma unroll
     for (int m = 32; m >= 1; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
     float sum = 0.0f, x[8] = {};
-#pragma unroll 4
-    for (int s = run; s < A.splits; s += 4) {
-        const float2 o = A.part_ml[s * pitch + row];
+    auto add = [&](float2 o, v4f a, v4f b) __attribute__((always_inline)) {
         // (an empty split, of which nothing counts; not one whose sum is NaN)
         const bool none = o.x == -__builtin_inff() && o.y == 0.0f;
         const float by = none ? 0.0f : o.x == top ? 1.0f : exp2_fast(o.x - top);
         sum += o.y * by;
-        if (d < A.dim) {
-            const v4f* const p = reinterpret_cast<const v4f*>(A.part + (s * pitch + row) * A.dim + d);
-            const v4f a = p[0], b = p[1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] += a[i] * by;
-                x[4 + i] += b[i] * by;
-            }
+        for (int i = 0; i < 4; ++i) {
+            x[i] += a[i] * by;
+            x[4 + i] += b[i] * by;
         }
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) add(ml[i], part[i][0], part[i][1]);
+    for (int s = run + 4 * kAhead; s < A.splits; s += 4) {
+        const v4f* const p = reinterpret_cast<const v4f*>(A.part + (s * pitch + row) * A.dim + d);
+        if (d < A.dim) add(A.part_ml[s * pitch + row], p[0], p[1]);
+        else add(A.part_ml[s * pitch + row], (v4f){0, 0, 0, 0}, (v4f){0, 0, 0, 0});
     }
 #pragma unroll
     for (int m = 16; m <= 32; m *= 2) {
