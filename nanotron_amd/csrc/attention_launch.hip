@@ -23,10 +23,11 @@ struct Choice {
     int64_t tiles;
 };
 // Rows of a group's heads that a wave's products have columns for, 32, are the few kernel's (us, for it and for the other: a token over 4096 keys, 32
-// heads of 128 over 8, 12.9 and 17.4; 32 such tokens over 8192 191 and 458; 32 tokens of 8 heads over 4096 15.7 and 17.2).  Both cut the keys where
-// there are fewer workgroups than the chip holds, into no less than 128 keys, a step of each of four waves (of 128 and 256 at least: a token over 512
-// keys 10.2 and 11.3, over 4096 12.9 and 12.6), and into no less than 512 keys (512 tokens over 8192 keys 85, 130 uncut, 95 with twice as
-// many runs; of 512 and 256 at least: 512 tokens of 32 heads of 128 24 and 34, 1500 of 2 heads 33 and 30).
+// heads of 128 over 8, 11.1 and 17.4; 32 such tokens over 8192 191 and 458; 32 tokens of 8 heads over 4096 14.2 and 17.2).  Both cut the keys where
+// there are fewer workgroups than the chip holds.  Few rows, into 128 keys at least, a step of each of four waves, and only beyond 512, which four steps
+// take as long as the launch that joins (uncut and cut, over 256 keys 8.4 and 10.4, 512 10.2 and 10.4, 640 11.1 and 10.4; into 128 and 256, 4096
+// keys 11.1 and 11.7).  More rows, into 512 keys at least (512 tokens over 8192 keys 85, 130 uncut, 95 with twice as many runs; of
+// 512 and 256 at least: 512 tokens of 32 heads of 128 24 and 34, 1500 of 2 heads 33 and 30).
 Choice choose(const ntops_attention_desc& d) {
     const int64_t cus = cu_count(), q_len = d.q_rows / d.sequences, k_len = d.k_rows / d.sequences;   // (of packed ones, on average)
     Choice c = {};
@@ -34,7 +35,7 @@ Choice choose(const ntops_attention_desc& d) {
     c.few = !d.cu_q && d.heads / d.kv_heads * q_len <= 32 && d.sequences * d.kv_heads <= ((int64_t)1 << 22);
     if (c.few) {
         const int64_t units = d.sequences * d.kv_heads;
-        c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len / 128));
+        c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len <= 512 ? 1 : k_len / 128));
         return c;
     }
     c.tiles = tiles_of(d, d.q_rows, kAttnQueries);
