@@ -19,8 +19,14 @@ template <int T>
 __device__ __forceinline__ float gradient_lift(const AttnArgs& A) {
     if constexpr (T == NTFP8_BF16) return 1.0f;
     uint32_t q = 0, v = 0;
-    for (int i = threadIdx.x & 63; i < A.most_q; i += 64) q = max(q, A.most[i]);
-    for (int i = threadIdx.x & 63; i < A.most_v; i += 64) v = max(v, A.most[kAttnMost + i]);
+    // (one trip to memory, not one for every 64)
+#pragma unroll
+    for (int n = 0; n < kAttnMost; n += 64) {
+        const int i = n + (threadIdx.x & 63);
+        const uint32_t x = i < A.most_q ? A.most[i] : 0u, y = i < A.most_v ? A.most[kAttnMost + i] : 0u;
+        q = max(q, x);
+        v = max(v, y);
+    }
     const float most = 2.0f * A.dim * __uint_as_float(wave_most(q)) * __uint_as_float(wave_most(v));
     if (!(most > 0.0f) || most > 1e30f || most < 1e-30f) return 1.0f;
     const int e = (int)(__float_as_uint(most) >> 23) - 127;   // 2^e <= most < 2^(e + 1)
