@@ -63,7 +63,8 @@ struct AttnArgs {
     float* k_part;
 };
 
-// the task of tile `t`; the longest come first
+// The task of tile `t`.  Under a causal mask the longest come first; else those of a sequence one behind the other, while its keys are in the L2 (16 sequences
+// of 1024, 16 heads of 128, forward 192 -> 168 us; causal 64 sequences of 512, both passes, would lose 2 %)
 __device__ __forceinline__ AttnTask attn_task(const AttnArgs& A, int t, int tile_rows, bool keys) {
     if (A.tasks) {
         AttnTask r = A.tasks[t];
@@ -77,7 +78,7 @@ __device__ __forceinline__ AttnTask attn_task(const AttnArgs& A, int t, int tile
         return r;
     }
     const int own_len = keys ? A.k_len : A.q_len, len = keys ? A.q_len : A.k_len;
-    const int per = (own_len + tile_rows - 1) / tile_rows, rank = t / A.sequences, seq = t - rank * A.sequences;
+    const int per = (own_len + tile_rows - 1) / tile_rows, seq = A.causal ? t % A.sequences : t / per, rank = A.causal ? t / A.sequences : t % per;
     const int at = (keys ? rank : per - 1 - rank) * tile_rows;
     return {seq * own_len + at, min(tile_rows, own_len - at), seq * len, len, at, seq, keys ? at - (A.k_len - A.q_len) : at + A.k_len - A.q_len, 0};
 }

@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
         for (int i = 0; i < 4; ++i) x[i] = s[g][r + i] = exp2_fast(__builtin_fmaf(s[g][r + i], A.c, -below));
         sum += (x[0] + x[1]) + (x[2] + x[3]);
     };
-    // One tile of keys that every row of the workgroup sees whole, with another behind it.  A wave issues one instruction after another, so their
+    // One tile of keys that every row of the workgroup sees whole.  A wave issues one instruction after another, so their
     // order is set here: between two products of 32 cycles each what is done beside them, and fragments read two pairs of products ahead.
     float most = steps > 0 ? largest() : 0.0f;
     auto whole_step = [&](int j) __attribute__((always_inline)) {
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
             for (int g = 0; g < 4; ++g) add_columns<T, DP>(out, tile, values, g, p[g]);
         }
     };
-    // Any tile: rows that do not see all of it, or nothing behind it.  One with values which are not finite is left for later (of the same tiles, for
+    // Any tile: rows that do not see all of it.  One with values which are not finite is left for later (of the same tiles, for
     // every wave): what such a tile needs would take registers from this loop
     bool left = false;
     auto step = [&](int j) __attribute__((always_inline)) {
@@ -275,8 +275,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
         if (!later) masked(key0, sv + stage, std::false_type{});
         if (j + 1 < steps) scores(sk + other, s);
     };
-    // tiles that every row sees whole, then the others and the last
-    const int whole = min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, clear = min(whole - first, steps - 1);
+    // tiles that every row sees whole (behind the last the next scores are made of zeros, beside its exponentials: less than a tile of its own kind), then the others
+    const int whole = min(task.len, A.causal ? task.shift + 1 : task.len) / kAttnStep, clear = min(whole - first, steps);
     int j = 0;
     for (; j < clear; ++j) whole_step(j);
     for (; j < steps; ++j) step(j);
@@ -295,6 +295,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
             masked(key0, sv, std::true_type{});
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (what was requested behind the last tile lands in this workgroup's LDS)
     const float all = both_sum(sum);
     const int64_t at = (int64_t)task.own + row;
     if (A.splits > 1) {
