@@ -41,22 +41,22 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
     const bool values = (int)blockIdx.x >= q_groups;
     const int own = values ? blockIdx.x - q_groups : blockIdx.x, groups = values ? gridDim.x - q_groups : q_groups;
     const int heads = values ? A.kv_heads : A.heads, own_len = values ? A.k_len : A.q_len;
-    const int64_t rows = values ? A.k_rows : A.q_rows;
+    const uint32_t items = (uint32_t)((values ? A.k_rows : A.q_rows) * heads);   // (2^27 at most)
     const int d = (threadIdx.x & 15) * 8;
     const int* const cu = values ? cu_k : cu_q;
+    const int begin = cu ? cu[0] : 0, end = cu ? cu[A.sequences] : 0;
     uint32_t most = 0;
-    for (int64_t item = (int64_t)own * 16 + (threadIdx.x >> 4); item < rows * heads; item += (int64_t)groups * 16) {
-        const int64_t row = item / heads;
-        const int head = (int)(item - row * heads);
-        const bool live = !cu || (row >= cu[0] && row < cu[A.sequences]);   // rows of no sequence may hold anything
+    for (uint32_t item = (uint32_t)own * 16 + (threadIdx.x >> 4); item < items; item += (uint32_t)groups * 16) {
+        const int row = (int)(item / (uint32_t)heads), head = (int)(item - (uint32_t)row * (uint32_t)heads);
+        const bool live = !cu || (row >= begin && row < end);   // rows of no sequence may hold anything
         float x[8] = {}, y[8] = {}, sum = 0.0f;
         if (live && d < A.dim) {
-            const int seq = A.tasks ? 0 : (int)(row / own_len);
-            const int64_t at = A.tasks ? row : row - (int64_t)seq * own_len;
+            const int seq = A.tasks ? 0 : row / own_len;
+            const int64_t at = A.tasks ? row : row - seq * own_len;
             const int64_t stride = values ? A.v_stride : A.do_stride, batch = values ? A.v_batch : A.do_batch, apart = values ? A.v_head : A.do_head;
             unpack<T, 8>(load_piece<T, 8>(values ? A.v : A.dout, seq * batch + at * stride + head * apart + d), x);
             if (!values) {
-                const int64_t at_out = (row * heads + head) * A.dim + d;
+                const int64_t at_out = (int64_t)item * A.dim + d;
                 unpack<T, 8>(load_piece<T, 8>(A.o, at_out), y);
                 if (A.low) {
                     const v2i_attn low = *reinterpret_cast<const v2i_attn*>(A.low + at_out);
