@@ -328,10 +328,12 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
         // fragments are read two products ahead.  A wave issues one instruction after another, so their order is set here.
         constexpr int kProducts = DP / 16;   // of a run
         v4i fq[3], fg[2], fv[2], p[2], ds[2];
-        auto fetch_q = [&](int i) __attribute__((always_inline)) { fq[i % 3] = tile.rows_anew(sq, at, 0, i); };
+        // (short heads have registers for the fragments' addresses: 8192 causal tokens, 16 heads of 64, both passes 805 -> 768 us)
+        auto rows = [&](uint8_t* array, int begin, int i) __attribute__((always_inline)) { return DP == 64 ? tile.rows(array + begin, 0, i) : tile.rows_anew(array, begin, 0, i); };
+        auto fetch_q = [&](int i) __attribute__((always_inline)) { fq[i % 3] = rows(sq, at, i); };
         auto fetch_g = [&](int i) __attribute__((always_inline)) {
-            fg[i & 1] = tile.rows_anew(sg, at, 0, i);
-            fv[i & 1] = tile.rows_anew(sv, mine, 0, i);
+            fg[i & 1] = rows(sg, at, i);
+            fv[i & 1] = rows(sv, mine, i);
         };
         fetch_q(0);
         fetch_q(1);
@@ -348,7 +350,11 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
         };
         v4i fa[3];
         // fragment x of the products for dv, and those for dk behind them
-        auto fetch_a = [&](int x) __attribute__((always_inline)) { fa[x % 3] = tile.columns_anew(x < kProducts ? sg : sq, at, x % kProducts / (DP / 32), x % (DP / 32)); };
+        auto fetch_a = [&](int x) __attribute__((always_inline)) {
+            uint8_t* const from = x < kProducts ? sg : sq;
+            const int block = x % kProducts / (DP / 32), e = x % (DP / 32);
+            fa[x % 3] = DP == 64 ? tile.columns(from + at, block, e) : tile.columns_anew(from, at, block, e);
+        };
 #pragma unroll
         for (int i = 0; i < kProducts; ++i) {
             if (i + 1 < kProducts) fetch_g(i + 1);
