@@ -3,7 +3,7 @@
 // One kernel owns queries and makes dq, one owns keys and makes dk and dv; both make the scores again, seven products where five
 // would do, so that every sum is made in one place and order: no atomics, the same bits for the same inputs.
 //
-// Bound by the products: 16384 causal tokens, 32 heads of 128 over 8, in bf16 take 6.4 ms, 0.86 PFLOP/s of the five products and 1.2 of the seven that are
+// Bound by the products: 16384 causal tokens, 32 heads of 128 over 8, in bf16 take 6.4 to 6.8 ms, 0.86 PFLOP/s of the five products and 1.2 of the seven that are
 // made, 71 % of the matrix instructions' slots at the 1.5 GHz that the power limit leaves; 4096 tokens 431 us.  delta is memory, 4.8 TB/s.
 //
 // fp16: ds is a gradient and may be smaller than that type's normal numbers, and p in a long row is.  p is kept times 2^8, ds
