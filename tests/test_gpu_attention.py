@@ -283,18 +283,16 @@ def test_what_is_not_seen_does_not_arrive(dtype, bad):
 @pytest.mark.parametrize("dtype, dim, heads, kv_heads", [(torch.bfloat16, 128, 4, 2), (torch.float16, 80, 2, 2), (torch.float16, 64, 6, 1)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_bad_values_in_several_tiles(dtype, dim, heads, kv_heads, causal):
-    """Values that are not finite, in tiles of several steps, reach the rows that see them and the elements that they are in; what they do not reach is
-    added up in another order, so that it may be off by roundings of what the sums hold on the way, not by more."""
+    """Values that are not finite, in tiles of several steps, reach the rows that see them and the elements that they are in, and nothing else."""
     lengths, rows = [333, 5, 270], (333 + 5 + 64, 333 + 5 + 200)
     n, first = sum(lengths), 338
     q, k, v, do = inputs(n, heads, kv_heads, dim, dtype, seed=8)
     cu = offsets(lengths)
-    clean = step(q, k, v, do, cu_seqlens=cu, causal=causal)
-    u = U[dtype]
+    want, bound = exact(q, k, v, do, [(x, x) for x in lengths], causal)
 
     def same(got, name, at):
-        c = clean[("out", "dq", "dk", "dv").index(name)]
-        near(got[at], c[at].double(), (c[at].double().abs() + 1e-3 + 0.5 * (name != "out") * c.double().abs().max()) * 4 * u, name)
+        i = ("out", "dq", "dk", "dv").index(name)
+        near(got[at], want[i][at], bound[i][at], name)
 
     # a value: its element of the rows behind it, of the heads that share it; gradients of the rows in front of it
     bad = v.clone()
@@ -341,7 +339,6 @@ def test_bad_values_behind_a_few_tokens(dtype, dim, keys):
     g = torch.Generator().manual_seed(keys)
     q, k, v = (torch.randn(3, n, h, dim, generator=g).to(dtype).to(DEV) for n, h in ((6, 4), (keys, 2), (keys, 2)))
     with torch.no_grad():
-        clean = attention(q, k, v)
         bad = v.clone()
         bad[1, keys - 3, 1, 4], bad[1, keys - 2, 0, 9] = math.inf, math.nan
         out = attention(q, k, bad)
@@ -349,8 +346,9 @@ def test_bad_values_behind_a_few_tokens(dtype, dim, keys):
         hit[1, 3:, 2:, 4] = True
         hit[1, 4:, :2, 9] = True
         assert torch.equal(~torch.isfinite(out), hit)
-        # (one score more or less in a sum, in another order)
-        near(out[~hit], clean[~hit].double(), (clean[~hit].double().abs() + v.double().abs().max()) * 4 * U[dtype], "elements beside")
+        flat = [t.flatten(0, 1) for t in (q, k, v)]
+        want, bound = exact(*flat, torch.zeros_like(flat[0]), [(6, keys)] * 3)
+        near(out[~hit], want[0].view_as(out)[~hit], bound[0].view_as(out)[~hit], "elements beside")
         bad = k.clone()
         bad[2, keys - 1] = math.nan
         out = attention(q, bad, v)
@@ -587,6 +585,18 @@ def test_many_short_sequences():
     for o, a, name in zip(got, exact_, ("out", "dq", "dk", "dv")):
         # (sequences of three: the bound of a rounding of every operand, twice)
         assert ((o.double() - a).norm() / a.norm()).item() < 4 * U[q.dtype], name
+
+
+def test_sequences_of_every_length_beside_each_other():
+    """1500 sequences of 0 to 140 rows and a few of many tiles: more than a lane of the plan's kernel each, of one tile and of several."""
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 141, (1500,), generator=g).tolist()
+    lengths[7], lengths[1023], lengths[1024], lengths[1499] = 700, 1300, 129, 257
+    n = sum(lengths)
+    q, k, v, do = inputs(n, 1, 1, 64, torch.bfloat16, seed=6)
+    cu = offsets(lengths)
+    for causal in (True, False):
+        check(q, k, v, do, [(x, x) for x in lengths], causal, cu_seqlens=cu)
 
 
 def test_refusals():
