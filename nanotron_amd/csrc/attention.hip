@@ -163,6 +163,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
         vs.load(sv, first * kAttnStep, task.len, wave);
         scores(sk, s);
     }
+    const bool idle = wave * 32 >= task.rows;   // a wave without rows brings its part of the tiles
     const int lead = task.shift + wave * 32;                                            // the last key that the wave's first row sees
     const int last_key = A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1;   // and that this lane's does
     // a row's maximum of a tile's scores, in two chains
@@ -204,6 +205,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
         wg_barrier();
         ks.load(sk + stage, key0 + 2 * kAttnStep, task.len, wave);
         vs.load(sv + other, key0 + kAttnStep, task.len, wave);
+        if (idle) return;
         const float below = raise(most);
         constexpr int kPairs = DP / 16;   // of products of the next scores
         v4i fk[3][2], p[4];
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
         }
         const bool later = attn_any_wave(odd[j & 1]);
         left |= later;
-        if (A.causal && key0 > lead + 31) return;   // (uniform in the wave; so are the tiles behind this one)
+        if (idle || (A.causal && key0 > lead + 31)) return;   // (uniform in the wave; so are the tiles behind this one)
         if (!later) masked(key0, sv + stage, std::false_type{});
         if (j + 1 < steps) scores(sk + other, s);
     };

@@ -145,6 +145,7 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
             left |= not_finite;
             if (not_finite != (kHow == kSingly)) return;
         }
+        if (wave * 32 >= task.rows) return;   // (without rows, it brings its part of the tiles)
         const int lead = task.shift + wave * 32;   // the last key that the wave's first row sees
         if (kMask && A.causal && key0 > lead + 31) return;   // (uniform in the wave)
         const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0, last_half = last - 4 * (lane >> 5);
@@ -310,6 +311,7 @@ __device__ __forceinline__ void attention_dkv(const AttnArgs& A, int group, uint
             left |= not_finite;
             if (not_finite != (kHow == kSingly)) return;
         }
+        if (wave * 32 >= task.rows) return;
         const int lead = task.shift + wave * 32;   // the first query that sees the wave's first key
         if (kMask && A.causal && row0 + kAttnKeyStep - 1 < lead) return;
         const int from = A.causal ? lead + (lane & 31) - row0 : 0, to = task.len - row0, half = 4 * (lane_anew() >> 5);   // rows of the tile that see this lane's key
