@@ -184,7 +184,8 @@ int ntops_rotary(const ntops_rotary_desc* d, void* stream);
  * out_low (as out, a byte an element, aligned to 8; may be NULL): what a forward call's rounding of out left out, 8 more bits of
  * significand, with which a backward call's dq and dk lose less.
  * workspace: ntops_attention_workspace(d, backward) bytes, aligned to 256.  plan (packed sequences, may be NULL): ntops_attention_plan(d) bytes,
- * aligned to 256, that a forward call fills and the backward call of the same sizes and offsets reads; without it each makes its own.
+ * aligned to 256, that a forward call fills and the backward call of the same sizes and offsets reads; without it each makes its own (in its
+ * workspace, which is the larger for it).
  * Backward: dq, dk, dv (dense, dtype, each may be NULL) from dout (strides as q's) and the q, k, v, out and lse of the forward call.
  * The same inputs give the same bits.  fp16: p and ds are kept with powers of two on them, so that gradients below its normal range survive. */
 typedef struct ntops_attention_desc {

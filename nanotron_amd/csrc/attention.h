@@ -42,6 +42,7 @@ struct AttnArgs {
     int64_t q_batch, k_batch, v_batch, do_batch;       // and sequences of equal lengths
     const AttnTask* tasks;                             // or NULL: `sequences` of q_len and k_len rows
     int64_t tiles;
+    int tile_heads;   // heads of a group that the waves of a workgroup take (of 32 queries), 1: all its waves take one (of 128)
     int sequences, q_len, k_len;
     int64_t q_rows, k_rows;
     int heads, kv_heads, group, dim, causal;
@@ -63,6 +64,7 @@ struct AttnArgs {
     float* k_part;
 };
 
+__host__ __device__ constexpr int attn_chunks(int group, int tile_heads) { return (group + tile_heads - 1) / tile_heads; }
 // The task of tile `t`.  Under a causal mask the longest come first; else those of a sequence one behind the other, while its keys are in the L2 (16 sequences
 // of 1024, 16 heads of 128, forward 192 -> 168 us; causal 64 sequences of 512, both passes, would lose 2 %)
 __device__ __forceinline__ AttnTask attn_task(const AttnArgs& A, int t, int tile_rows, bool keys) {

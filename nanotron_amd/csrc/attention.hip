@@ -120,8 +120,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
     __shared__ __attribute__((aligned(16))) int odd[2][kAttnWaves];   // [stage]: a wave's part of the values is not finite throughout
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // heads that share keys go to one XCD: workgroups are dealt to the eight in turn
-    const int t = blockIdx.x / A.heads, pick = blockIdx.x - t * A.heads;
-    const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
+    const bool shared = A.tile_heads > 1;   // the waves take heads of their own (the last ones may have none) and the same queries
+    const int picks = A.kv_heads * attn_chunks(A.group, A.tile_heads), t = blockIdx.x / picks, pick = blockIdx.x - t * picks;
+    const int kv = pick % A.kv_heads, inside = pick / A.kv_heads * A.tile_heads + (shared ? wave : 0), head = kv * A.group + inside, wave_row = shared ? 0 : wave * 32;
     const AttnTask task = attn_task(A, t, kAttnQueries, false);
     if (task.rows <= 0) return;
     const int64_t q0 = attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head;
@@ -140,8 +141,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
     ks.init(A.k, k0, A.k_stride, A.dim, wave, lane);
     vs.init(A.v, v0, A.v_stride, A.dim, wave, lane);
     if (steps > 0) ks.load(sk, first * kAttnStep, task.len, wave);
-    const int row = wave * 32 + (lane & 31);
-    const bool live = row < task.rows;
+    const int row = wave_row + (lane & 31);
+    const bool live = row < task.rows && inside < A.group;
     v4i q[DP / 16];
     load_own<DP>(q, A.q, q0 + row * A.q_stride, A.dim, live, lane);
     v16f out[DP / 32], s[2];
@@ -163,8 +164,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
         vs.load(sv, first * kAttnStep, task.len, wave);
         scores(sk, s);
     }
-    const bool idle = wave * 32 >= task.rows;   // a wave without rows brings its part of the tiles
-    const int lead = task.shift + wave * 32;                                            // the last key that the wave's first row sees
+    const bool idle = wave_row >= task.rows || inside >= A.group;   // a wave without rows brings its part of the tiles
+    const int lead = task.shift + wave_row;                                             // the last key that the wave's first row sees
     const int last_key = A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1;   // and that this lane's does
     // a row's maximum of a tile's scores, in two chains
     auto largest = [&]() __attribute__((always_inline)) {
@@ -574,7 +575,7 @@ int run_attention_plan(const int* cu_q, const int* cu_k, int sequences, int q_ro
 int run_attention_forward_kernels(const AttnArgs& A, int dtype, bool few, hipStream_t st) {
     return with_attn(dtype, A.dim, [&](auto t, auto d) {
         constexpr int T = decltype(t)::value, DP = decltype(d)::value;
-        const dim3 grid((unsigned)(few ? (int64_t)A.sequences * A.kv_heads : A.tiles * A.heads), (unsigned)A.splits);
+        const dim3 grid((unsigned)(few ? (int64_t)A.sequences * A.kv_heads : A.tiles * A.kv_heads * attn_chunks(A.group, A.tile_heads)), (unsigned)A.splits);
         if (few) attention_few_kernel<T, DP><<<grid, 64 * kAttnWaves, 0, st>>>(A);
         else attention_forward_kernel<T, DP><<<grid, 64 * kAttnWaves, 0, st>>>(A);
         if (const int rc = launch_status(); rc != NTFP8_OK || A.splits <= 1) return rc;

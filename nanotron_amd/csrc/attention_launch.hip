@@ -19,7 +19,7 @@ int64_t tiles_of(const ntops_attention_desc& d, int64_t rows, int64_t tile) {
 
 struct Choice {
     bool few;
-    int splits;
+    int splits, queries, tile_heads;
     int64_t tiles;
 };
 // Rows of a group's heads that a wave's products have columns for, 32, are the few kernel's (us, for it and for the other: a token over 4096 keys, 32
@@ -31,15 +31,18 @@ struct Choice {
 Choice choose(const ntops_attention_desc& d) {
     const int64_t cus = cu_count(), q_len = d.q_rows / d.sequences, k_len = d.k_rows / d.sequences;   // (of packed ones, on average)
     Choice c = {};
-    c.splits = 1;
+    c.splits = 1, c.queries = kAttnQueries, c.tile_heads = 1;
     c.few = !d.cu_q && d.heads / d.kv_heads * q_len <= 32 && d.sequences * d.kv_heads <= ((int64_t)1 << 22);
     if (c.few) {
         const int64_t units = d.sequences * d.kv_heads;
         c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len <= 512 ? 1 : k_len / 128));
         return c;
     }
-    c.tiles = tiles_of(d, d.q_rows, kAttnQueries);
-    const int64_t groups = c.tiles * d.heads, room = 2 * cus;
+    const int group = d.heads / d.kv_heads;
+    const bool shared = d.cu_q && !d.plan && group >= 3 && q_len <= 32;
+    c.queries = shared ? 32 : kAttnQueries, c.tile_heads = shared ? kAttnWaves : 1;
+    c.tiles = tiles_of(d, d.q_rows, c.queries);
+    const int64_t groups = c.tiles * d.kv_heads * attn_chunks(group, c.tile_heads), room = 2 * cus;
     if (groups < room) c.splits = (int)std::max<int64_t>(1, std::min(room / groups, k_len / 512));
     return c;
 }
@@ -58,8 +61,8 @@ int key_splits(const ntops_attention_desc& d) {
 struct Plan {
     int64_t q_tiles, k_tiles, keys_at, bytes;
 };
-Plan plan_of(const ntops_attention_desc& d) {
-    Plan p = {tiles_of(d, d.q_rows, kAttnQueries), tiles_of(d, d.k_rows, kAttnKeys), 0, 0};
+Plan plan_of(const ntops_attention_desc& d, int queries = kAttnQueries) {
+    Plan p = {tiles_of(d, d.q_rows, queries), tiles_of(d, d.k_rows, kAttnKeys), 0, 0};
     p.keys_at = up(p.q_tiles * (int64_t)sizeof(AttnTask), 256);
     p.bytes = p.keys_at + up(p.k_tiles * (int64_t)sizeof(AttnTask), 256);
     return p;
@@ -76,7 +79,7 @@ Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c) 
         at += up(bytes, 256);
         return here;
     };
-    l.plan = take(d.cu_q && !d.plan ? plan_of(d).bytes : 0);
+    l.plan = take(d.cu_q && !d.plan ? plan_of(d, backward ? kAttnQueries : c.queries).bytes : 0);
     if (backward) {
         l.delta = take(d.q_rows * d.heads * 4);
         l.most = take(d.dtype == NTFP8_F16 ? 2 * kAttnMost * 4 : 0);
@@ -109,18 +112,24 @@ AttnArgs args_of(const ntops_attention_desc& d) {
 // What a launch has to hold: workgroups, and threads, in 32 bits
 bool attention_fits(const ntops_attention_desc& d) {
     constexpr int64_t kMost = (int64_t)1 << 22;
-    return choose(d).tiles * d.heads <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
+    return choose(d).tiles * d.kv_heads * attn_chunks(d.heads / d.kv_heads, choose(d).tile_heads) <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
 }
 
 int64_t attention_plan(const ntops_attention_desc& d) { return d.cu_q ? plan_of(d).bytes : 0; }
 
-int64_t attention_workspace(const ntops_attention_desc& d, bool backward) { return layout_of(d, backward, choose(d)).bytes; }
+int64_t attention_workspace(const ntops_attention_desc& d, bool backward) {
+    if (backward) return layout_of(d, true, {}).bytes;
+    // (what a forward call takes differs with a plan, which its descriptor may have got since)
+    ntops_attention_desc with = d, without = d;
+    with.plan = reinterpret_cast<void*>(256), without.plan = nullptr;
+    return std::max(layout_of(with, false, choose(with)).bytes, layout_of(without, false, choose(without)).bytes);
+}
 
 namespace {
 // the tasks of a call's sequences at `at`; those of keys where a backward pass reads them
-int make_plan(const ntops_attention_desc& d, char* at, bool keys, hipStream_t st) {
-    const Plan p = plan_of(d);
-    return run_attention_plan(d.cu_q, d.cu_k, (int)d.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, kAttnQueries, kAttnKeys, (int)p.q_tiles, (int)p.k_tiles,
+int make_plan(const ntops_attention_desc& d, char* at, int queries, bool keys, hipStream_t st) {
+    const Plan p = plan_of(d, queries);
+    return run_attention_plan(d.cu_q, d.cu_k, (int)d.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, queries, kAttnKeys, (int)p.q_tiles, (int)p.k_tiles,
                               reinterpret_cast<AttnTask*>(at), keys ? reinterpret_cast<AttnTask*>(at + p.keys_at) : nullptr, st);
 }
 }  // namespace
@@ -130,12 +139,12 @@ int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
     const Layout l = layout_of(d, false, c);
     char* const ws = static_cast<char*>(d.workspace);
     AttnArgs a = args_of(d);
-    a.tiles = c.tiles, a.splits = c.splits;
+    a.tiles = c.tiles, a.splits = c.splits, a.tile_heads = c.tile_heads;
     if (c.splits > 1) a.part = reinterpret_cast<float*>(ws + l.part), a.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
     if (d.cu_q) {
         char* const plan = d.plan ? static_cast<char*>(d.plan) : ws + l.plan;
         a.tasks = reinterpret_cast<AttnTask*>(plan);
-        if (const int rc = make_plan(d, plan, d.plan != nullptr, st)) return rc;
+        if (const int rc = make_plan(d, plan, c.queries, d.plan != nullptr, st)) return rc;
     }
     return run_attention_forward_kernels(a, d.dtype, c.few, st);
 }
@@ -154,7 +163,7 @@ int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
         a.tasks = reinterpret_cast<AttnTask*>(plan);
         k_list = reinterpret_cast<AttnTask*>(plan + p.keys_at);
         if (!d.plan)
-            if (const int rc = make_plan(d, plan, true, st)) return rc;
+            if (const int rc = make_plan(d, plan, kAttnQueries, true, st)) return rc;
     }
     return run_attention_backward_kernels(a, k_list, p.k_tiles, d.cu_q, d.cu_k, d.dtype, st);
 }

@@ -567,6 +567,33 @@ def test_rows_far_apart():
     assert torch.equal(attention(view, k[:4], v[:4]), attention(q[:4], k[:4], v[:4]))
 
 
+@pytest.mark.parametrize("heads, kv_heads, dim", [(8, 2, 128), (6, 2, 64), (5, 1, 80), (12, 2, 64), (4, 4, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_tokens_over_caches_of_different_lengths(heads, kv_heads, dim, causal):
+    """Packed sequences of a few queries each over keys of their own, and one of many queries between them, without gradients."""
+    lengths = [(1, 900), (1, 1), (0, 50), (3, 0), (2, 65), (1, 2000), (33, 40), (1, 64), (7, 3), (90, 300), (1, 129), (1, 511), (1, 7), (1, 70), (2, 2), (1, 1)]
+    for dtype in (torch.bfloat16, torch.float16):
+        n, m = sum(a for a, _ in lengths), sum(b for _, b in lengths)
+        q, k, v, do = inputs(n, heads, kv_heads, dim, dtype, keys=m, seed=heads)
+        want, bound = exact(q, k, v, do, lengths, causal)
+        with torch.no_grad():
+            out = attention(q, k, v, cu_seqlens=offsets(lengths), cu_seqlens_k=offsets(lengths, 1), causal=causal)
+        near(out, want[0], bound[0], "out")
+        # a cache that is not finite (the one key of the second sequence) is that of its own queries
+        bad = v.clone()
+        bad[900] = math.nan
+        with torch.no_grad():
+            other = attention(q, k, bad, cu_seqlens=offsets(lengths), cu_seqlens_k=offsets(lengths, 1), causal=causal)
+        rows = torch.arange(n, device=DEV) != 1
+        assert torch.equal(other[rows], out[rows]) and not torch.isfinite(other[1]).any()
+        # rows of no sequence
+        pad = torch.full((40, heads, dim), math.inf, dtype=dtype, device=DEV)
+        with torch.no_grad():
+            more = attention(torch.cat([q, pad]), k, v, cu_seqlens=offsets(lengths), cu_seqlens_k=offsets(lengths, 1), causal=causal)
+        near(more[:n], want[0], bound[0], "out")
+        assert not more[n:].any()
+
+
 def test_many_short_sequences():
     """More sequences than a workgroup of the plan has threads."""
     g = torch.Generator().manual_seed(1)
