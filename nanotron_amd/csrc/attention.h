@@ -84,6 +84,17 @@ __device__ __forceinline__ AttnTask attn_task(const AttnArgs& A, int t, int tile
     const int at = (keys ? rank : per - 1 - rank) * tile_rows;
     return {seq * own_len + at, min(tile_rows, own_len - at), seq * len, len, at, seq, keys ? at - (A.k_len - A.q_len) : at + A.k_len - A.q_len, 0};
 }
+// What a wave of the kernels that own queries has: tile, head of keys, head inside its group, first row in the tile.  Either its workgroup's waves share a head
+// and take 32 of 128 rows each, or the same 32 rows of heads of their own (the last ones may have none).  Heads that share keys go to one XCD:
+// workgroups are dealt to the eight in turn.
+struct AttnOwn {
+    int tile, kv, inside, row;
+};
+__device__ __forceinline__ AttnOwn attn_own(const AttnArgs& A, int group, int wave) {
+    const bool shared = A.tile_heads > 1;
+    const int picks = A.kv_heads * attn_chunks(A.group, A.tile_heads), tile = group / picks, pick = group - tile * picks, chunk = pick / A.kv_heads;
+    return {tile, pick - chunk * A.kv_heads, chunk * A.tile_heads + (shared ? wave : 0), shared ? 0 : wave * 32};
+}
 // element offset of a run of rows: packed ones are counted over all sequences, others within theirs
 __device__ __forceinline__ int64_t attn_rows(const AttnArgs& A, int64_t packed, int seq, int at, int64_t stride, int64_t batch) {
     return A.tasks ? packed * stride : seq * batch + at * stride;

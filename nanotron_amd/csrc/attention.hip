@@ -119,11 +119,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
     __shared__ __attribute__((aligned(1024))) uint8_t sv[2 * Tile::kBytes];
     __shared__ __attribute__((aligned(16))) int odd[2][kAttnWaves];   // [stage]: a wave's part of the values is not finite throughout
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // heads that share keys go to one XCD: workgroups are dealt to the eight in turn
-    const bool shared = A.tile_heads > 1;   // the waves take heads of their own (the last ones may have none) and the same queries
-    const int picks = A.kv_heads * attn_chunks(A.group, A.tile_heads), t = blockIdx.x / picks, pick = blockIdx.x - t * picks;
-    const int kv = pick % A.kv_heads, inside = pick / A.kv_heads * A.tile_heads + (shared ? wave : 0), head = kv * A.group + inside, wave_row = shared ? 0 : wave * 32;
-    const AttnTask task = attn_task(A, t, kAttnQueries, false);
+    const AttnOwn own = attn_own(A, blockIdx.x, wave);
+    const int kv = own.kv, inside = own.inside, head = kv * A.group + inside, wave_row = own.row;
+    const AttnTask task = attn_task(A, own.tile, A.tile_heads > 1 ? 32 : kAttnQueries, false);
     if (task.rows <= 0) return;
     const int64_t q0 = attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head;
     const int64_t k0 = attn_rows(A, task.other, task.seq, 0, A.k_stride, A.k_batch) + kv * A.k_head;

@@ -93,9 +93,9 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
     uint8_t *const sk = lds, *const sv = lds + 2 * Tile::kBytes;
     int(*const odd)[kAttnWaves] = reinterpret_cast<int(*)[kAttnWaves]>(lds + 4 * Tile::kBytes);   // [stage]: a wave's part of the keys is not finite throughout
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = group / A.heads, pick = group - t * A.heads;
-    const int kv = pick % A.kv_heads, head = kv * A.group + pick / A.kv_heads;
-    const AttnTask task = attn_task(A, t, kAttnQueries, false);
+    const AttnOwn own = attn_own(A, group, wave);
+    const int kv = own.kv, head = kv * A.group + own.inside;
+    const AttnTask task = attn_task(A, own.tile, A.tile_heads > 1 ? 32 : kAttnQueries, false);
     if (task.rows <= 0) return;
     const int64_t k0 = attn_rows(A, task.other, task.seq, 0, A.k_stride, A.k_batch) + kv * A.k_head;
     const int64_t v0 = attn_rows(A, task.other, task.seq, 0, A.v_stride, A.v_batch) + kv * A.v_head;
@@ -109,8 +109,8 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
         ks.load(sk, 0, task.len, wave);
         vs.load(sv, 0, task.len, wave);
     }
-    const int row = wave * 32 + (lane & 31);
-    const bool live = row < task.rows;
+    const int row = own.row + (lane & 31);
+    const bool live = row < task.rows && own.inside < A.group;
     v4i q[DP / 16], g[DP / 16];
     load_own<DP>(q, A.q, attn_rows(A, task.own, task.seq, task.at, A.q_stride, A.q_batch) + head * A.q_head + row * A.q_stride, A.dim, live, lane);
     load_own<DP>(g, A.dout, attn_rows(A, task.own, task.seq, task.at, A.do_stride, A.do_batch) + head * A.do_head + row * A.do_stride, A.dim, live, lane);
@@ -145,8 +145,8 @@ __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8
             left |= not_finite;
             if (not_finite != (kHow == kSingly)) return;
         }
-        if (wave * 32 >= task.rows) return;   // (without rows, it brings its part of the tiles)
-        const int lead = task.shift + wave * 32;   // the last key that the wave's first row sees
+        if (own.row >= task.rows || own.inside >= A.group) return;   // (without rows, it brings its part of the tiles)
+        const int lead = task.shift + own.row;   // the last key that the wave's first row sees
         if (kMask && A.causal && key0 > lead + 31) return;   // (uniform in the wave)
         const int last = (A.causal ? min(task.len - 1, lead + (lane & 31)) : task.len - 1) - key0, last_half = last - 4 * (lane >> 5);
         // Runs of products, of two blocks of 32 keys: scores and dout v^T of the one, of the other, then dq; beside each the arithmetic of the run
@@ -481,7 +481,7 @@ int run_attention_backward_kernels(const AttnArgs& A, const AttnTask* k_tasks, i
         if (const int rc = launch_status(); rc != NTFP8_OK) return rc;
         const bool keys = A.dk || A.dv;
         const int64_t k_groups = keys ? k_tiles * A.kv_heads * A.k_splits : 0;
-        const int64_t groups = k_groups + (A.dq ? A.tiles * A.heads : 0);
+        const int64_t groups = k_groups + (A.dq ? A.tiles * A.kv_heads * attn_chunks(A.group, A.tile_heads) : 0);
         if (groups == 0) return (int)NTFP8_OK;   // (no keys, and dq not asked for)
         attention_backward_kernel<T, DP><<<(unsigned)groups, 64 * kAttnWaves, 0, st>>>(B, k_tasks, (int)k_groups);
         if (const int rc = launch_status(); rc != NTFP8_OK) return rc;

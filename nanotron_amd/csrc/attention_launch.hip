@@ -17,9 +17,22 @@ int64_t tiles_of(const ntops_attention_desc& d, int64_t rows, int64_t tile) {
     return d.sequences * ((rows / d.sequences + tile - 1) / tile);
 }
 
+// Heads of a group whose 32 queries a workgroup's waves take, or 1, and 128 queries of that one: what leaves fewer waves without rows; of packed sequences,
+// whose tiles end anywhere, also where that is equal, up to a length that makes no difference.  (us: a token of 32 sequences over 8192 keys each, packed, 32
+// heads of 128 over 8, 214 and 385 by one head; 64 causal sequences of 16384 tokens, forward 131 and 147, both passes 525 and 560; 4 sequences of 64
+// over 2000 keys 31 and 36.  64 causal sequences of a batch of 512, equal waves: 302 and 290.)
+constexpr int64_t kSharedRows = 1024;
+int tile_heads_of(const ntops_attention_desc& d) {
+    const int64_t rows = std::max<int64_t>(1, d.q_rows / d.sequences);   // (of packed ones, on average)
+    const int group = d.heads / d.kv_heads;
+    const int64_t apart = (rows + 31) / 32 * attn_chunks(group, kAttnWaves), one = (rows + kAttnQueries - 1) / kAttnQueries * group;
+    return group > 1 && rows <= kSharedRows && (apart < one || (d.cu_q && apart == one)) ? kAttnWaves : 1;
+}
+int queries_of(const ntops_attention_desc& d) { return tile_heads_of(d) > 1 ? 32 : kAttnQueries; }
+
 struct Choice {
     bool few;
-    int splits, queries, tile_heads;
+    int splits;
     int64_t tiles;
 };
 // Rows of a group's heads that a wave's products have columns for, 32, are the few kernel's (us, for it and for the other: a token over 4096 keys, 32
@@ -31,18 +44,15 @@ struct Choice {
 Choice choose(const ntops_attention_desc& d) {
     const int64_t cus = cu_count(), q_len = d.q_rows / d.sequences, k_len = d.k_rows / d.sequences;   // (of packed ones, on average)
     Choice c = {};
-    c.splits = 1, c.queries = kAttnQueries, c.tile_heads = 1;
+    c.splits = 1;
     c.few = !d.cu_q && d.heads / d.kv_heads * q_len <= 32 && d.sequences * d.kv_heads <= ((int64_t)1 << 22);
     if (c.few) {
         const int64_t units = d.sequences * d.kv_heads;
         c.splits = (int)std::max<int64_t>(1, std::min((cus + units - 1) / units, k_len <= 512 ? 1 : k_len / 128));
         return c;
     }
-    const int group = d.heads / d.kv_heads;
-    const bool shared = d.cu_q && !d.plan && group >= 3 && q_len <= 32;
-    c.queries = shared ? 32 : kAttnQueries, c.tile_heads = shared ? kAttnWaves : 1;
-    c.tiles = tiles_of(d, d.q_rows, c.queries);
-    const int64_t groups = c.tiles * d.kv_heads * attn_chunks(group, c.tile_heads), room = 2 * cus;
+    c.tiles = tiles_of(d, d.q_rows, queries_of(d));
+    const int64_t groups = c.tiles * d.kv_heads * attn_chunks(d.heads / d.kv_heads, tile_heads_of(d)), room = 2 * cus;
     if (groups < room) c.splits = (int)std::max<int64_t>(1, std::min(room / groups, k_len / 512));
     return c;
 }
@@ -61,8 +71,8 @@ int key_splits(const ntops_attention_desc& d) {
 struct Plan {
     int64_t q_tiles, k_tiles, keys_at, bytes;
 };
-Plan plan_of(const ntops_attention_desc& d, int queries = kAttnQueries) {
-    Plan p = {tiles_of(d, d.q_rows, queries), tiles_of(d, d.k_rows, kAttnKeys), 0, 0};
+Plan plan_of(const ntops_attention_desc& d) {
+    Plan p = {tiles_of(d, d.q_rows, queries_of(d)), tiles_of(d, d.k_rows, kAttnKeys), 0, 0};
     p.keys_at = up(p.q_tiles * (int64_t)sizeof(AttnTask), 256);
     p.bytes = p.keys_at + up(p.k_tiles * (int64_t)sizeof(AttnTask), 256);
     return p;
@@ -79,7 +89,7 @@ Layout layout_of(const ntops_attention_desc& d, bool backward, const Choice& c) 
         at += up(bytes, 256);
         return here;
     };
-    l.plan = take(d.cu_q && !d.plan ? plan_of(d, backward ? kAttnQueries : c.queries).bytes : 0);
+    l.plan = take(d.cu_q && !d.plan ? plan_of(d).bytes : 0);
     if (backward) {
         l.delta = take(d.q_rows * d.heads * 4);
         l.most = take(d.dtype == NTFP8_F16 ? 2 * kAttnMost * 4 : 0);
@@ -101,7 +111,7 @@ AttnArgs args_of(const ntops_attention_desc& d) {
     a.q_batch = d.q_batch, a.k_batch = d.k_batch, a.v_batch = d.v_batch, a.do_batch = d.do_batch;
     a.sequences = (int)d.sequences, a.q_len = (int)(d.q_rows / d.sequences), a.k_len = (int)(d.k_rows / d.sequences);
     a.q_rows = d.q_rows, a.k_rows = d.k_rows;
-    a.heads = d.heads, a.kv_heads = d.kv_heads, a.group = d.heads / d.kv_heads, a.dim = d.head_dim, a.causal = d.causal;
+    a.tile_heads = tile_heads_of(d), a.heads = d.heads, a.kv_heads = d.kv_heads, a.group = d.heads / d.kv_heads, a.dim = d.head_dim, a.causal = d.causal;
     a.c = d.scale * kLog2E, a.scale = d.scale;
     a.out = d.out, a.o = d.out, a.low = d.out_low, a.lse = d.lse, a.dq = d.dq, a.dk = d.dk, a.dv = d.dv, a.splits = 1;
     return a;
@@ -112,24 +122,20 @@ AttnArgs args_of(const ntops_attention_desc& d) {
 // What a launch has to hold: workgroups, and threads, in 32 bits
 bool attention_fits(const ntops_attention_desc& d) {
     constexpr int64_t kMost = (int64_t)1 << 22;
-    return choose(d).tiles * d.kv_heads * attn_chunks(d.heads / d.kv_heads, choose(d).tile_heads) <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
+    return tiles_of(d, d.q_rows, queries_of(d)) * d.kv_heads * attn_chunks(d.heads / d.kv_heads, tile_heads_of(d)) <= kMost && tiles_of(d, d.q_rows, kAttnQueries) * d.heads <= kMost && tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads <= kMost;
 }
 
 int64_t attention_plan(const ntops_attention_desc& d) { return d.cu_q ? plan_of(d).bytes : 0; }
 
 int64_t attention_workspace(const ntops_attention_desc& d, bool backward) {
-    if (backward) return layout_of(d, true, {}).bytes;
-    // (what a forward call takes differs with a plan, which its descriptor may have got since)
-    ntops_attention_desc with = d, without = d;
-    with.plan = reinterpret_cast<void*>(256), without.plan = nullptr;
-    return std::max(layout_of(with, false, choose(with)).bytes, layout_of(without, false, choose(without)).bytes);
+    return layout_of(d, backward, choose(d)).bytes;
 }
 
 namespace {
 // the tasks of a call's sequences at `at`; those of keys where a backward pass reads them
-int make_plan(const ntops_attention_desc& d, char* at, int queries, bool keys, hipStream_t st) {
-    const Plan p = plan_of(d, queries);
-    return run_attention_plan(d.cu_q, d.cu_k, (int)d.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, queries, kAttnKeys, (int)p.q_tiles, (int)p.k_tiles,
+int make_plan(const ntops_attention_desc& d, char* at, bool keys, hipStream_t st) {
+    const Plan p = plan_of(d);
+    return run_attention_plan(d.cu_q, d.cu_k, (int)d.sequences, (int)d.q_rows, (int)d.k_rows, d.causal, queries_of(d), kAttnKeys, (int)p.q_tiles, (int)p.k_tiles,
                               reinterpret_cast<AttnTask*>(at), keys ? reinterpret_cast<AttnTask*>(at + p.keys_at) : nullptr, st);
 }
 }  // namespace
@@ -139,12 +145,12 @@ int run_attention_forward(const ntops_attention_desc& d, hipStream_t st) {
     const Layout l = layout_of(d, false, c);
     char* const ws = static_cast<char*>(d.workspace);
     AttnArgs a = args_of(d);
-    a.tiles = c.tiles, a.splits = c.splits, a.tile_heads = c.tile_heads;
+    a.tiles = c.tiles, a.splits = c.splits;
     if (c.splits > 1) a.part = reinterpret_cast<float*>(ws + l.part), a.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
     if (d.cu_q) {
         char* const plan = d.plan ? static_cast<char*>(d.plan) : ws + l.plan;
         a.tasks = reinterpret_cast<AttnTask*>(plan);
-        if (const int rc = make_plan(d, plan, c.queries, d.plan != nullptr, st)) return rc;
+        if (const int rc = make_plan(d, plan, d.plan != nullptr, st)) return rc;
     }
     return run_attention_forward_kernels(a, d.dtype, c.few, st);
 }
@@ -163,7 +169,7 @@ int run_attention_backward(const ntops_attention_desc& d, hipStream_t st) {
         a.tasks = reinterpret_cast<AttnTask*>(plan);
         k_list = reinterpret_cast<AttnTask*>(plan + p.keys_at);
         if (!d.plan)
-            if (const int rc = make_plan(d, plan, kAttnQueries, true, st)) return rc;
+            if (const int rc = make_plan(d, plan, true, st)) return rc;
     }
     return run_attention_backward_kernels(a, k_list, p.k_tiles, d.cu_q, d.cu_k, d.dtype, st);
 }
