@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(const Plan
 }
 
 // ------------------------------------------------------------------------------------------------ prompts
-// A workgroup owns 128 queries of one head, a wave 32 of them, and walks their keys 64 at a time: scores of 64 keys by 32
+// A workgroup owns 128 queries of one head, a wave 32 of them (or 32 queries of four heads, a wave each: AttnOwn), and walks their keys 64 at a time: scores of 64 keys by 32
 // queries, the running maximum and sum, and the product with the values, into out^T [elements][queries]: the queries are the columns of both products,
 // one a lane, so a row's maximum and sum stay in a lane (and its twin of the other half) and the scores are the second operand of the next product as
 // they come.  Tiles of keys and values travel straight into LDS.  The scores of the next tile are made while the exponentials of this one are: products

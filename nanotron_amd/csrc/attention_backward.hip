@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void attention_delta_kernel(const AttnArgs A, 
 // How a tile is taken: all its rows and keys see each other, or some do not, or these hold values that are not finite
 constexpr int kWhole = 0, kMasked = 1, kSingly = 2;
 
-// dq of 128 queries of one head, 32 a wave
+// dq of 128 queries of one head, 32 a wave, or of 32 of four heads
 template <int T, int DP>
 __device__ __forceinline__ void attention_dq(const AttnArgs& A, int group, uint8_t* lds) {
     typedef AttnTile<DP> Tile;
