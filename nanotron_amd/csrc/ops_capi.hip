@@ -101,12 +101,12 @@ int64_t reach(int64_t rows, int64_t stride, int64_t heads, int64_t head, int64_t
 int check_rotary(const ntops_rotary_desc& d) {
     if (!dtype_ok(d.dtype) || (d.position_bits != 32 && d.position_bits != 64)) return NTFP8_ERR_ENUM;
     if (d.heads < 0 || d.kv_heads < 0 || (d.heads > 0 && (!d.q || !d.q_out)) || (d.kv_heads > 0 && (!d.k || !d.k_out)) || !d.positions || !d.frequencies) return NTFP8_ERR_NULL;
-    if (d.tokens <= 0 || d.tokens > 0x7fffffff || d.heads + d.kv_heads < 1 || d.heads + d.kv_heads > 16384 || d.head_dim < 1 || d.pairs < 1 || 2 * d.pairs > d.head_dim ||
-        d.position_count < 1)
-        return NTFP8_ERR_SIZE;
+    const int64_t heads = (int64_t)d.heads + d.kv_heads;
+    if (d.tokens <= 0 || d.tokens > 0x7fffffff || heads < 1 || heads > 16384 || d.head_dim < 1 || d.pairs < 1 || d.pairs > d.head_dim / 2 || d.position_count < 1) return NTFP8_ERR_SIZE;
     constexpr int64_t kMost = (int64_t)1 << 31;   // elements from token to token and from head to head
     for (const int64_t v : {d.q_stride, d.q_head, d.k_stride, d.k_head})
         if (v < 0 || v > kMost) return NTFP8_ERR_SIZE;
+    if ((d.heads && d.q_stride > kMostElements / d.tokens) || (d.kv_heads && d.k_stride > kMostElements / d.tokens)) return NTFP8_ERR_SIZE;
     if (d.head_dim > 2048 || !(d.scale == d.scale)) return NTFP8_ERR_UNSUPPORTED;
     const size_t s = size_of(d.dtype);
     if (!aligned(d.q, s) || !aligned(d.k, s) || !aligned(d.q_out, s) || !aligned(d.k_out, s) || !aligned(d.positions, d.position_bits / 8) || !aligned(d.frequencies, 8))
@@ -114,8 +114,8 @@ int check_rotary(const ntops_rotary_desc& d) {
     const int64_t b = (int64_t)s;
     const Range in[] = {{d.heads ? d.q : nullptr, reach(d.tokens, d.q_stride, d.heads, d.q_head, d.head_dim) * b},
                         {d.kv_heads ? d.k : nullptr, reach(d.tokens, d.k_stride, d.kv_heads, d.k_head, d.head_dim) * b},
-                        {d.positions, d.position_count * d.position_bits / 8},
-                        {d.frequencies, 8 * d.pairs}};
+                        {d.positions, std::min(d.position_count, d.tokens) * d.position_bits / 8},
+                        {d.frequencies, 8 * (int64_t)d.pairs}};
     const Range out[] = {{d.heads ? d.q_out : nullptr, d.tokens * d.heads * d.head_dim * b}, {d.kv_heads ? d.k_out : nullptr, d.tokens * d.kv_heads * d.head_dim * b}};
     return collide(in, out) ? NTFP8_ERR_ALIAS : NTFP8_OK;
 }
