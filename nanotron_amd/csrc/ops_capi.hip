@@ -141,6 +141,11 @@ int check_attention(const ntops_attention_desc& d) {
         if (v < 0 || v > ((int64_t)1 << 24) || v % 8 != 0) return NTFP8_ERR_SIZE;
     for (const int64_t v : {d.q_head, d.k_head, d.v_head, d.do_head, d.q_batch, d.k_batch, d.v_batch, d.do_batch})
         if (v < 0 || v > kMostElements || v % 8 != 0) return NTFP8_ERR_SIZE;
+    // (where they are used, all heads and sequences together lie within that too)
+    const int64_t most = kMostElements / d.heads, most_kv = kMostElements / d.kv_heads, most_batch = d.cu_q ? kMostElements : kMostElements / d.sequences;
+    if (d.q_head > most || d.k_head > most_kv || d.v_head > most_kv || (d.dout && d.do_head > most) || d.q_batch > most_batch || d.k_batch > most_batch || d.v_batch > most_batch ||
+        (d.dout && d.do_batch > most_batch))
+        return NTFP8_ERR_SIZE;
     for (const void* p : {d.q, d.k, d.v, d.dout, (const void*)d.out, (const void*)d.dq, (const void*)d.dk, (const void*)d.dv})
         if (!aligned(p, 16)) return NTFP8_ERR_ALIGN;
     return aligned(d.lse, 4) && aligned(d.cu_q, 4) && aligned(d.cu_k, 4) && aligned(d.workspace, 256) && aligned(d.plan, 256) && aligned(d.out_low, 8) ? NTFP8_OK : NTFP8_ERR_ALIGN;
