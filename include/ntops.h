@@ -177,7 +177,7 @@ int ntops_rotary(const ntops_rotary_desc* d, void* stream);
  * lengths q_rows / sequences and k_rows / sequences, q_batch, k_batch, v_batch elements apart.
  * causal: row i of a sequence of n queries and m keys sees the keys 0 .. m - n + i, so that the last rows of both belong together.  A
  * row that sees no key, and a row of q that belongs to no sequence, is 0, and so are its gradients; what is in rows of k and v
- * that a row does not see, NaN say, does not reach it.
+ * that a row does not see, NaN say, does not reach it.  A row whose keys all score minus infinity is 0 / 0: it and its gradients are NaN.
  * head_dim <= 128, a multiple of 8; scale 1e-30 to 1e30; dtype NTFP8_BF16 or NTFP8_F16.  Scores, maxima, sums and outputs are fp32 until the one rounding of
  * out; the softmax's numerators are rounded to dtype for the product with v.  out is dense; lse [heads][q_rows] fp32 (minus the logarithm of a row's
  * sum of exponentials, over scale) is what a backward pass needs, NULL if none follows.  q_rows * heads and k_rows * kv_heads at most 2^27.

@@ -370,9 +370,16 @@ __device__ __forceinline__ float both_sum(float v) {
     return __uint_as_float(x) + __uint_as_float(y);
 }
 
-// what is kept of a row's maximum (base 2) and sum for the backward pass, and whether it sees anything
-__device__ __forceinline__ bool attn_any(float sum) { return sum > 0.0f || sum != sum; }
-__device__ __forceinline__ float attn_lse(const AttnArgs& A, float top, float sum) { return attn_any(sum) ? -(top + log2f(sum)) / A.c : -__builtin_inff(); }
+// The maximum (base 2) of a row is minus infinity where it sees no key.  Where it sees some that all score minus infinity (an infinity in the query, a
+// product beyond fp32) or NaN it is this instead, so that the row's sum, 0, makes the 0 / 0 that its softmax is, while beside a run of keys with
+// scores it counts nothing: exp2(this - their maximum) is 0
+constexpr float kAttnLowest = -3.4028234663852886e38f;
+__device__ __forceinline__ float attn_top(float top, bool sees) { return sees && top == -__builtin_inff() ? kAttnLowest : top; }
+// what a row's outputs are multiplied by, and what is kept of its maximum and sum for the backward pass
+__device__ __forceinline__ float attn_over(float top, float sum) { return top == -__builtin_inff() ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ float attn_lse(const AttnArgs& A, float top, float sum) {
+    return top == -__builtin_inff() ? top : sum == 0.0f ? __builtin_nanf("") : -(top + log2f(sum)) / A.c;
+}
 
 // calls f with the type and the head's size rounded up to what the kernels are built for
 template <typename F>

@@ -307,6 +307,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (what was requested behind the last tile lands in this workgroup's LDS)
     const float all = both_sum(sum);
+    top = attn_top(top, steps > 0 && first * kAttnStep <= last_key);   // (of this run's keys)
     const int64_t at = (int64_t)task.own + row;
     if (A.splits > 1) {
         if (!live) return;
@@ -321,7 +322,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
             }
         return;
     }
-    store_rows<T, DP>(out, attn_any(all) ? 1.0f / all : 0.0f, A.out, (at * A.heads + head) * A.dim, A.dim, live, lane, A.low);
+    store_rows<T, DP>(out, attn_over(top, all), A.out, (at * A.heads + head) * A.dim, A.dim, live, lane, A.low);
     if (A.lse && live && lane < 32) A.lse[head * A.q_rows + at] = attn_lse(A, top, all);
 }
 
@@ -445,6 +446,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         }
     }
     sum = both_sum(sum);
+    top = attn_top(top, steps > 0 && first * kFewStep <= min(len - 1, last_row));   // (of this wave's keys)
     if (lane < kFewRows) ml[wave][lane] = make_float2(top, sum);
     __syncthreads();
     float all_top = -__builtin_inff(), all_sum = 0.0f;
@@ -453,9 +455,9 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
 #pragma unroll
     for (int w = 0; w < kAttnWaves; ++w) {
         const float2 o = ml[w][row];
-        if (o.x != -__builtin_inff() || o.y != 0.0f) all_sum += o.y * (o.x == all_top ? 1.0f : exp2_fast(o.x - all_top));
+        if (o.x != -__builtin_inff()) all_sum += o.y * (o.x == all_top ? 1.0f : exp2_fast(o.x - all_top));
     }
-    const float mine = top == -__builtin_inff() ? (sum != sum ? 1.0f : 0.0f) : top == all_top ? 1.0f : exp2_fast(top - all_top);
+    const float mine = top == -__builtin_inff() ? 0.0f : top == all_top ? 1.0f : exp2_fast(top - all_top);
     // the waves' outputs, [wave][element][row] in the stages that they no longer need, added up in the order of the waves
     float* const at = reinterpret_cast<float*>(&sk[0][0]);
     static_assert(sizeof(sk[0]) >= sizeof(float) * 64 * kFewRows && sizeof(sk) + sizeof(sv) >= sizeof(float) * kAttnWaves * DP * kFewRows, "");
@@ -475,7 +477,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         const int in = r / n, tok = r - in * n, hd = kv * A.group + in;
         const int64_t out_row = (int64_t)seq * n + tok;
         const int64_t to = ((int64_t)blockIdx.y * A.q_rows + out_row) * A.heads + hd;
-        const float by = A.splits > 1 ? 1.0f : attn_any(all_sum) ? 1.0f / all_sum : 0.0f;
+        const float by = A.splits > 1 ? 1.0f : attn_over(all_top, all_sum);
         for (int d = (threadIdx.x >> 5) * 8; d < A.dim; d += 64) {
             const float* const from = d < 64 ? at : over;
             float x[8] = {};
@@ -526,9 +528,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
     for (int m = 32; m >= 1; m /= 2) top = fmaxf(top, __shfl_xor(top, m));
     float sum = 0.0f, x[8] = {};
     auto add = [&](float2 o, v4f a, v4f b) __attribute__((always_inline)) {
-        // (an empty split, of which nothing counts; not one whose sum is NaN)
-        const bool none = o.x == -__builtin_inff() && o.y == 0.0f;
-        const float by = none ? 0.0f : o.x == top ? 1.0f : exp2_fast(o.x - top);
+        // (of a split of which the row sees nothing, nothing counts)
+        const float by = o.x == -__builtin_inff() ? 0.0f : o.x == top ? 1.0f : exp2_fast(o.x - top);
         sum += o.y * by;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -551,7 +552,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs A) {
     }
     if (run != 0) return;
     if (d < A.dim) {
-        const float over = attn_any(sum) ? 1.0f / sum : 0.0f;
+        const float over = attn_over(top, sum);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= over;
         store_piece<T, 8>(A.out, row * A.dim + d, x);

@@ -18,7 +18,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: 
     heads is a multiple of kv_heads: head h reads key head `h // (heads // kv_heads)`.  causal: of n queries and m keys of a sequence query i
     sees the keys 0 .. m - n + i, so the last ones belong together.  A query that sees no key has output 0 and no gradient, and so
     have rows before the first sequence and behind the last.  Whatever keys and values hold that a query does not see (NaN in padding,
-    tokens to come) does not reach it.  scale: 1 / sqrt(head_dim) by default.
+    tokens to come) does not reach it.  A query whose keys all score minus infinity has NaN, as its softmax is 0 / 0: an overflow stays to be
+    seen.  scale: 1 / sqrt(head_dim) by default.
 
     bfloat16 or float16, head_dim a multiple of 8 up to 128.  Products run on the matrix cores with fp32 sums; maxima and sums are fp32; the
     softmax's numerators, and in backward the scores' gradients, are rounded to the type of q for the products they go into.  Rows are read where they are
