@@ -468,7 +468,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             float* const to = e < 2 ? at : over;
-            to[(wave * 64 + 32 * (e & 1) + place_of(r, lane)) * kFewRows + row] = mine == 0.0f ? 0.0f : out[e][r] * mine;
+            to[(wave * 64 + 32 * (e & 1) + place_of(r, lane)) * kFewRows + row] = out[e][r] * mine;   // (0 times what is not finite is NaN, as within a wave)
         }
     __syncthreads();
     // 8 threads a row, 8 elements at a time
