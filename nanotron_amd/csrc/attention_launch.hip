@@ -62,6 +62,7 @@ Choice choose(const ntops_attention_desc& d) {
 // of 128 over 8, for two, two and a half, three and four a CU: 1024 tokens 64, 65, 73, 91; 2048 160, 153, 161, 173; 4096 648, 474, 473, 485.  For
 // 8, 10 and 16 steps at least: 512 tokens of these heads 38, 40, 45; 1500 of 2 heads of 128 47, 45, 41; 1000 of 4 of 64 over one 29, 27, 27.
 int key_splits(const ntops_attention_desc& d) {
+    if (d.k_rows == 0) return 1;   // (nothing to add up: a launch of no workgroups is an error)
     const int64_t rows = std::min(d.q_rows, d.q_rows / d.sequences * (d.cu_q && d.sequences > 1 ? 2 : 1));
     const int64_t units = std::max<int64_t>(1, tiles_of(d, d.k_rows, kAttnKeys) * d.kv_heads), steps = (rows + kAttnKeyStep - 1) / kAttnKeyStep * (d.heads / d.kv_heads);
     return (int)std::max<int64_t>(1, std::min(5 * cu_count() / 2 / units, steps / 10));
