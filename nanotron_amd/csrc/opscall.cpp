@@ -480,7 +480,8 @@ Attended attended(const Tensor& x) {
     a.t = walks(x) ? x : x.contiguous();
     if (!walks(a.t)) a.t = a.t.clone(at::MemoryFormat::Contiguous);   // (a dense view that begins off a 16-byte boundary)
     const int64_t n = a.t.dim(), dim = a.t.size(-1);
-    const auto stride = [&](int64_t i) { return a.t.size(i) > 1 ? a.t.stride(i) : dim; };
+    // (a dimension of one element, or a tensor of none, may have any distance: nothing walks it)
+    const auto stride = [&](int64_t i) { return a.t.size(i) > 1 && a.t.numel() ? a.t.stride(i) : dim; };
     a.head = stride(n - 2), a.row = stride(n - 3), a.batch = n == 4 ? stride(0) : 0;
     return a;
 }
