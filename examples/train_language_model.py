@@ -70,6 +70,7 @@ class DecoderBlock(nn.Module):
 class LanguageModel(nn.Module):
     def __init__(self, vocab: int, hidden: int, layers: int, device="cuda", heads: int = 0, kv_heads: int = 0):
         super().__init__()
+        self.decoder = heads > 0
         self.embedding = nn.Embedding(vocab, hidden, device=device, dtype=torch.bfloat16)
         self.blocks = nn.ModuleList(DecoderBlock(hidden, heads, kv_heads or heads, device) if heads else Block(hidden, device) for _ in range(layers))
         self.norm = RMSNorm(hidden, device=device) if heads else LayerNorm(hidden, device=device)
@@ -82,7 +83,7 @@ class LanguageModel(nn.Module):
         requantize_fp8_weights(self)
 
     def forward(self, tokens: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
-        if not isinstance(self.blocks[0], DecoderBlock):
+        if not self.decoder:
             x = self.embedding(tokens)
             for b in self.blocks:
                 x = b(x)
@@ -94,7 +95,7 @@ class LanguageModel(nn.Module):
         x, residual = self.embedding(tokens.flatten()), None
         for b in self.blocks:
             x, residual = b(x, residual, positions, cu_seqlens)
-        y, _ = self.norm(x, residual)
+        y = self.norm(x) if residual is None else self.norm(x, residual)[0]
         return linear_cross_entropy(y, self.head, labels.flatten())
 
 
