@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (what was requested behind the last tile lands in this workgroup's LDS)
     const float all = both_sum(sum);
-    top = attn_top(top, steps > 0 && first * kAttnStep <= last_key);   // (of this run's keys)
+    top = attn_top(top, first * kAttnStep <= last_key);   // (of this run's keys)
     const int64_t at = (int64_t)task.own + row;
     if (A.splits > 1) {
         if (!live) return;
@@ -446,7 +446,7 @@ __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const
         }
     }
     sum = both_sum(sum);
-    top = attn_top(top, steps > 0 && first * kFewStep <= min(len - 1, last_row));   // (of this wave's keys)
+    top = attn_top(top, first * kFewStep <= min(len - 1, last_row));   // (of this wave's keys)
     if (lane < kFewRows) ml[wave][lane] = make_float2(top, sum);
     __syncthreads();
     float all_top = -__builtin_inff(), all_sum = 0.0f;
