@@ -140,3 +140,24 @@ def test_what_outs_rounding_leaves_out_reaches_the_gradients(n, m, dtype):
     # and the bound tells: delta made of the rounded out alone would leave more than it in many rows
     off = ((G @ (o.to(dtype).double() - o))[..., None] * K[0, 0] * dim ** -0.5).abs()
     assert ((off > limit).any(-1).double().mean() > 0.25).item()
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+@pytest.mark.parametrize("used", [[100, 3, 0, 57], [1, 1, 100, 99], [0, 0, 0, 1]])
+def test_a_batched_cache_that_is_used_up_to_lengths_of_its_own(used, tokens):
+    """Packed: a sequence for what is in use, and one of no queries for the room behind it, which may hold anything."""
+    room, heads, kv_heads, dim, b = 100, 8, 2, 64, len(used)
+    g = torch.Generator().manual_seed(tokens)
+    q = torch.randn(b, tokens, heads, dim, generator=g).bfloat16().to(DEV)
+    k, v = (torch.randn(b, room, kv_heads, dim, generator=g).bfloat16().to(DEV) for _ in range(2))
+    at = torch.tensor(used, device=DEV)
+    behind = torch.arange(room, device=DEV)[None] >= at[:, None]
+    k[behind], v[behind] = math.nan, math.inf
+    starts = torch.arange(b, device=DEV) * room
+    cu_k = torch.cat([torch.stack([starts, starts + at], 1).flatten(), torch.tensor([b * room], device=DEV)]).int()
+    cu = (torch.arange(2 * b + 1, device=DEV).add(1).div(2, rounding_mode="floor") * tokens).int()
+    with torch.no_grad():
+        out = attention(q.flatten(0, 1), k.flatten(0, 1), v.flatten(0, 1), cu_seqlens=cu, cu_seqlens_k=cu_k).view_as(q)
+    for i, n in enumerate(used):
+        want, bound = exact(q[i], k[i, :n], v[i, :n], torch.zeros_like(q[i]), [(tokens, n)])
+        near(out[i], want[0], bound[0], f"sequence {i}")
