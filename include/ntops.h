@@ -186,8 +186,9 @@ int ntops_rotary(const ntops_rotary_desc* d, void* stream);
  * workspace: ntops_attention_workspace(d, backward) bytes, aligned to 256.  plan (packed sequences, may be NULL): ntops_attention_plan(d) bytes,
  * aligned to 256, that a forward call fills and the backward call of the same sizes and offsets reads; without it each makes its own (in its
  * workspace, which is the larger for it).
- * Backward: dq, dk, dv (dense, dtype, each may be NULL) from dout (strides as q's) and the q, k, v, out and lse of the forward call.
- * The same inputs give the same bits.  fp16: p and ds are kept with powers of two on them, so that gradients below its normal range survive. */
+ * Backward: dq, dk, dv (dense, dtype, each may be NULL) from dout (do_stride, do_head, do_batch, with the limits of q's) and the q, k, v, out and lse of the forward call.
+ * The same inputs give the same bits.  fp16: p and ds are kept with powers of two on them, ds with one a call, from the largest finite dout and v, so that gradients
+ * below its normal range survive that are no more than 2^28 below 2 head_dim times these. */
 typedef struct ntops_attention_desc {
     const void* q;
     const void* k;

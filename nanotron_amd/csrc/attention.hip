@@ -109,8 +109,8 @@ __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(const Plan
 // they come.  Tiles of keys and values travel straight into LDS.  The scores of the next tile are made while the exponentials of this one are: products
 // and arithmetic then share a wave's time.
 //
-// Bound by the products: 16384 causal tokens, 32 heads of 128 over 8, in bf16 take 2.0 to 2.1 ms, 1.1 PFLOP/s, with 65 % of the matrix instructions' slots taken at
-// the 1.5 GHz that the power limit leaves (all-zero operands, the same instructions: 1.48 PFLOP/s); 4096 tokens 152 us.  Tried: 64 queries a
+// Bound by the products: 16384 causal tokens, 32 heads of 128 over 8, in bf16 take 2.0 to 2.1 ms, 1.1 PFLOP/s, with 63 to 65 % of the matrix instructions' slots taken at
+// the 1.5 to 1.6 GHz that the power limit leaves (all-zero operands, the same instructions: 1.48 PFLOP/s); 4096 tokens 152 to 156 us.  Tried: 64 queries a
 // wave, which halves the reads of LDS but moves sums between register files (slower); three and four tiles ahead, and waves of raised priority (nothing).
 template <int T, int DP>
 __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attention_forward_kernel(const AttnArgs A) {
@@ -330,8 +330,8 @@ __global__ __launch_bounds__(64 * kAttnWaves, attn_workgroups(DP)) void attentio
 // Where the queries of a group of heads are 32 rows or fewer (a token, or a few, of every sequence) the keys are the work: the rows
 // (head in its group, query) share them, every wave takes keys of its own, 32 at a time through LDS of its own without a
 // barrier, and the waves' results are joined at the end; workgroups' (`splits` of a sequence) by a second launch.
-// Bound by memory: 32 tokens over caches of 8192, 8 heads of 128 in bf16, are 1.07 GB in 191 us, 5.6 TB/s.  One token over 4096 keys is latency, 8.6 us
-// here (a launch, the trip for keys and values, 8 products in a row, the waves' join) and 3.5 for the second launch.
+// Bound by memory: 32 tokens over caches of 8192, 8 heads of 128 in bf16, are 1.07 GB in 190 us, 5.7 TB/s.  One token over 4096 keys is latency, 8.2 to
+// 8.6 us here (a launch, the trip for keys and values, 8 products in a row, the waves' join) and 3.5 to 3.9 for the second launch.
 constexpr int kFewStep = 32, kFewRows = 32;
 template <int T, int DP>
 __global__ __launch_bounds__(64 * kAttnWaves, 1) void attention_few_kernel(const AttnArgs A) {

@@ -4,10 +4,11 @@
 // would do, so that every sum is made in one place and order: no atomics, the same bits for the same inputs.
 //
 // Bound by the products: 16384 causal tokens, 32 heads of 128 over 8, in bf16 take 6.4 to 6.8 ms, 0.86 PFLOP/s of the five products and 1.2 of the seven that are
-// made, 71 % of the matrix instructions' slots at the 1.5 GHz that the power limit leaves; 4096 tokens 431 us.  delta is memory, 4.8 TB/s.
+// made, 70 % of the matrix instructions' slots at the 1.4 to 1.5 GHz that the power limit leaves; 4096 tokens 431 to 438 us.  delta is memory, 4.8 TB/s.
 //
 // fp16: ds is a gradient and may be smaller than that type's normal numbers, and p in a long row is.  p is kept times 2^8, ds
-// times the power of two that the largest magnitudes of dout and v allow it without overflow.
+// times the power of two that the largest magnitudes of dout and v allow it without overflow.  That one serves the call: what is 2^28 below 2 dim |dout| |v|
+// of the largest of all its sequences goes into that type's subnormals.
 #include "attention.h"
 
 namespace ntfp8 {

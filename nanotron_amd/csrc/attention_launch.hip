@@ -19,7 +19,7 @@ int64_t tiles_of(const ntops_attention_desc& d, int64_t rows, int64_t tile) {
 
 // Heads of a group whose 32 queries a workgroup's waves take, or 1, and 128 queries of that one: what leaves fewer waves without rows; of packed sequences,
 // whose tiles end anywhere, also where that is equal, up to a length that makes no difference.  (us: a token of 32 sequences over 8192 keys each, packed, 32
-// heads of 128 over 8, 214 and 385 by one head; 64 causal sequences of 16384 tokens, forward 131 and 147, both passes 525 and 560; 4 sequences of 64
+// heads of 128 over 8, 204 to 214 and 385 by one head; 64 causal sequences of 16384 tokens, forward 131 and 147, both passes 525 and 560; 4 sequences of 64
 // over 2000 keys 31 and 36.  64 causal sequences of a batch of 512, equal waves: 302 and 290.)
 constexpr int64_t kSharedRows = 1024;
 int tile_heads_of(const ntops_attention_desc& d) {
@@ -40,7 +40,9 @@ struct Choice {
 // there are fewer workgroups than the chip holds.  Few rows, into 128 keys at least, a step of each of four waves, and only beyond 512, which four steps
 // take as long as the launch that joins (uncut and cut, over 256 keys 8.4 and 10.4, 512 10.2 and 10.4, 640 11.1 and 10.4; into 128 and 256, 4096
 // keys 11.1 and 11.7).  More rows, into 512 keys at least (512 tokens over 8192 keys 85, 130 uncut, 95 with twice as many runs; of
-// 512 and 256 at least: 512 tokens of 32 heads of 128 24 and 34, 1500 of 2 heads 33 and 30).
+// 512 and 256 at least: 512 tokens of 32 heads of 128 24 and 34, 1500 of 2 heads 33 and 30).  Packed sequences are cut by their average length, which is all that the
+// host knows: a token each, 32 heads of 128 over 8, over 32 caches of 260 to 16380 keys in even steps 319 us for 213 at the copy's rate, of 128 to 32768 evenly in their
+// logarithm 515 for 145, over one of 32768 and 31 of 100, uncut, 511 for 29.
 Choice choose(const ntops_attention_desc& d) {
     const int64_t cus = cu_count(), q_len = d.q_rows / d.sequences, k_len = d.k_rows / d.sequences;   // (of packed ones, on average)
     Choice c = {};

@@ -4,7 +4,9 @@
 //
 // Bound by memory.  A row lives in the registers of the threads that read it, so that both norms cost one read; h is rounded to the type of
 // the residual stream before the second norm reads it, as the backward pass does, which has it from memory.
-// 16384 rows of 4096, bf16 with an fp32 residual stream, both norms and a gate: 805 MB forward in 160 us, 5.0 TB/s, 1208 MB backward in 245, 4.9 TB/s.
+// 16384 rows of 4096, bf16 with an fp32 residual stream, both norms and a gate: 805 MB forward in 153 us, 1208 MB backward in 229, 5.3 TB/s.  Backward with a norm behind the block or
+// a gate over more than 8192 elements of 16 bits holds two pieces of every row and vector a thread, of which 105 to 110 registers are spilled: 4096 rows of 16384, both norms and a
+// gate, 574 us, 2.1 TB/s (without them 215, 5.0; forward 176, 4.6).
 #include "ops_common.h"
 
 namespace ntfp8 {

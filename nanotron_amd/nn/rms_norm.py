@@ -29,14 +29,15 @@ def residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[
     post_weight and a channel's gate are optional, float32 or of the type of x, of one type.  Arithmetic is fp32; the gradients of
     weights and of a channel's gate are summed in fp32 within a workgroup and in 64 bits over them, in an order that depends on the
     sizes alone, so gradients repeat bit for bit.  Rows that are dense in themselves (a slice of a wider 2-D tensor) are read where they
-    are.  Up to 16384 columns of a 16-bit x, 8192 of float32.  ValueError / TypeError for what does not fit; differentiable once."""
+    are.  Up to 16384 columns of a 16-bit x, 8192 of float32 (backward with a post_weight or a gate takes 2.5 times as long an element beyond 8192 columns of a 16-bit
+    x).  ValueError / TypeError for what does not fit; differentiable once."""
     y, h = _ops.host.rms_norm(x, residual, weight, post_weight, gate, eps, residual_scale)
     return y, h
 
 
 class RMSNorm(nn.Module):
-    """`rms_norm` as a module, with the constructor of torch.nn.RMSNorm for one normalised dimension.  Called with a residual as
-    well, it is `residual_rms_norm` and returns (y, h); `post_norm` and `gate` then say whether the block's output has a norm of its own
+    """`rms_norm` as a module, with the constructor of torch.nn.RMSNorm for one normalised dimension, but for `eps`, a number here (there None by
+    default, the epsilon of the type).  Called with a residual as well, it is `residual_rms_norm` and returns (y, h); `post_norm` and `gate` then say whether the block's output has a norm of its own
     (`post_weight`) and a learned gate for each channel (`gate`, at `gate_init`).  `dtype` is that of the weights, which may stay
     float32 beside 16-bit activations."""
 
